@@ -176,6 +176,80 @@ int ts5hip_argmax(ts5hip_ctx *ctx, const float *x, int n, int rows, int32_t *out
  * of engine/src/engine.cpp:19-33). */
 int ts5hip_topk(ts5hip_ctx *ctx, const float *x, int n, int k, float *vals_dev, int32_t *ids_dev);
 
+/* ---- trees of drafts, key weights, eviction, block-sparse attention: device pointers, asynchronous on
+ * the context's stream, as above. No counterpart in the reference (its verify batch is a chain of
+ * consecutive positions and its caches keep and read every key).
+ *
+ * kv_type TS5HIP_KV_Q8: k, v int8 [cache][n_head_kv][n_ctx][head_dim], ks, vs f16 [..][head_dim / 32]; V
+ * counts within f16's range (65504). TS5HIP_KV_F16: k, v f16, ks and vs null. B caches lie back to back.
+ * Head dimension 64, 128 or 256, up to 16 query heads a KV head, n_ctx x head_dim x value bytes a KV head
+ * below 2 GiB. q, out, cache values and bounds are 16-byte aligned. Counts on the device
+ * (n_keys_dev, n_past_dev) are taken into 0..n_ctx. A query without a key gets zeros. Scratch is the
+ * context's: it grows on the first call of a size, and no two streams use it. ---- */
+
+/* ts5hip_rope_kv_append with each token's RoPE position pos_dev[t] (0..n_pos - 1, the rows of rope_cs) apart
+ * from its cache slot *slot0_dev + t: the drafts of a tree that share a depth share a position, and an
+ * evicted cache has fewer slots than positions. Either cache type; a token whose position or slot is out
+ * of range is left out, its row of q_out too. */
+int ts5hip_rope_kv_append_at(ts5hip_ctx *ctx, const float *qkv, int ntok, const int32_t *pos_dev,
+                             const int32_t *slot0_dev, int n_head, int n_head_kv, int head_dim, int n_rot, int neox,
+                             const float *rope_cs, int n_pos, int n_ctx, int kv_type, const float *bias,
+                             const float *q_norm, const float *k_norm, float eps, float *q_out, void *k, void *ks,
+                             void *v, void *vs);
+/* Attention of a tree of n_tree (1..64) drafted tokens over each of B caches: the tokens' K and V are at
+ * slots n_past_dev[b] .. + n_tree - 1, and token t of cache b reads every key below n_past_dev[b] and key
+ * n_past_dev[b] + j for each set bit j of mask_dev[b * n_tree + t] (its ancestors and itself; bits from n_tree
+ * on count as clear). Infinite or NaN values of tokens that a row's mask leaves out do not reach it.
+ * q, out: [B][n_tree][n_head * head_dim]. */
+int ts5hip_attn_tree(ts5hip_ctx *ctx, const float *q, int B, int n_tree, int n_head, int n_head_kv, int head_dim,
+                     int kv_type, const void *k, const void *ks, const void *v, const void *vs, int n_ctx,
+                     const int32_t *n_past_dev, const uint64_t *mask_dev, float scale, float *out);
+/* The accepted path of a tree to the front, in place: cache b's rows at slots slots_dev[b * n + i] (1 <= n <= 64)
+ * to slots slot0_dev[b] + i, all read before any is written. A row whose slot or place is not in
+ * the cache (-1 pads a shorter path) is left out. */
+int ts5hip_kv_path(ts5hip_ctx *ctx, int B, int n_head_kv, int head_dim, int kv_type, void *k, void *ks, void *v, void *vs,
+                   int n_ctx, const int32_t *slots_dev, int n, const int32_t *slot0_dev);
+/* ts5hip_attn_decode of one query per cache (n_keys_dev[b] keys each) that also adds up what each key was
+ * worth: acc_out[b][h][j] = acc[b][h][j] + the softmax weights of key j over KV head h's query heads, for
+ * j < n_keys_dev[b]; later entries stay as they are. acc, acc_out: [B][n_head_kv][n_ctx], the same
+ * array or not overlapping. */
+int ts5hip_attn_decode_weights(ts5hip_ctx *ctx, const float *q, int B, int n_head, int n_head_kv, int head_dim,
+                               int kv_type, const void *k, const void *ks, const void *v, const void *vs, int n_ctx,
+                               const int32_t *n_keys_dev, float scale, float *out, const float *acc, float *acc_out);
+/* ts5hip_attn_prompt (nq queries, 1..4096, at positions pos0 .. over one cache, causal) with the same sums, over the
+ * chunk's queries too. */
+int ts5hip_attn_prompt_weights(ts5hip_ctx *ctx, const float *q, int nq, int n_head, int n_head_kv, int head_dim,
+                               int kv_type, const void *k, const void *ks, const void *v, const void *vs, int n_ctx,
+                               int pos0, float scale, float *out, const float *acc, float *acc_out);
+/* Cuts each of B caches back to n_keep keys a KV head, in another cache of n_ctx_out slots: the first n_first
+ * and the last n_last of its n_keys_dev[b] keys, then those of the largest acc (ties to the lowest slot, NaN
+ * last), in slot order; all of them where there are no more than n_keep. Each KV head keeps its own. acc_out
+ * [B][n_head_kv][n_ctx_out] gets their sums and zeros behind them; kept_dev [B][n_head_kv][n_keep] their slots
+ * (-1 behind the last); n_out_dev [B] (may be null) the keys kept. Cache rows behind them stay as they are. The
+ * outputs overlap none of the inputs. */
+int ts5hip_kv_evict(ts5hip_ctx *ctx, int B, int n_head_kv, int head_dim, int kv_type, const void *k, const void *ks,
+                    const void *v, const void *vs, int n_ctx, const int32_t *n_keys_dev, const float *acc, int n_keep,
+                    int n_first, int n_last, int n_ctx_out, void *k_out, void *ks_out, void *v_out, void *vs_out,
+                    float *acc_out, int32_t *kept_dev, int32_t *n_out_dev);
+/* Bytes of the bounds of B caches in blocks of 16, 32, 64 or 128 keys: f16
+ * [B][n_head_kv][ceil(n_ctx / block)][lowest, highest][head_dim]; -1 for other blocks. */
+int64_t ts5hip_kv_bounds_bytes(int B, int n_head_kv, int head_dim, int n_ctx, int block);
+/* The bounds of the blocks that hold each cache's last n_new keys (of n_keys_dev[b]): each dimension's lowest
+ * and highest cached K value over the block's keys, rounded outwards to f16; NaN is passed over. Called after
+ * keys are appended (or overwritten after a rewind); other blocks' bounds stay. */
+int ts5hip_kv_block_bounds(ts5hip_ctx *ctx, int B, int n_head_kv, int head_dim, int kv_type, const void *k,
+                           const void *ks, int n_ctx, const int32_t *n_keys_dev, int n_new, int block, void *bounds);
+/* Attention over n_pick blocks of keys a query and KV head: the last block, the first, then those of
+ * the highest scores (ties to the lowest block), a block's score being the largest over the group's heads of
+ * sum_d max(q_d lowest_d, q_d highest_d), which no key of the block exceeds; NaN ranks first. Scores are fp64:
+ * equal choices for equal inputs. n_keys_dev and kv_per_batch as ts5hip_attn_decode has them; scale > 0.
+ * The last block needs no bounds. picked_dev [B][n_head_kv][n_pick] (may be null): the
+ * blocks read, ascending, -1 behind the last. */
+int ts5hip_attn_sparse(ts5hip_ctx *ctx, const float *q, int B, int n_head, int n_head_kv, int head_dim, int kv_type,
+                       const void *k, const void *ks, const void *v, const void *vs, int n_ctx,
+                       const int32_t *n_keys_dev, int kv_per_batch, const void *bounds, int block, int n_pick,
+                       float scale, float *out, int32_t *picked_dev);
+
 /* ---- the sampler: Engine::sample (engine/src/engine.cpp:16-46) on host, std::mt19937_64 ---- */
 ts5hip_sampler *ts5hip_sampler_new(uint64_t seed);
 void ts5hip_sampler_free(ts5hip_sampler *s);

@@ -1,0 +1,660 @@
+"""Attention of trees of drafts, key weights, eviction and block-sparse attention over q8 and f16 caches, through the C
+ABI, against float64 numpy.
+
+Tolerance of an attention output (Tol): a query enters as two fp16 planes, each rounded by half a step, so q keeps 2^-22
+of its size (and 2^-23 from the scale's product) and a score is off by at most 2 * 2^-22 sum |q k|; its fp32 sums add
+less than that again. A weight is off by that relative amount twice (numerator and normaliser), and by the
+roundings of the exponential, of its own two planes and of sums of n terms in any order: 16 + 4 sqrt(n) half steps of
+fp32 cover six standard deviations of independent roundings. An output is off by its weights' error times sum p |v|."""
+import numpy as np
+import pytest
+
+from tokenstation5_amd import ts5hip
+
+pytestmark = pytest.mark.gpu
+Q8, F16 = ts5hip.KV_Q8, ts5hip.KV_F16
+# (query heads, KV heads, head dimension)
+HEADS = [(4, 4, 64), (14, 2, 64), (32, 8, 128), (5, 1, 128), (16, 1, 128), (8, 4, 256), (6, 2, 256)]
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    c = ts5hip.Context(0)
+    yield c
+    c.close()
+
+
+class Cache:
+    """B caches of random K and V in host and device memory; k, v: their float64 values [B][HKV][slots][HD]."""
+
+    def __init__(self, ctx, rng, kv, B, HKV, slots, HD, std=1.0):
+        self.ctx, self.kv, self.B, self.HKV, self.slots, self.HD = ctx, kv, B, HKV, slots, HD
+        self.raw = {}
+        for n in "kv":
+            x = rng.standard_normal((B, HKV, slots, HD)).astype(np.float32) * np.float32(std)
+            if kv == F16:
+                self.raw[n] = x.astype(np.float16)
+            else:
+                r = x.reshape(B, HKV, slots, HD // 32, 32)
+                sc = (np.abs(r).max(-1) / np.float32(127)).astype(np.float16)
+                self.raw[n] = np.clip(np.rint(r / sc.astype(np.float32)[..., None]), -127, 127).astype(np.int8).reshape(x.shape)
+                self.raw[n + "s"] = sc
+        self.send()
+
+    def send(self):
+        self.dev = {n: self.ctx.to_device(a) for n, a in self.raw.items()}
+        return self
+
+    def values(self, n):
+        with np.errstate(invalid="ignore"):
+            x = self.raw[n].astype(np.float64)
+            if self.kv == Q8:
+                x = x * np.repeat(self.raw[n + "s"].astype(np.float64), 32, axis=-1)
+        return x
+
+    def fetch(self):
+        return {n: d.download(self.raw[n].dtype, self.raw[n].shape) for n, d in self.dev.items()}
+
+    @property
+    def args(self):
+        """kv type, k, ks, v, vs, slots as the entry points take them."""
+        d = self.dev
+        return self.kv, d["k"], d.get("ks"), d["v"], d.get("vs"), self.slots
+
+
+def attend(q, k, v, seen, scale):
+    """q [r][HD] over k, v [n][HD]; seen [r][n]: (out, weights, tolerance of out [r][HD], of the weights [r][n])."""
+    with np.errstate(invalid="ignore"):
+        s = np.where(seen, (q[:, None, :] * np.where(seen.any(0)[:, None], k, 0)[None]).sum(-1) * scale, -np.inf)
+    r, n = s.shape
+    if n == 0 or not seen.any():
+        return np.zeros_like(q), np.zeros((r, n)), np.zeros_like(q) + 1e-30, np.zeros((r, n)) + 1e-30
+    m = np.where(seen.any(1), s.max(1), 0)[:, None]
+    p = np.where(seen, np.exp(s - m), 0)
+    l = p.sum(1, keepdims=True)
+    p = p / np.where(l > 0, l, 1)
+    vz = np.where(seen.any(0)[:, None], v, 0)
+    size = np.abs(scale) * (np.abs(q) @ np.abs(np.where(seen.any(0)[:, None], k, 0)).T)
+    ds = np.where(seen, 4 * 2.0 ** -22 * size, 0).max(1, keepdims=True)
+    rel = 2 * ds + 2.0 ** -24 * (16 + 4 * np.sqrt(n))
+    return p @ vz, p, rel * (p @ np.abs(vz)) + 1e-30, rel * p + 1e-30
+
+
+def tree_seen(mask, n, T):
+    bits = (mask[:, None] >> np.arange(T, dtype=np.uint64)) & np.uint64(1)
+    return np.concatenate([np.ones((T, n), bool), bits.astype(bool)], 1)
+
+
+def random_masks(rng, B, T):
+    out = np.zeros((B, T), np.uint64)
+    for b in range(B):
+        for t in range(T):
+            p = int(rng.integers(-1, t)) if t else -1
+            out[b, t] = (int(out[b, p]) if p >= 0 else 0) | 1 << t
+    return out
+
+
+def check_rows(got, want, tol, what):
+    err = np.abs(got.astype(np.float64) - want)
+    assert np.all(err <= tol), (what, float((err / tol).max()), np.argwhere(err > tol)[:3].tolist())
+
+
+def run_tree(ctx, c, q, T, past, mask, scale, H, out=None):
+    B = c.B
+    out = out or ctx.alloc(q.nbytes)
+    ctx.attn_tree(ctx.to_device(q), B, T, H, c.HKV, c.HD, *c.args, ctx.to_device(np.asarray(past, np.int32)),
+                  ctx.to_device(mask), scale, out)
+    return out.download(np.float32, q.shape)
+
+
+def check_tree(c, q, T, past, mask, scale, H, got, what):
+    k, v, G = c.values("k"), c.values("v"), H // c.HKV
+    for b in range(c.B):
+        n = past[b]
+        seen = tree_seen(mask[b], n, T)
+        for h in range(H):
+            want, _, tol, _ = attend(q[b, :, h].astype(np.float64), k[b, h // G, :n + T], v[b, h // G, :n + T], seen, scale)
+            check_rows(got[b, :, h], want, tol, (*what, b, h))
+
+
+# ---- trees ---------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kv", [Q8, F16])
+@pytest.mark.parametrize("H,HKV,HD", HEADS)
+@pytest.mark.parametrize("B,T,past", [(1, 1, [0]), (1, 7, [40]), (2, 21, [130, 0]), (3, 64, [5, 333, 192])])
+def test_tree(ctx, kv, H, HKV, HD, B, T, past):
+    rng = np.random.default_rng([H, HD, T, kv])
+    c = Cache(ctx, rng, kv, B, HKV, max(past) + T + 3, HD)
+    q = rng.standard_normal((B, T, H, HD)).astype(np.float32)
+    mask = random_masks(rng, B, T)
+    scale = 1 / np.sqrt(HD)
+    got = run_tree(ctx, c, q, T, past, mask, scale, H)
+    check_tree(c, q, T, past, mask, scale, H, got, (kv, H, HD))
+
+
+@pytest.mark.parametrize("kv", [Q8, F16])
+@pytest.mark.parametrize("H,HKV,HD", [(14, 2, 64), (32, 8, 128), (8, 4, 256)])
+def test_tree_long(ctx, kv, H, HKV, HD):
+    """Past keys over many workgroups, units that end inside a slice and inside the tree."""
+    rng = np.random.default_rng([1, H, kv])
+    T, past = 33, [2001]
+    c = Cache(ctx, rng, kv, 1, HKV, 2048, HD)
+    q = rng.standard_normal((1, T, H, HD)).astype(np.float32)
+    mask = random_masks(rng, 1, T)
+    T2 = T  # slots 2001 .. 2033 of 2048
+    got = run_tree(ctx, c, q, T2, past, mask, 0.1, H)
+    check_tree(c, q, T2, past, mask, 0.1, H, got, (kv, H, HD))
+
+
+@pytest.mark.parametrize("kv", [Q8, F16])
+def test_tree_masks(ctx, kv):
+    """Rows that see nothing (zeros), bits past the tree (clear), tokens that do not see themselves."""
+    H, HKV, HD, T = 8, 2, 128, 9
+    rng = np.random.default_rng(3)
+    c = Cache(ctx, rng, kv, 2, HKV, 64, HD)
+    q = rng.standard_normal((2, T, H, HD)).astype(np.float32)
+    mask = np.array([[0, 1 << 63, 1 << 9, 0x1FF, 1 << 8, 0xFFFFFFFFFFFFFE00, 2, 5, 0]] * 2, np.uint64)
+    got = run_tree(ctx, c, q, T, [0, 20], mask, 0.09, H)
+    clear = mask & np.uint64(0x1FF)
+    check_tree(c, q, T, [0, 20], clear, 0.09, H, got, (kv,))
+    assert np.all(got[0, [0, 1, 2, 5, 8]] == 0)
+
+
+@pytest.mark.parametrize("kv", [Q8, F16])
+@pytest.mark.parametrize("H,HKV,HD", [(14, 2, 64), (8, 2, 128), (8, 4, 256)])
+def test_tree_nonfinite_values_of_other_branches(ctx, kv, H, HKV, HD):
+    """NaN and infinities in keys and values that a row's mask leaves out, and in slots behind the tree,
+    do not reach it; those of keys that it takes do."""
+    T, past = 12, [37]
+    rng = np.random.default_rng(5)
+    c = Cache(ctx, rng, kv, 1, HKV, 80, HD)
+    for n in "kv":
+        raw = c.raw[n + "s"] if kv == Q8 else c.raw[n]
+        raw[0, :, 37 + 4], raw[0, :, 37 + 7], raw[0, :, 37 + T:] = np.nan, np.inf, np.nan
+    if kv == F16:
+        c.raw["v"][0, :, 37 + 9, :3] = [-np.inf, np.inf, np.nan]
+    c.send()
+    q = rng.standard_normal((1, T, H, HD)).astype(np.float32)
+    mask = np.array([[1 << t for t in range(T)]], np.uint64)
+    got = run_tree(ctx, c, q, T, past, mask, 0.1, H)
+    clean = [t for t in range(T) if t not in (4, 7, 9)]
+    k, v, G = c.values("k"), c.values("v"), H // HKV
+    seen = tree_seen(mask[0], 37, T)
+    for h in range(H):
+        want, _, tol, _ = attend(q[0, clean, h].astype(np.float64), k[0, h // G, :37 + T], v[0, h // G, :37 + T], seen[clean], 0.1)
+        check_rows(got[0, clean, h], want, tol, (kv, h))
+    assert np.all(np.isnan(got[0, 4]))
+    assert not np.any(np.isfinite(got[0, 7]))
+    if kv == F16:
+        assert np.all(got[0, 9, :, 0] == -np.inf) and np.all(got[0, 9, :, 1] == np.inf) and np.all(np.isnan(got[0, 9, :, 2]))
+        assert np.all(np.isfinite(got[0, 9, :, 3:]))
+
+
+def test_tree_counts_outside_the_cache(ctx):
+    """Counts in device memory are taken into the cache: -5 as 0, one past the end as the last that fits."""
+    rng = np.random.default_rng(6)
+    c = Cache(ctx, rng, Q8, 2, 2, 40, 128)
+    q = rng.standard_normal((2, 4, 4, 128)).astype(np.float32)
+    mask = random_masks(rng, 2, 4)
+    got = run_tree(ctx, c, q, 4, [-5, 1000], mask, 0.1, 4)
+    check_tree(c, q, 4, [0, 36], mask, 0.1, 4, got, ("counts",))
+
+
+def test_tree_large_scores(ctx):
+    """One key far above the others, and queries of very different sizes."""
+    rng = np.random.default_rng(8)
+    c = Cache(ctx, rng, F16, 1, 1, 700, 128)
+    q = (rng.standard_normal((1, 5, 4, 128)) * np.array([1e-6, 1, 30, 1e4, 0])[:, None, None]).astype(np.float32)
+    mask = random_masks(rng, 1, 5)
+    got = run_tree(ctx, c, q, 5, [600], mask, 0.09, 4)
+    check_tree(c, q, 5, [600], mask, 0.09, 4, got, ("scores",))
+
+
+def test_tree_of_a_chain_is_a_verify_batch(ctx):
+    """A chain of drafts as a tree: what ts5hip_attn_decode gives for consecutive positions."""
+    H, HKV, HD, T, past = 32, 8, 128, 5, 777
+    rng = np.random.default_rng(9)
+    c = Cache(ctx, rng, Q8, 1, HKV, 800, HD)
+    q = rng.standard_normal((1, T, H, HD)).astype(np.float32)
+    mask = np.array([[(2 << t) - 1 for t in range(T)]], np.uint64)
+    got = run_tree(ctx, c, q, T, [past], mask, 0.08, H)
+    out = ctx.alloc(q.nbytes)
+    d = c.dev
+    ctx.attn_decode(ctx.to_device(q), T, H, HKV, HD, d["k"], d["ks"], d["v"], d["vs"], 800,
+                    ctx.to_device(np.array([past], np.int32)), 0, 0.08, out)
+    want = out.download(np.float32, q.shape)
+    check_tree(c, q, T, [past], mask, 0.08, H, want, ("decode",))
+    check_tree(c, q, T, [past], mask, 0.08, H, got, ("tree",))
+
+
+# ---- RoPE positions apart from slots, and the accepted path -------------------------------------------------
+
+@pytest.mark.parametrize("kv", [Q8, F16])
+@pytest.mark.parametrize("H,HKV,HD,neox", [(14, 2, 64, 1), (8, 2, 128, 0), (4, 1, 256, 1)])
+def test_append_at(ctx, kv, H, HKV, HD, neox):
+    """Each token as a chunk of its own at its position gives, row for row, what one call with the positions
+    gives; a token out of range leaves its rows alone."""
+    rng = np.random.default_rng([HD, kv])
+    T, slots, n_pos = 6, 32, 64
+    qkv = rng.standard_normal((T, (H + 2 * HKV) * HD)).astype(np.float32)
+    pos = np.array([9, 10, 10, 11, 64, 3], np.int32)  # the fifth is past the table
+    cs = ctx.rope_table(HD, n_pos, 10000.0)
+    norm = (1 + 0.1 * rng.standard_normal((2, HD))).astype(np.float32)
+    nq, nk = ctx.to_device(norm[0]), ctx.to_device(norm[1])
+    bias = ctx.to_device(rng.standard_normal((H + 2 * HKV) * HD).astype(np.float32))
+    c = Cache(ctx, rng, kv, 1, HKV, slots, HD)
+    before = c.fetch()
+    q_out = ctx.to_device(np.full((T, H * HD), 7, np.float32))
+    kvt, k, ks, v, vs, _ = c.args
+    ctx.rope_kv_append_at(ctx.to_device(qkv), T, ctx.to_device(pos), ctx.to_device(np.array([20], np.int32)), H, HKV, HD,
+                          HD, neox, cs, n_pos, slots, kvt, q_out, k, ks, v, vs, bias, nq, nk)
+    got, got_q = c.fetch(), q_out.download(np.float32, (T, H * HD))
+    for t in range(T):
+        if pos[t] >= n_pos:
+            assert np.all(got_q[t] == 7)
+            assert all(np.array_equal(got[n][:, :, 20 + t], before[n][:, :, 20 + t]) for n in got)
+            continue
+        one = Cache(ctx, rng, kv, 1, HKV, n_pos, HD)
+        q1 = ctx.alloc(H * HD * 4)
+        at = ctx.to_device(np.array([pos[t]], np.int32))
+        row = ctx.to_device(qkv[t])
+        ctx.rope_kv_append_at(row, 1, at, at, H, HKV, HD, HD, neox, cs, n_pos, n_pos, kvt, q1, *one.args[1:5], bias, nq, nk)
+        if kv == Q8 and HD < 256:  # the entry point whose slot is the position
+            d = one.dev
+            ctx.rope_kv_append(row, 1, at, H, HKV, HD, HD, neox, cs, n_pos, q1, d["k"], d["ks"], d["v"], d["vs"], bias, nq, nk)
+        assert np.array_equal(q1.download(np.float32), got_q[t])
+        o = one.fetch()
+        assert all(np.array_equal(o[n][:, :, pos[t]], got[n][:, :, 20 + t]) for n in o)
+    keep = [s for s in range(slots) if not 20 <= s < 26]
+    assert all(np.array_equal(got[n][:, :, keep], before[n][:, :, keep]) for n in got)
+
+
+@pytest.mark.parametrize("kv", [Q8, F16])
+@pytest.mark.parametrize("HKV,HD", [(2, 64), (8, 128), (1, 256)])
+def test_path(ctx, kv, HKV, HD):
+    rng = np.random.default_rng([HD, 2])
+    c = Cache(ctx, rng, kv, 4, HKV, 200, HD)
+    slots = np.full((4, 64), -1, np.int32)
+    slots[0, :4] = [100, 103, 104, 109]          # a path of a tree at 100
+    slots[1, :64] = np.arange(64)[::-1] + 30     # overlapping, descending
+    slots[2, :3] = [200, 5, 2 ** 31 - 1]         # outside: left out
+    slots[3, :3] = [1, 2, 3]
+    slot0 = np.array([100, 40, 10, 198], np.int32)  # the last one's third row has no place
+    ctx.kv_path(4, HKV, HD, *c.args, ctx.to_device(slots), 64, ctx.to_device(slot0))
+    got = c.fetch()
+    for n, raw in c.raw.items():
+        want = raw.copy()
+        for b in range(4):
+            for i in range(64):
+                if 0 <= slots[b, i] < 200 and slot0[b] + i < 200:
+                    want[b, :, slot0[b] + i] = raw[b, :, slots[b, i]]
+        assert np.array_equal(got[n], want), n
+
+
+# ---- key weights ---------------------------------------------------------------------------------------
+
+def weights_want(c, b, q, n, seen, scale, H):
+    """q [rows][H][HD]: outputs, their tolerances, per KV head the weights' sums and theirs."""
+    k, v, G = c.values("k"), c.values("v"), H // c.HKV
+    out, tol = np.zeros(q.shape), np.zeros(q.shape)
+    add, add_tol = np.zeros((c.HKV, n)), np.zeros((c.HKV, n))
+    for h in range(H):
+        o, p, t, tp = attend(q[:, h].astype(np.float64), k[b, h // G, :n], v[b, h // G, :n], seen, scale)
+        out[:, h], tol[:, h] = o, t
+        add[h // G] += p.sum(0)
+        add_tol[h // G] += tp.sum(0)
+    return out, tol, add, add_tol
+
+
+def check_sums(acc, got, n, add, add_tol, terms, what):
+    want = acc[:, :n] + add
+    tol = add_tol + 2.0 ** -24 * (terms + 1) * np.abs(want)  # the sum of the terms, and the sum with acc
+    check_rows(got[:, :n], want, tol, what)
+
+
+@pytest.mark.parametrize("kv", [Q8, F16])
+@pytest.mark.parametrize("H,HKV,HD", HEADS)
+@pytest.mark.parametrize("lengths", [[1], [0, 17, 130, 257], [1000, 64]])
+def test_decode_weights(ctx, kv, H, HKV, HD, lengths):
+    B, slots = len(lengths), max(lengths) + 30
+    rng = np.random.default_rng([H, HD, B, kv])
+    c = Cache(ctx, rng, kv, B, HKV, slots, HD)
+    for n in "kv":  # what lies behind the keys is not read
+        for b, m in enumerate(lengths):
+            (c.raw[n + "s"] if kv == Q8 else c.raw[n])[b, :, m:] = np.nan
+    c.send()
+    q = rng.standard_normal((B, H, HD)).astype(np.float32)
+    acc = rng.random((B, HKV, slots)).astype(np.float32)
+    n_keys = ctx.to_device(np.array(lengths, np.int32))
+    scale = 1 / np.sqrt(HD)
+    for alias in (False, True):
+        d_acc = ctx.to_device(acc)
+        d_to = d_acc if alias else ctx.to_device(np.full_like(acc, 7))
+        out = ctx.to_device(np.full_like(q, 9))
+        ctx.attn_decode_weights(ctx.to_device(q), B, H, HKV, HD, *c.args, n_keys, scale, out, d_acc, d_to)
+        got, sums = out.download(np.float32, q.shape), d_to.download(np.float32, acc.shape)
+        for b, n in enumerate(lengths):
+            want, tol, add, add_tol = weights_want(c, b, q[b:b + 1], n, np.ones((1, n), bool), scale, H)
+            check_rows(got[b:b + 1], want, tol, (kv, H, HD, b))
+            check_sums(acc[b], sums[b], n, add, add_tol, H // HKV, (kv, H, HD, b))
+            assert np.array_equal(sums[b, :, n:], acc[b, :, n:] if alias else np.full_like(acc[b, :, n:], 7))
+
+
+@pytest.mark.parametrize("kv", [Q8, F16])
+@pytest.mark.parametrize("H,HKV,HD", HEADS)
+@pytest.mark.parametrize("nq,pos0", [(1, 0), (5, 0), (37, 100), (3, 700)])
+def test_prompt_weights(ctx, kv, H, HKV, HD, nq, pos0):
+    rng = np.random.default_rng([H, HD, nq, kv])
+    n = pos0 + nq
+    c = Cache(ctx, rng, kv, 1, HKV, n + 9, HD)
+    q = rng.standard_normal((nq, H, HD)).astype(np.float32)
+    acc = rng.random((1, HKV, n + 9)).astype(np.float32)
+    scale = 1 / np.sqrt(HD)
+    out, d_to = ctx.alloc(q.nbytes), ctx.to_device(np.full_like(acc, 7))
+    ctx.attn_prompt_weights(ctx.to_device(q), nq, H, HKV, HD, *c.args, pos0, scale, out, ctx.to_device(acc), d_to)
+    got, sums = out.download(np.float32, q.shape), d_to.download(np.float32, acc.shape)
+    seen = np.arange(n)[None] <= pos0 + np.arange(nq)[:, None]
+    want, tol, add, add_tol = weights_want(c, 0, q, n, seen, scale, H)
+    check_rows(got, want, tol, (kv, H, HD))
+    check_sums(acc[0], sums[0], n, add, add_tol, nq * H // HKV, (kv, H, HD))
+    assert np.all(sums[0, :, n:] == 7)
+
+
+def test_prompt_weights_long(ctx):
+    H, HKV, HD, nq, pos0 = 8, 2, 128, 300, 1000
+    rng = np.random.default_rng(21)
+    c = Cache(ctx, rng, Q8, 1, HKV, 1300, HD)
+    q = rng.standard_normal((nq, H, HD)).astype(np.float32)
+    acc = np.zeros((1, HKV, 1300), np.float32)
+    out, d_acc = ctx.alloc(q.nbytes), ctx.to_device(acc)
+    ctx.attn_prompt_weights(ctx.to_device(q), nq, H, HKV, HD, *c.args, pos0, 0.09, out, d_acc, d_acc)
+    seen = np.arange(1300)[None] <= pos0 + np.arange(nq)[:, None]
+    want, tol, add, add_tol = weights_want(c, 0, q, 1300, seen, 0.09, H)
+    check_rows(out.download(np.float32, q.shape), want, tol, ("out",))
+    check_sums(acc[0], d_acc.download(np.float32, acc.shape)[0], 1300, add, add_tol, nq * 4, ("sums",))
+
+
+@pytest.mark.parametrize("kv", [Q8, F16])
+def test_prompt_weights_nonfinite_later_keys(ctx, kv):
+    """An infinite value of a later token of the chunk does not reach the queries before it."""
+    H, HKV, HD, nq, pos0 = 8, 2, 128, 20, 50
+    rng = np.random.default_rng(22)
+    c = Cache(ctx, rng, kv, 1, HKV, 70, HD)
+    for n in "kv":
+        (c.raw[n + "s"] if kv == Q8 else c.raw[n])[0, :, 65] = np.nan
+    c.send()
+    q = rng.standard_normal((nq, H, HD)).astype(np.float32)
+    acc = np.zeros((1, HKV, 70), np.float32)
+    out, d_acc = ctx.alloc(q.nbytes), ctx.to_device(acc)
+    ctx.attn_prompt_weights(ctx.to_device(q), nq, H, HKV, HD, *c.args, pos0, 0.09, out, d_acc, d_acc)
+    got = out.download(np.float32, q.shape)
+    seen = np.arange(65)[None] <= pos0 + np.arange(15)[:, None]
+    want, tol, _, _ = weights_want(c, 0, q[:15], 65, seen, 0.09, H)
+    check_rows(got[:15], want, tol, (kv,))
+    assert np.all(np.isnan(got[15:]))
+
+
+# ---- eviction ------------------------------------------------------------------------------------------
+
+def evict_want(acc, n, keep, first, last):
+    if n <= keep:
+        return list(range(n))
+    key = [(0 if i < first or i >= n - last else 1, 1 if np.isnan(acc[i]) else 0, -acc[i] if not np.isnan(acc[i]) else 0, i)
+           for i in range(n)]
+    return sorted(sorted(range(n), key=lambda i: key[i])[:keep])
+
+
+@pytest.mark.parametrize("kv", [Q8, F16])
+@pytest.mark.parametrize("HKV,HD", [(2, 64), (8, 128), (1, 256)])
+@pytest.mark.parametrize("lengths,keep,first,last", [([1], 1, 0, 1), ([0, 300, 100], 100, 0, 0), ([2500, 101], 100, 4, 64),
+                                                     ([1500], 700, 0, 700), ([1030], 1029, 1, 1)])
+def test_evict(ctx, kv, HKV, HD, lengths, keep, first, last):
+    B, slots, slots_out = len(lengths), max(lengths) + 5, keep + 20
+    rng = np.random.default_rng([HD, keep])
+    c = Cache(ctx, rng, kv, B, HKV, slots, HD)
+    to = Cache(ctx, rng, kv, B, HKV, slots_out, HD)
+    before = to.fetch()
+    acc = np.round(rng.standard_normal((B, HKV, slots)) * 20).astype(np.float32)  # many ties, both zeros
+    acc[rng.random(acc.shape) < 0.05] = -0.0
+    acc[rng.random(acc.shape) < 0.02] = np.nan
+    acc[rng.random(acc.shape) < 0.02] = np.inf
+    acc[rng.random(acc.shape) < 0.02] = -np.inf
+    acc_out = ctx.to_device(np.full((B, HKV, slots_out), 5, np.float32))
+    kept, n_out = ctx.to_device(np.full((B, HKV, keep), 77, np.int32)), ctx.to_device(np.full(B, 77, np.int32))
+    d, t = c.dev, to.dev
+    ctx.kv_evict(B, HKV, HD, *c.args, ctx.to_device(np.array(lengths, np.int32)), ctx.to_device(acc), keep, first, last,
+                 slots_out, t["k"], t.get("ks"), t["v"], t.get("vs"), acc_out, kept, n_out)
+    got, sums = to.fetch(), acc_out.download(np.float32, (B, HKV, slots_out))
+    kept = kept.download(np.int32, (B, HKV, keep))
+    assert n_out.download(np.int32).tolist() == [min(n, keep) for n in lengths]
+    for b, n in enumerate(lengths):
+        for h in range(HKV):
+            rows = evict_want(acc[b, h], n, keep, first, last)
+            m = len(rows)
+            assert kept[b, h].tolist() == rows + [-1] * (keep - m), (b, h)
+            assert np.array_equal(sums[b, h], np.concatenate([acc[b, h, rows], np.zeros(slots_out - m, np.float32)]), equal_nan=True)
+            for name in got:
+                assert np.array_equal(got[name][b, h, :m], c.raw[name][b, h, rows]), name
+                assert np.array_equal(got[name][b, h, m:], before[name][b, h, m:]), name
+
+
+# ---- bounds and sparse attention ------------------------------------------------------------------------
+
+def f16_toward(x, up):
+    h = x.astype(np.float16)
+    wrong = h.astype(np.float64) < x if up else h.astype(np.float64) > x
+    return np.where(wrong, np.nextafter(h, np.float16(np.inf if up else -np.inf)), h)
+
+
+def bounds_want(k, n, block):
+    """k [slots][HD] float64: [blocks][2][HD] f16 over the first n rows (blocks past them NaN)."""
+    nb = -(-k.shape[0] // block)
+    out = np.full((nb, 2, k.shape[1]), np.nan, np.float16)
+    for i in range(-(-n // block)):
+        rows = k[i * block:min(n, (i + 1) * block)]
+        with np.errstate(over="ignore"):
+            out[i, 0] = f16_toward(np.fmin.reduce(rows, initial=np.inf), False)
+            out[i, 1] = f16_toward(np.fmax.reduce(rows, initial=-np.inf), True)
+    return out
+
+
+@pytest.mark.parametrize("kv", [Q8, F16])
+@pytest.mark.parametrize("HKV,HD", [(2, 64), (8, 128), (1, 256)])
+@pytest.mark.parametrize("block", [16, 32, 64, 128])
+def test_bounds(ctx, kv, HKV, HD, block):
+    """Whole caches, then some keys overwritten and only their blocks recomputed."""
+    rng = np.random.default_rng([HD, block])
+    lengths = [700, 1, 0, 257, 128]
+    B, slots = 5, 701
+    c = Cache(ctx, rng, kv, B, HKV, slots, HD, std=3e3 if kv == Q8 else 1.0)
+    raw = c.raw["ks"] if kv == Q8 else c.raw["k"]
+    raw[0, :, 70] = np.nan
+    raw[3, :, 3] = 0
+    c.send()
+    nb = -(-slots // block)
+    assert ctx.kv_bounds_bytes(B, HKV, HD, slots, block) == B * HKV * nb * 2 * HD * 2
+    mark = np.full((B, HKV, nb, 2, HD), 0x7777, np.uint16)
+    d = ctx.to_device(mark)
+    n_dev = ctx.to_device(np.array(lengths, np.int32))
+    ctx.kv_block_bounds(B, HKV, HD, kv, c.dev["k"], c.dev.get("ks"), slots, n_dev, slots, block, d)
+    got = d.download(np.uint16, mark.shape)
+    k = c.values("k")
+
+    def check(got, k):
+        for b, n in enumerate(lengths):
+            used = -(-n // block)
+            for h in range(HKV):
+                want = bounds_want(k[b, h], n, block)
+                # (NaN: one -0 or the other may come of equal zeros)
+                assert np.array_equal(got[b, h, :used].view(np.float16), want[:used]), (b, h)
+            assert np.all(got[b, :, used:] == 0x7777)
+
+    check(got, k)
+    c2 = Cache(ctx, rng, kv, B, HKV, slots, HD)
+    for n in c.raw:
+        for b, m in enumerate(lengths):
+            c.raw[n][b, :, max(m - 10, 0):m] = c2.raw[n][b, :, max(m - 10, 0):m]
+    c.send()
+    ctx.kv_block_bounds(B, HKV, HD, kv, c.dev["k"], c.dev.get("ks"), slots, n_dev, 10, block, d)
+    check(d.download(np.uint16, mark.shape), c.values("k"))
+
+
+def pick_want(q, bounds, nb, n_pick):
+    """q [G][HD], bounds [blocks][2][HD]: the blocks read, ascending."""
+    lo, hi = (bounds[:nb, i].astype(np.float64) for i in (0, 1))
+    q = q.astype(np.float64)
+    s = np.stack([np.where(x >= 0, x * hi, x * lo).sum(-1) for x in q]).max(0)
+    order = sorted(range(nb), key=lambda i: (i != nb - 1, i != 0, -s[i], i))
+    return sorted(order[:n_pick])
+
+
+def check_sparse(ctx, c, q, H, lengths, per, block, n_pick, scale, what):
+    """Query b of B; its cache b (per) or 0."""
+    B, HKV, HD, slots = q.shape[0], c.HKV, c.HD, c.slots
+    k, v, G = c.values("k"), c.values("v"), H // c.HKV
+    bounds = np.stack([[bounds_want(k[i, h], slots, block) for h in range(HKV)] for i in range(c.B)])
+    n_dev = ctx.to_device(np.array(lengths if per else lengths[:1], np.int32))
+    out, picked = ctx.to_device(np.full_like(q, 9)), ctx.to_device(np.full((B, HKV, n_pick), 77, np.int32))
+    args = (ctx.to_device(q), B, H, HKV, HD, *c.args, n_dev, per, ctx.to_device(bounds), block, n_pick, scale)
+    ctx.attn_sparse(*args, out, picked)
+    got, ids = out.download(np.float32, q.shape), picked.download(np.int32, (B, HKV, n_pick))
+    for b in range(B):
+        n = lengths[b] if per else min(lengths[0] + b + 1, slots)
+        nb, cb = -(-n // block), b if per else 0
+        for h in range(HKV):
+            blocks = pick_want(q[b, h * G:(h + 1) * G], bounds[cb, h], nb, n_pick)
+            assert ids[b, h].tolist() == blocks + [-1] * (n_pick - len(blocks)), (*what, b, h)
+            rows = np.array([r for i in blocks for r in range(i * block, min(n, (i + 1) * block))], int)
+            for j in range(G):
+                want, _, tol, _ = attend(q[b, h * G + j][None].astype(np.float64), k[cb, h, rows], v[cb, h, rows],
+                                         np.ones((1, len(rows)), bool), scale)
+                check_rows(got[b, h * G + j][None], want, tol, (*what, b, h, j))
+    again = ctx.alloc(q.nbytes)
+    ctx.attn_sparse(*args, again)  # without the blocks
+    assert np.array_equal(again.download(np.float32, q.shape), got)
+
+
+@pytest.mark.parametrize("kv", [Q8, F16])
+@pytest.mark.parametrize("H,HKV,HD", HEADS)
+@pytest.mark.parametrize("lengths,block,n_pick", [([1], 16, 1), ([0, 999, 64, 65], 64, 3), ([2000, 1985], 16, 40),
+                                                  ([700], 128, 9)])
+def test_sparse(ctx, kv, H, HKV, HD, lengths, block, n_pick):
+    rng = np.random.default_rng([H, HD, block, kv])
+    B = len(lengths)
+    c = Cache(ctx, rng, kv, B, HKV, max(lengths) + 7, HD)
+    q = rng.standard_normal((B, H, HD)).astype(np.float32)
+    check_sparse(ctx, c, q, H, lengths, 1, block, n_pick, 1 / np.sqrt(HD), (kv, H, HD))
+
+
+@pytest.mark.parametrize("kv", [Q8, F16])
+def test_sparse_batch_on_one_cache(ctx, kv):
+    """Consecutive queries of one cache, the last of them past its end."""
+    rng = np.random.default_rng(31)
+    c = Cache(ctx, rng, kv, 1, 2, 600, 128)
+    q = rng.standard_normal((7, 8, 128)).astype(np.float32)
+    check_sparse(ctx, c, q, 8, [595], 0, 32, 5, 0.09, (kv,))
+
+
+def test_sparse_equal_scores_and_many_blocks(ctx):
+    """Blocks of equal bounds go by their index; more blocks than one pass of the pick holds."""
+    rng = np.random.default_rng(32)
+    c = Cache(ctx, rng, F16, 1, 1, 16 * 1500, 64)
+    for n in "kv":
+        c.raw[n][0, 0] = np.tile(c.raw[n][0, 0, :16 * 5], (300, 1))
+    c.send()
+    q = rng.standard_normal((1, 4, 64)).astype(np.float32)
+    for n_pick in (1, 2, 3, 299, 303, 1499):
+        check_sparse(ctx, c, q, 4, [16 * 1500], 1, 16, n_pick, 0.1, (n_pick,))
+
+
+# ---- together ------------------------------------------------------------------------------------------
+
+def test_tree_step_then_decode(ctx):
+    """Append a tree at its depths, attend, keep a path, and decode: as if only the path had been appended."""
+    H, HKV, HD, T, past, n_pos = 8, 2, 128, 7, 90, 256
+    rng = np.random.default_rng(41)
+    cs = ctx.rope_table(HD, n_pos, 500000.0)
+    parent = [-1, 0, 0, 1, 2, 4, -1]
+    depth = [0] * T
+    mask = np.zeros((1, T), np.uint64)
+    for t, p in enumerate(parent):
+        depth[t] = depth[p] + 1 if p >= 0 else 0
+        mask[0, t] = (int(mask[0, p]) if p >= 0 else 0) | 1 << t
+    qkv = rng.standard_normal((T, (H + 2 * HKV) * HD)).astype(np.float32)
+    c = Cache(ctx, rng, Q8, 1, HKV, 128, HD)
+    straight = Cache(ctx, rng, Q8, 1, HKV, 128, HD)
+    straight.raw = {n: a.copy() for n, a in c.raw.items()}
+    straight.send()
+    n_past, q = ctx.to_device(np.array([past], np.int32)), ctx.alloc(T * H * HD * 4)
+    out = ctx.alloc(T * H * HD * 4)
+    pos = np.array([past + d for d in depth], np.int32)
+    ctx.rope_kv_append_at(ctx.to_device(qkv), T, ctx.to_device(pos), n_past, H, HKV, HD, HD, 0, cs, n_pos, 128, Q8, q,
+                          *c.args[1:5])
+    ctx.attn_tree(q, 1, T, H, HKV, HD, *c.args, n_past, ctx.to_device(mask), 0.09, out)
+    c.raw = c.fetch()
+    check_tree(c, q.download(np.float32, (1, T, H, HD)), T, [past], mask, 0.09, H, out.download(np.float32, (1, T, H, HD)), ("step",))
+    path = [0, 2, 4, 5]
+    ctx.kv_path(1, HKV, HD, *c.args, ctx.to_device(np.array([[past + t for t in path]], np.int32)), 4, n_past)
+    ctx.rope_kv_append(ctx.to_device(qkv[path]), 4, n_past, H, HKV, HD, HD, 0, cs, 128, q, *straight.args[1:5])
+    a, b = c.fetch(), straight.fetch()
+    assert all(np.array_equal(a[n][:, :, :past + 4], b[n][:, :, :past + 4]) for n in a)
+
+
+def test_evicted_conversation(ctx):
+    """A prompt's weights, a decode step's, eviction, a new key at its own position, bounds, sparse attention."""
+    H, HKV, HD, n, keep, n_pos, block = 8, 2, 128, 500, 200, 1024, 16
+    rng = np.random.default_rng(42)
+    c, to = Cache(ctx, rng, Q8, 1, HKV, 512, HD), Cache(ctx, rng, Q8, 1, HKV, 256, HD)
+    acc = ctx.to_device(np.zeros((1, HKV, 512), np.float32))
+    nq = 40
+    q = rng.standard_normal((nq + 1, H, HD)).astype(np.float32)
+    out = ctx.alloc(q.nbytes)
+    ctx.attn_prompt_weights(ctx.to_device(q[:nq]), nq, H, HKV, HD, *c.args, n - 1 - nq, 0.09, out, acc, acc)
+    ctx.attn_decode_weights(ctx.to_device(q[nq]), 1, H, HKV, HD, *c.args, ctx.to_device(np.array([n], np.int32)), 0.09, out,
+                            acc, acc)
+    sums = acc.download(np.float32, (HKV, 512))
+    assert np.allclose(sums.sum(1), (nq + 1) * H // HKV, rtol=1e-5)
+    acc_out, kept = ctx.alloc(HKV * 256 * 4), ctx.alloc(HKV * keep * 4)
+    n_out = ctx.alloc(4)
+    ctx.kv_evict(1, HKV, HD, *c.args, ctx.to_device(np.array([n], np.int32)), acc, keep, 4, 32, 256, *to.args[1:5], acc_out,
+                 kept, n_out)
+    kept = kept.download(np.int32, (HKV, keep))
+    assert all(kept[h].tolist() == evict_want(sums[h], n, keep, 4, 32) for h in range(HKV))
+    cs = ctx.rope_table(HD, n_pos, 500000.0)
+    qkv = rng.standard_normal((1, (H + 2 * HKV) * HD)).astype(np.float32)
+    dq = ctx.alloc(H * HD * 4)
+    ctx.rope_kv_append_at(ctx.to_device(qkv), 1, ctx.to_device(np.array([n], np.int32)), n_out, H, HKV, HD, HD, 0, cs, n_pos,
+                          256, Q8, dq, *to.args[1:5])
+    raw = to.fetch()
+    for h in range(HKV):
+        assert all(np.array_equal(raw[m][0, h, :keep], c.raw[m][0, h, kept[h]]) for m in raw)
+    to.raw = raw
+    check_sparse(ctx, to, dq.download(np.float32, (1, H, HD)), H, [keep + 1], 1, block, 6, 0.09, ("after",))
+
+
+def test_contexts_side_by_side(ctx):
+    """Two contexts' calls in flight at once, of other sizes in turn: each gives what it gives alone."""
+    other = ts5hip.Context(0)
+    rng = np.random.default_rng(51)
+    jobs = []
+    for i, (x, past) in enumerate([(ctx, 300), (other, 1200), (ctx, 900), (other, 64)]):
+        c = Cache(x, rng, Q8, 1, 8, 1400, 128)
+        q = x.to_device(rng.standard_normal((1, 9, 32, 128)).astype(np.float32))
+        mask, n = x.to_device(random_masks(rng, 1, 9)), x.to_device(np.array([past], np.int32))
+        jobs.append((x, c, q, mask, n, x.alloc(9 * 32 * 128 * 4)))
+
+    def go(x, c, q, mask, n, out):
+        x.attn_tree(q, 1, 9, 32, 8, 128, *c.args, n, mask, 0.09, out)
+
+    alone = []
+    for j in jobs:
+        go(*j)
+        alone.append(j[5].download(np.float32))
+    for j in jobs:
+        j[5].zero()
+    ctx.sync(), other.sync()
+    for j in jobs:
+        go(*j)
+    for j, want in zip(jobs, alone):
+        assert np.array_equal(j[5].download(np.float32), want)
+    other.close()

@@ -34,16 +34,20 @@ namespace ts5hip {
 __device__ inline float block_sum64(float v) { return wave_sum(v); }
 
 // grid (H + 2*HKV, ntok), 64 threads (one wave): thread i holds values 2i, 2i+1
-// (and 2i + 128, 2i + 129 at head dimension 256).
+// (and 2i + 128, 2i + 129 at head dimension 256). With AT, token t's RoPE position is at[t] (below
+// n_pos, else the token is left out, as one past the cache is), not its slot.
+template <bool AT>
 __global__ __launch_bounds__(64) void k_rope_kv(const float *__restrict__ qkv, int64_t qkv_stride,
                                                 const float *__restrict__ bias, const float *__restrict__ q_norm,
                                                 const float *__restrict__ k_norm, float eps,
                                                 const float2 *__restrict__ rope_cs, int n_rot, int neox,
                                                 const int32_t *__restrict__ pos0p, int H, int HKV, int HD,
-                                                int n_ctx, float *__restrict__ q_out, KvLayer kv, int kv_f16) {
+                                                int n_ctx, float *__restrict__ q_out, KvLayer kv, int kv_f16,
+                                                const int32_t *__restrict__ at, int n_pos) {
     __shared__ float v[256];
     const int hh = blockIdx.x, t = blockIdx.y, i = threadIdx.x;
-    const int pos = pos0p[0] + t;
+    const int pos = pos0p[0] + t, turn = AT ? at[t] : pos;
+    if (AT && (turn < 0 || turn >= n_pos || pos < 0 || pos >= n_ctx)) return;
     const float *src = qkv + (int64_t)t * qkv_stride + (int64_t)hh * HD;
     const bool is_q = hh < H, is_k = !is_q && hh < H + HKV;
     for (int j = i; j < HD; j += 64) v[j] = src[j] + (bias ? bias[(int64_t)hh * HD + j] : 0.f);
@@ -61,7 +65,7 @@ __global__ __launch_bounds__(64) void k_rope_kv(const float *__restrict__ qkv, i
     if (is_q || is_k) {
         for (int r = i; r < n_rot / 2; r += 64) {
             const int a = neox ? r : 2 * r, b = neox ? r + n_rot / 2 : 2 * r + 1;
-            const float2 cs = rope_cs[(int64_t)pos * (n_rot / 2) + r];
+            const float2 cs = rope_cs[(int64_t)turn * (n_rot / 2) + r];
             float x0 = v[a], x1 = v[b];
             rope_pair(x0, x1, cs.x, cs.y);
             v[a] = x0;
@@ -256,8 +260,17 @@ hipError_t launch_rope_kv(const float *qkv, int64_t qkv_stride, const float *bia
                           const float *k_norm, float eps, const float *rope_cs, int n_rot, int neox,
                           const int32_t *pos0, int H, int HKV, int HD, int n_ctx, int ntok, float *q_out, KvLayer kv,
                           int kv_f16, hipStream_t s) {
-    hipLaunchKernelGGL(k_rope_kv, dim3(H + 2 * HKV, ntok), dim3(64), 0, s, qkv, qkv_stride, bias, q_norm, k_norm,
-                       eps, (const float2 *)rope_cs, n_rot, neox, pos0, H, HKV, HD, n_ctx, q_out, kv, kv_f16);
+    hipLaunchKernelGGL(k_rope_kv<false>, dim3(H + 2 * HKV, ntok), dim3(64), 0, s, qkv, qkv_stride, bias, q_norm, k_norm,
+                       eps, (const float2 *)rope_cs, n_rot, neox, pos0, H, HKV, HD, n_ctx, q_out, kv, kv_f16, nullptr, 0);
+    return hipGetLastError();
+}
+
+hipError_t launch_rope_kv_at(const float *qkv, int64_t qkv_stride, const float *bias, const float *q_norm,
+                             const float *k_norm, float eps, const float *rope_cs, int n_pos, int n_rot, int neox,
+                             const int32_t *at, const int32_t *slot0, int H, int HKV, int HD, int n_ctx, int ntok,
+                             float *q_out, KvLayer kv, int kv_f16, hipStream_t s) {
+    hipLaunchKernelGGL(k_rope_kv<true>, dim3(H + 2 * HKV, ntok), dim3(64), 0, s, qkv, qkv_stride, bias, q_norm, k_norm,
+                       eps, (const float2 *)rope_cs, n_rot, neox, slot0, H, HKV, HD, n_ctx, q_out, kv, kv_f16, at, n_pos);
     return hipGetLastError();
 }
 

@@ -1,0 +1,422 @@
+// Attention of several rows of queries over a KV cache, on the core of
+// attn_rows.h: a tree of drafted tokens, a prompt chunk whose key weights are
+// summed, and one query a cache whose scores are kept for that sum.
+#include <algorithm>
+
+#include "attn_rows.h"
+
+namespace ts5hip {
+
+struct RowsArgs {
+    const float *q;  // [B][T][H * HD]
+    KvLayer kv;      // B caches
+    int n_ctx, H, HKV, T, n_split;
+    const int32_t *n_keys;  // per cache: the keys before the T tokens (tree), or all keys (one query)
+    const uint64_t *mask;   // [B][T], tree
+    int pos0;               // position of the first token (causal)
+    int mode;
+    float scale;
+    float *part;    // [B][HKV][T * G][n_split][HD + 4]: m, l, -, -, O
+    float *out;     // [B][T][H * HD]
+    float *lse;     // [B][HKV][T * G] log2 of the sum of 2^score, or null
+    float *scores;  // [B][HKV][G][stride] log2-domain scores (one query)
+    int64_t stride;
+    uint4 *planes;  // [HKV][row tile][HD / 32][2][64] the rows' fp16 planes, and then
+    float *p2e;     // [HKV][row tile][16] their 2^e, or null (causal)
+};
+enum { ROWS_TREE = 0, ROWS_CAUSAL = 1, ROWS_ONE = 2 };
+
+// The keys before the tokens (tree) or of the sequence, inside the cache whatever the caller's
+// device memory holds.
+__device__ inline int rows_count(const RowsArgs &a, int b) {
+    if (a.mode == ROWS_CAUSAL) return a.pos0;
+    return max(0, min(a.n_keys[b], a.mode == ROWS_TREE ? a.n_ctx - a.T : a.n_ctx));
+}
+// Keys that slices divide, and the keys of token t's row.
+__device__ inline int rows_all(const RowsArgs &a, int n) { return a.mode == ROWS_ONE ? n : n + a.T; }
+__device__ inline int rows_reach(const RowsArgs &a, int n, int t) { return a.mode == ROWS_CAUSAL ? n + t + 1 : rows_all(a, n); }
+
+// grid (n_split, HKV * row blocks of 16 NT, B): one slice of the keys for 16 NT rows,
+// row r = G t + j being head j of token t. The waves take the slice's units in turn.
+template <int HD, bool F16, int KT, int NT, int NW, bool ONE>
+__global__ __launch_bounds__(64 * NW) void k_attn_rows(RowsArgs a) {
+    using S = RowsShape<HD, F16, KT>;
+    __shared__ RowsLds<HD, NW> L;
+    __shared__ int nonfinite;  // a masked unit left out infinite or NaN values
+    if (!ONE && threadIdx.x == 0) nonfinite = 0;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int rl = lane & 15, kq = lane >> 4;
+    const int G = a.H / a.HKV, R = a.T * G, nrb = (R + 16 * NT - 1) / (16 * NT);
+    const int split = blockIdx.x, kvh = blockIdx.y / nrb, r0 = blockIdx.y % nrb * 16 * NT, b = blockIdx.z;
+    const int rows = min(R - r0, 16 * NT);
+    const int n = rows_count(a, b), chunk = rows_chunk(rows_all(a, n), a.n_split);
+    const int kbeg = split * chunk, kend = min(kbeg + chunk, rows_reach(a, n, (r0 + rows - 1) / G));
+    if (kbeg >= kend) return;  // the merge reads no partial of this slice
+    const int full = a.mode == ROWS_CAUSAL ? n + r0 / G + 1 : n;  // keys before it are every row's
+    const RowsKv kv = rows_kv<HD, F16>(a.kv, ((int64_t)b * a.HKV + kvh) * a.n_ctx, kend);
+    const int units = (kend - kbeg + S::UNIT - 1) / S::UNIT;
+    RowsUnit<HD, F16, KT> nxt;
+    auto at = [&](int u, int (&kb)[KT]) {
+#pragma unroll
+        for (int t = 0; t < KT; t++) kb[t] = kbeg + u * S::UNIT + 16 * t;
+    };
+    int kb[KT];
+    at(wave, kb);
+    rows_load<HD, F16, KT>(nxt, kv, kb, rl, kq);
+
+    RowsQ<HD, NT> q;
+    rows_query<HD, NT>(q, a.scale, kq, [&](int qt) -> const float * {
+        const int r = r0 + 16 * qt + rl;
+        return r < R ? a.q + (((int64_t)b * a.T + r / G) * a.H + kvh * G + r % G) * HD : nullptr;
+    });
+    int seen[NT];       // keys before it are the row's
+    uint64_t bits[NT];  // and then those of n + its set bits
+#pragma unroll
+    for (int qt = 0; qt < NT; qt++) {
+        const int r = r0 + 16 * qt + rl;
+        seen[qt] = r >= R ? 0 : a.mode == ROWS_CAUSAL ? n + r / G + 1 : n;
+        bits[qt] = 0;
+        if (!ONE && a.mode == ROWS_TREE && r < R) bits[qt] = a.mask[(int64_t)b * a.T + r / G] & (~0ull >> (64 - a.T));
+    }
+    if (!ONE && a.planes && split == 0 && wave == 0) {
+        const int tiles = (R + 15) / 16;
+#pragma unroll
+        for (int qt = 0; qt < NT; qt++) {
+            const int tile = r0 / 16 + qt;
+            if (tile >= tiles) break;
+            uint4 *p = a.planes + ((int64_t)kvh * tiles + tile) * (HD / 32) * 2 * 64 + lane;
+#pragma unroll
+            for (int c = 0; c < HD / 32; c++) {
+                p[(2 * c) * 64] = __builtin_bit_cast(uint4, q.h[qt][c]);
+                p[(2 * c + 1) * 64] = __builtin_bit_cast(uint4, q.l[qt][c]);
+            }
+            if (kq == 0) a.p2e[((int64_t)kvh * tiles + tile) * 16 + rl] = q.p2e[qt];
+        }
+    }
+    RowsSum<HD, NT> sum;
+    rows_clear<HD, NT>(sum);
+    if (!ONE) __syncthreads();  // the flag is set
+    const int64_t row0 = ((int64_t)b * a.HKV + kvh) * R + r0;
+    for (int u = wave; u < units; u += NW) {
+        const RowsUnit<HD, F16, KT> cur = nxt;
+        int kn[KT];
+        at(u, kb);
+        at(u + NW, kn);
+        rows_load<HD, F16, KT>(nxt, kv, kn, rl, kq);  // (past the slice: zeros, no memory access)
+        if constexpr (ONE) {
+            auto put = [&](int, int key, const float (&s)[4]) {
+                if (rl < rows && key < kend)
+                    *(float4 *)(a.scores + (row0 + rl) * a.stride + key) =
+                        make_float4(s[0] * q.p2e[0], s[1] * q.p2e[0], s[2] * q.p2e[0], s[3] * q.p2e[0]);
+            };
+            if (kb[0] + S::UNIT <= kend)
+                rows_unit<HD, F16, KT, NT, false, false>(cur, q, sum, kb, kq, [](int, int) { return 15u; }, put);
+            else
+                rows_unit<HD, F16, KT, NT, true, false>(cur, q, sum, kb, kq, [&](int, int key) { return rows_below(key, kend); }, put);
+        } else {
+            auto put = [](int, int, const float (&)[4]) {};
+            if (kb[0] + S::UNIT <= full)
+                rows_unit<HD, F16, KT, NT, false, false>(cur, q, sum, kb, kq, [](int, int) { return 15u; }, put);
+            else if (rows_unit<HD, F16, KT, NT, true, true>(
+                         cur, q, sum, kb, kq,
+                         [&](int qt, int key) { return rows_below(key, seen[qt]) | rows_window(bits[qt], key - n); },
+                         put))
+                nonfinite = 1;
+        }
+    }
+    rows_combine<HD, NT, NW>(L, sum, rows, wave, rl, kq, [&](int r, int d, float4 o, float m, float l) {
+        const int t = (r0 + r) / G, j = (r0 + r) % G;
+        if (!ONE && nonfinite) {  // those of the keys that the row takes, of the units that are not every row's
+            const uint64_t own = a.mode == ROWS_TREE ? a.mask[(int64_t)b * a.T + t] & (~0ull >> (64 - a.T)) : 0;
+            const int reach = a.mode == ROWS_CAUSAL ? n + t + 1 : n;
+            const int first = kbeg + max(full - kbeg, 0) / S::UNIT * S::UNIT;
+            for (int key = first; key < kend; key++) {
+                if (key >= reach && !(key >= n && key - n < 64 && (own >> (key - n) & 1))) continue;
+                const int64_t slot = ((int64_t)b * a.HKV + kvh) * a.n_ctx + key;
+                o.x += rows_nonfinite<HD, F16>(a.kv, slot, d), o.y += rows_nonfinite<HD, F16>(a.kv, slot, d + 1);
+                o.z += rows_nonfinite<HD, F16>(a.kv, slot, d + 2), o.w += rows_nonfinite<HD, F16>(a.kv, slot, d + 3);
+            }
+        }
+        if (!ONE && a.n_split == 1) {
+            const float inv = 1.0f / l;
+            *(float4 *)(a.out + (((int64_t)b * a.T + t) * a.H + kvh * G + j) * HD + d) =
+                l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+            if (a.lse && d == 0) a.lse[row0 + r] = l == 0.f ? INFINITY : m + __log2f(l);
+            return;
+        }
+        float *p = a.part + ((row0 + r) * a.n_split + split) * (HD + 4);
+        if (d == 0) *(float4 *)p = make_float4(m, l, 0.f, 0.f);
+        *(float4 *)(p + 4 + d) = o;
+    });
+}
+
+// A thread per 4 outputs.
+template <int HD>
+__global__ __launch_bounds__(256) void k_rows_merge(RowsArgs a, int64_t rows) {
+    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x, row = e / (HD / 4);
+    if (row >= rows) return;
+    const int d = 4 * (int)(e % (HD / 4)), G = a.H / a.HKV, R = a.T * G;
+    const int b = (int)(row / ((int64_t)a.HKV * R)), kvh = (int)(row / R % a.HKV), r = (int)(row % R), t = r / G;
+    const int n = rows_count(a, b), chunk = rows_chunk(rows_all(a, n), a.n_split);
+    const int used = (rows_reach(a, n, t) + chunk - 1) / chunk;
+    float M, l;
+    const float4 o = rows_merge(a.part + row * a.n_split * (HD + 4), used, HD + 4, d, M, l);
+    const float inv = 1.0f / l;
+    *(float4 *)(a.out + (((int64_t)b * a.T + t) * a.H + kvh * G + r % G) * HD + d) =
+        l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    if (a.lse && d == 0) a.lse[row] = l == 0.f ? INFINITY : M + __log2f(l);
+}
+
+// One query a cache: the merge (the workgroups of the first keys) and acc_out = acc +
+// the group's weights 2^(score - lse). grid (key blocks of 1024, HKV, B).
+template <int HD>
+__global__ __launch_bounds__(256) void k_one_weights(RowsArgs a, const float *acc, float *acc_out) {
+    __shared__ float lse[ROWS_MAX_G];
+    const int kvh = blockIdx.y, b = blockIdx.z, G = a.H / a.HKV, tid = threadIdx.x;
+    const int n = rows_count(a, b), chunk = rows_chunk(n, a.n_split), used = (n + chunk - 1) / chunk;
+    const int64_t head = (int64_t)b * a.HKV + kvh, row0 = head * G;
+    const int k0 = blockIdx.x * 1024 + 4 * tid;
+    if (blockIdx.x == 0) {
+        for (int e = tid; e < G * (HD / 4); e += 256) {
+            const int g = e / (HD / 4), d = 4 * (e % (HD / 4));
+            float M, l;
+            const float4 o = rows_merge(a.part + (row0 + g) * a.n_split * (HD + 4), used, HD + 4, d, M, l);
+            const float inv = 1.0f / l;
+            *(float4 *)(a.out + (((int64_t)b * a.H) + kvh * G + g) * HD + d) =
+                l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+        }
+    }
+    if (blockIdx.x * 1024 >= n) return;
+    if (tid < G) {
+        const float *p = a.part + (row0 + tid) * a.n_split * (HD + 4);
+        float M = -INFINITY, l = 0.f;
+        for (int s = 0; s < used; s++) M = fmaxf(M, p[(int64_t)s * (HD + 4)]);
+        for (int s = 0; s < used; s++) {
+            const float2 ml = *(const float2 *)(p + (int64_t)s * (HD + 4));
+            if (ml.x != -INFINITY) l = fmaf(__builtin_amdgcn_exp2f(ml.x - M), ml.y, l);
+        }
+        lse[tid] = M + __log2f(l);
+    }
+    __syncthreads();
+    float w[4] = {0.f, 0.f, 0.f, 0.f};
+    if (k0 >= n) return;
+    for (int g = 0; g < G; g++) {
+        const float4 s = *(const float4 *)(a.scores + (row0 + g) * a.stride + k0);
+        w[0] += __builtin_amdgcn_exp2f(s.x - lse[g]), w[1] += __builtin_amdgcn_exp2f(s.y - lse[g]);
+        w[2] += __builtin_amdgcn_exp2f(s.z - lse[g]), w[3] += __builtin_amdgcn_exp2f(s.w - lse[g]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (k0 + i < n) acc_out[head * a.n_ctx + k0 + i] = acc[head * a.n_ctx + k0 + i] + w[i];
+}
+
+// A prompt chunk's weights summed over its queries, for each key: a wave holds a unit's
+// K and goes over every row tile's planes, sums 2^(score - lse) in its lanes, and
+// adds the lanes at the end. grid (key blocks of 4 units, HKV).
+template <int HD, bool F16, int KT>
+__global__ __launch_bounds__(256) void k_prompt_weights(RowsArgs a, const float *acc, float *acc_out) {
+    using S = RowsShape<HD, F16, KT>;
+    constexpr int NC = S::NC;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int rl = lane & 15, kq = lane >> 4, kvh = blockIdx.y;
+    const int G = a.H / a.HKV, R = a.T * G, tiles = (R + 15) / 16, n = a.pos0 + a.T;
+    const int k0 = (blockIdx.x * 4 + wave) * S::UNIT;
+    if (k0 >= n) return;
+    const RowsKv kv = rows_kv<HD, F16>(a.kv, (int64_t)kvh * a.n_ctx, n);
+    RowsUnit<HD, F16, KT> u;
+    ar_h8 ka[KT][NC];
+    float ks[KT][NC][4], w[KT][4];
+#pragma unroll
+    for (int t = 0; t < KT; t++) {
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+            rows_words<S::KW>(kv.k, ((uint32_t)(k0 + 16 * t + rl) * HD + 32 * c + 8 * kq) * S::VB, u.k[t][c]);
+        if constexpr (!F16) rows_words<2 * NC>(kv.ks, (uint32_t)(k0 + 16 * t + 4 * kq) * NC * 2, u.ks[t]);
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            ka[t][c] = rows_values<S::KW>(u.k[t][c]);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                ks[t][c][i] = F16 ? 1.f : h2f((u.ks[t][F16 ? 0 : (i * NC + c) / 2] >> (16 * (c & 1))) & 0xffff);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) w[t][i] = 0.f;
+    }
+    // The first row that sees key k0: token max(0, k0 - pos0).
+    const int first = max(0, k0 - a.pos0) * G / 16;
+    const uint4 *pl = a.planes + (int64_t)kvh * tiles * NC * 2 * 64 + lane;
+    for (int tile = first; tile < tiles; tile++) {
+        ar_h8 qh[NC], ql[NC];
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            qh[c] = __builtin_bit_cast(ar_h8, pl[((int64_t)tile * NC * 2 + 2 * c) * 64]);
+            ql[c] = __builtin_bit_cast(ar_h8, pl[((int64_t)tile * NC * 2 + 2 * c + 1) * 64]);
+        }
+        const int r = 16 * tile + rl;
+        const float p2e = a.p2e[((int64_t)kvh * tiles + tile) * 16 + rl];
+        const float lse = r < R ? a.lse[(int64_t)kvh * R + r] : INFINITY;
+        const int last = a.pos0 + r / G;  // the last key the row sees
+#pragma unroll
+        for (int t = 0; t < KT; t++) {
+            float s[4];
+            if constexpr (F16) {
+                ar_f4 D = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < NC; c++) {
+                    D = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[t][c], qh[c], D, 0, 0, 0);
+                    D = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[t][c], ql[c], D, 0, 0, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) s[i] = D[i];
+            } else {
+#pragma unroll
+                for (int c = 0; c < NC; c++) {
+                    ar_f4 D = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[t][c], qh[c], ar_f4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                    D = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[t][c], ql[c], D, 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) s[i] = c == 0 ? ks[t][c][i] * D[i] : fmaf(ks[t][c][i], D[i], s[i]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(s[i], p2e, -lse));
+                w[t][i] += k0 + 16 * t + 4 * kq + i <= last && r < R ? p : 0.f;
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < KT; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float x = row_sum_dpp(w[t][i]);
+            const int64_t key = k0 + 16 * t + 4 * kq + i;
+            if (rl == 0 && key < n) acc_out[(int64_t)kvh * a.n_ctx + key] = acc[(int64_t)kvh * a.n_ctx + key] + x;
+        }
+}
+
+// ---- host ----------------------------------------------------------------------------------------
+
+// Row tiles of a workgroup: they share each key's loads and conversion, as many as the
+// registers hold (the rows' planes and outputs take HD / 2 of them a tile).
+static int rows_tiles(int R, int HD) { return HD == 256 || R <= 16 ? 1 : HD == 128 || R <= 32 ? 2 : 4; }
+static int rows_blocks(int R, int HD) { return (R + 16 * rows_tiles(R, HD) - 1) / (16 * rows_tiles(R, HD)); }
+// Tiles of keys a unit.
+constexpr int rows_kt(int HD, int NT) { return HD == 256 || (HD == 128 && NT == 1) ? 1 : 2; }
+static int rows_splits(int items, int keys, int slots) {
+    const int most = std::min((keys + ROWS_MIN_KEYS - 1) / ROWS_MIN_KEYS, ROWS_MAX_SPLIT);
+    return std::max(1, std::min(slots / std::max(items, 1), most));
+}
+
+bool attn_rows_supported(int H, int HKV, int HD) {
+    return HKV > 0 && H > 0 && H % HKV == 0 && (HD == 64 || HD == 128 || HD == 256) && H / HKV <= ROWS_MAX_G;
+}
+
+template <int HD, bool F16>
+static hipError_t rows_launch(const RowsArgs &a, int B, bool one, hipStream_t s) {
+    const int R = a.T * (a.H / a.HKV);
+    const dim3 grid(a.n_split, a.HKV * rows_blocks(R, HD), B);
+    constexpr int NW = HD == 256 ? 4 : 8, K1 = rows_kt(HD, 1), K2 = rows_kt(HD, 2);
+    const int tiles = rows_tiles(R, HD);
+    if (one) {
+        hipLaunchKernelGGL((k_attn_rows<HD, F16, K1, 1, NW, true>), grid, dim3(64 * NW), 0, s, a);
+    } else if (tiles == 1) {
+        hipLaunchKernelGGL((k_attn_rows<HD, F16, K1, 1, NW, false>), grid, dim3(64 * NW), 0, s, a);
+    } else if constexpr (HD <= 128) {
+        if (tiles == 2) {
+            hipLaunchKernelGGL((k_attn_rows<HD, F16, K2, 2, 4, false>), grid, dim3(256), 0, s, a);
+        } else if constexpr (HD == 64) {
+            hipLaunchKernelGGL((k_attn_rows<HD, F16, K2, 4, 4, false>), grid, dim3(256), 0, s, a);
+        }
+    }
+    return hipGetLastError();
+}
+template <int HD>
+static hipError_t rows_launch_merge(const RowsArgs &a, int B, hipStream_t s) {
+    const int64_t rows = (int64_t)B * a.H * a.T;
+    hipLaunchKernelGGL(k_rows_merge<HD>, dim3((unsigned)((rows * (HD / 4) + 255) / 256)), dim3(256), 0, s, a, rows);
+    return hipGetLastError();
+}
+static int tree_splits(int B, int T, int H, int HKV, int HD, int n_ctx, int n_cu) {
+    return rows_splits(B * HKV * rows_blocks(T * (H / HKV), HD), n_ctx, n_cu);
+}
+size_t attn_tree_scratch_bytes(int B, int T, int H, int HKV, int HD, int n_ctx, int n_cu) {
+    const int ns = tree_splits(B, T, H, HKV, HD, n_ctx, n_cu);
+    return ns > 1 ? (size_t)B * T * H * ns * (HD + 4) * sizeof(float) : 0;
+}
+hipError_t launch_attn_tree(const float *q, int B, int T, int H, int HKV, int HD, KvLayer kv, int kv_f16, int n_ctx,
+                            const int32_t *n_past, const uint64_t *mask, float scale, float *part, float *out, int n_cu,
+                            hipStream_t s) {
+    RowsArgs a{};
+    a.q = q, a.kv = kv, a.n_ctx = n_ctx, a.H = H, a.HKV = HKV, a.T = T, a.n_keys = n_past, a.mask = mask;
+    a.mode = ROWS_TREE, a.scale = scale, a.part = part, a.out = out;
+    a.n_split = tree_splits(B, T, H, HKV, HD, n_ctx, n_cu);
+    return rows_by_shape(HD, kv_f16, [&](auto hd, auto f16) {
+        const hipError_t e = rows_launch<decltype(hd)::value, decltype(f16)::value>(a, B, false, s);
+        return e != hipSuccess || a.n_split == 1 ? e : rows_launch_merge<decltype(hd)::value>(a, B, s);
+    });
+}
+
+static int one_splits(int B, int HKV, int n_ctx, int n_cu) { return rows_splits(B * HKV, n_ctx, n_cu); }
+static int64_t one_stride(int n_ctx) { return ((int64_t)n_ctx + 31) / 32 * 32; }
+size_t attn_one_weights_scratch_bytes(int B, int H, int HKV, int HD, int n_ctx, int n_cu) {
+    return (size_t)B * H * (one_stride(n_ctx) + (size_t)one_splits(B, HKV, n_ctx, n_cu) * (HD + 4)) * sizeof(float);
+}
+hipError_t launch_attn_one_weights(const float *q, int B, int H, int HKV, int HD, KvLayer kv, int kv_f16, int n_ctx,
+                                   const int32_t *n_keys, float scale, void *scratch, float *out, const float *acc,
+                                   float *acc_out, int n_cu, hipStream_t s) {
+    RowsArgs a{};
+    a.q = q, a.kv = kv, a.n_ctx = n_ctx, a.H = H, a.HKV = HKV, a.T = 1, a.n_keys = n_keys;
+    a.mode = ROWS_ONE, a.scale = scale, a.out = out, a.stride = one_stride(n_ctx);
+    a.n_split = one_splits(B, HKV, n_ctx, n_cu);
+    a.scores = (float *)scratch, a.part = a.scores + (int64_t)B * H * a.stride;
+    return rows_by_shape(HD, kv_f16, [&](auto hd, auto f16) {
+        constexpr int D = decltype(hd)::value;
+        const hipError_t e = rows_launch<D, decltype(f16)::value>(a, B, true, s);
+        if (e != hipSuccess) return e;
+        hipLaunchKernelGGL(k_one_weights<D>, dim3((n_ctx + 1023) / 1024, HKV, B), dim3(256), 0, s, a, acc, acc_out);
+        return hipGetLastError();
+    });
+}
+
+struct PromptWeightsScratch {
+    int ns;
+    size_t part, planes, p2e, lse;  // bytes
+};
+static PromptWeightsScratch prompt_scratch(int nq, int H, int HKV, int HD, int n_keys, int n_cu) {
+    const int R = nq * (H / HKV), tiles = (R + 15) / 16;
+    PromptWeightsScratch p;
+    p.ns = rows_splits(HKV * rows_blocks(R, HD), n_keys, 2 * n_cu);
+    p.part = p.ns > 1 ? (size_t)nq * H * p.ns * (HD + 4) * sizeof(float) : 0;
+    p.planes = (size_t)HKV * tiles * HD / 32 * 2 * 64 * sizeof(uint4);
+    p.p2e = (size_t)HKV * tiles * 16 * sizeof(float);
+    p.lse = (size_t)HKV * R * sizeof(float);
+    return p;
+}
+size_t attn_prompt_weights_scratch_bytes(int nq, int H, int HKV, int HD, int n_keys, int n_cu) {
+    const PromptWeightsScratch p = prompt_scratch(nq, H, HKV, HD, n_keys, n_cu);
+    return p.part + p.planes + p.p2e + p.lse;
+}
+hipError_t launch_attn_prompt_weights(const float *q, int nq, int H, int HKV, int HD, KvLayer kv, int kv_f16, int n_ctx,
+                                      int pos0, float scale, void *scratch, float *out, const float *acc,
+                                      float *acc_out, int n_cu, hipStream_t s) {
+    const PromptWeightsScratch p = prompt_scratch(nq, H, HKV, HD, pos0 + nq, n_cu);
+    uint8_t *base = (uint8_t *)scratch;
+    RowsArgs a{};
+    a.q = q, a.kv = kv, a.n_ctx = n_ctx, a.H = H, a.HKV = HKV, a.T = nq, a.pos0 = pos0;
+    a.mode = ROWS_CAUSAL, a.scale = scale, a.out = out, a.n_split = p.ns;
+    a.planes = (uint4 *)base, a.p2e = (float *)(base + p.planes), a.lse = (float *)(base + p.planes + p.p2e);
+    a.part = (float *)(base + p.planes + p.p2e + p.lse);
+    return rows_by_shape(HD, kv_f16, [&](auto hd, auto f16) {
+        constexpr int D = decltype(hd)::value;
+        constexpr bool F = decltype(f16)::value;
+        hipError_t e = rows_launch<D, F>(a, 1, false, s);
+        if (e == hipSuccess && a.n_split > 1) e = rows_launch_merge<D>(a, 1, s);
+        if (e != hipSuccess) return e;
+        constexpr int KT = D == 256 ? 1 : 2, per = 4 * 16 * KT;
+        hipLaunchKernelGGL((k_prompt_weights<D, F, KT>), dim3((pos0 + nq + per - 1) / per, HKV), dim3(256), 0, s, a, acc,
+                           acc_out);
+        return hipGetLastError();
+    });
+}
+
+}  // namespace ts5hip

@@ -1,0 +1,267 @@
+// Attention over the blocks of a cache that a bound on their scores picks for each query:
+//  k_block_bounds  lowest and highest cached value of each dimension over a block's keys,
+//                  rounded outwards to f16;
+//  k_block_scores  for each block, the highest score that a key inside its bounds could have
+//                  with any head of the KV head's group: max over heads of sum_d max(q_d lo_d,
+//                  q_d hi_d). In fp64: a rounded score could pick another block, and another block
+//                  is another output;
+//  k_block_pick    the last block, the first, then the highest scores, ties to the lowest
+//                  block, ascending;
+//  k_attn_picked   attention over the picked blocks' keys (attn_rows.h), split over workgroups,
+//  k_picked_merge  which this joins.
+#include <algorithm>
+
+#include "attn_rows.h"
+#include "radix_pick.h"
+
+namespace ts5hip {
+
+// ---- bounds ----------------------------------------------------------------------------------------
+
+// x to f16, down (up) to the next value where the nearest is above (below) it.
+__device__ inline _Float16 f16_towards(float x, bool up) {
+    const _Float16 h = (_Float16)x;
+    const float y = (float)h;
+    if (up ? !(y < x) : !(y > x)) return h;
+    uint16_t b = __builtin_bit_cast(uint16_t, h);
+    if ((b & 0x7fff) == 0) b = up ? 0x0001 : 0x8001;
+    else b += ((b >> 15) == 0) == up ? 1 : -1;
+    return __builtin_bit_cast(_Float16, b);
+}
+
+// A wave per block: LPR lanes a row, 16 bytes each. grid (ceil(blocks / 4), HKV, B) of the blocks that hold a cache's
+// last n_new keys.
+template <int HD, bool F16>
+__global__ __launch_bounds__(256) void k_block_bounds(KvLayer kv, int HKV, int n_ctx, const int32_t *n_keys, int n_new,
+                                                      int block, int n_blocks, _Float16 *bounds) {
+    constexpr int VB = F16 ? 2 : 1, LPR = HD * VB / 16, RPW = 64 / LPR, V = 16 / VB;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, kvh = blockIdx.y, b = blockIdx.z;
+    const int n = max(0, min(n_keys[b], n_ctx));
+    const int blk = max(n - n_new, 0) / block + (int)blockIdx.x * 4 + wave;
+    if ((int64_t)blk * block >= n) return;
+    const int64_t slot0 = ((int64_t)b * HKV + kvh) * n_ctx;
+    const int first = blk * block, last = min(n, first + block), d0 = lane % LPR * V;
+    float lo[V], hi[V];
+#pragma unroll
+    for (int j = 0; j < V; j++) lo[j] = INFINITY, hi[j] = -INFINITY;
+    for (int r = first + lane / LPR; r < last; r += RPW) {
+        const u32x4 w = *(const u32x4 *)(kv.k + ((slot0 + r) * HD + d0) * VB);
+        float sc = 1.f;
+        if constexpr (!F16) sc = h2f(kv.ks[(slot0 + r) * (HD / 32) + d0 / 32]);
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            float x;
+            if constexpr (F16) x = h2f((w[j / 2] >> (16 * (j & 1))) & 0xffff);
+            else x = (float)(int8_t)(w[j / 4] >> (8 * (j & 3))) * sc;
+            lo[j] = fminf(lo[j], x), hi[j] = fmaxf(hi[j], x);  // (NaN: passed over)
+        }
+    }
+#pragma unroll
+    for (int o = LPR; o < 64; o <<= 1)
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            lo[j] = fminf(lo[j], __shfl_xor(lo[j], o, 64));
+            hi[j] = fmaxf(hi[j], __shfl_xor(hi[j], o, 64));
+        }
+    if (lane < LPR) {
+        _Float16 *p = bounds + (((int64_t)b * HKV + kvh) * n_blocks + blk) * 2 * HD + d0;
+#pragma unroll
+        for (int j = 0; j < V; j++) p[j] = f16_towards(lo[j], false), p[HD + j] = f16_towards(hi[j], true);
+    }
+}
+
+hipError_t launch_block_bounds(int B, int HKV, int HD, KvLayer kv, int kv_f16, int n_ctx, const int32_t *n_keys,
+                               int n_new, int block, void *bounds, hipStream_t s) {
+    const int nb = (n_ctx + block - 1) / block, most = std::min(nb, (n_new + block - 1) / block + 1);
+    const dim3 grid((most + 3) / 4, HKV, B);
+    auto go = [&](auto hd, auto f16) {
+        hipLaunchKernelGGL((k_block_bounds<decltype(hd)::value, decltype(f16)::value>), grid, dim3(256), 0, s, kv, HKV,
+                           n_ctx, n_keys, n_new, block, nb, (_Float16 *)bounds);
+        return hipGetLastError();
+    };
+    return rows_by_shape(HD, kv_f16, go);
+}
+
+// ---- scores and the pick ---------------------------------------------------------------------------
+
+struct SparseArgs {
+    const float *q;  // [B][H * HD]
+    KvLayer kv;
+    int n_ctx, H, HKV, B, per_batch, block, n_pick, n_split;
+    const int32_t *n_keys;
+    const _Float16 *bounds;  // [caches][HKV][n_blocks][2][HD]
+    int n_blocks;
+    float scale;
+    double *scores;   // [B][HKV][n_blocks]
+    int32_t *picked;  // [B][HKV][n_pick], -1 past the blocks there are
+    float *part;      // [B][HKV][G][n_split][HD + 4]
+    float *out;
+};
+__device__ inline int sparse_count(const SparseArgs &a, int b) {
+    return max(0, min(a.per_batch ? a.n_keys[b] : a.n_keys[0] + b + 1, a.n_ctx));
+}
+
+// HD / 8 lanes a block, 8 dims each. grid (ceil(n_blocks / SCORE_BLOCKS), HKV, B).
+constexpr int SCORE_BLOCKS = 64;
+template <int HD>
+__global__ __launch_bounds__(256) void k_block_scores(SparseArgs a) {
+    constexpr int LPB = HD / 8, BPW = 64 / LPB;
+    __shared__ __align__(16) double q[ROWS_MAX_G][HD];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, kvh = blockIdx.y, b = blockIdx.z;
+    const int n = sparse_count(a, b), nb = (n + a.block - 1) / a.block, G = a.H / a.HKV;
+    const int first = blockIdx.x * SCORE_BLOCKS;
+    if (first >= nb - 1 || nb <= a.n_pick) return;  // the last block is read in any case, and so are all that fit
+    for (int e = threadIdx.x; e < G * HD; e += 256) q[e / HD][e % HD] = (double)a.q[((int64_t)b * a.H + kvh * G) * HD + e];
+    __syncthreads();
+    const int64_t head = (int64_t)(a.per_batch ? b : 0) * a.HKV + kvh;
+    const int d0 = lane % LPB * 8;
+    for (int blk = first + wave * BPW + lane / LPB; blk < first + SCORE_BLOCKS; blk += 4 * BPW) {
+        double best = -INFINITY;
+        const int at = min(blk, nb - 1);
+        const _Float16 *p = a.bounds + (head * a.n_blocks + at) * 2 * HD + d0;
+        const ar_h8 lo = *(const ar_h8 *)p, hi = *(const ar_h8 *)(p + HD);
+        for (int g = 0; g < G; g++) {
+            double s = 0;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const double x = q[g][d0 + j];
+                s = fma(x, (double)(float)(x >= 0 ? hi[j] : lo[j]), s);
+            }
+#pragma unroll
+            for (int o = LPB / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+            if (!(s <= best)) best = s != s ? INFINITY : s;  // (NaN ranks first)
+        }
+        if (blk < nb && lane % LPB == 0) a.scores[((int64_t)b * a.HKV + kvh) * a.n_blocks + blk] = best;
+    }
+}
+
+__global__ __launch_bounds__(PICK_NT) void k_block_pick(SparseArgs a) {
+    __shared__ PickLds L;
+    const int kvh = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+    const int n = sparse_count(a, b), nb = (n + a.block - 1) / a.block;
+    int32_t *out = a.picked + ((int64_t)b * a.HKV + kvh) * a.n_pick;
+    if (nb <= a.n_pick) {
+        for (int i = tid; i < a.n_pick; i += PICK_NT) out[i] = i < nb ? i : -1;
+        return;
+    }
+    const double *sc = a.scores + ((int64_t)b * a.HKV + kvh) * a.n_blocks;
+    if (tid == 0) out[a.n_pick - 1] = nb - 1;
+    if (a.n_pick == 1) return;
+    radix_pick<64>(L, nb - 1, a.n_pick - 1, [&](int i) { return i == 0 ? ~0ull : order_key(sc[i]); },
+                   [&](int place, int i) { out[place] = i; });
+}
+
+// ---- attention over the picked blocks ----------------------------------------------------------------
+
+// Units (KT tiles of 16 keys) of the picked blocks of query b, and a slice's share.
+__device__ inline int sparse_units(const SparseArgs &a, int b, int KT) {
+    const int nb = (sparse_count(a, b) + a.block - 1) / a.block;
+    return (min(nb, a.n_pick) * (a.block / 16) + KT - 1) / KT;
+}
+
+// grid (n_split, HKV, B): one slice of the picked units for the G heads of a KV head.
+template <int HD, bool F16, int KT, int NW>
+__global__ __launch_bounds__(64 * NW) void k_attn_picked(SparseArgs a) {
+    __shared__ RowsLds<HD, NW> L;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int rl = lane & 15, kq = lane >> 4;
+    const int split = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z, G = a.H / a.HKV;
+    const int n = sparse_count(a, b), units = sparse_units(a, b, KT), per = (units + a.n_split - 1) / a.n_split;
+    const int u0 = split * per, u1 = min(units, u0 + per);
+    if (u0 >= u1) return;
+    const int tpb = a.block / 16, tiles = min((n + a.block - 1) / a.block, a.n_pick) * tpb;
+    const int32_t *list = a.picked + ((int64_t)b * a.HKV + kvh) * a.n_pick;
+    const RowsKv kv = rows_kv<HD, F16>(a.kv, ((int64_t)(a.per_batch ? b : 0) * a.HKV + kvh) * a.n_ctx, n);
+    auto at = [&](int u, int (&kb)[KT]) {
+#pragma unroll
+        for (int t = 0; t < KT; t++) {
+            const int tile = u * KT + t, i = tile < tiles && u < u1 ? tile : -1;
+            kb[t] = i < 0 ? n : list[i / tpb] * a.block + i % tpb * 16;  // (none: zeros, no memory access)
+        }
+    };
+    RowsUnit<HD, F16, KT> nxt;
+    int kb[KT], kn[KT];
+    at(u0 + wave, kn);
+    rows_load<HD, F16, KT>(nxt, kv, kn, rl, kq);
+    RowsQ<HD, 1> q;
+    rows_query<HD, 1>(q, a.scale, kq,
+                      [&](int) { return rl < G ? a.q + ((int64_t)b * a.H + kvh * G + rl) * HD : nullptr; });
+    RowsSum<HD, 1> sum;
+    rows_clear<HD, 1>(sum);
+    for (int u = u0 + wave; u < u1; u += NW) {
+        const RowsUnit<HD, F16, KT> cur = nxt;
+#pragma unroll
+        for (int t = 0; t < KT; t++) kb[t] = kn[t];
+        at(u + NW, kn);
+        rows_load<HD, F16, KT>(nxt, kv, kn, rl, kq);
+        rows_unit<HD, F16, KT, 1, true, false>(cur, q, sum, kb, kq, [&](int, int key) { return rows_below(key, n); },
+                                               [](int, int, const float (&)[4]) {});
+    }
+    const int64_t row0 = ((int64_t)b * a.HKV + kvh) * G;
+    rows_combine<HD, 1, NW>(L, sum, G, wave, rl, kq, [&](int r, int d, float4 o, float m, float l) {
+        float *p = a.part + ((row0 + r) * a.n_split + split) * (HD + 4);
+        if (d == 0) *(float4 *)p = make_float4(m, l, 0.f, 0.f);
+        *(float4 *)(p + 4 + d) = o;
+    });
+}
+
+template <int HD, int KT>
+__global__ __launch_bounds__(256) void k_picked_merge(SparseArgs a, int64_t rows) {
+    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x, row = e / (HD / 4);
+    if (row >= rows) return;
+    const int d = 4 * (int)(e % (HD / 4)), b = (int)(row / a.H);
+    const int units = sparse_units(a, b, KT), per = (units + a.n_split - 1) / a.n_split;
+    const int used = units ? (units + per - 1) / per : 0;
+    float M, l;
+    const float4 o = rows_merge(a.part + row * a.n_split * (HD + 4), used, HD + 4, d, M, l);
+    const float inv = 1.0f / l;
+    *(float4 *)(a.out + row * HD + d) =
+        l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+}
+
+struct SparseScratch {
+    int n_blocks, n_split;
+    size_t scores, picked, part;
+};
+static SparseScratch sparse_scratch(int B, int H, int HKV, int HD, int n_ctx, int block, int n_pick, int n_cu) {
+    SparseScratch p;
+    p.n_blocks = (n_ctx + block - 1) / block;
+    const int64_t keys = (int64_t)std::min(n_pick, p.n_blocks) * block;
+    // Every workgroup a unit a wave at least; one round of two workgroups a CU.
+    const int most = (int)std::min<int64_t>((keys + 63) / 64, ROWS_MAX_SPLIT);
+    p.n_split = std::max(1, std::min(2 * n_cu / std::max(1, B * HKV), most));
+    p.scores = align_up((size_t)B * HKV * p.n_blocks * sizeof(double), 256);
+    p.picked = align_up((size_t)B * HKV * n_pick * sizeof(int32_t), 256);
+    p.part = (size_t)B * H * p.n_split * (HD + 4) * sizeof(float);
+    return p;
+}
+size_t attn_sparse_scratch_bytes(int B, int H, int HKV, int HD, int n_ctx, int block, int n_pick, int n_cu) {
+    const SparseScratch p = sparse_scratch(B, H, HKV, HD, n_ctx, block, n_pick, n_cu);
+    return p.scores + p.picked + p.part;
+}
+hipError_t launch_attn_sparse(const float *q, int B, int H, int HKV, int HD, KvLayer kv, int kv_f16, int n_ctx,
+                              const int32_t *n_keys, int per_batch, const void *bounds, int block, int n_pick,
+                              float scale, void *scratch, float *out, int32_t *picked, int n_cu, hipStream_t s) {
+    const SparseScratch p = sparse_scratch(B, H, HKV, HD, n_ctx, block, n_pick, n_cu);
+    uint8_t *base = (uint8_t *)scratch;
+    SparseArgs a{};
+    a.q = q, a.kv = kv, a.n_ctx = n_ctx, a.H = H, a.HKV = HKV, a.B = B, a.per_batch = per_batch, a.block = block;
+    a.n_pick = n_pick, a.n_split = p.n_split, a.n_keys = n_keys, a.bounds = (const _Float16 *)bounds;
+    a.n_blocks = p.n_blocks, a.scale = scale, a.out = out;
+    a.scores = (double *)base, a.picked = picked ? picked : (int32_t *)(base + p.scores);
+    a.part = (float *)(base + p.scores + p.picked);
+    const dim3 sg((p.n_blocks + SCORE_BLOCKS - 1) / SCORE_BLOCKS, HKV, B);
+    return rows_by_shape(HD, kv_f16, [&](auto hd, auto f16) {
+        constexpr int D = decltype(hd)::value, KT = D == 64 ? 2 : 1, NW = 4;
+        constexpr bool F = decltype(f16)::value;
+        hipLaunchKernelGGL(k_block_scores<D>, sg, dim3(256), 0, s, a);
+        hipLaunchKernelGGL(k_block_pick, dim3(HKV, B), dim3(PICK_NT), 0, s, a);
+        hipLaunchKernelGGL((k_attn_picked<D, F, KT, NW>), dim3(p.n_split, HKV, B), dim3(64 * NW), 0, s, a);
+        const int64_t rows = (int64_t)B * H;
+        hipLaunchKernelGGL((k_picked_merge<D, KT>), dim3((unsigned)((rows * (D / 4) + 255) / 256)), dim3(256), 0, s, a,
+                           rows);
+        return hipGetLastError();
+    });
+}
+
+}  // namespace ts5hip

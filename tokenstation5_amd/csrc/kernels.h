@@ -108,6 +108,11 @@ hipError_t launch_rope_kv(const float *qkv, int64_t qkv_stride, const float *bia
                           const float *k_norm, float eps, const float *rope_cs, int n_rot, int neox,
                           const int32_t *pos0, int H, int HKV, int HD, int n_ctx, int ntok, float *q_out, KvLayer kv,
                           int kv_f16, hipStream_t s);
+// The same with each token's RoPE position at[t] (below n_pos, the table's rows) apart from its slot *slot0 + t.
+hipError_t launch_rope_kv_at(const float *qkv, int64_t qkv_stride, const float *bias, const float *q_norm,
+                             const float *k_norm, float eps, const float *rope_cs, int n_pos, int n_rot, int neox,
+                             const int32_t *at, const int32_t *slot0, int H, int HKV, int HD, int n_ctx, int ntok,
+                             float *q_out, KvLayer kv, int kv_f16, hipStream_t s);
 bool attn_supported(int H, int HKV, int HD);
 // Flash decode (attention.hip: k_attn). q rows of B queries; with rope each
 // row holds the token's raw q, k, v ((H + 2 HKV) HD values), and q (with
@@ -168,6 +173,42 @@ hipError_t launch_kv_read(KvLayer kv, int which, int HKV, int HD, int n_ctx, int
                           hipStream_t s);
 hipError_t launch_kv_write(KvLayer kv, int which, int HKV, int HD, int n_ctx, int pos0, int n, int kv_f16,
                            const float *in, hipStream_t s);
+
+// attn_rows.hip: head dimension 64, 128 or 256, at most 16 query heads a KV head; scratch of the
+// size that the function beside each launcher gives, 16-byte aligned.
+bool attn_rows_supported(int H, int HKV, int HD);
+// T tokens (at most 64) of each of B caches: every key below n_past[b], and of the T after them those of its mask's bits.
+size_t attn_tree_scratch_bytes(int B, int T, int H, int HKV, int HD, int n_ctx, int n_cu);
+hipError_t launch_attn_tree(const float *q, int B, int T, int H, int HKV, int HD, KvLayer kv, int kv_f16, int n_ctx,
+                            const int32_t *n_past, const uint64_t *mask, float scale, float *scratch, float *out,
+                            int n_cu, hipStream_t s);
+// One query a cache, and acc_out = acc + the weights of each KV head's keys [B][HKV][n_ctx].
+size_t attn_one_weights_scratch_bytes(int B, int H, int HKV, int HD, int n_ctx, int n_cu);
+hipError_t launch_attn_one_weights(const float *q, int B, int H, int HKV, int HD, KvLayer kv, int kv_f16, int n_ctx,
+                                   const int32_t *n_keys, float scale, void *scratch, float *out, const float *acc,
+                                   float *acc_out, int n_cu, hipStream_t s);
+// nq consecutive queries over one cache, causal, and the same sums.
+size_t attn_prompt_weights_scratch_bytes(int nq, int H, int HKV, int HD, int n_keys, int n_cu);
+hipError_t launch_attn_prompt_weights(const float *q, int nq, int H, int HKV, int HD, KvLayer kv, int kv_f16, int n_ctx,
+                                      int pos0, float scale, void *scratch, float *out, const float *acc,
+                                      float *acc_out, int n_cu, hipStream_t s);
+
+// attn_sparse.hip: f16 bounds [B][HKV][ceil(n_ctx / block)][lowest, highest][HD] of the blocks that hold each cache's
+// last n_new keys; attention over the n_pick blocks that they pick (picked [B][HKV][n_pick] may be null).
+hipError_t launch_block_bounds(int B, int HKV, int HD, KvLayer kv, int kv_f16, int n_ctx, const int32_t *n_keys,
+                               int n_new, int block, void *bounds, hipStream_t s);
+size_t attn_sparse_scratch_bytes(int B, int H, int HKV, int HD, int n_ctx, int block, int n_pick, int n_cu);
+hipError_t launch_attn_sparse(const float *q, int B, int H, int HKV, int HD, KvLayer kv, int kv_f16, int n_ctx,
+                              const int32_t *n_keys, int per_batch, const void *bounds, int block, int n_pick,
+                              float scale, void *scratch, float *out, int32_t *picked, int n_cu, hipStream_t s);
+
+// kv_cache.hip
+hipError_t launch_kv_evict(int B, int HKV, int HD, KvLayer kv, int kv_f16, int n_ctx, const int32_t *n_keys,
+                           const float *acc, int n_keep, int n_first, int n_last, int n_ctx_out, KvLayer to,
+                           float *acc_out, int32_t *kept, int32_t *n_out, hipStream_t s);
+constexpr int KV_PATH_MAX = 64;  // rows of a path
+hipError_t launch_kv_path(int B, int HKV, int HD, KvLayer kv, int kv_f16, int n_ctx, const int32_t *slots, int n,
+                          const int32_t *slot0, hipStream_t s);
 
 // sample.hip
 size_t argmax_scratch_bytes(int rows);

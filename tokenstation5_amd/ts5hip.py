@@ -82,6 +82,21 @@ _SIGS = {
                                           _f32, _i32, _vp]),
     "ts5hip_attn_prompt": (_i32, [_vp, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _i32, _f32, _vp]),
     "ts5hip_attn_prompt_f16": (_i32, [_vp, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _i32, _i32, _f32, _vp]),
+    "ts5hip_rope_kv_append_at": (_i32, [_vp, _vp, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _i32, _i32, _i32,
+                                        _vp, _vp, _vp, _f32, _vp, _vp, _vp, _vp, _vp]),
+    "ts5hip_attn_tree": (_i32, [_vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _f32,
+                                _vp]),
+    "ts5hip_kv_path": (_i32, [_vp, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _vp, _i32, _vp]),
+    "ts5hip_attn_decode_weights": (_i32, [_vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _vp, _f32,
+                                          _vp, _vp, _vp]),
+    "ts5hip_attn_prompt_weights": (_i32, [_vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _i32, _f32,
+                                          _vp, _vp, _vp]),
+    "ts5hip_kv_evict": (_i32, [_vp, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _i32, _i32, _i32, _i32,
+                               _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "ts5hip_kv_bounds_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32]),
+    "ts5hip_kv_block_bounds": (_i32, [_vp, _i32, _i32, _i32, _i32, _vp, _vp, _i32, _vp, _i32, _i32, _vp]),
+    "ts5hip_attn_sparse": (_i32, [_vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _vp, _i32, _vp, _i32,
+                                  _i32, _f32, _vp, _vp]),
     "ts5hip_argmax": (_i32, [_vp, _vp, _i32, _i32, _vp]),
     "ts5hip_topk": (_i32, [_vp, _vp, _i32, _i32, _vp, _vp]),
     "ts5hip_sampler_new": (_vp, [_u64]),
@@ -347,6 +362,52 @@ class Context:
     def attn_prompt_f16(self, q, nq, H, HKV, HD, k16, v16, n_ctx, pos0, scale, out):
         self.check(lib().ts5hip_attn_prompt_f16(self.h, _ptr(q), nq, H, HKV, HD, _ptr(k16), _ptr(v16), n_ctx, pos0,
                                                 scale, _ptr(out)))
+
+    def rope_kv_append_at(self, qkv, ntok, pos_dev, slot0_dev, H, HKV, HD, n_rot, neox, rope_cs, n_pos, n_ctx, kv, q_out,
+                          k, ks, v, vs, bias=None, q_norm=None, k_norm=None, eps=1e-6):
+        self.check(lib().ts5hip_rope_kv_append_at(self.h, _ptr(qkv), ntok, _ptr(pos_dev), _ptr(slot0_dev), H, HKV, HD,
+                                                  n_rot, int(neox), _ptr(rope_cs), n_pos, n_ctx, kv, _ptr(bias),
+                                                  _ptr(q_norm), _ptr(k_norm), eps, _ptr(q_out), _ptr(k), _ptr(ks),
+                                                  _ptr(v), _ptr(vs)))
+
+    def attn_tree(self, q, B, n_tree, H, HKV, HD, kv, k, ks, v, vs, n_ctx, n_past_dev, mask_dev, scale, out):
+        self.check(lib().ts5hip_attn_tree(self.h, _ptr(q), B, n_tree, H, HKV, HD, kv, _ptr(k), _ptr(ks), _ptr(v),
+                                          _ptr(vs), n_ctx, _ptr(n_past_dev), _ptr(mask_dev), scale, _ptr(out)))
+
+    def kv_path(self, B, HKV, HD, kv, k, ks, v, vs, n_ctx, slots_dev, n, slot0_dev):
+        self.check(lib().ts5hip_kv_path(self.h, B, HKV, HD, kv, _ptr(k), _ptr(ks), _ptr(v), _ptr(vs), n_ctx,
+                                        _ptr(slots_dev), n, _ptr(slot0_dev)))
+
+    def attn_decode_weights(self, q, B, H, HKV, HD, kv, k, ks, v, vs, n_ctx, n_keys_dev, scale, out, acc, acc_out):
+        self.check(lib().ts5hip_attn_decode_weights(self.h, _ptr(q), B, H, HKV, HD, kv, _ptr(k), _ptr(ks), _ptr(v),
+                                                    _ptr(vs), n_ctx, _ptr(n_keys_dev), scale, _ptr(out), _ptr(acc),
+                                                    _ptr(acc_out)))
+
+    def attn_prompt_weights(self, q, nq, H, HKV, HD, kv, k, ks, v, vs, n_ctx, pos0, scale, out, acc, acc_out):
+        self.check(lib().ts5hip_attn_prompt_weights(self.h, _ptr(q), nq, H, HKV, HD, kv, _ptr(k), _ptr(ks), _ptr(v),
+                                                    _ptr(vs), n_ctx, pos0, scale, _ptr(out), _ptr(acc), _ptr(acc_out)))
+
+    def kv_evict(self, B, HKV, HD, kv, k, ks, v, vs, n_ctx, n_keys_dev, acc, n_keep, n_first, n_last, n_ctx_out, k_out,
+                 ks_out, v_out, vs_out, acc_out, kept_dev, n_out_dev=None):
+        self.check(lib().ts5hip_kv_evict(self.h, B, HKV, HD, kv, _ptr(k), _ptr(ks), _ptr(v), _ptr(vs), n_ctx,
+                                         _ptr(n_keys_dev), _ptr(acc), n_keep, n_first, n_last, n_ctx_out, _ptr(k_out),
+                                         _ptr(ks_out), _ptr(v_out), _ptr(vs_out), _ptr(acc_out), _ptr(kept_dev),
+                                         _ptr(n_out_dev)))
+
+    @staticmethod
+    def kv_bounds_bytes(B: int, HKV: int, HD: int, n_ctx: int, block: int) -> int:
+        return lib().ts5hip_kv_bounds_bytes(B, HKV, HD, n_ctx, block)
+
+    def kv_block_bounds(self, B, HKV, HD, kv, k, ks, n_ctx, n_keys_dev, n_new, block, bounds):
+        self.check(lib().ts5hip_kv_block_bounds(self.h, B, HKV, HD, kv, _ptr(k), _ptr(ks), n_ctx, _ptr(n_keys_dev),
+                                                n_new, block, _ptr(bounds)))
+
+    def attn_sparse(self, q, B, H, HKV, HD, kv, k, ks, v, vs, n_ctx, n_keys_dev, kv_per_batch, bounds, block, n_pick,
+                    scale, out, picked_dev=None):
+        self.check(lib().ts5hip_attn_sparse(self.h, _ptr(q), B, H, HKV, HD, kv, _ptr(k), _ptr(ks), _ptr(v), _ptr(vs),
+                                            n_ctx, _ptr(n_keys_dev), int(kv_per_batch), _ptr(bounds), block, n_pick,
+                                            scale, _ptr(out), _ptr(picked_dev)))
+
     def argmax(self, x, n, rows, out):
         self.check(lib().ts5hip_argmax(self.h, _ptr(x), n, rows, _ptr(out)))
 
