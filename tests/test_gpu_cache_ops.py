@@ -658,3 +658,45 @@ def test_contexts_side_by_side(ctx):
     for j, want in zip(jobs, alone):
         assert np.array_equal(j[5].download(np.float32), want)
     other.close()
+
+
+@pytest.mark.parametrize("HD", [64, 128, 256])
+def test_queries_that_are_no_numbers(ctx, HD):
+    """A NaN query gets NaN from every entry point, its neighbours what they get without it."""
+    H, HKV, n = 4, 2, 200
+    rng = np.random.default_rng(HD)
+    c = Cache(ctx, rng, Q8, 2, HKV, n, HD)
+    q = rng.standard_normal((2, 3, H, HD)).astype(np.float32)
+    mask = random_masks(rng, 2, 3)
+    clean = run_tree(ctx, c, q, 3, [150, 20], mask, 0.1, H)
+    q[1, 1, 2] = np.nan
+    got = run_tree(ctx, c, q, 3, [150, 20], mask, 0.1, H)
+    assert np.all(np.isnan(got[1, 1, 2]))
+    got[1, 1, 2] = clean[1, 1, 2]
+    assert np.array_equal(got, clean)
+    n_keys = ctx.to_device(np.array([n, 7], np.int32))
+    acc, out = ctx.to_device(np.zeros((2, HKV, n), np.float32)), ctx.alloc(2 * H * HD * 4)
+    one = ctx.to_device(q[1, :2])  # the second query's third head
+    ctx.attn_decode_weights(one, 2, H, HKV, HD, *c.args, n_keys, 0.1, out, acc, acc)
+    o = out.download(np.float32, (2, H, HD))
+    assert np.all(np.isnan(o[1, 2])) and np.all(np.isfinite(o[0])) and np.all(np.isfinite(o[1, [0, 1, 3]]))
+    bounds = ctx.to_device(np.zeros((2, HKV, 13, 2, HD), np.float16))
+    ctx.attn_sparse(one, 2, H, HKV, HD, *c.args, n_keys, 1, bounds, 16, 4, 0.1, out)
+    o = out.download(np.float32, (2, H, HD))
+    assert np.all(np.isnan(o[1, 2])) and np.all(np.isfinite(o[0])) and np.all(np.isfinite(o[1, [0, 1, 3]]))
+
+
+def test_evict_many_keys(ctx):
+    """More keys than a workgroup's registers hold, with ties across their chunks."""
+    rng = np.random.default_rng(61)
+    n, keep = 70000, 40000
+    c, to = Cache(ctx, rng, Q8, 1, 2, n, 64), Cache(ctx, rng, Q8, 1, 2, keep, 64)
+    acc = rng.integers(0, 50, (1, 2, n)).astype(np.float32)
+    acc_out, kept = ctx.alloc(2 * keep * 4), ctx.alloc(2 * keep * 4)
+    ctx.kv_evict(1, 2, 64, *c.args, ctx.to_device(np.array([n], np.int32)), ctx.to_device(acc), keep, 5, 1000, keep,
+                 *to.args[1:5], acc_out, kept)
+    kept, got = kept.download(np.int32, (2, keep)), to.fetch()
+    for h in range(2):
+        rows = evict_want(acc[0, h], n, keep, 5, 1000)
+        assert kept[h].tolist() == rows
+        assert all(np.array_equal(got[m][0, h], c.raw[m][0, h, rows]) for m in got)

@@ -10,8 +10,9 @@
 //    bits, the planes' products are exact and summed in fp32); q8: K as exact
 //    integers, one product per 32-value scale group, then S += ks * R.
 //  * online softmax per row in the log2 domain; the rows are the lanes'
-//    columns. The reference is the running maximum less 7, so that weights go to
-//    128 and their lo plane stays out of the fp16 subnormals.
+//    columns. The reference is a running maximum less 7, so that weights go past
+//    128 and their lo plane stays out of the fp16 subnormals; it follows the true
+//    maximum only once that is 4 above it (weights to 2^11), so that the sums are rarely scaled.
 //  * O^T (dims x rows) += V^T . P^T. The D layout of S^T (lane: keys 4 kq .. + 3 of
 //    each tile) is the B layout of P^T, so P stays in registers as hi + lo. For V^T
 //    the lane in MFMA row m = lane & 15 and key group kq = lane >> 4 loads keys 4 kq ..
@@ -30,6 +31,7 @@ namespace ts5hip {
 typedef _Float16 ar_h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 ar_h4 __attribute__((ext_vector_type(4)));
 typedef _Float16 ar_h2 __attribute__((ext_vector_type(2)));
+typedef float ar_f2 __attribute__((ext_vector_type(2)));
 typedef float ar_f4 __attribute__((ext_vector_type(4)));
 
 constexpr float AR_LOG2E = 1.4426950408889634f;
@@ -130,8 +132,22 @@ __device__ inline ar_h8 rows_values(const uint32_t (&w)[N]) {
     }
 }
 
+// Two fp32 as fp16 pairs hi + lo, x = hi + lo to about 22 bits.
+__device__ inline void rows_split(float x0, float x1, uint32_t &hi, uint32_t &lo) {
+    const ar_f2 x = {x0, x1};
+    const ar_h2 h = __builtin_convertvector(x, ar_h2);  // v_cvt_pk_f16_f32
+    hi = __builtin_bit_cast(uint32_t, h);
+    ar_f2 r;  // x - h: one instruction a half
+    float r0, r1;
+    asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r0) : "v"(hi), "v"(x0));
+    asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r1) : "v"(hi), "v"(x1));
+    r[0] = r0, r[1] = r1;
+    lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, ar_h2));
+}
+
 // The lane's rows (its MFMA columns), row 16 qt + rl of the wave's: B operands of dims
-// 32 c + 8 kq .. + 7, and 2^e. A null row is zero.
+// 32 c + 8 kq .. + 7, and 2^e. row(qt, ok) is the row's address; not ok: an address to read from, and zeros
+// (a load under a branch would wait for the one before it).
 template <int HD, int NT>
 struct RowsQ {
     ar_h8 h[NT][HD / 32], l[NT][HD / 32];
@@ -142,15 +158,16 @@ __device__ inline void rows_query(RowsQ<HD, NT> &q, float scale, int kq, Row row
     constexpr int NC = HD / 32;
 #pragma unroll
     for (int qt = 0; qt < NT; qt++) {
-        const float *p = row(qt);
+        bool ok;
+        const float *p = row(qt, ok);
+        const float by = scale * AR_LOG2E;
         float v[NC][8], amax = 0.f;
 #pragma unroll
         for (int c = 0; c < NC; c++) {
-            float4 x0 = make_float4(0.f, 0.f, 0.f, 0.f), x1 = x0;
-            if (p) x0 = *(const float4 *)(p + 32 * c + 8 * kq), x1 = *(const float4 *)(p + 32 * c + 8 * kq + 4);
+            const float4 x0 = *(const float4 *)(p + 32 * c + 8 * kq), x1 = *(const float4 *)(p + 32 * c + 8 * kq + 4);
             const float f[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[c][j] = f[j] * (scale * AR_LOG2E), amax = fmaxf(amax, fabsf(v[c][j]));
+            for (int j = 0; j < 8; j++) v[c][j] = ok ? f[j] * by : 0.f, amax = fmaxf(amax, fabsf(v[c][j]));
         }
         amax = max_xor32(max_xor16(amax));
         const int e = amax > 0.f ? max(ilogbf(amax) - 13, -100) : 0;
@@ -160,10 +177,19 @@ __device__ inline void rows_query(RowsQ<HD, NT> &q, float scale, int kq, Row row
         for (int c = 0; c < NC; c++)
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                const float f = v[c][j] * sc;
-                q.h[qt][c][j] = (_Float16)f;
-                q.l[qt][c][j] = (_Float16)(f - (float)q.h[qt][c][j]);
+                v[c][j] *= sc;
             }
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            u32x4 h, l;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                uint32_t hj, lj;
+                rows_split(v[c][2 * j], v[c][2 * j + 1], hj, lj);
+                h[j] = hj, l[j] = lj;
+            }
+            q.h[qt][c] = __builtin_bit_cast(ar_h8, h), q.l[qt][c] = __builtin_bit_cast(ar_h8, l);
+        }
     }
 }
 
@@ -232,29 +258,32 @@ template <int HD, bool F16, int KT>
 struct RowsScale {
     ar_h2 s[KT][2];
 };
+// The pair (key a, key b) of dim j of value dwords wa, wb, times their scales (q8).
+template <bool F16>
+__device__ inline void rows_value_pair(uint32_t wa, uint32_t wb, int j, ar_h2 sc, uint32_t &hi, uint32_t &lo) {
+    if constexpr (F16) {
+        hi = __builtin_amdgcn_perm(wb, wa, j & 1 ? 0x07060302u : 0x05040100u);
+        lo = 0;
+    } else {
+        const ar_h2 k1152 = {(_Float16)1152.0f, (_Float16)1152.0f};
+        const uint32_t b = __builtin_amdgcn_perm(wb ^ 0x80808080u, wa ^ 0x80808080u, 0x0c000c00u | (uint32_t)(4 + j) << 16 | (uint32_t)j);
+        const ar_h2 v = __builtin_bit_cast(ar_h2, b | 0x64006400u) - k1152;
+        const ar_h2 h = v * sc;
+        hi = __builtin_bit_cast(uint32_t, h);
+        lo = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(v, sc, -h));
+    }
+}
 template <int HD, bool F16, int KT>
 __device__ inline void rows_value_tile(const RowsUnit<HD, F16, KT> &u, const RowsScale<HD, F16, KT> &sc, int dt,
                                        uint32_t (&hi)[2 * KT],
                                        uint32_t (&lo)[2 * KT]) {
-    const ar_h2 k1152 = {(_Float16)1152.0f, (_Float16)1152.0f};
+    constexpr int PW = F16 ? 2 : 4;  // dims a dword
 #pragma unroll
     for (int t = 0; t < KT; t++)
 #pragma unroll
-        for (int p = 0; p < 2; p++) {
-            if constexpr (F16) {
-                hi[2 * t + p] = __builtin_amdgcn_perm(u.v[t][2 * p + 1][dt / 2], u.v[t][2 * p][dt / 2],
-                                                      dt & 1 ? 0x07060302u : 0x05040100u);
-                lo[2 * t + p] = 0;
-            } else {
-                const uint32_t x0 = u.v[t][2 * p][dt / 4] ^ 0x80808080u, x1 = u.v[t][2 * p + 1][dt / 4] ^ 0x80808080u;
-                const uint32_t j = dt & 3;
-                const uint32_t b = __builtin_amdgcn_perm(x1, x0, 0x0c000c00u | (4 + j) << 16 | j);
-                const ar_h2 v = __builtin_bit_cast(ar_h2, b | 0x64006400u) - k1152;
-                const ar_h2 h = v * sc.s[t][p];
-                hi[2 * t + p] = __builtin_bit_cast(uint32_t, h);
-                lo[2 * t + p] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(v, sc.s[t][p], -h));
-            }
-        }
+        for (int p = 0; p < 2; p++)
+            rows_value_pair<F16>(u.v[t][2 * p][dt / PW], u.v[t][2 * p + 1][dt / PW], dt % PW, sc.s[t][p], hi[2 * t + p],
+                                 lo[2 * t + p]);
 }
 template <int KT>
 struct RowsOp;
@@ -270,6 +299,21 @@ struct RowsOp<2> {
     __device__ static T of(const uint32_t (&w)[4]) { return __builtin_bit_cast(T, u32x4{w[0], w[1], w[2], w[3]}); }
     __device__ static ar_f4 mfma(T a, T b, ar_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
+
+// The rows' reference for weights of scores up to mx (log2 domain): raised, and the sums
+// scaled, where some row's maximum is past it by ROWS_SLACK. Returns what scores are taken less.
+constexpr float ROWS_SLACK = 4.f;
+template <int HD, int NT>
+__device__ inline float rows_reference(RowsSum<HD, NT> &a, int qt, float mx) {
+    mx -= 7.f;
+    if (__builtin_amdgcn_ballot_w64(mx > a.m[qt] + ROWS_SLACK)) {
+        const float mn = fmaxf(a.m[qt], mx), alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(a.m[qt] - mn);
+        a.m[qt] = mn, a.l[qt] *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < HD / 16; dt++) a.o[qt][dt] *= alpha;
+    }
+    return a.m[qt] == -INFINITY ? 0.f : a.m[qt];  // (no key yet: every weight is 0)
+}
 
 // Bits 0..3: which of keys key .. + 3 lie below n.
 __device__ inline uint32_t rows_below(int key, int n) { return (1u << max(0, min(n - key, 4))) - 1u; }
@@ -306,26 +350,21 @@ __device__ inline bool rows_unit(const RowsUnit<HD, F16, KT> &u, const RowsQ<HD,
         }
 #pragma unroll
         for (int t = 0; t < KT; t++) put(qt, kb[t] + 4 * kq, s[t][qt]);
-        mx = fmaf(max_xor32(max_xor16(mx)), q.p2e[qt], -7.f);
-        const float mn = fmaxf(a.m[qt], mx), m0 = mn == -INFINITY ? 0.f : mn;  // (no key yet: every weight is 0)
-        const float alpha = __builtin_amdgcn_exp2f(a.m[qt] - m0);
+        const float m0 = rows_reference(a, qt, max_xor32(max_xor16(mx)) * q.p2e[qt]);
         float sum = 0.f;
+        uint32_t hi[2 * KT], lo[2 * KT];
 #pragma unroll
         for (int t = 0; t < KT; t++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float p = __builtin_amdgcn_exp2f(fmaf(s[t][qt][i], q.p2e[qt], -m0));
-                sum += p;
-                const _Float16 h = (_Float16)p;
-                ph[qt][4 * t + i] = h;
-                pl[qt][4 * t + i] = (_Float16)(p - (float)h);
+            for (int i = 0; i < 2; i++) {
+                const float p0 = __builtin_amdgcn_exp2f(fmaf(s[t][qt][2 * i], q.p2e[qt], -m0));
+                const float p1 = __builtin_amdgcn_exp2f(fmaf(s[t][qt][2 * i + 1], q.p2e[qt], -m0));
+                sum += p0 + p1;
+                rows_split(p0, p1, hi[2 * t + i], lo[2 * t + i]);
             }
+        ph[qt] = Op::of(hi), pl[qt] = Op::of(lo);
         sum = add_xor32(add_xor16(sum));
-        a.m[qt] = mn, a.l[qt] = a.l[qt] * alpha + sum;
-        if (__builtin_amdgcn_ballot_w64(alpha != 1.0f)) {
-#pragma unroll
-            for (int dt = 0; dt < S::NDT; dt++) a.o[qt][dt] *= alpha;
-        }
+        a.l[qt] += sum;
     }
     RowsScale<HD, F16, KT> sc;
     if constexpr (!F16) {
@@ -420,10 +459,11 @@ __device__ inline void rows_combine(RowsLds<HD, NW> &L, const RowsSum<HD, NT> &a
             float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < NW; w++) {
-                const float x = L.m[w][r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(L.m[w][r] - M);
-                if (x == 0.f) continue;  // (a wave with no key of the row)
+                const float lw = L.l[w][r];
+                const float x = lw != lw ? lw : L.m[w][r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(L.m[w][r] - M);
+                if (x == 0.f) continue;  // (a wave with no key of the row; NaN scores have no maximum)
                 const float4 p = *(const float4 *)&L.o[w][r][d];
-                l = fmaf(x, L.l[w][r], l);
+                l = fmaf(x, lw, l);
                 o.x = fmaf(x, p.x, o.x), o.y = fmaf(x, p.y, o.y), o.z = fmaf(x, p.z, o.z), o.w = fmaf(x, p.w, o.w);
             }
             emit(16 * qt + r, d, o, M, l);
@@ -431,33 +471,75 @@ __device__ inline void rows_combine(RowsLds<HD, NW> &L, const RowsSum<HD, NT> &a
     }
 }
 
-// Slices of n keys: as many as asked for, of at least ROWS_MIN_KEYS keys each,
-// whole units; and how many of them hold keys.
+// Keys of each of n_split slices of n keys: at least ROWS_MIN_KEYS, and whole blocks of k_attn_tile
+// (a slice that ended inside one would count the zeros behind it).
 constexpr int ROWS_MIN_KEYS = 128;
 constexpr int ROWS_MAX_SPLIT = 64;
 __host__ __device__ inline int rows_chunk(int n, int n_split) {
     int c = (n + n_split - 1) / n_split;
     c = c < ROWS_MIN_KEYS ? ROWS_MIN_KEYS : c;
-    return (c + 31) / 32 * 32;
+    return (c + 63) / 64 * 64;
 }
 
 constexpr int ROWS_MAX_G = 16;  // query heads a KV head, where one row tile holds a query's
 
-// sum_s 2^(m_s - M) (O_s, l_s) over the first `used` slices of a row, in order:
-// 4 dims from d on.
-__device__ inline float4 rows_merge(const float *p, int used, int rec, int d, float &M, float &l) {
+// sum_s 2^(m_s - M) (O_s, l_s) over the first `used` slices of a row's partials p: HD / 4 x SG of a
+// workgroup's 256 threads a row, 4 dims a thread and every SG-th slice, eight of them
+// requested before the first is used (one at a time their latencies add up: 32 slices took 27 us, now
+// 3); the SG parts join in LDS in order. Every thread of the workgroup calls it; the result is the SG = 0 part's.
+constexpr int JOIN_SG = 4;
+struct RowsJoin {
+    __align__(16) float4 o[256];
+    float2 ml[256];
+};
+template <int HD, int SG>
+__device__ inline float4 rows_join(RowsJoin &J, const float *p, int used, float &M, float &l) {
+    constexpr int REC = HD + 4, L4 = HD / 4, AHEAD = 8;
+    const int tid = threadIdx.x, sg = tid / L4 % SG, d = 4 * (tid % L4);
     M = -INFINITY, l = 0.f;
-    for (int s = 0; s < used; s++) M = fmaxf(M, p[(int64_t)s * rec]);
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < used; s++) {
-        const float2 ml = *(const float2 *)(p + (int64_t)s * rec);
-        const float4 x = *(const float4 *)(p + (int64_t)s * rec + 4 + d);
-        const float w = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - M);
-        if (w == 0.f) continue;
-        l = fmaf(w, ml.y, l);
+    auto add = [&](float m, float pl, float4 x) {
+        const float mn = fmaxf(M, m);
+        if (l != l || pl != pl) {  // a row of NaN scores has no maximum
+            l = NAN, o = make_float4(NAN, NAN, NAN, NAN);
+            return;
+        }
+        if (mn == -INFINITY) return;
+        const float a = __builtin_amdgcn_exp2f(M - mn), w = __builtin_amdgcn_exp2f(m - mn);
+        M = mn;
+        if (a == 0.f) o = make_float4(0.f, 0.f, 0.f, 0.f), l = 0.f;  // (nothing yet: no 0 times an infinity)
+        else o.x *= a, o.y *= a, o.z *= a, o.w *= a, l *= a;
+        if (w == 0.f) return;
+        l = fmaf(w, pl, l);
         o.x = fmaf(w, x.x, o.x), o.y = fmaf(w, x.y, o.y), o.z = fmaf(w, x.z, o.z), o.w = fmaf(w, x.w, o.w);
+    };
+    for (int s0 = sg; s0 < used; s0 += AHEAD * SG) {
+        float2 ml[AHEAD];
+        float4 x[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+            const float *r = p + (int64_t)min(s0 + i * SG, used - 1) * REC;
+            ml[i] = *(const float2 *)r, x[i] = *(const float4 *)(r + 4 + d);
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++)
+            if (s0 + i * SG < used) add(ml[i].x, ml[i].y, x[i]);
+    }
+    if constexpr (SG > 1) {
+        __syncthreads();
+        J.o[tid] = o, J.ml[tid] = make_float2(M, l);
+        __syncthreads();
+        if (sg == 0) {
+#pragma unroll
+            for (int i = 1; i < SG; i++) add(J.ml[tid + i * L4].x, J.ml[tid + i * L4].y, J.o[tid + i * L4]);
+        }
     }
     return o;
+}
+// The row's output.
+__device__ inline float4 rows_over(float4 o, float l) {
+    const float inv = 1.0f / l;
+    return l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
 // f(head dimension, whether f16) with both as constants.

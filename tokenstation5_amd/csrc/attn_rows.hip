@@ -36,6 +36,21 @@ __device__ inline int rows_count(const RowsArgs &a, int b) {
 __device__ inline int rows_all(const RowsArgs &a, int n) { return a.mode == ROWS_ONE ? n : n + a.T; }
 __device__ inline int rows_reach(const RowsArgs &a, int n, int t) { return a.mode == ROWS_CAUSAL ? n + t + 1 : rows_all(a, n); }
 
+// The infinite and NaN values of keys first .. kend - 1 that token t's rows take, onto dims d .. + 3 of a row:
+// the products left them out there.
+template <int HD, bool F16>
+__device__ inline void rows_add_nonfinite(const RowsArgs &a, int b, int kvh, int t, int n, int first, int kend, int d,
+                                          float4 &o) {
+    const uint64_t own = a.mode == ROWS_TREE ? a.mask[(int64_t)b * a.T + t] & (~0ull >> (64 - a.T)) : 0;
+    const int reach = a.mode == ROWS_CAUSAL ? n + t + 1 : n;
+    for (int key = first; key < kend; key++) {
+        if (key >= reach && !(key >= n && key - n < 64 && (own >> (key - n) & 1))) continue;
+        const int64_t slot = ((int64_t)b * a.HKV + kvh) * a.n_ctx + key;
+        o.x += rows_nonfinite<HD, F16>(a.kv, slot, d), o.y += rows_nonfinite<HD, F16>(a.kv, slot, d + 1);
+        o.z += rows_nonfinite<HD, F16>(a.kv, slot, d + 2), o.w += rows_nonfinite<HD, F16>(a.kv, slot, d + 3);
+    }
+}
+
 // grid (n_split, HKV * row blocks of 16 NT, B): one slice of the keys for 16 NT rows,
 // row r = G t + j being head j of token t. The waves take the slice's units in turn.
 template <int HD, bool F16, int KT, int NT, int NW, bool ONE>
@@ -65,9 +80,10 @@ __global__ __launch_bounds__(64 * NW) void k_attn_rows(RowsArgs a) {
     rows_load<HD, F16, KT>(nxt, kv, kb, rl, kq);
 
     RowsQ<HD, NT> q;
-    rows_query<HD, NT>(q, a.scale, kq, [&](int qt) -> const float * {
-        const int r = r0 + 16 * qt + rl;
-        return r < R ? a.q + (((int64_t)b * a.T + r / G) * a.H + kvh * G + r % G) * HD : nullptr;
+    rows_query<HD, NT>(q, a.scale, kq, [&](int qt, bool &ok) -> const float * {
+        const int r = min(r0 + 16 * qt + rl, R - 1);
+        ok = r0 + 16 * qt + rl < R;
+        return a.q + (((int64_t)b * a.T + r / G) * a.H + kvh * G + r % G) * HD;
     });
     int seen[NT];       // keys before it are the row's
     uint64_t bits[NT];  // and then those of n + its set bits
@@ -97,24 +113,38 @@ __global__ __launch_bounds__(64 * NW) void k_attn_rows(RowsArgs a) {
     rows_clear<HD, NT>(sum);
     if (!ONE) __syncthreads();  // the flag is set
     const int64_t row0 = ((int64_t)b * a.HKV + kvh) * R + r0;
-    for (int u = wave; u < units; u += NW) {
-        const RowsUnit<HD, F16, KT> cur = nxt;
-        int kn[KT];
-        at(u, kb);
-        at(u + NW, kn);
-        rows_load<HD, F16, KT>(nxt, kv, kn, rl, kq);  // (past the slice: zeros, no memory access)
-        if constexpr (ONE) {
-            auto put = [&](int, int key, const float (&s)[4]) {
-                if (rl < rows && key < kend)
-                    *(float4 *)(a.scores + (row0 + rl) * a.stride + key) =
-                        make_float4(s[0] * q.p2e[0], s[1] * q.p2e[0], s[2] * q.p2e[0], s[3] * q.p2e[0]);
-            };
-            if (kb[0] + S::UNIT <= kend)
-                rows_unit<HD, F16, KT, NT, false, false>(cur, q, sum, kb, kq, [](int, int) { return 15u; }, put);
-            else
-                rows_unit<HD, F16, KT, NT, true, false>(cur, q, sum, kb, kq, [&](int, int key) { return rows_below(key, kend); }, put);
-        } else {
-            auto put = [](int, int, const float (&)[4]) {};
+    if constexpr (ONE) {
+        // Two units ahead: an iteration's loads go out as soon as their registers are
+        // free, and it ends nowhere else, so that a wait for one unit leaves the next in flight.
+        auto put = [&](int, int key, const float (&s)[4]) {
+            if (rl < rows && key < kend)
+                *(float4 *)(a.scores + (row0 + rl) * a.stride + key) =
+                    make_float4(s[0] * q.p2e[0], s[1] * q.p2e[0], s[2] * q.p2e[0], s[3] * q.p2e[0]);
+        };
+        auto seen4 = [&](int, int key) { return rows_below(key, kend); };
+        RowsUnit<HD, F16, KT> far;
+        at(wave + NW, kb);
+        rows_load<HD, F16, KT>(far, kv, kb, rl, kq);
+        for (int u = wave; u < units; u += 2 * NW) {
+            RowsUnit<HD, F16, KT> cur = nxt;
+            at(u + 2 * NW, kb);
+            rows_load<HD, F16, KT>(nxt, kv, kb, rl, kq);  // (past the slice: zeros, no memory access)
+            at(u, kb);
+            rows_unit<HD, F16, KT, NT, true, false>(cur, q, sum, kb, kq, seen4, put);
+            cur = far;
+            at(u + 3 * NW, kb);
+            rows_load<HD, F16, KT>(far, kv, kb, rl, kq);
+            at(u + NW, kb);  // (past the slice: no key of it is taken)
+            rows_unit<HD, F16, KT, NT, true, false>(cur, q, sum, kb, kq, seen4, put);
+        }
+    } else {
+        auto put = [](int, int, const float (&)[4]) {};
+        for (int u = wave; u < units; u += NW) {
+            const RowsUnit<HD, F16, KT> cur = nxt;
+            int kn[KT];
+            at(u, kb);
+            at(u + NW, kn);
+            rows_load<HD, F16, KT>(nxt, kv, kn, rl, kq);
             if (kb[0] + S::UNIT <= full)
                 rows_unit<HD, F16, KT, NT, false, false>(cur, q, sum, kb, kq, [](int, int) { return 15u; }, put);
             else if (rows_unit<HD, F16, KT, NT, true, true>(
@@ -126,21 +156,10 @@ __global__ __launch_bounds__(64 * NW) void k_attn_rows(RowsArgs a) {
     }
     rows_combine<HD, NT, NW>(L, sum, rows, wave, rl, kq, [&](int r, int d, float4 o, float m, float l) {
         const int t = (r0 + r) / G, j = (r0 + r) % G;
-        if (!ONE && nonfinite) {  // those of the keys that the row takes, of the units that are not every row's
-            const uint64_t own = a.mode == ROWS_TREE ? a.mask[(int64_t)b * a.T + t] & (~0ull >> (64 - a.T)) : 0;
-            const int reach = a.mode == ROWS_CAUSAL ? n + t + 1 : n;
-            const int first = kbeg + max(full - kbeg, 0) / S::UNIT * S::UNIT;
-            for (int key = first; key < kend; key++) {
-                if (key >= reach && !(key >= n && key - n < 64 && (own >> (key - n) & 1))) continue;
-                const int64_t slot = ((int64_t)b * a.HKV + kvh) * a.n_ctx + key;
-                o.x += rows_nonfinite<HD, F16>(a.kv, slot, d), o.y += rows_nonfinite<HD, F16>(a.kv, slot, d + 1);
-                o.z += rows_nonfinite<HD, F16>(a.kv, slot, d + 2), o.w += rows_nonfinite<HD, F16>(a.kv, slot, d + 3);
-            }
-        }
+        if (!ONE && nonfinite)
+            rows_add_nonfinite<HD, F16>(a, b, kvh, t, n, kbeg + max(full - kbeg, 0) / S::UNIT * S::UNIT, kend, d, o);
         if (!ONE && a.n_split == 1) {
-            const float inv = 1.0f / l;
-            *(float4 *)(a.out + (((int64_t)b * a.T + t) * a.H + kvh * G + j) * HD + d) =
-                l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+            *(float4 *)(a.out + (((int64_t)b * a.T + t) * a.H + kvh * G + j) * HD + d) = rows_over(o, l);
             if (a.lse && d == 0) a.lse[row0 + r] = l == 0.f ? INFINITY : m + __log2f(l);
             return;
         }
@@ -150,52 +169,320 @@ __global__ __launch_bounds__(64 * NW) void k_attn_rows(RowsArgs a) {
     });
 }
 
-// A thread per 4 outputs.
-template <int HD>
+// ---- many rows: the keys converted once for a workgroup --------------------------------------------------
+// 64 NT rows, each of four waves 16 NT of them, over one slice of the keys in blocks of 16 NKT.
+// The waves read a block's K and V while they compute the one before, convert a share of it each into the MFMA
+// operands' own layout in LDS (16 bytes a lane, so that no read or write meets a bank twice:
+// K [tile][chunk][lane], V hi and lo [tile pair][dim tile][lane]), and take all of it against
+// their own rows. Each key is converted once for 64 NT rows instead of once for 16 NT, and two
+// workgroups a CU fill each other's waits: k_attn_rows, one wave a SIMD, took 191 us where this takes
+// TILE_US (4 trees of 64 tokens, 32/8 heads, up to 8192 keys). What bounds it: the matrix cores and
+// the vector ALU in turn.
+template <int HD, bool F16>
+struct TileShape {
+    static constexpr int NT = HD == 256 ? 1 : 2, NKT = HD == 256 ? 2 : 4, KEYS = 16 * NKT, ROWS = 64 * NT;
+    static constexpr int WPT = 4 / NKT;  // waves that share a key tile's conversion
+    static constexpr int NC = HD / 32, NDT = HD / 16, CW = NC / WPT, DW = NDT / WPT;  // chunks and dims of a lane's share
+    static constexpr int VB = F16 ? 2 : 1, KW = F16 ? 4 : 2, VW = DW * VB / 4;
+};
+template <int HD, bool F16>
+struct TileLds {
+    using S = TileShape<HD, F16>;
+    uint4 k[S::NKT][S::NC][64];
+    uint2 vh[S::NKT / 2][S::NDT][64][2];
+    uint2 vl[F16 ? 1 : S::NKT / 2][F16 ? 1 : S::NDT][64][2];
+    __align__(16) float ks[F16 ? 1 : S::NKT][F16 ? 1 : S::NC][16];
+    int nonfinite;
+};
+
+template <int HD, bool F16>
+__global__ __launch_bounds__(256, 2) void k_attn_tile(RowsArgs a) {
+    using S = TileShape<HD, F16>;
+    constexpr int NT = S::NT, NKT = S::NKT, NC = S::NC, NDT = S::NDT;
+    __shared__ TileLds<HD, F16> L;
+    if (threadIdx.x == 0) L.nonfinite = 0;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int rl = lane & 15, kq = lane >> 4;
+    const int G = a.H / a.HKV, R = a.T * G, nrb = (R + S::ROWS - 1) / S::ROWS;
+    const int split = blockIdx.x, kvh = blockIdx.y / nrb, r0 = blockIdx.y % nrb * S::ROWS, b = blockIdx.z;
+    const int n = rows_count(a, b), chunk = rows_chunk(rows_all(a, n), a.n_split);
+    const int kbeg = split * chunk, kend = min(kbeg + chunk, rows_reach(a, n, (min(R, r0 + S::ROWS) - 1) / G));
+    if (kbeg >= kend) return;  // the merge reads no partial of this slice
+    const int full = a.mode == ROWS_CAUSAL ? n + r0 / G + 1 : n;  // keys before it are every row's
+    const RowsKv kv = rows_kv<HD, F16>(a.kv, ((int64_t)b * a.HKV + kvh) * a.n_ctx, kend);
+    // The lane's share of a block: tile wave / WPT; K of key rl, chunks c0 ..; V of keys 4 kq .. + 3, dims
+    // NDT rl + d0 ..; the K scale of key rl, chunk c0 + kq.
+    const int tile = wave / S::WPT, c0 = wave % S::WPT * S::CW, d0 = wave % S::WPT * S::DW;
+    uint32_t rk[S::CW][S::KW], rv[4][S::VW];
+    uint16_t rks = 0, rvs[4];
+    auto load = [&](int kb) {
+        const int key = kb + 16 * tile;
+#pragma unroll
+        for (int c = 0; c < S::CW; c++)
+            rows_words<S::KW>(kv.k, ((uint32_t)(key + rl) * HD + 32 * (c0 + c) + 8 * kq) * S::VB, rk[c]);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            rows_words<S::VW>(kv.v, ((uint32_t)(key + 4 * kq + i) * HD + NDT * rl + d0) * S::VB, rv[i]);
+            if constexpr (!F16)
+                rvs[i] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(
+                    kv.vs, ((uint32_t)(key + 4 * kq + i) * NC + (NDT * rl + d0) / 32) * 2, 0, 0);
+        }
+        if constexpr (!F16)
+            rks = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(kv.ks, ((uint32_t)(key + rl) * NC + c0 + kq % S::CW) * 2, 0, 0);
+    };
+    auto convert = [&](auto m) {
+        constexpr bool masked = decltype(m)::value;
+#pragma unroll
+        for (int c = 0; c < S::CW; c++) L.k[tile][c0 + c][lane] = __builtin_bit_cast(uint4, rows_values<S::KW>(rk[c]));
+        if constexpr (!F16) {
+            if (kq < S::CW) L.ks[tile][c0 + kq][rl] = h2f(rks);
+        }
+        constexpr int PW = F16 ? 2 : 4;
+        ar_h2 sc[2] = {};
+        if constexpr (!F16) {
+            sc[0] = __builtin_bit_cast(ar_h2, (uint32_t)rvs[0] | (uint32_t)rvs[1] << 16);
+            sc[1] = __builtin_bit_cast(ar_h2, (uint32_t)rvs[2] | (uint32_t)rvs[3] << 16);
+        }
+        uint32_t any = 0;
+#pragma unroll
+        for (int d = 0; d < S::DW; d++) {
+            uint32_t hi[2], lo[2];
+#pragma unroll
+            for (int p = 0; p < 2; p++) {
+                rows_value_pair<F16>(rv[2 * p][d / PW], rv[2 * p + 1][d / PW], d % PW, sc[p], hi[p], lo[p]);
+                if constexpr (masked) {  // infinite and NaN values out: they are added where the rows are written
+                    uint32_t keep = 0;
+                    if ((hi[p] & 0x7c00u) != 0x7c00u) keep |= 0xffffu;
+                    if ((hi[p] & 0x7c000000u) != 0x7c000000u) keep |= 0xffff0000u;
+                    any |= ~keep, hi[p] &= keep, lo[p] &= keep;
+                }
+            }
+            L.vh[tile / 2][d0 + d][lane][tile & 1] = make_uint2(hi[0], hi[1]);
+            if constexpr (!F16) L.vl[tile / 2][d0 + d][lane][tile & 1] = make_uint2(lo[0], lo[1]);
+        }
+        if (masked && __builtin_amdgcn_ballot_w64(any != 0)) L.nonfinite = 1;
+    };
+    load(kbeg);
+
+    const int w0 = r0 + 16 * NT * wave;  // the wave's first row
+    RowsQ<HD, NT> q;
+    rows_query<HD, NT>(q, a.scale, kq, [&](int qt, bool &ok) -> const float * {
+        const int r = min(w0 + 16 * qt + rl, R - 1);
+        ok = w0 + 16 * qt + rl < R;
+        return a.q + (((int64_t)b * a.T + r / G) * a.H + kvh * G + r % G) * HD;
+    });
+    int seen[NT];       // keys before it are the row's
+    uint64_t bits[NT];  // and then those of n + its set bits
+#pragma unroll
+    for (int qt = 0; qt < NT; qt++) {
+        const int r = w0 + 16 * qt + rl;
+        seen[qt] = r >= R ? 0 : a.mode == ROWS_CAUSAL ? n + r / G + 1 : n;
+        bits[qt] = 0;
+        if (a.mode == ROWS_TREE) {
+            const uint64_t m = a.mask[(int64_t)b * a.T + min(r, R - 1) / G] & (~0ull >> (64 - a.T));
+            bits[qt] = r < R ? m : 0;
+        }
+    }
+    if (a.planes && split == 0) {
+        const int tiles = (R + 15) / 16;
+#pragma unroll
+        for (int qt = 0; qt < NT; qt++) {
+            const int row_tile = w0 / 16 + qt;
+            if (row_tile >= tiles) break;
+            uint4 *p = a.planes + ((int64_t)kvh * tiles + row_tile) * NC * 2 * 64 + lane;
+#pragma unroll
+            for (int c = 0; c < NC; c++) {
+                p[(2 * c) * 64] = __builtin_bit_cast(uint4, q.h[qt][c]);
+                p[(2 * c + 1) * 64] = __builtin_bit_cast(uint4, q.l[qt][c]);
+            }
+            if (kq == 0) a.p2e[((int64_t)kvh * tiles + row_tile) * 16 + rl] = q.p2e[qt];
+        }
+    }
+    RowsSum<HD, NT> sum;
+    rows_clear<HD, NT>(sum);
+    const int wfull = a.mode == ROWS_CAUSAL ? n + w0 / G + 1 : n;  // every row of the wave's
+    const int wreach = w0 < R ? rows_reach(a, n, (min(R, w0 + 16 * NT) - 1) / G) : 0;
+
+    for (int kb = kbeg; kb < kend; kb += S::KEYS) {
+        __syncthreads();  // every wave is done with the last block
+        if (kb + S::KEYS > full) convert(std::true_type{});
+        else convert(std::false_type{});
+        load(kb + S::KEYS);  // (past the slice: zeros, no memory access)
+        __syncthreads();
+        if (kb >= wreach) continue;
+        float s[NKT][NT][4];
+#pragma unroll
+        for (int t = 0; t < NKT; t++) {
+            if constexpr (F16) {
+                ar_f4 D[NT];
+#pragma unroll
+                for (int qt = 0; qt < NT; qt++) D[qt] = ar_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < NC; c++) {
+                    const ar_h8 ka = __builtin_bit_cast(ar_h8, L.k[t][c][lane]);
+#pragma unroll
+                    for (int qt = 0; qt < NT; qt++) {
+                        D[qt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q.h[qt][c], D[qt], 0, 0, 0);
+                        D[qt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q.l[qt][c], D[qt], 0, 0, 0);
+                    }
+                }
+#pragma unroll
+                for (int qt = 0; qt < NT; qt++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) s[t][qt][i] = D[qt][i];
+            } else {
+#pragma unroll
+                for (int c = 0; c < NC; c++) {
+                    const ar_h8 ka = __builtin_bit_cast(ar_h8, L.k[t][c][lane]);
+                    const float4 k4 = *(const float4 *)&L.ks[t][c][4 * kq];
+                    const float ks[4] = {k4.x, k4.y, k4.z, k4.w};
+#pragma unroll
+                    for (int qt = 0; qt < NT; qt++) {
+                        ar_f4 D = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q.h[qt][c], ar_f4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                        D = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q.l[qt][c], D, 0, 0, 0);
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            s[t][qt][i] = c == 0 ? ks[i] * D[i] : fmaf(ks[i], D[i], s[t][qt][i]);
+                    }
+                }
+            }
+        }
+        if (kb + S::KEYS > wfull) {
+#pragma unroll
+            for (int t = 0; t < NKT; t++)
+#pragma unroll
+                for (int qt = 0; qt < NT; qt++) {
+                    const int key = kb + 16 * t + 4 * kq;
+                    const uint32_t take = rows_below(key, seen[qt]) | rows_window(bits[qt], key - n);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) s[t][qt][i] = take & 1u << i ? s[t][qt][i] : -INFINITY;
+                }
+        }
+        uint32_t ph[NT][2 * NKT], pl[NT][2 * NKT];
+#pragma unroll
+        for (int qt = 0; qt < NT; qt++) {
+            float mx = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < NKT; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) mx = fmaxf(mx, s[t][qt][i]);
+            const float m0 = rows_reference(sum, qt, max_xor32(max_xor16(mx)) * q.p2e[qt]);
+            float l = 0.f;
+#pragma unroll
+            for (int t = 0; t < NKT; t++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const float p0 = __builtin_amdgcn_exp2f(fmaf(s[t][qt][2 * i], q.p2e[qt], -m0));
+                    const float p1 = __builtin_amdgcn_exp2f(fmaf(s[t][qt][2 * i + 1], q.p2e[qt], -m0));
+                    l += p0 + p1;
+                    rows_split(p0, p1, ph[qt][2 * t + i], pl[qt][2 * t + i]);
+                }
+            l = add_xor32(add_xor16(l));
+            sum.l[qt] += l;
+        }
+#pragma unroll
+        for (int dt = 0; dt < NDT; dt++)
+#pragma unroll
+            for (int k2 = 0; k2 < NKT / 2; k2++) {
+                const ar_h8 vh = *(const ar_h8 *)&L.vh[k2][dt][lane];
+                ar_h8 vl;
+                if constexpr (!F16) vl = *(const ar_h8 *)&L.vl[k2][dt][lane];
+#pragma unroll
+                for (int qt = 0; qt < NT; qt++) {
+                    const ar_h8 h = __builtin_bit_cast(ar_h8, u32x4{ph[qt][4 * k2], ph[qt][4 * k2 + 1], ph[qt][4 * k2 + 2], ph[qt][4 * k2 + 3]});
+                    const ar_h8 l = __builtin_bit_cast(ar_h8, u32x4{pl[qt][4 * k2], pl[qt][4 * k2 + 1], pl[qt][4 * k2 + 2], pl[qt][4 * k2 + 3]});
+                    sum.o[qt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, h, sum.o[qt][dt], 0, 0, 0);
+                    if constexpr (!F16) sum.o[qt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, h, sum.o[qt][dt], 0, 0, 0);
+                    sum.o[qt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, l, sum.o[qt][dt], 0, 0, 0);
+                }
+            }
+    }
+
+    const bool extra = L.nonfinite;  // (set before a barrier that every wave has passed)
+#pragma unroll
+    for (int qt = 0; qt < NT; qt++) {
+        const int r = w0 + 16 * qt + rl, t = r / G;
+        if (r >= R) continue;
+        const int64_t row = ((int64_t)b * a.HKV + kvh) * R + r;
+        float *p = a.n_split == 1 ? a.out + (((int64_t)b * a.T + t) * a.H + kvh * G + r % G) * HD
+                                  : a.part + (row * a.n_split + split) * (HD + 4) + 4;
+        if (kq == 0) {
+            if (a.n_split > 1) *(float4 *)(p - 4) = make_float4(sum.m[qt], sum.l[qt], 0.f, 0.f);
+            else if (a.lse) a.lse[row] = sum.l[qt] == 0.f ? INFINITY : sum.m[qt] + __log2f(sum.l[qt]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int d = 0; d < NDT; d += 4) {
+                const float4 o = make_float4(sum.o[qt][d][i], sum.o[qt][d + 1][i], sum.o[qt][d + 2][i], sum.o[qt][d + 3][i]);
+                *(float4 *)(p + NDT * (4 * kq + i) + d) = a.n_split == 1 ? rows_over(o, sum.l[qt]) : o;
+            }
+        if (extra) {  // (onto a quotient as onto its numerator)
+#pragma unroll 1
+            for (int dim = NDT * 4 * kq; dim < NDT * 4 * (kq + 1); dim += 4) {
+                float4 o = *(const float4 *)(p + dim);
+                rows_add_nonfinite<HD, F16>(a, b, kvh, t, n, kbeg + max(full - kbeg, 0) / S::KEYS * S::KEYS, kend, dim, o);
+                *(float4 *)(p + dim) = o;
+            }
+        }
+    }
+}
+
+// The slices' join, 256 / (HD / 4 x SG) rows a workgroup.
+template <int HD, int SG>
 __global__ __launch_bounds__(256) void k_rows_merge(RowsArgs a, int64_t rows) {
-    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x, row = e / (HD / 4);
-    if (row >= rows) return;
-    const int d = 4 * (int)(e % (HD / 4)), G = a.H / a.HKV, R = a.T * G;
-    const int b = (int)(row / ((int64_t)a.HKV * R)), kvh = (int)(row / R % a.HKV), r = (int)(row % R), t = r / G;
+    constexpr int TPR = HD / 4 * SG;  // threads a row
+    __shared__ RowsJoin J;
+    const int64_t row = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR, at = min(row, rows - 1);
+    const int d = 4 * ((int)threadIdx.x % (HD / 4)), G = a.H / a.HKV, R = a.T * G;
+    const int b = (int)(at / ((int64_t)a.HKV * R)), kvh = (int)(at / R % a.HKV), r = (int)(at % R), t = r / G;
     const int n = rows_count(a, b), chunk = rows_chunk(rows_all(a, n), a.n_split);
     const int used = (rows_reach(a, n, t) + chunk - 1) / chunk;
     float M, l;
-    const float4 o = rows_merge(a.part + row * a.n_split * (HD + 4), used, HD + 4, d, M, l);
-    const float inv = 1.0f / l;
-    *(float4 *)(a.out + (((int64_t)b * a.T + t) * a.H + kvh * G + r % G) * HD + d) =
-        l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    const float4 o = rows_join<HD, SG>(J, a.part + at * a.n_split * (HD + 4), used, M, l);
+    if (row >= rows || threadIdx.x % TPR >= HD / 4) return;
+    *(float4 *)(a.out + (((int64_t)b * a.T + t) * a.H + kvh * G + r % G) * HD + d) = rows_over(o, l);
     if (a.lse && d == 0) a.lse[row] = l == 0.f ? INFINITY : M + __log2f(l);
 }
 
-// One query a cache: the merge (the workgroups of the first keys) and acc_out = acc +
-// the group's weights 2^(score - lse). grid (key blocks of 1024, HKV, B).
+// One query a cache: the join (the first workgroup of a KV head) and acc_out = acc + the group's
+// weights 2^(score - lse). grid (1 + key blocks of 1024, HKV, B).
 template <int HD>
 __global__ __launch_bounds__(256) void k_one_weights(RowsArgs a, const float *acc, float *acc_out) {
+    __shared__ RowsJoin J;
     __shared__ float lse[ROWS_MAX_G];
+    constexpr int TPR = HD / 4 * JOIN_SG;
     const int kvh = blockIdx.y, b = blockIdx.z, G = a.H / a.HKV, tid = threadIdx.x;
     const int n = rows_count(a, b), chunk = rows_chunk(n, a.n_split), used = (n + chunk - 1) / chunk;
     const int64_t head = (int64_t)b * a.HKV + kvh, row0 = head * G;
-    const int k0 = blockIdx.x * 1024 + 4 * tid;
     if (blockIdx.x == 0) {
-        for (int e = tid; e < G * (HD / 4); e += 256) {
-            const int g = e / (HD / 4), d = 4 * (e % (HD / 4));
+        for (int g0 = 0; g0 < G; g0 += 256 / TPR) {
+            const int g = g0 + tid / TPR;
             float M, l;
-            const float4 o = rows_merge(a.part + (row0 + g) * a.n_split * (HD + 4), used, HD + 4, d, M, l);
-            const float inv = 1.0f / l;
-            *(float4 *)(a.out + (((int64_t)b * a.H) + kvh * G + g) * HD + d) =
-                l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+            const float4 o = rows_join<HD, JOIN_SG>(J, a.part + (row0 + min(g, G - 1)) * a.n_split * (HD + 4), used, M, l);
+            if (g < G && tid % TPR < HD / 4)
+                *(float4 *)(a.out + (row0 + g) * HD + 4 * (tid % TPR)) = rows_over(o, l);
         }
+        return;
     }
-    if (blockIdx.x * 1024 >= n) return;
-    if (tid < G) {
-        const float *p = a.part + (row0 + tid) * a.n_split * (HD + 4);
-        float M = -INFINITY, l = 0.f;
-        for (int s = 0; s < used; s++) M = fmaxf(M, p[(int64_t)s * (HD + 4)]);
-        for (int s = 0; s < used; s++) {
-            const float2 ml = *(const float2 *)(p + (int64_t)s * (HD + 4));
-            if (ml.x != -INFINITY) l = fmaf(__builtin_amdgcn_exp2f(ml.x - M), ml.y, l);
+    const int k0 = ((int)blockIdx.x - 1) * 1024 + 4 * tid;
+    if (k0 - 4 * tid >= n) return;
+    {  // 16 lanes a head over the slices' m and l
+        const int g = tid / 16, s0 = tid % 16;
+        float m[ROWS_MAX_SPLIT / 16], l[ROWS_MAX_SPLIT / 16], M = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < ROWS_MAX_SPLIT / 16; i++) {
+            const int s = s0 + 16 * i;
+            const bool in = g < G && s < used;
+            const float2 ml = *(const float2 *)(a.part + ((row0 + (in ? g : 0)) * a.n_split + (in ? s : 0)) * (HD + 4));
+            m[i] = in ? ml.x : -INFINITY, l[i] = in ? ml.y : 0.f, M = fmaxf(M, m[i]);
         }
-        lse[tid] = M + __log2f(l);
+        M = row_max_dpp(M);
+#pragma unroll
+        for (int i = 0; i < ROWS_MAX_SPLIT / 16; i++)
+            if (m[i] != -INFINITY) sum = fmaf(__builtin_amdgcn_exp2f(m[i] - M), l[i], sum);
+        sum = row_sum_dpp(sum);
+        if (s0 == 0) lse[g] = M + __log2f(sum);
     }
     __syncthreads();
     float w[4] = {0.f, 0.f, 0.f, 0.f};
@@ -296,10 +583,13 @@ __global__ __launch_bounds__(256) void k_prompt_weights(RowsArgs a, const float 
 
 // ---- host ----------------------------------------------------------------------------------------
 
-// Row tiles of a workgroup: they share each key's loads and conversion, as many as the
-// registers hold (the rows' planes and outputs take HD / 2 of them a tile).
-static int rows_tiles(int R, int HD) { return HD == 256 || R <= 16 ? 1 : HD == 128 || R <= 32 ? 2 : 4; }
-static int rows_blocks(int R, int HD) { return (R + 16 * rows_tiles(R, HD) - 1) / (16 * rows_tiles(R, HD)); }
+// Rows a KV head has of a sequence's tokens go to k_attn_rows, whose waves split the keys, while
+// one or two row tiles hold them, and past that to k_attn_tile, whose waves split the rows.
+static bool rows_tile(int R, int HD) { return R > (HD == 256 ? 16 : 32); }
+static int rows_blocks(int R, int HD) {
+    const int per = rows_tile(R, HD) ? (HD == 256 ? 64 : 128) : HD == 256 || R <= 16 ? 16 : 32;
+    return (R + per - 1) / per;
+}
 // Tiles of keys a unit.
 constexpr int rows_kt(int HD, int NT) { return HD == 256 || (HD == 128 && NT == 1) ? 1 : 2; }
 static int rows_splits(int items, int keys, int slots) {
@@ -316,28 +606,28 @@ static hipError_t rows_launch(const RowsArgs &a, int B, bool one, hipStream_t s)
     const int R = a.T * (a.H / a.HKV);
     const dim3 grid(a.n_split, a.HKV * rows_blocks(R, HD), B);
     constexpr int NW = HD == 256 ? 4 : 8, K1 = rows_kt(HD, 1), K2 = rows_kt(HD, 2);
-    const int tiles = rows_tiles(R, HD);
     if (one) {
         hipLaunchKernelGGL((k_attn_rows<HD, F16, K1, 1, NW, true>), grid, dim3(64 * NW), 0, s, a);
-    } else if (tiles == 1) {
+    } else if (rows_tile(R, HD)) {
+        hipLaunchKernelGGL((k_attn_tile<HD, F16>), grid, dim3(256), 0, s, a);
+    } else if (HD == 256 || R <= 16) {
         hipLaunchKernelGGL((k_attn_rows<HD, F16, K1, 1, NW, false>), grid, dim3(64 * NW), 0, s, a);
     } else if constexpr (HD <= 128) {
-        if (tiles == 2) {
-            hipLaunchKernelGGL((k_attn_rows<HD, F16, K2, 2, 4, false>), grid, dim3(256), 0, s, a);
-        } else if constexpr (HD == 64) {
-            hipLaunchKernelGGL((k_attn_rows<HD, F16, K2, 4, 4, false>), grid, dim3(256), 0, s, a);
-        }
+        hipLaunchKernelGGL((k_attn_rows<HD, F16, K2, 2, 4, false>), grid, dim3(256), 0, s, a);
     }
     return hipGetLastError();
 }
 template <int HD>
 static hipError_t rows_launch_merge(const RowsArgs &a, int B, hipStream_t s) {
     const int64_t rows = (int64_t)B * a.H * a.T;
-    hipLaunchKernelGGL(k_rows_merge<HD>, dim3((unsigned)((rows * (HD / 4) + 255) / 256)), dim3(256), 0, s, a, rows);
+    const auto grid = [&](int tpr) { return dim3((unsigned)((rows + 256 / tpr - 1) / (256 / tpr))); };
+    if (a.n_split <= 8) hipLaunchKernelGGL((k_rows_merge<HD, 1>), grid(HD / 4), dim3(256), 0, s, a, rows);
+    else hipLaunchKernelGGL((k_rows_merge<HD, JOIN_SG>), grid(HD / 4 * JOIN_SG), dim3(256), 0, s, a, rows);
     return hipGetLastError();
 }
 static int tree_splits(int B, int T, int H, int HKV, int HD, int n_ctx, int n_cu) {
-    return rows_splits(B * HKV * rows_blocks(T * (H / HKV), HD), n_ctx, n_cu);
+    const int R = T * (H / HKV);
+    return rows_splits(B * HKV * rows_blocks(R, HD), n_ctx, rows_tile(R, HD) ? 2 * n_cu : n_cu);
 }
 size_t attn_tree_scratch_bytes(int B, int T, int H, int HKV, int HD, int n_ctx, int n_cu) {
     const int ns = tree_splits(B, T, H, HKV, HD, n_ctx, n_cu);
@@ -373,7 +663,8 @@ hipError_t launch_attn_one_weights(const float *q, int B, int H, int HKV, int HD
         constexpr int D = decltype(hd)::value;
         const hipError_t e = rows_launch<D, decltype(f16)::value>(a, B, true, s);
         if (e != hipSuccess) return e;
-        hipLaunchKernelGGL(k_one_weights<D>, dim3((n_ctx + 1023) / 1024, HKV, B), dim3(256), 0, s, a, acc, acc_out);
+        hipLaunchKernelGGL(k_one_weights<D>, dim3(1 + (n_ctx + 1023) / 1024, HKV, B), dim3(256), 0, s, a, acc,
+                           acc_out);
         return hipGetLastError();
     });
 }

@@ -101,42 +101,74 @@ __device__ inline int sparse_count(const SparseArgs &a, int b) {
     return max(0, min(a.per_batch ? a.n_keys[b] : a.n_keys[0] + b + 1, a.n_ctx));
 }
 
-// HD / 8 lanes a block, 8 dims each. grid (ceil(n_blocks / SCORE_BLOCKS), HKV, B).
-constexpr int SCORE_BLOCKS = 64;
+template <int CTRL>
+__device__ inline double dpp_f64(double x) {
+    const uint64_t u = (uint64_t)__double_as_longlong(x);
+    const uint32_t l = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xF, 0xF, true);
+    const uint32_t h = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, true);
+    return __longlong_as_double((long long)((uint64_t)h << 32 | l));
+}
+
+// HD / 8 lanes a block, 8 dims and four blocks a lane; a head's four sums over the lanes go together:
+// two exchanges within a quad leave each of its lanes the quad's sum of one block, and only that goes
+// on to the other quads. grid (ceil(n_blocks / blocks a workgroup), HKV, B).
+template <int HD>
+constexpr int score_blocks() { return 4 * 4 * 64 / (HD / 8); }
 template <int HD>
 __global__ __launch_bounds__(256) void k_block_scores(SparseArgs a) {
     constexpr int LPB = HD / 8, BPW = 64 / LPB;
-    __shared__ __align__(16) double q[ROWS_MAX_G][HD];
+    __shared__ __align__(16) float q[ROWS_MAX_G][HD];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, kvh = blockIdx.y, b = blockIdx.z;
     const int n = sparse_count(a, b), nb = (n + a.block - 1) / a.block, G = a.H / a.HKV;
-    const int first = blockIdx.x * SCORE_BLOCKS;
+    const int first = blockIdx.x * score_blocks<HD>();
     if (first >= nb - 1 || nb <= a.n_pick) return;  // the last block is read in any case, and so are all that fit
-    for (int e = threadIdx.x; e < G * HD; e += 256) q[e / HD][e % HD] = (double)a.q[((int64_t)b * a.H + kvh * G) * HD + e];
-    __syncthreads();
+    for (int e = threadIdx.x; e < G * HD; e += 256) q[e / HD][e % HD] = a.q[((int64_t)b * a.H + kvh * G) * HD + e];
     const int64_t head = (int64_t)(a.per_batch ? b : 0) * a.HKV + kvh;
-    const int d0 = lane % LPB * 8;
-    for (int blk = first + wave * BPW + lane / LPB; blk < first + SCORE_BLOCKS; blk += 4 * BPW) {
-        double best = -INFINITY;
-        const int at = min(blk, nb - 1);
-        const _Float16 *p = a.bounds + (head * a.n_blocks + at) * 2 * HD + d0;
-        const ar_h8 lo = *(const ar_h8 *)p, hi = *(const ar_h8 *)(p + HD);
-        for (int g = 0; g < G; g++) {
-            double s = 0;
+    const int d0 = lane % LPB * 8, blk0 = first + wave * 4 * BPW + lane / LPB;
+    u32x4 lo[4], hi[4];
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const double x = q[g][d0 + j];
-                s = fma(x, (double)(float)(x >= 0 ? hi[j] : lo[j]), s);
-            }
-#pragma unroll
-            for (int o = LPB / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-            if (!(s <= best)) best = s != s ? INFINITY : s;  // (NaN ranks first)
-        }
-        if (blk < nb && lane % LPB == 0) a.scores[((int64_t)b * a.HKV + kvh) * a.n_blocks + blk] = best;
+    for (int p = 0; p < 4; p++) {
+        const _Float16 *at = a.bounds + (head * a.n_blocks + min(blk0 + p * BPW, nb - 1)) * 2 * HD + d0;
+        lo[p] = *(const u32x4 *)at, hi[p] = *(const u32x4 *)(at + HD);
     }
+    __syncthreads();
+    double best = -INFINITY;  // of block pass 2 * (lane & 1) + (lane >> 1 & 1)
+    for (int g = 0; g < G; g++) {
+        double x[8], s[4] = {0, 0, 0, 0};
+        uint32_t neg[4];  // the halves whose query value takes the lowest
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float x0 = q[g][d0 + 2 * j], x1 = q[g][d0 + 2 * j + 1];
+            x[2 * j] = x0, x[2 * j + 1] = x1;
+            neg[j] = (x0 >= 0.f ? 0u : 0xffffu) | (x1 >= 0.f ? 0u : 0xffff0000u);
+        }
+#pragma unroll
+        for (int p = 0; p < 4; p++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint32_t w = (lo[p][j] & neg[j]) | (hi[p][j] & ~neg[j]);
+                s[p] = fma(x[2 * j], (double)h2f(w & 0xffff), s[p]);
+                s[p] = fma(x[2 * j + 1], (double)h2f(w >> 16), s[p]);
+            }
+        const bool odd = lane & 1, two = lane & 2;
+        const double a0 = (odd ? s[2] : s[0]) + dpp_f64<0xB1>(odd ? s[0] : s[2]);  // quad_perm [1,0,3,2]
+        const double a1 = (odd ? s[3] : s[1]) + dpp_f64<0xB1>(odd ? s[1] : s[3]);
+        double t = (two ? a1 : a0) + dpp_f64<0x4E>(two ? a0 : a1);  // quad_perm [2,3,0,1]
+        if constexpr (LPB == 8) {
+            t += __shfl_xor(t, 4, 64);
+        } else {
+            t += dpp_f64<0x124>(t);  // row_ror:4
+            t += dpp_f64<0x128>(t);  // row_ror:8
+            if constexpr (LPB == 32) t += __shfl_xor(t, 16, 64);
+        }
+        if (!(t <= best)) best = t != t ? INFINITY : t;  // (NaN ranks first)
+    }
+    const int blk = blk0 + (2 * (lane & 1) + (lane >> 1 & 1)) * BPW;
+    if (lane % LPB < 4 && blk < nb) a.scores[((int64_t)b * a.HKV + kvh) * a.n_blocks + blk] = best;
 }
 
 __global__ __launch_bounds__(PICK_NT) void k_block_pick(SparseArgs a) {
-    __shared__ PickLds L;
+    __shared__ PickLds<uint64_t, 8192> L;
     const int kvh = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
     const int n = sparse_count(a, b), nb = (n + a.block - 1) / a.block;
     int32_t *out = a.picked + ((int64_t)b * a.HKV + kvh) * a.n_pick;
@@ -147,8 +179,9 @@ __global__ __launch_bounds__(PICK_NT) void k_block_pick(SparseArgs a) {
     const double *sc = a.scores + ((int64_t)b * a.HKV + kvh) * a.n_blocks;
     if (tid == 0) out[a.n_pick - 1] = nb - 1;
     if (a.n_pick == 1) return;
-    radix_pick<64>(L, nb - 1, a.n_pick - 1, [&](int i) { return i == 0 ? ~0ull : order_key(sc[i]); },
-                   [&](int place, int i) { out[place] = i; });
+    radix_pick(L, nb - 1, a.n_pick - 1, [&](int i) { return sc[i]; },
+               [&](int i, double x) { return i == 0 ? ~(uint64_t)0 : order_key(x); },
+               [&](int place, int i) { out[place] = i; });
 }
 
 // ---- attention over the picked blocks ----------------------------------------------------------------
@@ -185,7 +218,10 @@ __global__ __launch_bounds__(64 * NW) void k_attn_picked(SparseArgs a) {
     rows_load<HD, F16, KT>(nxt, kv, kn, rl, kq);
     RowsQ<HD, 1> q;
     rows_query<HD, 1>(q, a.scale, kq,
-                      [&](int) { return rl < G ? a.q + ((int64_t)b * a.H + kvh * G + rl) * HD : nullptr; });
+                      [&](int, bool &ok) {
+                          ok = rl < G;
+                          return a.q + ((int64_t)b * a.H + kvh * G + min(rl, G - 1)) * HD;
+                      });
     RowsSum<HD, 1> sum;
     rows_clear<HD, 1>(sum);
     for (int u = u0 + wave; u < u1; u += NW) {
@@ -207,16 +243,15 @@ __global__ __launch_bounds__(64 * NW) void k_attn_picked(SparseArgs a) {
 
 template <int HD, int KT>
 __global__ __launch_bounds__(256) void k_picked_merge(SparseArgs a, int64_t rows) {
-    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x, row = e / (HD / 4);
-    if (row >= rows) return;
-    const int d = 4 * (int)(e % (HD / 4)), b = (int)(row / a.H);
-    const int units = sparse_units(a, b, KT), per = (units + a.n_split - 1) / a.n_split;
+    constexpr int TPR = HD / 4 * JOIN_SG;
+    __shared__ RowsJoin J;
+    const int64_t row = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR, at = min(row, rows - 1);
+    const int units = sparse_units(a, (int)(at / a.H), KT), per = (units + a.n_split - 1) / a.n_split;
     const int used = units ? (units + per - 1) / per : 0;
     float M, l;
-    const float4 o = rows_merge(a.part + row * a.n_split * (HD + 4), used, HD + 4, d, M, l);
-    const float inv = 1.0f / l;
-    *(float4 *)(a.out + row * HD + d) =
-        l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    const float4 o = rows_join<HD, JOIN_SG>(J, a.part + at * a.n_split * (HD + 4), used, M, l);
+    if (row < rows && threadIdx.x % TPR < HD / 4)
+        *(float4 *)(a.out + row * HD + 4 * (threadIdx.x % TPR)) = rows_over(o, l);
 }
 
 struct SparseScratch {
@@ -250,16 +285,16 @@ hipError_t launch_attn_sparse(const float *q, int B, int H, int HKV, int HD, KvL
     a.n_blocks = p.n_blocks, a.scale = scale, a.out = out;
     a.scores = (double *)base, a.picked = picked ? picked : (int32_t *)(base + p.scores);
     a.part = (float *)(base + p.scores + p.picked);
-    const dim3 sg((p.n_blocks + SCORE_BLOCKS - 1) / SCORE_BLOCKS, HKV, B);
     return rows_by_shape(HD, kv_f16, [&](auto hd, auto f16) {
         constexpr int D = decltype(hd)::value, KT = D == 64 ? 2 : 1, NW = 4;
         constexpr bool F = decltype(f16)::value;
-        hipLaunchKernelGGL(k_block_scores<D>, sg, dim3(256), 0, s, a);
+        hipLaunchKernelGGL(k_block_scores<D>, dim3((p.n_blocks + score_blocks<D>() - 1) / score_blocks<D>(), HKV, B), dim3(256),
+                           0, s, a);
         hipLaunchKernelGGL(k_block_pick, dim3(HKV, B), dim3(PICK_NT), 0, s, a);
         hipLaunchKernelGGL((k_attn_picked<D, F, KT, NW>), dim3(p.n_split, HKV, B), dim3(64 * NW), 0, s, a);
         const int64_t rows = (int64_t)B * H;
-        hipLaunchKernelGGL((k_picked_merge<D, KT>), dim3((unsigned)((rows * (D / 4) + 255) / 256)), dim3(256), 0, s, a,
-                           rows);
+        constexpr int RPW = 256 / (D / 4 * JOIN_SG);
+        hipLaunchKernelGGL((k_picked_merge<D, KT>), dim3((unsigned)((rows + RPW - 1) / RPW)), dim3(256), 0, s, a, rows);
         return hipGetLastError();
     });
 }

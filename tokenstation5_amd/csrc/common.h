@@ -292,6 +292,13 @@ __device__ inline float wave_max_dpp(float v) {
     v = dpp_max<0x143, 0xC, false>(v);
     return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
+// Max over each 16-lane row, in every lane of the row.
+__device__ inline float row_max_dpp(float v) {
+    v = dpp_max<0xB1, 0xF, true>(v);
+    v = dpp_max<0x4E, 0xF, true>(v);
+    v = dpp_max<0x141, 0xF, true>(v);
+    return dpp_max<0x140, 0xF, true>(v);
+}
 // v + the value of lane i ^ 16 (v_permlane16_swap), of lane i ^ 32
 // (v_permlane32_swap): VALU lane exchanges across 16-lane rows and wave halves.
 __device__ inline float add_xor16(float v) {

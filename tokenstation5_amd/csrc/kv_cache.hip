@@ -21,7 +21,7 @@ __device__ inline int evict_count(const EvictArgs &a, int b) { return max(0, min
 // The slots kept, ascending: the first and last ones, then those of the largest sums (NaN lowest),
 // ties to the lowest slot. grid (HKV, B).
 __global__ __launch_bounds__(PICK_NT) void k_evict_pick(EvictArgs a) {
-    __shared__ PickLds L;
+    __shared__ PickLds<uint32_t, 32768> L;
     const int kvh = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, n = evict_count(a, b);
     int32_t *kept = a.kept + ((int64_t)b * a.HKV + kvh) * a.n_keep;
     if (kvh == 0 && tid == 0 && a.n_out) a.n_out[b] = min(n, a.n_keep);
@@ -30,10 +30,9 @@ __global__ __launch_bounds__(PICK_NT) void k_evict_pick(EvictArgs a) {
         return;
     }
     const float *acc = a.acc + ((int64_t)b * a.HKV + kvh) * a.n_ctx;
-    radix_pick<32>(
-        L, n, a.n_keep,
-        [&](int i) -> uint32_t {
-            const float x = acc[i];
+    radix_pick(
+        L, n, a.n_keep, [&](int i) { return acc[i]; },
+        [&](int i, float x) -> uint32_t {
             if (i < a.n_first || i >= n - a.n_last) return 0xffffffffu;
             return x != x ? 0u : order_key(x);
         },
