@@ -146,47 +146,57 @@ __device__ inline void rows_split(float x0, float x1, uint32_t &hi, uint32_t &lo
 }
 
 // The lane's rows (its MFMA columns), row 16 qt + rl of the wave's: B operands of dims
-// 32 c + 8 kq .. + 7, and 2^e. row(qt, ok) is the row's address; not ok: an address to read from, and zeros
-// (a load under a branch would wait for the one before it).
+// 32 c + 8 kq .. + 7, and 2^e. row(qt, ok) is the row's address; a column without a row (not ok) has one to
+// read from all the same, since a load under a branch would wait for the one before it, and zeros (which
+// cost the matrix cores less power: copies of a row took 10 % longer).
 template <int HD, int NT>
 struct RowsQ {
     ar_h8 h[NT][HD / 32], l[NT][HD / 32];
     float p2e[NT];
 };
+template <int HD, int NT>
+struct RowsIn {
+    float4 x[NT][HD / 32][2];
+    bool ok[NT];
+};
 template <int HD, int NT, class Row>
-__device__ inline void rows_query(RowsQ<HD, NT> &q, float scale, int kq, Row row) {
-    constexpr int NC = HD / 32;
+__device__ inline void rows_request(RowsIn<HD, NT> &in, int kq, Row row) {
 #pragma unroll
     for (int qt = 0; qt < NT; qt++) {
-        bool ok;
-        const float *p = row(qt, ok);
-        const float by = scale * AR_LOG2E;
-        float v[NC][8], amax = 0.f;
+        const float *p = row(qt, in.ok[qt]) + 8 * kq;
 #pragma unroll
-        for (int c = 0; c < NC; c++) {
-            const float4 x0 = *(const float4 *)(p + 32 * c + 8 * kq), x1 = *(const float4 *)(p + 32 * c + 8 * kq + 4);
-            const float f[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+        for (int c = 0; c < HD / 32; c++)
+            in.x[qt][c][0] = *(const float4 *)(p + 32 * c), in.x[qt][c][1] = *(const float4 *)(p + 32 * c + 4);
+    }
+}
+template <int HD, int NT>
+__device__ inline void rows_query(RowsQ<HD, NT> &q, const RowsIn<HD, NT> &in, float scale) {
+    constexpr int NC = HD / 32;
+    const float by = scale * AR_LOG2E;
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[c][j] = ok ? f[j] * by : 0.f, amax = fmaxf(amax, fabsf(v[c][j]));
-        }
-        amax = max_xor32(max_xor16(amax));
-        const int e = amax > 0.f ? max(ilogbf(amax) - 13, -100) : 0;
-        const float sc = ldexpf(1.0f, -e);
-        q.p2e[qt] = ldexpf(1.0f, e);
+    for (int qt = 0; qt < NT; qt++) {
+        float amax = 0.f;
 #pragma unroll
         for (int c = 0; c < NC; c++)
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                v[c][j] *= sc;
+            for (int k = 0; k < 2; k++) {
+                const float4 x = in.x[qt][c][k];
+                amax = fmaxf(fmaxf(amax, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(x.z), fabsf(x.w)));
             }
+        amax = max_xor32(max_xor16(amax)) * fabsf(by);
+        const int e = amax > 0.f ? max(ilogbf(amax) - 13, -100) : 0;
+        const float sc = in.ok[qt] ? ldexpf(by, -e) : 0.f;  // (one rounding of q * by: the rest is a power of 2)
+        q.p2e[qt] = ldexpf(1.0f, e);
 #pragma unroll
         for (int c = 0; c < NC; c++) {
             u32x4 h, l;
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                uint32_t hj, lj;
-                rows_split(v[c][2 * j], v[c][2 * j + 1], hj, lj);
-                h[j] = hj, l[j] = lj;
+            for (int k = 0; k < 2; k++) {
+                const float4 x = in.x[qt][c][k];
+                uint32_t h0, l0, h1, l1;
+                rows_split(x.x * sc, x.y * sc, h0, l0);
+                rows_split(x.z * sc, x.w * sc, h1, l1);
+                h[2 * k] = h0, h[2 * k + 1] = h1, l[2 * k] = l0, l[2 * k + 1] = l1;
             }
             q.h[qt][c] = __builtin_bit_cast(ar_h8, h), q.l[qt][c] = __builtin_bit_cast(ar_h8, l);
         }
@@ -195,7 +205,7 @@ __device__ inline void rows_query(RowsQ<HD, NT> &q, float scale, int kq, Row row
 
 template <int HD, int NT>
 struct RowsSum {
-    float m[NT], l[NT];
+    float m[NT], l[NT];    // (l: the lane's keys' share)
     ar_f4 o[NT][HD / 16];  // dim HD / 16 * (4 kq + i) + dt of row 16 qt + rl
 };
 template <int HD, int NT>
@@ -363,8 +373,7 @@ __device__ inline bool rows_unit(const RowsUnit<HD, F16, KT> &u, const RowsQ<HD,
                 rows_split(p0, p1, hi[2 * t + i], lo[2 * t + i]);
             }
         ph[qt] = Op::of(hi), pl[qt] = Op::of(lo);
-        sum = add_xor32(add_xor16(sum));
-        a.l[qt] += sum;
+        a.l[qt] += sum;  // (the lane's share: its four keys of each tile)
     }
     RowsScale<HD, F16, KT> sc;
     if constexpr (!F16) {
@@ -440,14 +449,15 @@ __device__ inline void rows_combine(RowsLds<HD, NW> &L, const RowsSum<HD, NT> &a
         const int nr = min(rows - 16 * qt, 16);  // (uniform: every thread leaves together)
         if (nr <= 0) return;
         __syncthreads();
+        const float sum = add_xor32(add_xor16(a.l[qt]));
         if (rl < nr) {
+            if (kq == 0) L.m[wave][rl] = a.m[qt], L.l[wave][rl] = sum;
 #pragma unroll
             for (int i = 0; i < 4; i++)
 #pragma unroll
                 for (int d = 0; d < NDT; d += 4)
                     *(float4 *)&L.o[wave][rl][NDT * (4 * kq + i) + d] =
                         make_float4(a.o[qt][d][i], a.o[qt][d + 1][i], a.o[qt][d + 2][i], a.o[qt][d + 3][i]);
-            if (kq == 0) L.m[wave][rl] = a.m[qt], L.l[wave][rl] = a.l[qt];
         }
         __syncthreads();
         for (int e = threadIdx.x; e < nr * (HD / 4); e += 64 * NW) {
@@ -471,12 +481,17 @@ __device__ inline void rows_combine(RowsLds<HD, NW> &L, const RowsSum<HD, NT> &a
     }
 }
 
+// x / d for 0 <= x < 2^26, x d < 2^36, as one multiplication by m = rows_magic(d): m d is less than d above
+// 2^36, so the error stays under x / 2^36 < 1 / d, and x m under 2^63.
+__host__ inline uint64_t rows_magic(int d) { return ((1ull << 36) + d - 1) / d; }
+__host__ __device__ inline int rows_div(int x, uint64_t m) { return (int)((uint64_t)(uint32_t)x * m >> 36); }
+
 // Keys of each of n_split slices of n keys: at least ROWS_MIN_KEYS, and whole blocks of k_attn_tile
 // (a slice that ended inside one would count the zeros behind it).
 constexpr int ROWS_MIN_KEYS = 128;
 constexpr int ROWS_MAX_SPLIT = 64;
-__host__ __device__ inline int rows_chunk(int n, int n_split) {
-    int c = (n + n_split - 1) / n_split;
+__host__ __device__ inline int rows_chunk(int n, int n_split, uint64_t split_m) {  // split_m = rows_magic(n_split)
+    int c = rows_div(n + n_split - 1, split_m);
     c = c < ROWS_MIN_KEYS ? ROWS_MIN_KEYS : c;
     return (c + 63) / 64 * 64;
 }

@@ -11,6 +11,8 @@ struct RowsArgs {
     const float *q;  // [B][T][H * HD]
     KvLayer kv;      // B caches
     int n_ctx, H, HKV, T, n_split;
+    int G, R, nrb;  // query heads a KV head, rows T * G, blocks of rows
+    uint64_t g_m, nrb_m, split_m;  // rows_magic of G, nrb, n_split
     const int32_t *n_keys;  // per cache: the keys before the T tokens (tree), or all keys (one query)
     const uint64_t *mask;   // [B][T], tree
     int pos0;               // position of the first token (causal)
@@ -35,6 +37,12 @@ __device__ inline int rows_count(const RowsArgs &a, int b) {
 // Keys that slices divide, and the keys of token t's row.
 __device__ inline int rows_all(const RowsArgs &a, int n) { return a.mode == ROWS_ONE ? n : n + a.T; }
 __device__ inline int rows_reach(const RowsArgs &a, int n, int t) { return a.mode == ROWS_CAUSAL ? n + t + 1 : rows_all(a, n); }
+
+// The query head (and output) of row r of KV head kvh: token r / G, head r % G of the group.
+__device__ inline int64_t rows_at(const RowsArgs &a, int b, int kvh, int r) {
+    const int t = rows_div(r, a.g_m);
+    return ((int64_t)b * a.T + t) * a.H + kvh * a.G + r - t * a.G;
+}
 
 // The infinite and NaN values of keys first .. kend - 1 that token t's rows take, onto dims d .. + 3 of a row:
 // the products left them out there.
@@ -61,13 +69,19 @@ __global__ __launch_bounds__(64 * NW) void k_attn_rows(RowsArgs a) {
     if (!ONE && threadIdx.x == 0) nonfinite = 0;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int rl = lane & 15, kq = lane >> 4;
-    const int G = a.H / a.HKV, R = a.T * G, nrb = (R + 16 * NT - 1) / (16 * NT);
-    const int split = blockIdx.x, kvh = blockIdx.y / nrb, r0 = blockIdx.y % nrb * 16 * NT, b = blockIdx.z;
+    const int G = a.G, R = a.R;
+    const int split = blockIdx.x, kvh = rows_div(blockIdx.y, a.nrb_m), r0 = ((int)blockIdx.y - kvh * a.nrb) * 16 * NT, b = blockIdx.z;
     const int rows = min(R - r0, 16 * NT);
-    const int n = rows_count(a, b), chunk = rows_chunk(rows_all(a, n), a.n_split);
-    const int kbeg = split * chunk, kend = min(kbeg + chunk, rows_reach(a, n, (r0 + rows - 1) / G));
+    RowsIn<HD, NT> in;  // requested before the counts that the keys' addresses wait for
+    rows_request<HD, NT>(in, kq, [&](int qt, bool &ok) {
+        const int r = r0 + 16 * qt + rl;
+        ok = r < R;
+        return a.q + rows_at(a, b, kvh, min(r, R - 1)) * HD;
+    });
+    const int n = rows_count(a, b), chunk = rows_chunk(rows_all(a, n), a.n_split, a.split_m);
+    const int kbeg = split * chunk, kend = min(kbeg + chunk, rows_reach(a, n, rows_div(r0 + rows - 1, a.g_m)));
     if (kbeg >= kend) return;  // the merge reads no partial of this slice
-    const int full = a.mode == ROWS_CAUSAL ? n + r0 / G + 1 : n;  // keys before it are every row's
+    const int full = a.mode == ROWS_CAUSAL ? n + rows_div(r0, a.g_m) + 1 : n;  // keys before it are every row's
     const RowsKv kv = rows_kv<HD, F16>(a.kv, ((int64_t)b * a.HKV + kvh) * a.n_ctx, kend);
     const int units = (kend - kbeg + S::UNIT - 1) / S::UNIT;
     RowsUnit<HD, F16, KT> nxt;
@@ -80,19 +94,18 @@ __global__ __launch_bounds__(64 * NW) void k_attn_rows(RowsArgs a) {
     rows_load<HD, F16, KT>(nxt, kv, kb, rl, kq);
 
     RowsQ<HD, NT> q;
-    rows_query<HD, NT>(q, a.scale, kq, [&](int qt, bool &ok) -> const float * {
-        const int r = min(r0 + 16 * qt + rl, R - 1);
-        ok = r0 + 16 * qt + rl < R;
-        return a.q + (((int64_t)b * a.T + r / G) * a.H + kvh * G + r % G) * HD;
-    });
+    rows_query<HD, NT>(q, in, a.scale);
     int seen[NT];       // keys before it are the row's
     uint64_t bits[NT];  // and then those of n + its set bits
 #pragma unroll
     for (int qt = 0; qt < NT; qt++) {
-        const int r = r0 + 16 * qt + rl;
-        seen[qt] = r >= R ? 0 : a.mode == ROWS_CAUSAL ? n + r / G + 1 : n;
+        const int r = r0 + 16 * qt + rl, t = rows_div(min(r, R - 1), a.g_m);
+        seen[qt] = r >= R ? 0 : a.mode == ROWS_CAUSAL ? n + t + 1 : n;
         bits[qt] = 0;
-        if (!ONE && a.mode == ROWS_TREE && r < R) bits[qt] = a.mask[(int64_t)b * a.T + r / G] & (~0ull >> (64 - a.T));
+        if (!ONE && a.mode == ROWS_TREE) {
+            const uint64_t m = a.mask[(int64_t)b * a.T + t] & (~0ull >> (64 - a.T));
+            bits[qt] = r < R ? m : 0;
+        }
     }
     if (!ONE && a.planes && split == 0 && wave == 0) {
         const int tiles = (R + 15) / 16;
@@ -155,11 +168,11 @@ __global__ __launch_bounds__(64 * NW) void k_attn_rows(RowsArgs a) {
         }
     }
     rows_combine<HD, NT, NW>(L, sum, rows, wave, rl, kq, [&](int r, int d, float4 o, float m, float l) {
-        const int t = (r0 + r) / G, j = (r0 + r) % G;
+        const int t = rows_div(r0 + r, a.g_m);
         if (!ONE && nonfinite)
             rows_add_nonfinite<HD, F16>(a, b, kvh, t, n, kbeg + max(full - kbeg, 0) / S::UNIT * S::UNIT, kend, d, o);
         if (!ONE && a.n_split == 1) {
-            *(float4 *)(a.out + (((int64_t)b * a.T + t) * a.H + kvh * G + j) * HD + d) = rows_over(o, l);
+            *(float4 *)(a.out + rows_at(a, b, kvh, r0 + r) * HD + d) = rows_over(o, l);
             if (a.lse && d == 0) a.lse[row0 + r] = l == 0.f ? INFINITY : m + __log2f(l);
             return;
         }
@@ -203,12 +216,19 @@ __global__ __launch_bounds__(256, 2) void k_attn_tile(RowsArgs a) {
     if (threadIdx.x == 0) L.nonfinite = 0;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int rl = lane & 15, kq = lane >> 4;
-    const int G = a.H / a.HKV, R = a.T * G, nrb = (R + S::ROWS - 1) / S::ROWS;
-    const int split = blockIdx.x, kvh = blockIdx.y / nrb, r0 = blockIdx.y % nrb * S::ROWS, b = blockIdx.z;
-    const int n = rows_count(a, b), chunk = rows_chunk(rows_all(a, n), a.n_split);
-    const int kbeg = split * chunk, kend = min(kbeg + chunk, rows_reach(a, n, (min(R, r0 + S::ROWS) - 1) / G));
+    const int G = a.G, R = a.R;
+    const int split = blockIdx.x, kvh = rows_div(blockIdx.y, a.nrb_m), r0 = ((int)blockIdx.y - kvh * a.nrb) * S::ROWS, b = blockIdx.z;
+    const int w0 = r0 + 16 * NT * wave;  // the wave's first row
+    RowsIn<HD, NT> in;  // requested before the counts that the keys' addresses wait for
+    rows_request<HD, NT>(in, kq, [&](int qt, bool &ok) {
+        const int r = w0 + 16 * qt + rl;
+        ok = r < R;
+        return a.q + rows_at(a, b, kvh, min(r, R - 1)) * HD;
+    });
+    const int n = rows_count(a, b), chunk = rows_chunk(rows_all(a, n), a.n_split, a.split_m);
+    const int kbeg = split * chunk, kend = min(kbeg + chunk, rows_reach(a, n, rows_div(min(R, r0 + S::ROWS) - 1, a.g_m)));
     if (kbeg >= kend) return;  // the merge reads no partial of this slice
-    const int full = a.mode == ROWS_CAUSAL ? n + r0 / G + 1 : n;  // keys before it are every row's
+    const int full = a.mode == ROWS_CAUSAL ? n + rows_div(r0, a.g_m) + 1 : n;  // keys before it are every row's
     const RowsKv kv = rows_kv<HD, F16>(a.kv, ((int64_t)b * a.HKV + kvh) * a.n_ctx, kend);
     // The lane's share of a block: tile wave / WPT; K of key rl, chunks c0 ..; V of keys 4 kq .. + 3, dims
     // NDT rl + d0 ..; the K scale of key rl, chunk c0 + kq.
@@ -264,22 +284,17 @@ __global__ __launch_bounds__(256, 2) void k_attn_tile(RowsArgs a) {
     };
     load(kbeg);
 
-    const int w0 = r0 + 16 * NT * wave;  // the wave's first row
     RowsQ<HD, NT> q;
-    rows_query<HD, NT>(q, a.scale, kq, [&](int qt, bool &ok) -> const float * {
-        const int r = min(w0 + 16 * qt + rl, R - 1);
-        ok = w0 + 16 * qt + rl < R;
-        return a.q + (((int64_t)b * a.T + r / G) * a.H + kvh * G + r % G) * HD;
-    });
+    rows_query<HD, NT>(q, in, a.scale);
     int seen[NT];       // keys before it are the row's
     uint64_t bits[NT];  // and then those of n + its set bits
 #pragma unroll
     for (int qt = 0; qt < NT; qt++) {
-        const int r = w0 + 16 * qt + rl;
-        seen[qt] = r >= R ? 0 : a.mode == ROWS_CAUSAL ? n + r / G + 1 : n;
+        const int r = w0 + 16 * qt + rl, t = rows_div(min(r, R - 1), a.g_m);
+        seen[qt] = r >= R ? 0 : a.mode == ROWS_CAUSAL ? n + t + 1 : n;
         bits[qt] = 0;
         if (a.mode == ROWS_TREE) {
-            const uint64_t m = a.mask[(int64_t)b * a.T + min(r, R - 1) / G] & (~0ull >> (64 - a.T));
+            const uint64_t m = a.mask[(int64_t)b * a.T + t] & (~0ull >> (64 - a.T));
             bits[qt] = r < R ? m : 0;
         }
     }
@@ -300,8 +315,8 @@ __global__ __launch_bounds__(256, 2) void k_attn_tile(RowsArgs a) {
     }
     RowsSum<HD, NT> sum;
     rows_clear<HD, NT>(sum);
-    const int wfull = a.mode == ROWS_CAUSAL ? n + w0 / G + 1 : n;  // every row of the wave's
-    const int wreach = w0 < R ? rows_reach(a, n, (min(R, w0 + 16 * NT) - 1) / G) : 0;
+    const int wfull = a.mode == ROWS_CAUSAL ? n + rows_div(w0, a.g_m) + 1 : n;  // every row of the wave's
+    const int wreach = w0 < R ? rows_reach(a, n, rows_div(min(R, w0 + 16 * NT) - 1, a.g_m)) : 0;
 
     for (int kb = kbeg; kb < kend; kb += S::KEYS) {
         __syncthreads();  // every wave is done with the last block
@@ -310,113 +325,151 @@ __global__ __launch_bounds__(256, 2) void k_attn_tile(RowsArgs a) {
         load(kb + S::KEYS);  // (past the slice: zeros, no memory access)
         __syncthreads();
         if (kb >= wreach) continue;
-        float s[NKT][NT][4];
+        // 32 keys at a time (a whole block's scores and weights would take 32 registers more).
+#pragma unroll 1
+        for (int half = 0; half < NKT / 2; half++) {
+            const int kh = kb + 32 * half;
+            if (kh >= wreach) break;
+            // S^T, two chunks of a tile at a time (so that other products lie between two on one
+            // accumulator); the next two are read from LDS before these are used.
+            float s[2][NT][4];
+            {
+                constexpr int STEPS = NC;
+                ar_h8 ka[2][2];
+                float4 k4[2][2];
+                ar_f4 D[F16 ? 1 : 2][NT];
+                auto fetch = [&](int step, int buf) {
+                    const int t = 2 * half + step / (NC / 2), c = step % (NC / 2) * 2;
 #pragma unroll
-        for (int t = 0; t < NKT; t++) {
-            if constexpr (F16) {
-                ar_f4 D[NT];
+                    for (int j = 0; j < 2; j++) {
+                        ka[buf][j] = __builtin_bit_cast(ar_h8, L.k[t][c + j][lane]);
+                        if constexpr (!F16) k4[buf][j] = *(const float4 *)&L.ks[t][c + j][4 * kq];
+                    }
+                };
+                fetch(0, 0);
 #pragma unroll
-                for (int qt = 0; qt < NT; qt++) D[qt] = ar_f4{0.f, 0.f, 0.f, 0.f};
+                for (int step = 0; step < STEPS; step++) {
+                    const int t = step / (NC / 2), c = step % (NC / 2) * 2, buf = step & 1;
+                    if (step + 1 < STEPS) fetch(step + 1, buf ^ 1);
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int c = 0; c < NC; c++) {
-                    const ar_h8 ka = __builtin_bit_cast(ar_h8, L.k[t][c][lane]);
+                    for (int plane = 0; plane < 2; plane++)
 #pragma unroll
-                    for (int qt = 0; qt < NT; qt++) {
-                        D[qt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q.h[qt][c], D[qt], 0, 0, 0);
-                        D[qt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q.l[qt][c], D[qt], 0, 0, 0);
+                        for (int j = 0; j < 2; j++)
+#pragma unroll
+                            for (int qt = 0; qt < NT; qt++) {
+                                const bool first = plane == 0 && (!F16 || (c == 0 && j == 0));
+                                ar_f4 &d = D[F16 ? 0 : j][qt];
+                                if (first) d = ar_f4{0.f, 0.f, 0.f, 0.f};
+                                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[buf][j], plane ? q.l[qt][c + j] : q.h[qt][c + j], d, 0, 0, 0);
+                            }
+                    if constexpr (F16) {
+                        if (c + 2 == NC) {
+#pragma unroll
+                            for (int qt = 0; qt < NT; qt++)
+#pragma unroll
+                                for (int i = 0; i < 4; i++) s[t][qt][i] = D[0][qt][i];
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 2; j++) {
+                            const float ks[4] = {k4[buf][j].x, k4[buf][j].y, k4[buf][j].z, k4[buf][j].w};
+#pragma unroll
+                            for (int qt = 0; qt < NT; qt++)
+#pragma unroll
+                                for (int i = 0; i < 4; i++)
+                                    s[t][qt][i] = c + j == 0 ? ks[i] * D[j][qt][i] : fmaf(ks[i], D[j][qt][i], s[t][qt][i]);
+                        }
                     }
                 }
+            }
+            if (kh + 32 > wfull) {
 #pragma unroll
-                for (int qt = 0; qt < NT; qt++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) s[t][qt][i] = D[qt][i];
-            } else {
-#pragma unroll
-                for (int c = 0; c < NC; c++) {
-                    const ar_h8 ka = __builtin_bit_cast(ar_h8, L.k[t][c][lane]);
-                    const float4 k4 = *(const float4 *)&L.ks[t][c][4 * kq];
-                    const float ks[4] = {k4.x, k4.y, k4.z, k4.w};
+                for (int t = 0; t < 2; t++)
 #pragma unroll
                     for (int qt = 0; qt < NT; qt++) {
-                        ar_f4 D = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q.h[qt][c], ar_f4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-                        D = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q.l[qt][c], D, 0, 0, 0);
+                        const int key = kh + 16 * t + 4 * kq;
+                        const uint32_t take = rows_below(key, seen[qt]) | rows_window(bits[qt], key - n);
 #pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            s[t][qt][i] = c == 0 ? ks[i] * D[i] : fmaf(ks[i], D[i], s[t][qt][i]);
+                        for (int i = 0; i < 4; i++) s[t][qt][i] = take & 1u << i ? s[t][qt][i] : -INFINITY;
+                    }
+            }
+            uint32_t ph[NT][4], pl[NT][4];
+#pragma unroll
+            for (int qt = 0; qt < NT; qt++) {
+                float mx = -INFINITY;
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) mx = fmaxf(mx, s[t][qt][i]);
+                const float m0 = rows_reference(sum, qt, max_xor32(max_xor16(mx)) * q.p2e[qt]);
+                float l = 0.f;
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[t][qt][2 * i], q.p2e[qt], -m0));
+                        const float p1 = __builtin_amdgcn_exp2f(fmaf(s[t][qt][2 * i + 1], q.p2e[qt], -m0));
+                        l += p0 + p1;
+                        rows_split(p0, p1, ph[qt][2 * t + i], pl[qt][2 * t + i]);
+                    }
+                sum.l[qt] += l;  // (the lane's share: its four keys of each tile)
+            }
+            // O^T, two dim tiles at a time, the next two's values read before.
+            {
+                constexpr int STEPS = NDT / 2;
+                ar_h8 vh[2][2], vl[2][2];
+                auto fetch = [&](int step, int buf) {
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        vh[buf][j] = *(const ar_h8 *)&L.vh[half][step * 2 + j][lane];
+                        if constexpr (!F16) vl[buf][j] = *(const ar_h8 *)&L.vl[half][step * 2 + j][lane];
+                    }
+                };
+                fetch(0, 0);
+#pragma unroll
+                for (int step = 0; step < STEPS; step++) {
+                    const int d = step * 2, buf = step & 1;
+                    if (step + 1 < STEPS) fetch(step + 1, buf ^ 1);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int term = 0; term < 3; term++) {  // Vh Ph, Vl Ph, Vh Pl
+                        if (F16 && term == 1) continue;
+#pragma unroll
+                        for (int j = 0; j < 2; j++)
+#pragma unroll
+                            for (int qt = 0; qt < NT; qt++) {
+                                const uint32_t *p = term == 2 ? pl[qt] : ph[qt];
+                                const ar_h8 w = __builtin_bit_cast(ar_h8, u32x4{p[0], p[1], p[2], p[3]});
+                                sum.o[qt][d + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(term == 1 ? vl[buf][j] : vh[buf][j], w,
+                                                                                         sum.o[qt][d + j], 0, 0, 0);
+                            }
                     }
                 }
             }
         }
-        if (kb + S::KEYS > wfull) {
-#pragma unroll
-            for (int t = 0; t < NKT; t++)
-#pragma unroll
-                for (int qt = 0; qt < NT; qt++) {
-                    const int key = kb + 16 * t + 4 * kq;
-                    const uint32_t take = rows_below(key, seen[qt]) | rows_window(bits[qt], key - n);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) s[t][qt][i] = take & 1u << i ? s[t][qt][i] : -INFINITY;
-                }
-        }
-        uint32_t ph[NT][2 * NKT], pl[NT][2 * NKT];
-#pragma unroll
-        for (int qt = 0; qt < NT; qt++) {
-            float mx = -INFINITY;
-#pragma unroll
-            for (int t = 0; t < NKT; t++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) mx = fmaxf(mx, s[t][qt][i]);
-            const float m0 = rows_reference(sum, qt, max_xor32(max_xor16(mx)) * q.p2e[qt]);
-            float l = 0.f;
-#pragma unroll
-            for (int t = 0; t < NKT; t++)
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const float p0 = __builtin_amdgcn_exp2f(fmaf(s[t][qt][2 * i], q.p2e[qt], -m0));
-                    const float p1 = __builtin_amdgcn_exp2f(fmaf(s[t][qt][2 * i + 1], q.p2e[qt], -m0));
-                    l += p0 + p1;
-                    rows_split(p0, p1, ph[qt][2 * t + i], pl[qt][2 * t + i]);
-                }
-            l = add_xor32(add_xor16(l));
-            sum.l[qt] += l;
-        }
-#pragma unroll
-        for (int dt = 0; dt < NDT; dt++)
-#pragma unroll
-            for (int k2 = 0; k2 < NKT / 2; k2++) {
-                const ar_h8 vh = *(const ar_h8 *)&L.vh[k2][dt][lane];
-                ar_h8 vl;
-                if constexpr (!F16) vl = *(const ar_h8 *)&L.vl[k2][dt][lane];
-#pragma unroll
-                for (int qt = 0; qt < NT; qt++) {
-                    const ar_h8 h = __builtin_bit_cast(ar_h8, u32x4{ph[qt][4 * k2], ph[qt][4 * k2 + 1], ph[qt][4 * k2 + 2], ph[qt][4 * k2 + 3]});
-                    const ar_h8 l = __builtin_bit_cast(ar_h8, u32x4{pl[qt][4 * k2], pl[qt][4 * k2 + 1], pl[qt][4 * k2 + 2], pl[qt][4 * k2 + 3]});
-                    sum.o[qt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, h, sum.o[qt][dt], 0, 0, 0);
-                    if constexpr (!F16) sum.o[qt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, h, sum.o[qt][dt], 0, 0, 0);
-                    sum.o[qt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, l, sum.o[qt][dt], 0, 0, 0);
-                }
-            }
     }
+#pragma unroll
+    for (int qt = 0; qt < NT; qt++) sum.l[qt] = add_xor32(add_xor16(sum.l[qt]));
 
     const bool extra = L.nonfinite;  // (set before a barrier that every wave has passed)
 #pragma unroll
     for (int qt = 0; qt < NT; qt++) {
-        const int r = w0 + 16 * qt + rl, t = r / G;
+        const int r = w0 + 16 * qt + rl, t = rows_div(r, a.g_m);
         if (r >= R) continue;
         const int64_t row = ((int64_t)b * a.HKV + kvh) * R + r;
-        float *p = a.n_split == 1 ? a.out + (((int64_t)b * a.T + t) * a.H + kvh * G + r % G) * HD
-                                  : a.part + (row * a.n_split + split) * (HD + 4) + 4;
+        float *p = a.n_split == 1 ? a.out + rows_at(a, b, kvh, r) * HD : a.part + (row * a.n_split + split) * (HD + 4) + 4;
         if (kq == 0) {
             if (a.n_split > 1) *(float4 *)(p - 4) = make_float4(sum.m[qt], sum.l[qt], 0.f, 0.f);
             else if (a.lse) a.lse[row] = sum.l[qt] == 0.f ? INFINITY : sum.m[qt] + __log2f(sum.l[qt]);
         }
+        const float by = a.n_split > 1 ? 1.f : sum.l[qt] == 0.f ? 0.f : 1.0f / sum.l[qt];
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int d = 0; d < NDT; d += 4) {
-                const float4 o = make_float4(sum.o[qt][d][i], sum.o[qt][d + 1][i], sum.o[qt][d + 2][i], sum.o[qt][d + 3][i]);
-                *(float4 *)(p + NDT * (4 * kq + i) + d) = a.n_split == 1 ? rows_over(o, sum.l[qt]) : o;
-            }
+            for (int d = 0; d < NDT; d += 4)
+                *(float4 *)(p + NDT * (4 * kq + i) + d) = make_float4(sum.o[qt][d][i] * by, sum.o[qt][d + 1][i] * by,
+                                                                      sum.o[qt][d + 2][i] * by, sum.o[qt][d + 3][i] * by);
         if (extra) {  // (onto a quotient as onto its numerator)
 #pragma unroll 1
             for (int dim = NDT * 4 * kq; dim < NDT * 4 * (kq + 1); dim += 4) {
@@ -434,14 +487,14 @@ __global__ __launch_bounds__(256) void k_rows_merge(RowsArgs a, int64_t rows) {
     constexpr int TPR = HD / 4 * SG;  // threads a row
     __shared__ RowsJoin J;
     const int64_t row = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR, at = min(row, rows - 1);
-    const int d = 4 * ((int)threadIdx.x % (HD / 4)), G = a.H / a.HKV, R = a.T * G;
-    const int b = (int)(at / ((int64_t)a.HKV * R)), kvh = (int)(at / R % a.HKV), r = (int)(at % R), t = r / G;
-    const int n = rows_count(a, b), chunk = rows_chunk(rows_all(a, n), a.n_split);
+    const int d = 4 * ((int)threadIdx.x % (HD / 4)), R = a.R;
+    const int b = (int)(at / ((int64_t)a.HKV * R)), kvh = (int)(at / R % a.HKV), r = (int)(at % R), t = rows_div(r, a.g_m);
+    const int n = rows_count(a, b), chunk = rows_chunk(rows_all(a, n), a.n_split, a.split_m);
     const int used = (rows_reach(a, n, t) + chunk - 1) / chunk;
     float M, l;
     const float4 o = rows_join<HD, SG>(J, a.part + at * a.n_split * (HD + 4), used, M, l);
     if (row >= rows || threadIdx.x % TPR >= HD / 4) return;
-    *(float4 *)(a.out + (((int64_t)b * a.T + t) * a.H + kvh * G + r % G) * HD + d) = rows_over(o, l);
+    *(float4 *)(a.out + rows_at(a, b, kvh, r) * HD + d) = rows_over(o, l);
     if (a.lse && d == 0) a.lse[row] = l == 0.f ? INFINITY : M + __log2f(l);
 }
 
@@ -453,7 +506,7 @@ __global__ __launch_bounds__(256) void k_one_weights(RowsArgs a, const float *ac
     __shared__ float lse[ROWS_MAX_G];
     constexpr int TPR = HD / 4 * JOIN_SG;
     const int kvh = blockIdx.y, b = blockIdx.z, G = a.H / a.HKV, tid = threadIdx.x;
-    const int n = rows_count(a, b), chunk = rows_chunk(n, a.n_split), used = (n + chunk - 1) / chunk;
+    const int n = rows_count(a, b), chunk = rows_chunk(n, a.n_split, a.split_m), used = (n + chunk - 1) / chunk;
     const int64_t head = (int64_t)b * a.HKV + kvh, row0 = head * G;
     if (blockIdx.x == 0) {
         for (int g0 = 0; g0 < G; g0 += 256 / TPR) {
@@ -498,8 +551,9 @@ __global__ __launch_bounds__(256) void k_one_weights(RowsArgs a, const float *ac
 }
 
 // A prompt chunk's weights summed over its queries, for each key: a wave holds a unit's
-// K and goes over every row tile's planes, sums 2^(score - lse) in its lanes, and
-// adds the lanes at the end. grid (key blocks of 4 units, HKV).
+// K and goes over every fourth row tile's planes (the next one's requested before this one's products),
+// sums 2^(score - lse) in its lanes, and the workgroup adds lanes and waves in order at the end. grid
+// (units, HKV).
 template <int HD, bool F16, int KT>
 __global__ __launch_bounds__(256) void k_prompt_weights(RowsArgs a, const float *acc, float *acc_out) {
     using S = RowsShape<HD, F16, KT>;
@@ -507,8 +561,8 @@ __global__ __launch_bounds__(256) void k_prompt_weights(RowsArgs a, const float 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int rl = lane & 15, kq = lane >> 4, kvh = blockIdx.y;
     const int G = a.H / a.HKV, R = a.T * G, tiles = (R + 15) / 16, n = a.pos0 + a.T;
-    const int k0 = (blockIdx.x * 4 + wave) * S::UNIT;
-    if (k0 >= n) return;
+    const int k0 = blockIdx.x * S::UNIT;
+    __shared__ float part[4][KT][16];
     const RowsKv kv = rows_kv<HD, F16>(a.kv, (int64_t)kvh * a.n_ctx, n);
     RowsUnit<HD, F16, KT> u;
     ar_h8 ka[KT][NC];
@@ -532,17 +586,29 @@ __global__ __launch_bounds__(256) void k_prompt_weights(RowsArgs a, const float 
     // The first row that sees key k0: token max(0, k0 - pos0).
     const int first = max(0, k0 - a.pos0) * G / 16;
     const uint4 *pl = a.planes + (int64_t)kvh * tiles * NC * 2 * 64 + lane;
-    for (int tile = first; tile < tiles; tile++) {
-        ar_h8 qh[NC], ql[NC];
+    struct Tile {
+        uint4 h[NC], l[NC];
+        float p2e, lse;
+    } nxt;
+    auto request = [&](int tile) {
+        const int at = min(tile, tiles - 1);
 #pragma unroll
         for (int c = 0; c < NC; c++) {
-            qh[c] = __builtin_bit_cast(ar_h8, pl[((int64_t)tile * NC * 2 + 2 * c) * 64]);
-            ql[c] = __builtin_bit_cast(ar_h8, pl[((int64_t)tile * NC * 2 + 2 * c + 1) * 64]);
+            nxt.h[c] = pl[((int64_t)at * NC * 2 + 2 * c) * 64];
+            nxt.l[c] = pl[((int64_t)at * NC * 2 + 2 * c + 1) * 64];
         }
+        nxt.p2e = a.p2e[((int64_t)kvh * tiles + at) * 16 + rl];
+        nxt.lse = a.lse[(int64_t)kvh * R + min(16 * at + rl, R - 1)];
+    };
+    request(first + wave);
+    for (int tile = first + wave; tile < tiles; tile += 4) {
+        ar_h8 qh[NC], ql[NC];
+#pragma unroll
+        for (int c = 0; c < NC; c++) qh[c] = __builtin_bit_cast(ar_h8, nxt.h[c]), ql[c] = __builtin_bit_cast(ar_h8, nxt.l[c]);
+        const float p2e = nxt.p2e, lse = nxt.lse;
+        request(tile + 4);
         const int r = 16 * tile + rl;
-        const float p2e = a.p2e[((int64_t)kvh * tiles + tile) * 16 + rl];
-        const float lse = r < R ? a.lse[(int64_t)kvh * R + r] : INFINITY;
-        const int last = a.pos0 + r / G;  // the last key the row sees
+        const int last = a.pos0 + rows_div(r, a.g_m);  // the last key the row sees
 #pragma unroll
         for (int t = 0; t < KT; t++) {
             float s[4];
@@ -576,9 +642,14 @@ __global__ __launch_bounds__(256) void k_prompt_weights(RowsArgs a, const float 
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const float x = row_sum_dpp(w[t][i]);
-            const int64_t key = k0 + 16 * t + 4 * kq + i;
-            if (rl == 0 && key < n) acc_out[(int64_t)kvh * a.n_ctx + key] = acc[(int64_t)kvh * a.n_ctx + key] + x;
+            if (rl == 0) part[wave][t][4 * kq + i] = x;
         }
+    __syncthreads();
+    const int e = threadIdx.x;
+    if (e < S::UNIT && k0 + e < n) {
+        const float x = (part[0][e / 16][e % 16] + part[1][e / 16][e % 16]) + (part[2][e / 16][e % 16] + part[3][e / 16][e % 16]);
+        acc_out[(int64_t)kvh * a.n_ctx + k0 + e] = acc[(int64_t)kvh * a.n_ctx + k0 + e] + x;
+    }
 }
 
 // ---- host ----------------------------------------------------------------------------------------
@@ -601,10 +672,16 @@ bool attn_rows_supported(int H, int HKV, int HD) {
     return HKV > 0 && H > 0 && H % HKV == 0 && (HD == 64 || HD == 128 || HD == 256) && H / HKV <= ROWS_MAX_G;
 }
 
+// The arguments that follow from the others.
+static void rows_derive(RowsArgs &a, int HD) {
+    a.G = a.H / a.HKV, a.R = a.T * a.G, a.nrb = rows_blocks(a.R, HD);
+    a.g_m = rows_magic(a.G), a.nrb_m = rows_magic(a.nrb), a.split_m = rows_magic(a.n_split);
+}
+
 template <int HD, bool F16>
 static hipError_t rows_launch(const RowsArgs &a, int B, bool one, hipStream_t s) {
-    const int R = a.T * (a.H / a.HKV);
-    const dim3 grid(a.n_split, a.HKV * rows_blocks(R, HD), B);
+    const int R = a.R;
+    const dim3 grid(a.n_split, a.HKV * a.nrb, B);
     constexpr int NW = HD == 256 ? 4 : 8, K1 = rows_kt(HD, 1), K2 = rows_kt(HD, 2);
     if (one) {
         hipLaunchKernelGGL((k_attn_rows<HD, F16, K1, 1, NW, true>), grid, dim3(64 * NW), 0, s, a);
@@ -640,13 +717,16 @@ hipError_t launch_attn_tree(const float *q, int B, int T, int H, int HKV, int HD
     a.q = q, a.kv = kv, a.n_ctx = n_ctx, a.H = H, a.HKV = HKV, a.T = T, a.n_keys = n_past, a.mask = mask;
     a.mode = ROWS_TREE, a.scale = scale, a.part = part, a.out = out;
     a.n_split = tree_splits(B, T, H, HKV, HD, n_ctx, n_cu);
+    rows_derive(a, HD);
     return rows_by_shape(HD, kv_f16, [&](auto hd, auto f16) {
         const hipError_t e = rows_launch<decltype(hd)::value, decltype(f16)::value>(a, B, false, s);
         return e != hipSuccess || a.n_split == 1 ? e : rows_launch_merge<decltype(hd)::value>(a, B, s);
     });
 }
 
-static int one_splits(int B, int HKV, int n_ctx, int n_cu) { return rows_splits(B * HKV, n_ctx, n_cu); }
+// Two rounds of workgroups: sequences of different lengths leave less of the last one idle (16 of 12288 to 16384
+// keys: 122 us, 127 in one round, 130 in four).
+static int one_splits(int B, int HKV, int n_ctx, int n_cu) { return rows_splits(B * HKV, n_ctx, 2 * n_cu); }
 static int64_t one_stride(int n_ctx) { return ((int64_t)n_ctx + 31) / 32 * 32; }
 size_t attn_one_weights_scratch_bytes(int B, int H, int HKV, int HD, int n_ctx, int n_cu) {
     return (size_t)B * H * (one_stride(n_ctx) + (size_t)one_splits(B, HKV, n_ctx, n_cu) * (HD + 4)) * sizeof(float);
@@ -659,6 +739,7 @@ hipError_t launch_attn_one_weights(const float *q, int B, int H, int HKV, int HD
     a.mode = ROWS_ONE, a.scale = scale, a.out = out, a.stride = one_stride(n_ctx);
     a.n_split = one_splits(B, HKV, n_ctx, n_cu);
     a.scores = (float *)scratch, a.part = a.scores + (int64_t)B * H * a.stride;
+    rows_derive(a, HD);
     return rows_by_shape(HD, kv_f16, [&](auto hd, auto f16) {
         constexpr int D = decltype(hd)::value;
         const hipError_t e = rows_launch<D, decltype(f16)::value>(a, B, true, s);
@@ -697,13 +778,14 @@ hipError_t launch_attn_prompt_weights(const float *q, int nq, int H, int HKV, in
     a.mode = ROWS_CAUSAL, a.scale = scale, a.out = out, a.n_split = p.ns;
     a.planes = (uint4 *)base, a.p2e = (float *)(base + p.planes), a.lse = (float *)(base + p.planes + p.p2e);
     a.part = (float *)(base + p.planes + p.p2e + p.lse);
+    rows_derive(a, HD);
     return rows_by_shape(HD, kv_f16, [&](auto hd, auto f16) {
         constexpr int D = decltype(hd)::value;
         constexpr bool F = decltype(f16)::value;
         hipError_t e = rows_launch<D, F>(a, 1, false, s);
         if (e == hipSuccess && a.n_split > 1) e = rows_launch_merge<D>(a, 1, s);
         if (e != hipSuccess) return e;
-        constexpr int KT = D == 256 ? 1 : 2, per = 4 * 16 * KT;
+        constexpr int KT = D == 256 ? 1 : 2, per = 16 * KT;
         hipLaunchKernelGGL((k_prompt_weights<D, F, KT>), dim3((pos0 + nq + per - 1) / per, HKV), dim3(256), 0, s, a, acc,
                            acc_out);
         return hipGetLastError();

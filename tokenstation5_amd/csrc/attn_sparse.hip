@@ -199,6 +199,11 @@ __global__ __launch_bounds__(64 * NW) void k_attn_picked(SparseArgs a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int rl = lane & 15, kq = lane >> 4;
     const int split = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z, G = a.H / a.HKV;
+    RowsIn<HD, 1> in;  // requested before the counts that the keys' addresses wait for
+    rows_request<HD, 1>(in, kq, [&](int, bool &ok) {
+        ok = rl < G;
+        return a.q + ((int64_t)b * a.H + kvh * G + min(rl, G - 1)) * HD;
+    });
     const int n = sparse_count(a, b), units = sparse_units(a, b, KT), per = (units + a.n_split - 1) / a.n_split;
     const int u0 = split * per, u1 = min(units, u0 + per);
     if (u0 >= u1) return;
@@ -217,11 +222,7 @@ __global__ __launch_bounds__(64 * NW) void k_attn_picked(SparseArgs a) {
     at(u0 + wave, kn);
     rows_load<HD, F16, KT>(nxt, kv, kn, rl, kq);
     RowsQ<HD, 1> q;
-    rows_query<HD, 1>(q, a.scale, kq,
-                      [&](int, bool &ok) {
-                          ok = rl < G;
-                          return a.q + ((int64_t)b * a.H + kvh * G + min(rl, G - 1)) * HD;
-                      });
+    rows_query<HD, 1>(q, in, a.scale);
     RowsSum<HD, 1> sum;
     rows_clear<HD, 1>(sum);
     for (int u = u0 + wave; u < u1; u += NW) {
