@@ -62,7 +62,7 @@ __device__ inline void rows_add_nonfinite(const RowsArgs &a, int b, int kvh, int
 // grid (n_split, HKV * row blocks of 16 NT, B): one slice of the keys for 16 NT rows,
 // row r = G t + j being head j of token t. The waves take the slice's units in turn.
 template <int HD, bool F16, int KT, int NT, int NW, bool ONE>
-__global__ __launch_bounds__(64 * NW) void k_attn_rows(RowsArgs a) {
+__global__ __launch_bounds__(64 * NW, ONE && HD <= 128 ? 3 : 1) void k_attn_rows(RowsArgs a) {
     using S = RowsShape<HD, F16, KT>;
     __shared__ RowsLds<HD, NW> L;
     __shared__ int nonfinite;  // a masked unit left out infinite or NaN values
@@ -127,27 +127,19 @@ __global__ __launch_bounds__(64 * NW) void k_attn_rows(RowsArgs a) {
     if (!ONE) __syncthreads();  // the flag is set
     const int64_t row0 = ((int64_t)b * a.HKV + kvh) * R + r0;
     if constexpr (ONE) {
-        // Two units ahead: an iteration's loads go out as soon as their registers are
-        // free, and it ends nowhere else, so that a wait for one unit leaves the next in flight.
+        // One unit ahead in three waves a SIMD; two ahead in two waves is no faster (122 us), and in three it
+        // spills (170 us).
         auto put = [&](int, int key, const float (&s)[4]) {
             if (rl < rows && key < kend)
                 *(float4 *)(a.scores + (row0 + rl) * a.stride + key) =
                     make_float4(s[0] * q.p2e[0], s[1] * q.p2e[0], s[2] * q.p2e[0], s[3] * q.p2e[0]);
         };
         auto seen4 = [&](int, int key) { return rows_below(key, kend); };
-        RowsUnit<HD, F16, KT> far;
-        at(wave + NW, kb);
-        rows_load<HD, F16, KT>(far, kv, kb, rl, kq);
-        for (int u = wave; u < units; u += 2 * NW) {
-            RowsUnit<HD, F16, KT> cur = nxt;
-            at(u + 2 * NW, kb);
+        for (int u = wave; u < units; u += NW) {
+            const RowsUnit<HD, F16, KT> cur = nxt;
+            at(u + NW, kb);
             rows_load<HD, F16, KT>(nxt, kv, kb, rl, kq);  // (past the slice: zeros, no memory access)
             at(u, kb);
-            rows_unit<HD, F16, KT, NT, true, false>(cur, q, sum, kb, kq, seen4, put);
-            cur = far;
-            at(u + 3 * NW, kb);
-            rows_load<HD, F16, KT>(far, kv, kb, rl, kq);
-            at(u + NW, kb);  // (past the slice: no key of it is taken)
             rows_unit<HD, F16, KT, NT, true, false>(cur, q, sum, kb, kq, seen4, put);
         }
     } else {
@@ -551,18 +543,21 @@ __global__ __launch_bounds__(256) void k_one_weights(RowsArgs a, const float *ac
 }
 
 // A prompt chunk's weights summed over its queries, for each key: a wave holds a unit's
-// K and goes over every fourth row tile's planes (the next one's requested before this one's products),
-// sums 2^(score - lse) in its lanes, and the workgroup adds lanes and waves in order at the end. grid
-// (units, HKV).
+// K and goes over every other row tile's planes (the next one's requested before this one's products),
+// sums 2^(score - lse) in its lanes, and the workgroup adds lanes and waves in order at the end. Four
+// waves with units of their own take the same row tiles: the L1 serves three of them
+// (waves that shared a unit instead read 540 MB of planes from the L2 for 256 queries over 4096 keys, 32 us).
+// grid (blocks of PW_UNITS units, HKV).
+constexpr int PW_UNITS = 4, PW_ROWS = 2;
 template <int HD, bool F16, int KT>
-__global__ __launch_bounds__(256) void k_prompt_weights(RowsArgs a, const float *acc, float *acc_out) {
+__global__ __launch_bounds__(64 * PW_UNITS * PW_ROWS) void k_prompt_weights(RowsArgs a, const float *acc, float *acc_out) {
     using S = RowsShape<HD, F16, KT>;
     constexpr int NC = S::NC;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int rl = lane & 15, kq = lane >> 4, kvh = blockIdx.y;
     const int G = a.H / a.HKV, R = a.T * G, tiles = (R + 15) / 16, n = a.pos0 + a.T;
-    const int k0 = blockIdx.x * S::UNIT;
-    __shared__ float part[4][KT][16];
+    const int unit = wave % PW_UNITS, rows = wave / PW_UNITS, k0 = (blockIdx.x * PW_UNITS + unit) * S::UNIT;
+    __shared__ float part[PW_ROWS][PW_UNITS][KT][16];
     const RowsKv kv = rows_kv<HD, F16>(a.kv, (int64_t)kvh * a.n_ctx, n);
     RowsUnit<HD, F16, KT> u;
     ar_h8 ka[KT][NC];
@@ -584,7 +579,7 @@ __global__ __launch_bounds__(256) void k_prompt_weights(RowsArgs a, const float 
         for (int i = 0; i < 4; i++) w[t][i] = 0.f;
     }
     // The first row that sees key k0: token max(0, k0 - pos0).
-    const int first = max(0, k0 - a.pos0) * G / 16;
+    const int first = k0 < n ? max(0, k0 - a.pos0) * G / 16 : tiles;
     const uint4 *pl = a.planes + (int64_t)kvh * tiles * NC * 2 * 64 + lane;
     struct Tile {
         uint4 h[NC], l[NC];
@@ -600,13 +595,13 @@ __global__ __launch_bounds__(256) void k_prompt_weights(RowsArgs a, const float 
         nxt.p2e = a.p2e[((int64_t)kvh * tiles + at) * 16 + rl];
         nxt.lse = a.lse[(int64_t)kvh * R + min(16 * at + rl, R - 1)];
     };
-    request(first + wave);
-    for (int tile = first + wave; tile < tiles; tile += 4) {
+    request(first + rows);
+    for (int tile = first + rows; tile < tiles; tile += PW_ROWS) {
         ar_h8 qh[NC], ql[NC];
 #pragma unroll
         for (int c = 0; c < NC; c++) qh[c] = __builtin_bit_cast(ar_h8, nxt.h[c]), ql[c] = __builtin_bit_cast(ar_h8, nxt.l[c]);
         const float p2e = nxt.p2e, lse = nxt.lse;
-        request(tile + 4);
+        request(tile + PW_ROWS);
         const int r = 16 * tile + rl;
         const int last = a.pos0 + rows_div(r, a.g_m);  // the last key the row sees
 #pragma unroll
@@ -642,13 +637,15 @@ __global__ __launch_bounds__(256) void k_prompt_weights(RowsArgs a, const float 
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const float x = row_sum_dpp(w[t][i]);
-            if (rl == 0) part[wave][t][4 * kq + i] = x;
+            if (rl == 0) part[rows][unit][t][4 * kq + i] = x;
         }
     __syncthreads();
-    const int e = threadIdx.x;
-    if (e < S::UNIT && k0 + e < n) {
-        const float x = (part[0][e / 16][e % 16] + part[1][e / 16][e % 16]) + (part[2][e / 16][e % 16] + part[3][e / 16][e % 16]);
-        acc_out[(int64_t)kvh * a.n_ctx + k0 + e] = acc[(int64_t)kvh * a.n_ctx + k0 + e] + x;
+    const int e = threadIdx.x, key = blockIdx.x * PW_UNITS * S::UNIT + e;
+    if (e < PW_UNITS * S::UNIT && key < n) {
+        float x = 0.f;
+#pragma unroll
+        for (int r = 0; r < PW_ROWS; r++) x += part[r][e / S::UNIT][e % S::UNIT / 16][e % 16];
+        acc_out[(int64_t)kvh * a.n_ctx + key] = acc[(int64_t)kvh * a.n_ctx + key] + x;
     }
 }
 
@@ -684,7 +681,7 @@ static hipError_t rows_launch(const RowsArgs &a, int B, bool one, hipStream_t s)
     const dim3 grid(a.n_split, a.HKV * a.nrb, B);
     constexpr int NW = HD == 256 ? 4 : 8, K1 = rows_kt(HD, 1), K2 = rows_kt(HD, 2);
     if (one) {
-        hipLaunchKernelGGL((k_attn_rows<HD, F16, K1, 1, NW, true>), grid, dim3(64 * NW), 0, s, a);
+        hipLaunchKernelGGL((k_attn_rows<HD, F16, K1, 1, 4, true>), grid, dim3(256), 0, s, a);
     } else if (rows_tile(R, HD)) {
         hipLaunchKernelGGL((k_attn_tile<HD, F16>), grid, dim3(256), 0, s, a);
     } else if (HD == 256 || R <= 16) {
@@ -724,9 +721,9 @@ hipError_t launch_attn_tree(const float *q, int B, int T, int H, int HKV, int HD
     });
 }
 
-// Two rounds of workgroups: sequences of different lengths leave less of the last one idle (16 of 12288 to 16384
-// keys: 122 us, 127 in one round, 130 in four).
-static int one_splits(int B, int HKV, int n_ctx, int n_cu) { return rows_splits(B * HKV, n_ctx, 2 * n_cu); }
+// Two rounds of the three workgroups that a CU holds: sequences of different lengths leave less of the
+// last one idle (16 of 12288 to 16384 keys: 121 us, 125 in one round, 132 in one and a third).
+static int one_splits(int B, int HKV, int n_ctx, int n_cu) { return rows_splits(B * HKV, n_ctx, 6 * n_cu); }
 static int64_t one_stride(int n_ctx) { return ((int64_t)n_ctx + 31) / 32 * 32; }
 size_t attn_one_weights_scratch_bytes(int B, int H, int HKV, int HD, int n_ctx, int n_cu) {
     return (size_t)B * H * (one_stride(n_ctx) + (size_t)one_splits(B, HKV, n_ctx, n_cu) * (HD + 4)) * sizeof(float);
@@ -785,9 +782,9 @@ hipError_t launch_attn_prompt_weights(const float *q, int nq, int H, int HKV, in
         hipError_t e = rows_launch<D, F>(a, 1, false, s);
         if (e == hipSuccess && a.n_split > 1) e = rows_launch_merge<D>(a, 1, s);
         if (e != hipSuccess) return e;
-        constexpr int KT = D == 256 ? 1 : 2, per = 16 * KT;
-        hipLaunchKernelGGL((k_prompt_weights<D, F, KT>), dim3((pos0 + nq + per - 1) / per, HKV), dim3(256), 0, s, a, acc,
-                           acc_out);
+        constexpr int KT = D == 256 ? 1 : 2, per = PW_UNITS * 16 * KT;
+        hipLaunchKernelGGL((k_prompt_weights<D, F, KT>), dim3((pos0 + nq + per - 1) / per, HKV),
+                           dim3(64 * PW_UNITS * PW_ROWS), 0, s, a, acc, acc_out);
         return hipGetLastError();
     });
 }
