@@ -181,7 +181,9 @@ __device__ inline void rows_query(RowsQ<HD, NT> &q, const RowsIn<HD, NT> &in, fl
 #pragma unroll
             for (int k = 0; k < 2; k++) {
                 const float4 x = in.x[qt][c][k];
-                amax = fmaxf(fmaxf(amax, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(x.z), fabsf(x.w)));
+                // (fmaxf quiets each operand first: three instructions a value)
+                asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(amax) : "v"(x.x), "v"(x.y));
+                asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(amax) : "v"(x.z), "v"(x.w));
             }
         amax = max_xor32(max_xor16(amax)) * fabsf(by);
         const int e = amax > 0.f ? max(ilogbf(amax) - 13, -100) : 0;
@@ -486,13 +488,13 @@ __device__ inline void rows_combine(RowsLds<HD, NW> &L, const RowsSum<HD, NT> &a
 __host__ inline uint64_t rows_magic(int d) { return ((1ull << 36) + d - 1) / d; }
 __host__ __device__ inline int rows_div(int x, uint64_t m) { return (int)((uint64_t)(uint32_t)x * m >> 36); }
 
-// Keys of each of n_split slices of n keys: at least ROWS_MIN_KEYS, and whole blocks of k_attn_tile
-// (a slice that ended inside one would count the zeros behind it).
+// Keys of each of n_split slices of n keys: at least `least`, and whole blocks of k_attn_tile (a slice that
+// ended inside one would count the zeros behind it).
 constexpr int ROWS_MIN_KEYS = 128;
 constexpr int ROWS_MAX_SPLIT = 64;
-__host__ __device__ inline int rows_chunk(int n, int n_split, uint64_t split_m) {  // split_m = rows_magic(n_split)
+__host__ __device__ inline int rows_chunk(int n, int n_split, uint64_t split_m, int least) {  // split_m = rows_magic(n_split)
     int c = rows_div(n + n_split - 1, split_m);
-    c = c < ROWS_MIN_KEYS ? ROWS_MIN_KEYS : c;
+    c = c < least ? least : c;
     return (c + 63) / 64 * 64;
 }
 

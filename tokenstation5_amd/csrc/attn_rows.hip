@@ -12,6 +12,7 @@ struct RowsArgs {
     KvLayer kv;      // B caches
     int n_ctx, H, HKV, T, n_split;
     int G, R, nrb;  // query heads a KV head, rows T * G, blocks of rows
+    int least;      // keys a slice takes at least
     uint64_t g_m, nrb_m, split_m;  // rows_magic of G, nrb, n_split
     const int32_t *n_keys;  // per cache: the keys before the T tokens (tree), or all keys (one query)
     const uint64_t *mask;   // [B][T], tree
@@ -78,7 +79,7 @@ __global__ __launch_bounds__(64 * NW, ONE && HD <= 128 ? 3 : 1) void k_attn_rows
         ok = r < R;
         return a.q + rows_at(a, b, kvh, min(r, R - 1)) * HD;
     });
-    const int n = rows_count(a, b), chunk = rows_chunk(rows_all(a, n), a.n_split, a.split_m);
+    const int n = rows_count(a, b), chunk = rows_chunk(rows_all(a, n), a.n_split, a.split_m, a.least);
     const int kbeg = split * chunk, kend = min(kbeg + chunk, rows_reach(a, n, rows_div(r0 + rows - 1, a.g_m)));
     if (kbeg >= kend) return;  // the merge reads no partial of this slice
     const int full = a.mode == ROWS_CAUSAL ? n + rows_div(r0, a.g_m) + 1 : n;  // keys before it are every row's
@@ -217,7 +218,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_tile(RowsArgs a) {
         ok = r < R;
         return a.q + rows_at(a, b, kvh, min(r, R - 1)) * HD;
     });
-    const int n = rows_count(a, b), chunk = rows_chunk(rows_all(a, n), a.n_split, a.split_m);
+    const int n = rows_count(a, b), chunk = rows_chunk(rows_all(a, n), a.n_split, a.split_m, a.least);
     const int kbeg = split * chunk, kend = min(kbeg + chunk, rows_reach(a, n, rows_div(min(R, r0 + S::ROWS) - 1, a.g_m)));
     if (kbeg >= kend) return;  // the merge reads no partial of this slice
     const int full = a.mode == ROWS_CAUSAL ? n + rows_div(r0, a.g_m) + 1 : n;  // keys before it are every row's
@@ -481,7 +482,7 @@ __global__ __launch_bounds__(256) void k_rows_merge(RowsArgs a, int64_t rows) {
     const int64_t row = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR, at = min(row, rows - 1);
     const int d = 4 * ((int)threadIdx.x % (HD / 4)), R = a.R;
     const int b = (int)(at / ((int64_t)a.HKV * R)), kvh = (int)(at / R % a.HKV), r = (int)(at % R), t = rows_div(r, a.g_m);
-    const int n = rows_count(a, b), chunk = rows_chunk(rows_all(a, n), a.n_split, a.split_m);
+    const int n = rows_count(a, b), chunk = rows_chunk(rows_all(a, n), a.n_split, a.split_m, a.least);
     const int used = (rows_reach(a, n, t) + chunk - 1) / chunk;
     float M, l;
     const float4 o = rows_join<HD, SG>(J, a.part + at * a.n_split * (HD + 4), used, M, l);
@@ -498,7 +499,7 @@ __global__ __launch_bounds__(256) void k_one_weights(RowsArgs a, const float *ac
     __shared__ float lse[ROWS_MAX_G];
     constexpr int TPR = HD / 4 * JOIN_SG;
     const int kvh = blockIdx.y, b = blockIdx.z, G = a.H / a.HKV, tid = threadIdx.x;
-    const int n = rows_count(a, b), chunk = rows_chunk(n, a.n_split, a.split_m), used = (n + chunk - 1) / chunk;
+    const int n = rows_count(a, b), chunk = rows_chunk(n, a.n_split, a.split_m, a.least), used = (n + chunk - 1) / chunk;
     const int64_t head = (int64_t)b * a.HKV + kvh, row0 = head * G;
     if (blockIdx.x == 0) {
         for (int g0 = 0; g0 < G; g0 += 256 / TPR) {
@@ -660,8 +661,15 @@ static int rows_blocks(int R, int HD) {
 }
 // Tiles of keys a unit.
 constexpr int rows_kt(int HD, int NT) { return HD == 256 || (HD == 128 && NT == 1) ? 1 : 2; }
-static int rows_splits(int items, int keys, int slots) {
-    const int most = std::min((keys + ROWS_MIN_KEYS - 1) / ROWS_MIN_KEYS, ROWS_MAX_SPLIT);
+// A slice reads at least half as many bytes of keys and values as its rows' queries and partials take
+// (84 rows over 4096 keys of 32/8 heads: 128 keys a slice 27.5 us with the join, 192 25.3, 256 26.7, 384 30.8).
+static int rows_least(int R, int HD, int kv_f16) {
+    const int rows = std::min(R, HD == 256 ? 64 : 128), key = 2 * (kv_f16 ? 2 * HD : HD + HD / 16);
+    const int n = rows * (2 * HD + 4) * 4 / (2 * key);
+    return std::max(ROWS_MIN_KEYS, (n + 63) / 64 * 64);
+}
+static int rows_splits(int items, int keys, int slots, int least) {
+    const int most = std::min((keys + least - 1) / least, ROWS_MAX_SPLIT);
     return std::max(1, std::min(slots / std::max(items, 1), most));
 }
 
@@ -670,7 +678,8 @@ bool attn_rows_supported(int H, int HKV, int HD) {
 }
 
 // The arguments that follow from the others.
-static void rows_derive(RowsArgs &a, int HD) {
+static void rows_derive(RowsArgs &a, int HD, int kv_f16) {
+    a.least = rows_least(a.T * (a.H / a.HKV), HD, kv_f16);
     a.G = a.H / a.HKV, a.R = a.T * a.G, a.nrb = rows_blocks(a.R, HD);
     a.g_m = rows_magic(a.G), a.nrb_m = rows_magic(a.nrb), a.split_m = rows_magic(a.n_split);
 }
@@ -699,12 +708,13 @@ static hipError_t rows_launch_merge(const RowsArgs &a, int B, hipStream_t s) {
     else hipLaunchKernelGGL((k_rows_merge<HD, JOIN_SG>), grid(HD / 4 * JOIN_SG), dim3(256), 0, s, a, rows);
     return hipGetLastError();
 }
-static int tree_splits(int B, int T, int H, int HKV, int HD, int n_ctx, int n_cu) {
+static int tree_splits(int B, int T, int H, int HKV, int HD, int kv_f16, int n_ctx, int n_cu) {
     const int R = T * (H / HKV);
-    return rows_splits(B * HKV * rows_blocks(R, HD), n_ctx, rows_tile(R, HD) ? 2 * n_cu : n_cu);
+    return rows_splits(B * HKV * rows_blocks(R, HD), n_ctx, rows_tile(R, HD) ? 2 * n_cu : n_cu,
+                       rows_least(R, HD, kv_f16));
 }
-size_t attn_tree_scratch_bytes(int B, int T, int H, int HKV, int HD, int n_ctx, int n_cu) {
-    const int ns = tree_splits(B, T, H, HKV, HD, n_ctx, n_cu);
+size_t attn_tree_scratch_bytes(int B, int T, int H, int HKV, int HD, int kv_f16, int n_ctx, int n_cu) {
+    const int ns = tree_splits(B, T, H, HKV, HD, kv_f16, n_ctx, n_cu);
     return ns > 1 ? (size_t)B * T * H * ns * (HD + 4) * sizeof(float) : 0;
 }
 hipError_t launch_attn_tree(const float *q, int B, int T, int H, int HKV, int HD, KvLayer kv, int kv_f16, int n_ctx,
@@ -713,8 +723,8 @@ hipError_t launch_attn_tree(const float *q, int B, int T, int H, int HKV, int HD
     RowsArgs a{};
     a.q = q, a.kv = kv, a.n_ctx = n_ctx, a.H = H, a.HKV = HKV, a.T = T, a.n_keys = n_past, a.mask = mask;
     a.mode = ROWS_TREE, a.scale = scale, a.part = part, a.out = out;
-    a.n_split = tree_splits(B, T, H, HKV, HD, n_ctx, n_cu);
-    rows_derive(a, HD);
+    a.n_split = tree_splits(B, T, H, HKV, HD, kv_f16, n_ctx, n_cu);
+    rows_derive(a, HD, kv_f16);
     return rows_by_shape(HD, kv_f16, [&](auto hd, auto f16) {
         const hipError_t e = rows_launch<decltype(hd)::value, decltype(f16)::value>(a, B, false, s);
         return e != hipSuccess || a.n_split == 1 ? e : rows_launch_merge<decltype(hd)::value>(a, B, s);
@@ -723,7 +733,7 @@ hipError_t launch_attn_tree(const float *q, int B, int T, int H, int HKV, int HD
 
 // Two rounds of the three workgroups that a CU holds: sequences of different lengths leave less of the
 // last one idle (16 of 12288 to 16384 keys: 121 us, 125 in one round, 132 in one and a third).
-static int one_splits(int B, int HKV, int n_ctx, int n_cu) { return rows_splits(B * HKV, n_ctx, 6 * n_cu); }
+static int one_splits(int B, int HKV, int n_ctx, int n_cu) { return rows_splits(B * HKV, n_ctx, 6 * n_cu, ROWS_MIN_KEYS); }
 static int64_t one_stride(int n_ctx) { return ((int64_t)n_ctx + 31) / 32 * 32; }
 size_t attn_one_weights_scratch_bytes(int B, int H, int HKV, int HD, int n_ctx, int n_cu) {
     return (size_t)B * H * (one_stride(n_ctx) + (size_t)one_splits(B, HKV, n_ctx, n_cu) * (HD + 4)) * sizeof(float);
@@ -736,7 +746,7 @@ hipError_t launch_attn_one_weights(const float *q, int B, int H, int HKV, int HD
     a.mode = ROWS_ONE, a.scale = scale, a.out = out, a.stride = one_stride(n_ctx);
     a.n_split = one_splits(B, HKV, n_ctx, n_cu);
     a.scores = (float *)scratch, a.part = a.scores + (int64_t)B * H * a.stride;
-    rows_derive(a, HD);
+    rows_derive(a, HD, kv_f16);
     return rows_by_shape(HD, kv_f16, [&](auto hd, auto f16) {
         constexpr int D = decltype(hd)::value;
         const hipError_t e = rows_launch<D, decltype(f16)::value>(a, B, true, s);
@@ -751,31 +761,31 @@ struct PromptWeightsScratch {
     int ns;
     size_t part, planes, p2e, lse;  // bytes
 };
-static PromptWeightsScratch prompt_scratch(int nq, int H, int HKV, int HD, int n_keys, int n_cu) {
+static PromptWeightsScratch prompt_scratch(int nq, int H, int HKV, int HD, int kv_f16, int n_keys, int n_cu) {
     const int R = nq * (H / HKV), tiles = (R + 15) / 16;
     PromptWeightsScratch p;
-    p.ns = rows_splits(HKV * rows_blocks(R, HD), n_keys, 2 * n_cu);
+    p.ns = rows_splits(HKV * rows_blocks(R, HD), n_keys, 2 * n_cu, rows_least(R, HD, kv_f16));
     p.part = p.ns > 1 ? (size_t)nq * H * p.ns * (HD + 4) * sizeof(float) : 0;
     p.planes = (size_t)HKV * tiles * HD / 32 * 2 * 64 * sizeof(uint4);
     p.p2e = (size_t)HKV * tiles * 16 * sizeof(float);
     p.lse = (size_t)HKV * R * sizeof(float);
     return p;
 }
-size_t attn_prompt_weights_scratch_bytes(int nq, int H, int HKV, int HD, int n_keys, int n_cu) {
-    const PromptWeightsScratch p = prompt_scratch(nq, H, HKV, HD, n_keys, n_cu);
+size_t attn_prompt_weights_scratch_bytes(int nq, int H, int HKV, int HD, int kv_f16, int n_keys, int n_cu) {
+    const PromptWeightsScratch p = prompt_scratch(nq, H, HKV, HD, kv_f16, n_keys, n_cu);
     return p.part + p.planes + p.p2e + p.lse;
 }
 hipError_t launch_attn_prompt_weights(const float *q, int nq, int H, int HKV, int HD, KvLayer kv, int kv_f16, int n_ctx,
                                       int pos0, float scale, void *scratch, float *out, const float *acc,
                                       float *acc_out, int n_cu, hipStream_t s) {
-    const PromptWeightsScratch p = prompt_scratch(nq, H, HKV, HD, pos0 + nq, n_cu);
+    const PromptWeightsScratch p = prompt_scratch(nq, H, HKV, HD, kv_f16, pos0 + nq, n_cu);
     uint8_t *base = (uint8_t *)scratch;
     RowsArgs a{};
     a.q = q, a.kv = kv, a.n_ctx = n_ctx, a.H = H, a.HKV = HKV, a.T = nq, a.pos0 = pos0;
     a.mode = ROWS_CAUSAL, a.scale = scale, a.out = out, a.n_split = p.ns;
     a.planes = (uint4 *)base, a.p2e = (float *)(base + p.planes), a.lse = (float *)(base + p.planes + p.p2e);
     a.part = (float *)(base + p.planes + p.p2e + p.lse);
-    rows_derive(a, HD);
+    rows_derive(a, HD, kv_f16);
     return rows_by_shape(HD, kv_f16, [&](auto hd, auto f16) {
         constexpr int D = decltype(hd)::value;
         constexpr bool F = decltype(f16)::value;

@@ -94,7 +94,8 @@ int ts5hip_attn_tree(ts5hip_ctx *ctx, const float *q, int B, int n_tree, int n_h
         return fail(ctx, TS5HIP_ERR_ARG, "q and out need 16-byte, masks 8-byte alignment");
     if (!ctx) return fail(nullptr, TS5HIP_ERR_ARG, "ctx is null");
     const OnDevice on(ctx->device);
-    if (int rc = ensure_scratch(ctx, attn_tree_scratch_bytes(B, n_tree, n_head, n_head_kv, head_dim, n_ctx, ctx->n_cu)))
+    if (int rc = ensure_scratch(ctx, attn_tree_scratch_bytes(B, n_tree, n_head, n_head_kv, head_dim, kv_type == KV_F16, n_ctx,
+                                                              ctx->n_cu)))
         return rc;
     TS5_HIP(ctx, launch_attn_tree(q, B, n_tree, n_head, n_head_kv, head_dim, layer(k, ks, v, vs), kv_type == KV_F16,
                                   n_ctx, n_past_dev, mask_dev, scale, (float *)ctx->scratch, out, ctx->n_cu,
@@ -144,8 +145,8 @@ int ts5hip_attn_prompt_weights(ts5hip_ctx *ctx, const float *q, int nq, int n_he
     if (!aligned(q, 16) || !aligned(out, 16)) return fail(ctx, TS5HIP_ERR_ARG, "q and out need 16-byte alignment");
     if (!ctx) return fail(nullptr, TS5HIP_ERR_ARG, "ctx is null");
     const OnDevice on(ctx->device);
-    if (int rc = ensure_scratch(ctx, attn_prompt_weights_scratch_bytes(nq, n_head, n_head_kv, head_dim, pos0 + nq,
-                                                                       ctx->n_cu)))
+    if (int rc = ensure_scratch(ctx, attn_prompt_weights_scratch_bytes(nq, n_head, n_head_kv, head_dim, kv_type == KV_F16,
+                                                                       pos0 + nq, ctx->n_cu)))
         return rc;
     TS5_HIP(ctx, launch_attn_prompt_weights(q, nq, n_head, n_head_kv, head_dim, layer(k, ks, v, vs), kv_type == KV_F16,
                                             n_ctx, pos0, scale, ctx->scratch, out, acc, acc_out, ctx->n_cu,

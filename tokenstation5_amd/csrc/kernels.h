@@ -178,7 +178,7 @@ hipError_t launch_kv_write(KvLayer kv, int which, int HKV, int HD, int n_ctx, in
 // size that the function beside each launcher gives, 16-byte aligned.
 bool attn_rows_supported(int H, int HKV, int HD);
 // T tokens (at most 64) of each of B caches: every key below n_past[b], and of the T after them those of its mask's bits.
-size_t attn_tree_scratch_bytes(int B, int T, int H, int HKV, int HD, int n_ctx, int n_cu);
+size_t attn_tree_scratch_bytes(int B, int T, int H, int HKV, int HD, int kv_f16, int n_ctx, int n_cu);
 hipError_t launch_attn_tree(const float *q, int B, int T, int H, int HKV, int HD, KvLayer kv, int kv_f16, int n_ctx,
                             const int32_t *n_past, const uint64_t *mask, float scale, float *scratch, float *out,
                             int n_cu, hipStream_t s);
@@ -188,7 +188,7 @@ hipError_t launch_attn_one_weights(const float *q, int B, int H, int HKV, int HD
                                    const int32_t *n_keys, float scale, void *scratch, float *out, const float *acc,
                                    float *acc_out, int n_cu, hipStream_t s);
 // nq consecutive queries over one cache, causal, and the same sums.
-size_t attn_prompt_weights_scratch_bytes(int nq, int H, int HKV, int HD, int n_keys, int n_cu);
+size_t attn_prompt_weights_scratch_bytes(int nq, int H, int HKV, int HD, int kv_f16, int n_keys, int n_cu);
 hipError_t launch_attn_prompt_weights(const float *q, int nq, int H, int HKV, int HD, KvLayer kv, int kv_f16, int n_ctx,
                                       int pos0, float scale, void *scratch, float *out, const float *acc,
                                       float *acc_out, int n_cu, hipStream_t s);
