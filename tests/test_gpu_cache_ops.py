@@ -375,9 +375,11 @@ def test_prompt_weights_long(ctx):
 
 
 @pytest.mark.parametrize("kv", [Q8, F16])
-def test_prompt_weights_nonfinite_later_keys(ctx, kv):
-    """An infinite value of a later token of the chunk does not reach the queries before it."""
-    H, HKV, HD, nq, pos0 = 8, 2, 128, 20, 50
+@pytest.mark.parametrize("H,HKV,HD", [(14, 2, 64), (2, 2, 128), (8, 2, 128), (32, 4, 128), (8, 4, 256), (16, 2, 256)])
+def test_prompt_weights_nonfinite_later_keys(ctx, kv, H, HKV, HD):
+    """NaN keys and values of a later token of the chunk do not reach the queries before it: rows for every form
+    of the kernel (one and two row tiles, four and eight waves)."""
+    nq, pos0 = 20, 50
     rng = np.random.default_rng(22)
     c = Cache(ctx, rng, kv, 1, HKV, 70, HD)
     for n in "kv":

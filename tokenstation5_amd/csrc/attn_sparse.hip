@@ -44,17 +44,25 @@ __global__ __launch_bounds__(256) void k_block_bounds(KvLayer kv, int HKV, int n
     float lo[V], hi[V];
 #pragma unroll
     for (int j = 0; j < V; j++) lo[j] = INFINITY, hi[j] = -INFINITY;
-    for (int r = first + lane / LPR; r < last; r += RPW) {
-        const u32x4 w = *(const u32x4 *)(kv.k + ((slot0 + r) * HD + d0) * VB);
-        float sc = 1.f;
-        if constexpr (!F16) sc = h2f(kv.ks[(slot0 + r) * (HD / 32) + d0 / 32]);
+    constexpr int AHEAD = 4;  // passes requested before the first is used (rows past the last: the last again)
+    for (int r0 = first + lane / LPR; r0 < last; r0 += AHEAD * RPW) {
+        u32x4 w[AHEAD];
+        uint16_t sc[AHEAD];
 #pragma unroll
-        for (int j = 0; j < V; j++) {
-            float x;
-            if constexpr (F16) x = h2f((w[j / 2] >> (16 * (j & 1))) & 0xffff);
-            else x = (float)(int8_t)(w[j / 4] >> (8 * (j & 3))) * sc;
-            lo[j] = fminf(lo[j], x), hi[j] = fmaxf(hi[j], x);  // (NaN: passed over)
+        for (int k = 0; k < AHEAD; k++) {
+            const int64_t r = slot0 + min(r0 + k * RPW, last - 1);
+            w[k] = *(const u32x4 *)(kv.k + (r * HD + d0) * VB);
+            if constexpr (!F16) sc[k] = kv.ks[r * (HD / 32) + d0 / 32];
         }
+#pragma unroll
+        for (int k = 0; k < AHEAD; k++)
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                float x;
+                if constexpr (F16) x = h2f((w[k][j / 2] >> (16 * (j & 1))) & 0xffff);
+                else x = (float)(int8_t)(w[k][j / 4] >> (8 * (j & 3))) * h2f(sc[k]);
+                lo[j] = fminf(lo[j], x), hi[j] = fmaxf(hi[j], x);  // (NaN: passed over)
+            }
     }
 #pragma unroll
     for (int o = LPR; o < 64; o <<= 1)

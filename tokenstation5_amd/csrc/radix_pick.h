@@ -5,7 +5,7 @@
 // it ends once a bin is taken whole. The keys are staged in LDS, sixteen requests at a time, and a
 // thread takes an odd number of neighbours there (an odd stride meets no bank twice), so that the
 // last pass is counts and bit masks of its own keys instead of ballots; the picked
-// indices go out through LDS in order. 32768 keys: 23 us (8-bit digits from memory: 60). Deterministic.
+// indices go out through LDS in order. 32768 keys: 27 us (8-bit digits from memory: 60). Deterministic.
 #pragma once
 #include "common.h"
 
@@ -27,12 +27,13 @@ struct PickLds {
 template <class L_>
 __device__ inline uint32_t pick_scan(L_ &L, uint32_t v, uint32_t &total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    uint32_t x = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t y = __shfl_up(x, o, 64);
-        if (lane >= o) x += y;
-    }
+    uint32_t x = v;  // the wave's inclusive sums by DPP: shifts within 16-lane rows, then the rows' last lanes on
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true);   // row_shr:1
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true);   // row_shr:2
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xE, true);   // row_shr:4
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xC, true);   // row_shr:8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
     __syncthreads();
     if (lane == 63) L.wave[wave] = x;
     __syncthreads();
@@ -125,15 +126,19 @@ __device__ inline void radix_pick(PickLds<T, CAP> &L, int n, int k, Fetch fetch,
         const uint32_t mine = (uint32_t)__popcll(above) | (uint32_t)__popcll(equal) << 16;
         const uint32_t before = pick_scan(L, mine, total);  // (its barriers: every key has been read)
         int eq = eq0 + (int)(before >> 16), place = (int)(before & 0xffff) + max(0, min(eq, left) - min(eq0, left));
-        for (uint64_t bits = above | equal; bits; bits &= bits - 1) {
-            const int j = __ffsll((unsigned long long)bits) - 1;
-            if ((above >> j & 1) || eq < left) L.key[place++] = (T)(i0 + j);
-            eq += (int)(equal >> j & 1);
+#pragma unroll
+        for (int w = 0; w < 2; w++) {  // (32 bits at a time)
+            const uint32_t a = (uint32_t)(above >> (32 * w)), e = (uint32_t)(equal >> (32 * w));
+            for (uint32_t bits = a | e; bits; bits &= bits - 1) {
+                const int j = __ffs((int)bits) - 1;
+                if ((a >> j & 1) || eq < left) L.key[place++] = (T)(i0 + 32 * w + j);
+                eq += (int)(e >> j & 1);
+            }
         }
         __syncthreads();
-        const int at = gt0 + min(eq0, left), gts = (int)(total & 0xffff), eqs = (int)(total >> 16);
+        const int first = gt0 + min(eq0, left), gts = (int)(total & 0xffff), eqs = (int)(total >> 16);
         const int taken = gts + min(eq0 + eqs, left) - min(eq0, left);
-        for (int i = tid; i < taken; i += PICK_NT) emit(at + i, c0 + (int)L.key[i]);
+        for (int i = tid; i < taken; i += PICK_NT) emit(first + i, c0 + (int)L.key[i]);
         gt0 += gts, eq0 += eqs;
         __syncthreads();
     }
