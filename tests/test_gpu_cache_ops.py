@@ -702,3 +702,82 @@ def test_evict_many_keys(ctx):
         rows = evict_want(acc[0, h], n, keep, 5, 1000)
         assert kept[h].tolist() == rows
         assert all(np.array_equal(got[m][0, h], c.raw[m][0, h, rows]) for m in got)
+
+
+def test_sparse_more_blocks_than_are_staged(ctx):
+    """Over 8192 blocks: the pick reads its scores again in every pass."""
+    rng = np.random.default_rng(71)
+    n, HD = 16 * 9001 - 3, 64
+    c = Cache(ctx, rng, F16, 1, 1, n + 3, HD)
+    q = rng.standard_normal((1, 2, HD)).astype(np.float32)
+    for n_pick in (7, 9000):
+        check_sparse(ctx, c, q, 2, [n], 1, 16, n_pick, 0.1, (n_pick,))
+
+
+def test_caches_past_4_gib(ctx):
+    """Rows whose byte offsets pass 32 bits, in the last of two caches of 4 KV heads of 1 GiB each."""
+    rng = np.random.default_rng(81)
+    HKV, HD, slots, H, B = 4, 256, 1 << 21, 8, 2
+    nbytes = B * HKV * slots * HD * 2
+    k, v = ctx.alloc(nbytes), ctx.alloc(nbytes)
+    ctx.kv_synth(1, nbytes // 2, F16, k)
+    ctx.kv_synth(2, nbytes // 2, F16, v)
+    n, T = [40, 900], 9
+
+    def rows(d, b, h, first, m):
+        return d.download(np.float16, (m, HD), offset=(((b * HKV + h) * slots) + first) * HD * 2).astype(np.float64)
+
+    q = rng.standard_normal((B, T, H, HD)).astype(np.float32)
+    mask = random_masks(rng, B, T)
+    args, n_dev = (F16, k, None, v, None, slots), ctx.to_device(np.array(n, np.int32))
+    out = ctx.alloc(q.nbytes)
+    ctx.attn_tree(ctx.to_device(q), B, T, H, HKV, HD, *args, n_dev, ctx.to_device(mask), 0.06, out)
+    got = out.download(np.float32, q.shape)
+    acc = ctx.to_device(np.zeros((B, HKV, slots), np.float32))
+    ctx.attn_decode_weights(ctx.to_device(q[:, 0]), B, H, HKV, HD, *args, n_dev, 0.06, out, acc, acc)
+    sums = [acc.download(np.float32, (900,), offset=((1 * HKV + h) * slots) * 4) for h in range(HKV)]
+    ko, vo = ctx.alloc(B * HKV * 128 * HD * 2), ctx.alloc(B * HKV * 128 * HD * 2)
+    acc_out, kept = ctx.alloc(B * HKV * 128 * 4), ctx.alloc(B * HKV * 100 * 4)
+    ctx.kv_evict(B, HKV, HD, *args, n_dev, acc, 100, 2, 10, 128, ko, None, vo, None, acc_out, kept)
+    kept = kept.download(np.int32, (B, HKV, 100))
+    bounds = ctx.alloc(ctx.kv_bounds_bytes(B, HKV, HD, slots, 64))
+    ctx.kv_block_bounds(B, HKV, HD, F16, k, None, slots, n_dev, 900, 64, bounds)
+    for h in range(HKV):
+        kk, vv = rows(k, 1, h, 0, n[1] + T), rows(v, 1, h, 0, n[1] + T)
+        for j in (2 * h, 2 * h + 1):
+            want, _, tol, _ = attend(q[1, :, j].astype(np.float64), kk, vv, tree_seen(mask[1], n[1], T), 0.06)
+            check_rows(got[1, :, j], want, tol, ("tree", j))
+        add, add_tol = np.zeros(n[1]), np.zeros(n[1])
+        for j in (2 * h, 2 * h + 1):
+            _, p, _, tp = attend(q[1, :1, j].astype(np.float64), kk[:n[1]], vv[:n[1]], np.ones((1, n[1]), bool), 0.06)
+            add, add_tol = add + p[0], add_tol + tp[0]
+        check_rows(sums[h], add, add_tol + 2.0 ** -24 * 3 * add, ("sums", h))
+        want_rows = evict_want(sums[h], n[1], 100, 2, 10)
+        assert kept[1, h].tolist() == want_rows
+        got_k = ko.download(np.float16, (100, HD), offset=(HKV + h) * 128 * HD * 2).astype(np.float64)
+        assert np.array_equal(got_k, kk[want_rows])
+        b = bounds.download(np.float16, (15, 2, HD), offset=(HKV + h) * (slots // 64) * HD * 4)
+        assert np.array_equal(b, bounds_want(kk[:n[1]], n[1], 64)[:15])
+
+
+def test_calls_repeat_bit_for_bit(ctx):
+    """The same calls again, other sizes in between on the same scratch: the same bits."""
+    rng = np.random.default_rng(91)
+    H, HKV, HD = 32, 8, 128
+    c = Cache(ctx, rng, Q8, 2, HKV, 3000, HD)
+    small = Cache(ctx, rng, F16, 1, 2, 300, 64)
+    q = ctx.to_device(rng.standard_normal((2, 40, H, HD)).astype(np.float32))
+    mask, past = ctx.to_device(random_masks(rng, 2, 40)), ctx.to_device(np.array([2900, 411], np.int32))
+    acc = ctx.to_device(np.zeros((2, HKV, 3000), np.float32))
+    first = None
+    for _ in range(3):
+        outs = [ctx.alloc(2 * 40 * H * HD * 4), ctx.alloc(2 * H * HD * 4), ctx.alloc(300 * H * HD * 4)]
+        sums = [ctx.to_device(np.zeros((2, HKV, 3000), np.float32)) for _ in range(2)]
+        ctx.attn_tree(q, 2, 40, H, HKV, HD, *c.args, past, mask, 0.09, outs[0])
+        ctx.attn_decode_weights(q, 2, H, HKV, HD, *c.args, past, 0.09, outs[1], acc, sums[0])
+        o = ctx.alloc(4 * 64 * 4)
+        ctx.attn_tree(q, 1, 1, 4, 2, 64, *small.args, ctx.to_device(np.array([200], np.int32)), mask, 0.1, o)
+        ctx.attn_prompt_weights(q, 80, H, HKV, HD, *c.args, 1500, 0.09, outs[2], acc, sums[1])
+        got = [d.download(np.uint32) for d in outs[:2] + sums]
+        first = first or got
+        assert all(np.array_equal(a, b) for a, b in zip(got, first))

@@ -182,7 +182,7 @@ __global__ __launch_bounds__(64 * NW, ONE && HD <= 128 ? 3 : 1) void k_attn_rows
 // K [tile][chunk][lane], V hi and lo [tile pair][dim tile][lane]), and take all of it against
 // their own rows. Each key is converted once for 64 NT rows instead of once for 16 NT, and two
 // workgroups a CU fill each other's waits: k_attn_rows, one wave a SIMD, took 191 us where this takes
-// TILE_US (4 trees of 64 tokens, 32/8 heads, up to 8192 keys). What bounds it: the matrix cores and
+// 95 (4 trees of 64 tokens, 32/8 heads, up to 8192 keys). What bounds it: the matrix cores and
 // the vector ALU in turn.
 template <int HD, bool F16>
 struct TileShape {

@@ -5,8 +5,11 @@
 // it ends once a bin is taken whole. The keys are staged in LDS, sixteen requests at a time, and a
 // thread takes an odd number of neighbours there (an odd stride meets no bank twice), so that the
 // last pass is counts and bit masks of its own keys instead of ballots; the picked
-// indices go out through LDS in order. 32768 keys: 27 us (8-bit digits from memory: 60). Deterministic.
+// indices go out through LDS in order. 32768 keys: 23 us (8-bit digits
+// read from memory: 60). Deterministic.
 #pragma once
+#include <type_traits>
+
 #include "common.h"
 
 namespace ts5hip {
@@ -56,7 +59,7 @@ __device__ inline void radix_pick(PickLds<T, CAP> &L, int n, int k, Fetch fetch,
     constexpr int BITS = 8 * sizeof(T), AHEAD = sizeof(T) == 4 ? 16 : 8;
     const int tid = threadIdx.x;
     auto per = [](int m) { return ((m + PICK_NT - 1) / PICK_NT) | 1; };  // neighbours a thread
-    auto stage = [&](int c0) {  // keys c0 .. of the chunk
+    auto stage = [&](int c0, auto counted) {  // keys c0 .. of the chunk; counted: their top digits too
         const int m = min(n - c0, CAP);
         __syncthreads();
         for (int i0 = tid; i0 < m; i0 += AHEAD * PICK_NT) {
@@ -67,11 +70,14 @@ __device__ inline void radix_pick(PickLds<T, CAP> &L, int n, int k, Fetch fetch,
             for (int j = 0; j < AHEAD; j++) asm volatile("" : "+v"(v[j]));  // (no load of one waits for the use of another)
 #pragma unroll
             for (int j = 0; j < AHEAD; j++)
-                if (i0 + j * PICK_NT < m) L.key[i0 + j * PICK_NT] = key(c0 + i0 + j * PICK_NT, v[j]);
+                if (i0 + j * PICK_NT < m) {
+                    const T x = key(c0 + i0 + j * PICK_NT, v[j]);
+                    L.key[i0 + j * PICK_NT] = x;
+                    if constexpr (decltype(counted)::value) atomicAdd(&L.hist[(int)(x >> (BITS - 12))], 1);
+                }
         }
         __syncthreads();
     };
-    if (n <= CAP) stage(0);
     T prefix = 0;   // of the k-th largest key, from bit `shift` on
     int left = k;   // of the keys with that prefix, as many are picked
     int shift = BITS;
@@ -83,12 +89,16 @@ __device__ inline void radix_pick(PickLds<T, CAP> &L, int n, int k, Fetch fetch,
         for (int j = 0; j < PICK_BINS / PICK_NT; j++) L.hist[j * PICK_NT + tid] = 0;
         __syncthreads();
         for (int c0 = 0; c0 < n; c0 += CAP) {
-            if (n > CAP) stage(c0);
+            if (above == BITS) {
+                stage(c0, std::true_type{});
+                continue;
+            }
+            if (n > CAP) stage(c0, std::false_type{});
             const int m = min(n - c0, CAP), p = per(m), i1 = min(m, (tid + 1) * p);
 #pragma unroll 4
             for (int i = tid * p; i < i1; i++) {
                 const T x = L.key[i];
-                if (above == BITS || x >> (above & (BITS - 1)) == prefix)
+                if (x >> above == prefix)
                     atomicAdd(&L.hist[(int)(x >> shift) & ((1 << width) - 1)], 1);
             }
         }
@@ -114,7 +124,7 @@ __device__ inline void radix_pick(PickLds<T, CAP> &L, int n, int k, Fetch fetch,
     // over the keys in LDS.
     int gt0 = 0, eq0 = 0;
     for (int c0 = 0; c0 < n; c0 += CAP) {
-        if (n > CAP) stage(c0);
+        if (n > CAP) stage(c0, std::false_type{});
         const int m = min(n - c0, CAP), p = per(m), i0 = tid * p, i1 = min(m, i0 + p);
         uint64_t above = 0, equal = 0;
 #pragma unroll 4
