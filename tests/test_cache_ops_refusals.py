@@ -53,7 +53,7 @@ OWN = {
               dict(v_out=P), dict(vs_out=2 * P), dict(k_out=None), dict(n_ctx_out=0)],
     "bounds": [dict(block=0), dict(block=48), dict(block=256), dict(n_new=0), dict(n_new=-3), dict(bounds=P + 8), dict(B=0)],
     "sparse": [dict(block=20), dict(n_pick=0), dict(n_pick=-1), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")),
-               dict(B=0), dict(H=7), dict(H=34), dict(bounds=P + 8), dict(q=P + 8), dict(out=P + 8)],
+               dict(B=0), dict(H=7), dict(H=34), dict(bounds=P + 8), dict(q=P + 8), dict(out=P + 8), dict(B=2049)],
 }
 
 

@@ -500,18 +500,19 @@ __host__ __device__ inline int rows_chunk(int n, int n_split, uint64_t split_m, 
 
 constexpr int ROWS_MAX_G = 16;  // query heads a KV head, where one row tile holds a query's
 
-// sum_s 2^(m_s - M) (O_s, l_s) over the first `used` slices of a row's partials p: HD / 4 x SG of a
+// sum_s 2^(m_s - M) (O_s, l_s) over the first `used` slices of a row's partials: HD / 4 x SG of a
 // workgroup's 256 threads a row, 4 dims a thread and every SG-th slice, eight of them
 // requested before the first is used (one at a time their latencies add up: 32 slices took 27 us, now
-// 3); the SG parts join in LDS in order. Every thread of the workgroup calls it; the result is the SG = 0 part's.
+// 5); the SG parts join in LDS in order. Every thread of the workgroup calls it; the result is the SG = 0 part's.
 constexpr int JOIN_SG = 4;
 struct RowsJoin {
     __align__(16) float4 o[256];
     float2 ml[256];
 };
-template <int HD, int SG>
-__device__ inline float4 rows_join(RowsJoin &J, const float *p, int used, float &M, float &l) {
-    constexpr int REC = HD + 4, L4 = HD / 4, AHEAD = 8;
+// load(s, d, ml, x) loads slice s's m and l and its dims d .. + 3.
+template <int HD, int SG, class Load>
+__device__ inline float4 rows_join(RowsJoin &J, int used, float &M, float &l, Load load) {
+    constexpr int L4 = HD / 4, AHEAD = 8;
     const int tid = threadIdx.x, sg = tid / L4 % SG, d = 4 * (tid % L4);
     M = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -534,10 +535,7 @@ __device__ inline float4 rows_join(RowsJoin &J, const float *p, int used, float 
         float2 ml[AHEAD];
         float4 x[AHEAD];
 #pragma unroll
-        for (int i = 0; i < AHEAD; i++) {
-            const float *r = p + (int64_t)min(s0 + i * SG, used - 1) * REC;
-            ml[i] = *(const float2 *)r, x[i] = *(const float4 *)(r + 4 + d);
-        }
+        for (int i = 0; i < AHEAD; i++) load(min(s0 + i * SG, used - 1), d, ml[i], x[i]);
 #pragma unroll
         for (int i = 0; i < AHEAD; i++)
             if (s0 + i * SG < used) add(ml[i].x, ml[i].y, x[i]);
@@ -552,6 +550,14 @@ __device__ inline float4 rows_join(RowsJoin &J, const float *p, int used, float 
         }
     }
     return o;
+}
+// Partials that an earlier launch wrote.
+template <int HD, int SG>
+__device__ inline float4 rows_join(RowsJoin &J, const float *p, int used, float &M, float &l) {
+    return rows_join<HD, SG>(J, used, M, l, [&](int s, int d, float2 &ml, float4 &x) {
+        const float *r = p + (int64_t)s * (HD + 4);
+        ml = *(const float2 *)r, x = *(const float4 *)(r + 4 + d);
+    });
 }
 // The row's output.
 __device__ inline float4 rows_over(float4 o, float l) {

@@ -7,8 +7,9 @@
 //                  is another output;
 //  k_block_pick    the last block, the first, then the highest scores, ties to the lowest
 //                  block, ascending;
-//  k_attn_picked   attention over the picked blocks' keys (attn_rows.h), split over workgroups,
-//  k_picked_merge  which this joins.
+//  k_attn_picked   attention over the picked blocks' keys (attn_rows.h), split over workgroups, of which
+//                  few are joined by the last to finish, many by
+//  k_picked_merge.
 #include <algorithm>
 
 #include "attn_rows.h"
@@ -103,6 +104,7 @@ struct SparseArgs {
     double *scores;   // [B][HKV][n_blocks]
     int32_t *picked;  // [B][HKV][n_pick], -1 past the blocks there are
     float *part;      // [B][HKV][G][n_split][HD + 4]
+    int *counters;    // [B * HKV], CTR_STRIDE ints apart, zero between launches
     float *out;
 };
 __device__ inline int sparse_count(const SparseArgs &a, int b) {
@@ -200,8 +202,12 @@ __device__ inline int sparse_units(const SparseArgs &a, int b, int KT) {
     return (min(nb, a.n_pick) * (a.block / 16) + KT - 1) / KT;
 }
 
-// grid (n_split, HKV, B): one slice of the picked units for the G heads of a KV head.
-template <int HD, bool F16, int KT, int NW>
+// grid (n_split, HKV, B): one slice of the picked units for the G heads of a KV head. Up to FUSED_SPLITS slices
+// the last workgroup joins them: partials of one launch go past the L2 and back, about 7 us behind 32
+// slices, where a launch of its own takes 5 (one query: 13 against 10.4 us in all), but next to nothing
+// behind 4 that end at different times (16 queries: 37 against 41 us).
+constexpr int FUSED_SPLITS = 8;
+template <int HD, bool F16, int KT, int NW, bool FUSED>
 __global__ __launch_bounds__(64 * NW) void k_attn_picked(SparseArgs a) {
     __shared__ RowsLds<HD, NW> L;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -214,7 +220,9 @@ __global__ __launch_bounds__(64 * NW) void k_attn_picked(SparseArgs a) {
     });
     const int n = sparse_count(a, b), units = sparse_units(a, b, KT), per = (units + a.n_split - 1) / a.n_split;
     const int u0 = split * per, u1 = min(units, u0 + per);
-    if (u0 >= u1) return;
+    if (FUSED && n == 0 && split == 0)  // no key: zeros
+        for (int e = threadIdx.x; e < G * HD; e += 64 * NW) a.out[(((int64_t)b * a.HKV + kvh) * G) * HD + e] = 0.f;
+    if (u0 >= u1) return;  // an empty slice: not counted, not joined
     const int tpb = a.block / 16, tiles = min((n + a.block - 1) / a.block, a.n_pick) * tpb;
     const int32_t *list = a.picked + ((int64_t)b * a.HKV + kvh) * a.n_pick;
     const RowsKv kv = rows_kv<HD, F16>(a.kv, ((int64_t)(a.per_batch ? b : 0) * a.HKV + kvh) * a.n_ctx, n);
@@ -242,12 +250,46 @@ __global__ __launch_bounds__(64 * NW) void k_attn_picked(SparseArgs a) {
         rows_unit<HD, F16, KT, 1, true, false>(cur, q, sum, kb, kq, [&](int, int key) { return rows_below(key, n); },
                                                [](int, int, const float (&)[4]) {});
     }
+    // For the last workgroup, which may run on another XCD, the partials go past this one's L2, and only when they
+    // are out does the workgroup count itself in.
+    const int used = (units + per - 1) / per;
     const int64_t row0 = ((int64_t)b * a.HKV + kvh) * G;
+    const __amdgpu_buffer_rsrc_t part = slice_rsrc(a.part + row0 * a.n_split * (HD + 4), (uint32_t)(G * a.n_split * (HD + 4) * 4));
     rows_combine<HD, 1, NW>(L, sum, G, wave, rl, kq, [&](int r, int d, float4 o, float m, float l) {
-        float *p = a.part + ((row0 + r) * a.n_split + split) * (HD + 4);
-        if (d == 0) *(float4 *)p = make_float4(m, l, 0.f, 0.f);
-        *(float4 *)(p + 4 + d) = o;
+        if (FUSED && used == 1) {
+            *(float4 *)(a.out + (row0 + r) * HD + d) = rows_over(o, l);
+            return;
+        }
+        const uint32_t at = (uint32_t)(r * a.n_split + split) * (HD + 4) * 4;
+        constexpr int POLICY = FUSED ? BUF_SC1 : 0;
+        if (d == 0) __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, make_float2(m, l)), part, at, 0, POLICY);
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), part, at + 16 + 4 * d, 0, POLICY);
     });
+    if (!FUSED || used == 1) return;
+    __shared__ RowsJoin J;
+    __shared__ int last;
+    wait_stores();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int *c = a.counters + (b * a.HKV + kvh) * CTR_STRIDE;
+        last = atomicAdd(c, 1) == used - 1;
+        if (last) st_dev(c, 0);
+    }
+    __syncthreads();
+    if (!last) return;
+    constexpr int TPR = HD / 4 * JOIN_SG;
+    static_assert(64 * NW == 256, "rows_join's threads");
+    for (int g0 = 0; g0 < G; g0 += 256 / TPR) {
+        const int g = g0 + (int)threadIdx.x / TPR;
+        float M, l;
+        const float4 o = rows_join<HD, JOIN_SG>(J, used, M, l, [&](int s, int d, float2 &ml, float4 &x) {
+            const uint32_t at = (uint32_t)(min(g, G - 1) * a.n_split + s) * (HD + 4) * 4;
+            ml = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(part, at, 0, BUF_SC1));
+            x = __builtin_bit_cast(float4, __builtin_amdgcn_raw_buffer_load_b128(part, at + 16 + 4 * d, 0, BUF_SC1));
+        });
+        if (g < G && threadIdx.x % TPR < HD / 4)
+            *(float4 *)(a.out + (row0 + g) * HD + 4 * (threadIdx.x % TPR)) = rows_over(o, l);
+    }
 }
 
 template <int HD, int KT>
@@ -285,7 +327,7 @@ size_t attn_sparse_scratch_bytes(int B, int H, int HKV, int HD, int n_ctx, int b
 }
 hipError_t launch_attn_sparse(const float *q, int B, int H, int HKV, int HD, KvLayer kv, int kv_f16, int n_ctx,
                               const int32_t *n_keys, int per_batch, const void *bounds, int block, int n_pick,
-                              float scale, void *scratch, float *out, int32_t *picked, int n_cu, hipStream_t s) {
+                              float scale, void *scratch, int *counters, float *out, int32_t *picked, int n_cu, hipStream_t s) {
     const SparseScratch p = sparse_scratch(B, H, HKV, HD, n_ctx, block, n_pick, n_cu);
     uint8_t *base = (uint8_t *)scratch;
     SparseArgs a{};
@@ -293,14 +335,18 @@ hipError_t launch_attn_sparse(const float *q, int B, int H, int HKV, int HD, KvL
     a.n_pick = n_pick, a.n_split = p.n_split, a.n_keys = n_keys, a.bounds = (const _Float16 *)bounds;
     a.n_blocks = p.n_blocks, a.scale = scale, a.out = out;
     a.scores = (double *)base, a.picked = picked ? picked : (int32_t *)(base + p.scores);
-    a.part = (float *)(base + p.scores + p.picked);
+    a.part = (float *)(base + p.scores + p.picked), a.counters = counters;
     return rows_by_shape(HD, kv_f16, [&](auto hd, auto f16) {
         constexpr int D = decltype(hd)::value, KT = D == 64 ? 2 : 1, NW = 4;
         constexpr bool F = decltype(f16)::value;
         hipLaunchKernelGGL(k_block_scores<D>, dim3((p.n_blocks + score_blocks<D>() - 1) / score_blocks<D>(), HKV, B), dim3(256),
                            0, s, a);
         hipLaunchKernelGGL(k_block_pick, dim3(HKV, B), dim3(PICK_NT), 0, s, a);
-        hipLaunchKernelGGL((k_attn_picked<D, F, KT, NW>), dim3(p.n_split, HKV, B), dim3(64 * NW), 0, s, a);
+        if (p.n_split <= FUSED_SPLITS) {
+            hipLaunchKernelGGL((k_attn_picked<D, F, KT, NW, true>), dim3(p.n_split, HKV, B), dim3(64 * NW), 0, s, a);
+            return hipGetLastError();
+        }
+        hipLaunchKernelGGL((k_attn_picked<D, F, KT, NW, false>), dim3(p.n_split, HKV, B), dim3(64 * NW), 0, s, a);
         const int64_t rows = (int64_t)B * H;
         constexpr int RPW = 256 / (D / 4 * JOIN_SG);
         hipLaunchKernelGGL((k_picked_merge<D, KT>), dim3((unsigned)((rows + RPW - 1) / RPW)), dim3(256), 0, s, a, rows);

@@ -211,6 +211,8 @@ int ts5hip_attn_sparse(ts5hip_ctx *ctx, const float *q, int B, int n_head, int n
     if (int rc = check_heads(ctx, n_head, n_head_kv, head_dim)) return rc;
     if (int rc = check_cache(ctx, B, n_head_kv, head_dim, kv_type, k, ks, v, vs, n_ctx, true)) return rc;
     if (!block_ok(block)) return fail(ctx, TS5HIP_ERR_UNSUPPORTED, "blocks of %d keys (16, 32, 64 or 128)", block);
+    if (B * n_head_kv > 4096)  // the joins' counters
+        return fail(ctx, TS5HIP_ERR_ARG, "batch of %d x %d KV heads", B, n_head_kv);
     if (n_pick < 1 || n_pick > (1 << 20) || !(scale > 0.f))
         return fail(ctx, TS5HIP_ERR_ARG, "%d blocks picked at scale %g (scores rank by a positive scale)", n_pick, scale);
     if (!aligned(q, 16) || !aligned(out, 16) || !aligned(bounds, 16))
@@ -221,8 +223,8 @@ int ts5hip_attn_sparse(ts5hip_ctx *ctx, const float *q, int B, int n_head, int n
                                                                ctx->n_cu)))
         return rc;
     TS5_HIP(ctx, launch_attn_sparse(q, B, n_head, n_head_kv, head_dim, layer(k, ks, v, vs), kv_type == KV_F16, n_ctx,
-                                    n_keys_dev, kv_per_batch != 0, bounds, block, n_pick, scale, ctx->scratch, out,
-                                    picked_dev, ctx->n_cu, ctx->stream));
+                                    n_keys_dev, kv_per_batch != 0, bounds, block, n_pick, scale, ctx->scratch,
+                                    ctx->counters, out, picked_dev, ctx->n_cu, ctx->stream));
     return TS5HIP_OK;
 }
 

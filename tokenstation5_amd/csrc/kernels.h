@@ -194,13 +194,15 @@ hipError_t launch_attn_prompt_weights(const float *q, int nq, int H, int HKV, in
                                       float *acc_out, int n_cu, hipStream_t s);
 
 // attn_sparse.hip: f16 bounds [B][HKV][ceil(n_ctx / block)][lowest, highest][HD] of the blocks that hold each cache's
-// last n_new keys; attention over the n_pick blocks that they pick (picked [B][HKV][n_pick] may be null).
+// last n_new keys; attention over the n_pick blocks that they pick (picked [B][HKV][n_pick] may be null; counters:
+// B * HKV of them CTR_STRIDE ints apart, zero before the first launch and after each).
 hipError_t launch_block_bounds(int B, int HKV, int HD, KvLayer kv, int kv_f16, int n_ctx, const int32_t *n_keys,
                                int n_new, int block, void *bounds, hipStream_t s);
 size_t attn_sparse_scratch_bytes(int B, int H, int HKV, int HD, int n_ctx, int block, int n_pick, int n_cu);
 hipError_t launch_attn_sparse(const float *q, int B, int H, int HKV, int HD, KvLayer kv, int kv_f16, int n_ctx,
                               const int32_t *n_keys, int per_batch, const void *bounds, int block, int n_pick,
-                              float scale, void *scratch, float *out, int32_t *picked, int n_cu, hipStream_t s);
+                              float scale, void *scratch, int *counters, float *out, int32_t *picked, int n_cu,
+                              hipStream_t s);
 
 // kv_cache.hip
 hipError_t launch_kv_evict(int B, int HKV, int HD, KvLayer kv, int kv_f16, int n_ctx, const int32_t *n_keys,
