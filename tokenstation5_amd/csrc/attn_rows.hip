@@ -61,7 +61,9 @@ __device__ inline void rows_add_nonfinite(const RowsArgs &a, int b, int kvh, int
 }
 
 // grid (n_split, HKV * row blocks of 16 NT, B): one slice of the keys for 16 NT rows,
-// row r = G t + j being head j of token t. The waves take the slice's units in turn.
+// row r = G t + j being head j of token t. The waves take the slice's units in turn. ONE: one query a
+// cache (16 of 12288 to 16384 keys, 32/8 heads of 128, q8: 504 MB in 120 us, 4.4 TB/s with the scores it
+// writes); latency bounds it, the vector ALU is busy 45 % of the time.
 template <int HD, bool F16, int KT, int NT, int NW, bool ONE>
 __global__ __launch_bounds__(64 * NW, ONE && HD <= 128 ? 3 : 1) void k_attn_rows(RowsArgs a) {
     using S = RowsShape<HD, F16, KT>;
@@ -182,8 +184,10 @@ __global__ __launch_bounds__(64 * NW, ONE && HD <= 128 ? 3 : 1) void k_attn_rows
 // K [tile][chunk][lane], V hi and lo [tile pair][dim tile][lane]), and take all of it against
 // their own rows. Each key is converted once for 64 NT rows instead of once for 16 NT, and two
 // workgroups a CU fill each other's waits: k_attn_rows, one wave a SIMD, took 191 us where this takes
-// 95 (4 trees of 64 tokens, 32/8 heads, up to 8192 keys). What bounds it: the matrix cores and
-// the vector ALU in turn.
+// 95 (4 trees of 64 tokens, 32/8 heads, up to 8192 keys). What bounds it: the matrix cores are busy for 34 % of the
+// time and the vector ALU for 45 %, mostly in turn, as the two waves of a SIMD wait for their own chains.
+// Eight waves with two blocks in LDS convert half as much a row and were slower (103 us), and so were higher
+// priorities around the products (94 and 60 against 94 and 58 us).
 template <int HD, bool F16>
 struct TileShape {
     static constexpr int NT = HD == 256 ? 1 : 2, NKT = HD == 256 ? 2 : 4, KEYS = 16 * NKT, ROWS = 64 * NT;
@@ -492,7 +496,8 @@ __global__ __launch_bounds__(256) void k_rows_merge(RowsArgs a, int64_t rows) {
 }
 
 // One query a cache: the join (the first workgroup of a KV head) and acc_out = acc + the group's
-// weights 2^(score - lse). grid (1 + key blocks of 1024, HKV, B).
+// weights 2^(score - lse). HBM bounds it: scores read, sums read and written, 60 MB in 14 us. grid (1 + key blocks of
+// 1024, HKV, B).
 template <int HD>
 __global__ __launch_bounds__(256) void k_one_weights(RowsArgs a, const float *acc, float *acc_out) {
     __shared__ RowsJoin J;
@@ -547,7 +552,7 @@ __global__ __launch_bounds__(256) void k_one_weights(RowsArgs a, const float *ac
 // K and goes over every other row tile's planes (the next one's requested before this one's products),
 // sums 2^(score - lse) in its lanes, and the workgroup adds lanes and waves in order at the end. Four
 // waves with units of their own take the same row tiles: the L1 serves three of them
-// (waves that shared a unit instead read 540 MB of planes from the L2 for 256 queries over 4096 keys, 32 us).
+// (256 queries over 4096 keys: 25 us; waves that shared a unit instead read 540 MB of planes from the L2, 32 us).
 // grid (blocks of PW_UNITS units, HKV).
 constexpr int PW_UNITS = 4, PW_ROWS = 2;
 template <int HD, bool F16, int KT>

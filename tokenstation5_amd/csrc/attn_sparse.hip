@@ -31,7 +31,8 @@ __device__ inline _Float16 f16_towards(float x, bool up) {
 }
 
 // A wave per block: LPR lanes a row, 16 bytes each. grid (ceil(blocks / 4), HKV, B) of the blocks that hold a cache's
-// last n_new keys.
+// last n_new keys. HBM bounds it: 4 caches of 12288 to 16384 keys of 8 heads of 128, f16, 125 MB in 22 us; one block
+// of each head 5.6 us, a launch and two round trips.
 template <int HD, bool F16>
 __global__ __launch_bounds__(256) void k_block_bounds(KvLayer kv, int HKV, int n_ctx, const int32_t *n_keys, int n_new,
                                                       int block, int n_blocks, _Float16 *bounds) {
@@ -121,7 +122,9 @@ __device__ inline double dpp_f64(double x) {
 
 // HD / 8 lanes a block, 8 dims and four blocks a lane; a head's four sums over the lanes go together:
 // two exchanges within a quad leave each of its lanes the quad's sum of one block, and only that goes
-// on to the other quads. grid (ceil(n_blocks / blocks a workgroup), HKV, B).
+// on to the other quads. 16 queries over 29000 blocks of 8 heads of 128 (59 MB): 16 us, the bytes and
+// the fp64 multiply-adds about even (30 us with a head's sum over all lanes by itself and q
+// converted for each block). grid (ceil(n_blocks / blocks a workgroup), HKV, B).
 template <int HD>
 constexpr int score_blocks() { return 4 * 4 * 64 / (HD / 8); }
 template <int HD>
@@ -202,7 +205,9 @@ __device__ inline int sparse_units(const SparseArgs &a, int b, int KT) {
     return (min(nb, a.n_pick) * (a.block / 16) + KT - 1) / KT;
 }
 
-// grid (n_split, HKV, B): one slice of the picked units for the G heads of a KV head. Up to FUSED_SPLITS slices
+// grid (n_split, HKV, B): one slice of the picked units for the G heads of a KV head, three workgroups a CU, each
+// wave's next unit requested before this one is used. 16 queries over 4096 keys each (142 MB): 36 us; latency
+// bounds it (the vector ALU is busy 45 % of the time). Up to FUSED_SPLITS slices
 // the last workgroup joins them: partials of one launch go past the L2 and back, about 7 us behind 32
 // slices, where a launch of its own takes 5 (one query: 13 against 10.4 us in all), but next to nothing
 // behind 4 that end at different times (16 queries: 37 against 41 us).
