@@ -183,9 +183,10 @@ int ts5hip_topk(ts5hip_ctx *ctx, const float *x, int n, int k, float *vals_dev, 
  * kv_type TS5HIP_KV_Q8: k, v int8 [cache][n_head_kv][n_ctx][head_dim], ks, vs f16 [..][head_dim / 32]; V
  * counts within f16's range (65504). TS5HIP_KV_F16: k, v f16, ks and vs null. B caches lie back to back.
  * Head dimension 64, 128 or 256, up to 16 query heads a KV head, n_ctx x head_dim x value bytes a KV head
- * below 2 GiB. q, out, cache values and bounds are 16-byte aligned. Counts on the device
- * (n_keys_dev, n_past_dev) are taken into 0..n_ctx. A query without a key gets zeros. Scratch is the
- * context's: it grows on the first call of a size, and no two streams use it. ---- */
+ * below 2 GiB, n_head_kv up to 512, B up to 4096. q, out, cache values and bounds are 16-byte aligned. Counts on the device
+ * (n_keys_dev, n_past_dev) are taken into 0..n_ctx. A query without a key gets zeros; one that is NaN
+ * or reads NaN keys gets NaN; one that reads infinite values, infinities or NaN there. Scratch is the context's: it
+ * grows on the first call of a size, and no two streams use it. ---- */
 
 /* ts5hip_rope_kv_append with each token's RoPE position pos_dev[t] (0..n_pos - 1, the rows of rope_cs) apart
  * from its cache slot *slot0_dev + t: the drafts of a tree that share a depth share a position, and an
@@ -217,7 +218,7 @@ int ts5hip_attn_decode_weights(ts5hip_ctx *ctx, const float *q, int B, int n_hea
                                int kv_type, const void *k, const void *ks, const void *v, const void *vs, int n_ctx,
                                const int32_t *n_keys_dev, float scale, float *out, const float *acc, float *acc_out);
 /* ts5hip_attn_prompt (nq queries, 1..4096, at positions pos0 .. over one cache, causal) with the same sums, over the
- * chunk's queries too. */
+ * chunk's queries too. nq x n_head up to 960000. */
 int ts5hip_attn_prompt_weights(ts5hip_ctx *ctx, const float *q, int nq, int n_head, int n_head_kv, int head_dim,
                                int kv_type, const void *k, const void *ks, const void *v, const void *vs, int n_ctx,
                                int pos0, float scale, float *out, const float *acc, float *acc_out);
@@ -242,7 +243,8 @@ int ts5hip_kv_block_bounds(ts5hip_ctx *ctx, int B, int n_head_kv, int head_dim, 
 /* Attention over n_pick blocks of keys a query and KV head: the last block, the first, then those of
  * the highest scores (ties to the lowest block), a block's score being the largest over the group's heads of
  * sum_d max(q_d lowest_d, q_d highest_d), which no key of the block exceeds; NaN ranks first. Scores are fp64:
- * equal choices for equal inputs. n_keys_dev and kv_per_batch as ts5hip_attn_decode has them; scale > 0.
+ * equal choices for equal inputs. n_keys_dev and kv_per_batch as ts5hip_attn_decode has them; scale > 0;
+ * B x n_head_kv up to 4096.
  * The last block needs no bounds. picked_dev [B][n_head_kv][n_pick] (may be null): the
  * blocks read, ascending, -1 behind the last. */
 int ts5hip_attn_sparse(ts5hip_ctx *ctx, const float *q, int B, int n_head, int n_head_kv, int head_dim, int kv_type,

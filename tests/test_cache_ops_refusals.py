@@ -86,4 +86,5 @@ def test_bounds_bytes():
     f = L().ts5hip_kv_bounds_bytes
     assert f(3, 8, 128, 1000, 64) == 3 * 8 * 16 * 2 * 128 * 2
     assert f(1, 1, 64, 1, 128) == 256
+    assert f(1, 1, 64, 2 ** 31 - 1, 128) == 2 ** 24 * 256
     assert [f(*a) for a in ((0, 1, 64, 1, 64), (1, 0, 64, 1, 64), (1, 1, 64, 0, 64), (1, 1, 64, 1, 8))] == [-1] * 4

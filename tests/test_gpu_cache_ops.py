@@ -688,6 +688,42 @@ def test_queries_that_are_no_numbers(ctx, HD):
     assert np.all(np.isnan(o[1, 2])) and np.all(np.isfinite(o[0])) and np.all(np.isfinite(o[1, [0, 1, 3]]))
 
 
+@pytest.mark.parametrize("kv", [Q8, F16])
+def test_weights_of_keys_that_are_no_numbers(ctx, kv):
+    """NaN keys that fill the first slices of a query's cache: every weight is NaN, not those of the slices' own keys
+    alone, and so is the output; another cache's stay what they are."""
+    H, HKV, HD, n = 4, 2, 128, 900
+    rng = np.random.default_rng([91, kv])
+    c = Cache(ctx, rng, kv, 2, HKV, n, HD)
+    (c.raw["ks"] if kv == Q8 else c.raw["k"])[1, :, :300] = np.nan
+    c.send()
+    q = ctx.to_device(rng.standard_normal((2, H, HD)).astype(np.float32))
+    n_keys, out = ctx.to_device(np.array([n, n], np.int32)), ctx.alloc(2 * H * HD * 4)
+    acc = ctx.to_device(np.zeros((2, HKV, n), np.float32))
+    ctx.attn_decode_weights(q, 2, H, HKV, HD, *c.args, n_keys, 0.1, out, acc, acc)
+    o, sums = out.download(np.float32, (2, H, HD)), acc.download(np.float32, (2, HKV, n))
+    assert np.all(np.isfinite(o[0])) and np.all(np.isfinite(sums[0]))
+    assert np.all(np.isnan(o[1])) and np.all(np.isnan(sums[1]))
+
+
+def test_sparse_more_picks_than_blocks(ctx):
+    """Every block there is, with the list and without: scratch for the blocks, not for the picks asked for."""
+    H, HKV, HD, n = 8, 2, 64, 333
+    rng = np.random.default_rng(93)
+    c = Cache(ctx, rng, F16, 1, HKV, n, HD)
+    q, n_keys = ctx.to_device(rng.standard_normal((1, H, HD)).astype(np.float32)), ctx.to_device(np.array([n], np.int32))
+    bounds = ctx.to_device(np.zeros((HKV, 21, 2, HD), np.float16))
+    outs = []
+    for n_pick in (21, 1 << 20):
+        for picked in (None, ctx.alloc(HKV * n_pick * 4)):
+            out = ctx.alloc(H * HD * 4)
+            ctx.attn_sparse(q, 1, H, HKV, HD, *c.args, n_keys, 0, bounds, 16, n_pick, 0.1, out, *([picked] if picked else []))
+            outs.append(out.download(np.float32))
+            if picked:
+                assert np.array_equal(picked.download(np.int32, (HKV, n_pick))[1, :23], [*range(21), -1, -1][:min(23, n_pick)])
+    assert all(np.array_equal(o, outs[0]) for o in outs) and np.all(np.isfinite(outs[0]))
+
+
 def test_evict_many_keys(ctx):
     """More keys than a workgroup's registers hold, with ties across their chunks."""
     rng = np.random.default_rng(61)

@@ -531,7 +531,8 @@ __global__ __launch_bounds__(256) void k_one_weights(RowsArgs a, const float *ac
         M = row_max_dpp(M);
 #pragma unroll
         for (int i = 0; i < ROWS_MAX_SPLIT / 16; i++)
-            if (m[i] != -INFINITY) sum = fmaf(__builtin_amdgcn_exp2f(m[i] - M), l[i], sum);
+            if (m[i] != -INFINITY || l[i] != l[i])  // (a slice of NaN scores has no maximum)
+                sum = fmaf(__builtin_amdgcn_exp2f(m[i] - M), l[i], sum);
         sum = row_sum_dpp(sum);
         if (s0 == 0) lse[g] = M + __log2f(sum);
     }

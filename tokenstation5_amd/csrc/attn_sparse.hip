@@ -322,7 +322,7 @@ static SparseScratch sparse_scratch(int B, int H, int HKV, int HD, int n_ctx, in
     const int most = (int)std::min<int64_t>((keys + 63) / 64, ROWS_MAX_SPLIT);
     p.n_split = std::max(1, std::min(2 * n_cu / std::max(1, B * HKV), most));
     p.scores = align_up((size_t)B * HKV * p.n_blocks * sizeof(double), 256);
-    p.picked = align_up((size_t)B * HKV * n_pick * sizeof(int32_t), 256);
+    p.picked = align_up((size_t)B * HKV * std::min(n_pick, p.n_blocks) * sizeof(int32_t), 256);
     p.part = (size_t)B * H * p.n_split * (HD + 4) * sizeof(float);
     return p;
 }
@@ -337,7 +337,7 @@ hipError_t launch_attn_sparse(const float *q, int B, int H, int HKV, int HD, KvL
     uint8_t *base = (uint8_t *)scratch;
     SparseArgs a{};
     a.q = q, a.kv = kv, a.n_ctx = n_ctx, a.H = H, a.HKV = HKV, a.B = B, a.per_batch = per_batch, a.block = block;
-    a.n_pick = n_pick, a.n_split = p.n_split, a.n_keys = n_keys, a.bounds = (const _Float16 *)bounds;
+    a.n_pick = picked ? n_pick : std::min(n_pick, p.n_blocks), a.n_split = p.n_split, a.n_keys = n_keys, a.bounds = (const _Float16 *)bounds;
     a.n_blocks = p.n_blocks, a.scale = scale, a.out = out;
     a.scores = (double *)base, a.picked = picked ? picked : (int32_t *)(base + p.scores);
     a.part = (float *)(base + p.scores + p.picked), a.counters = counters;

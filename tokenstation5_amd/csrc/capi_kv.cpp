@@ -186,7 +186,7 @@ static bool block_ok(int block) { return block == 16 || block == 32 || block == 
 
 int64_t ts5hip_kv_bounds_bytes(int B, int n_head_kv, int head_dim, int n_ctx, int block) {
     if (B < 1 || n_head_kv < 1 || head_dim < 1 || n_ctx < 1 || !block_ok(block)) return -1;
-    return (int64_t)B * n_head_kv * ((n_ctx + block - 1) / block) * head_dim * 4;
+    return (int64_t)B * n_head_kv * (((int64_t)n_ctx + block - 1) / block) * head_dim * 4;
 }
 
 int ts5hip_kv_block_bounds(ts5hip_ctx *ctx, int B, int n_head_kv, int head_dim, int kv_type, const void *k,
