@@ -19,8 +19,8 @@ struct EvictArgs {
 __device__ inline int evict_count(const EvictArgs &a, int b) { return max(0, min(a.n_keys[b], a.n_ctx)); }
 
 // The slots kept, ascending: the first and last ones, then those of the largest sums (NaN lowest),
-// ties to the lowest slot. One workgroup a KV head: its passes over the keys in LDS bound it (4100 keys 8.5 us, 32768
-// keys 23 us). grid (HKV, B).
+// ties to the lowest slot. One workgroup a KV head: its passes over the keys in LDS bound it (4100 keys 8.3 us, 32768
+// keys 21 us). grid (HKV, B).
 __global__ __launch_bounds__(PICK_NT) void k_evict_pick(EvictArgs a) {
     __shared__ PickLds<uint32_t, 32768> L;
     const int kvh = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, n = evict_count(a, b);
