@@ -60,11 +60,11 @@ __device__ inline void rows_add_nonfinite(const RowsArgs &a, int b, int kvh, int
     }
 }
 
-// grid (n_split, HKV * row blocks of 16 NT, B): one slice of the keys for 16 NT rows,
+// grid (n_split, HKV, B): one slice of the keys for a KV head's R <= 16 rows,
 // row r = G t + j being head j of token t. The waves take the slice's units in turn. ONE: one query a
 // cache (16 of 12288 to 16384 keys, 32/8 heads of 128, q8: 504 MB in 120 us, 4.4 TB/s with the scores it
 // writes); latency bounds it, the vector ALU is busy 45 % of the time.
-template <int HD, bool F16, int KT, int NT, int NW, bool ONE>
+template <int HD, bool F16, int KT, int NW, bool ONE>
 __global__ __launch_bounds__(64 * NW, ONE && HD <= 128 ? 3 : 1) void k_attn_rows(RowsArgs a) {
     using S = RowsShape<HD, F16, KT>;
     __shared__ RowsLds<HD, NW> L;
@@ -72,19 +72,17 @@ __global__ __launch_bounds__(64 * NW, ONE && HD <= 128 ? 3 : 1) void k_attn_rows
     if (!ONE && threadIdx.x == 0) nonfinite = 0;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int rl = lane & 15, kq = lane >> 4;
-    const int G = a.G, R = a.R;
-    const int split = blockIdx.x, kvh = rows_div(blockIdx.y, a.nrb_m), r0 = ((int)blockIdx.y - kvh * a.nrb) * 16 * NT, b = blockIdx.z;
-    const int rows = min(R - r0, 16 * NT);
-    RowsIn<HD, NT> in;  // requested before the counts that the keys' addresses wait for
-    rows_request<HD, NT>(in, kq, [&](int qt, bool &ok) {
-        const int r = r0 + 16 * qt + rl;
-        ok = r < R;
-        return a.q + rows_at(a, b, kvh, min(r, R - 1)) * HD;
+    const int R = a.R;
+    const int split = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
+    RowsIn<HD, 1> in;  // requested before the counts that the keys' addresses wait for
+    rows_request<HD, 1>(in, kq, [&](int, bool &ok) {
+        ok = rl < R;
+        return a.q + rows_at(a, b, kvh, min(rl, R - 1)) * HD;
     });
     const int n = rows_count(a, b), chunk = rows_chunk(rows_all(a, n), a.n_split, a.split_m, a.least);
-    const int kbeg = split * chunk, kend = min(kbeg + chunk, rows_reach(a, n, rows_div(r0 + rows - 1, a.g_m)));
+    const int kbeg = split * chunk, kend = min(kbeg + chunk, rows_reach(a, n, rows_div(R - 1, a.g_m)));
     if (kbeg >= kend) return;  // the merge reads no partial of this slice
-    const int full = a.mode == ROWS_CAUSAL ? n + rows_div(r0, a.g_m) + 1 : n;  // keys before it are every row's
+    const int full = a.mode == ROWS_CAUSAL ? n + 1 : n;  // keys before it are every row's
     const RowsKv kv = rows_kv<HD, F16>(a.kv, ((int64_t)b * a.HKV + kvh) * a.n_ctx, kend);
     const int units = (kend - kbeg + S::UNIT - 1) / S::UNIT;
     RowsUnit<HD, F16, KT> nxt;
@@ -96,44 +94,33 @@ __global__ __launch_bounds__(64 * NW, ONE && HD <= 128 ? 3 : 1) void k_attn_rows
     at(wave, kb);
     rows_load<HD, F16, KT>(nxt, kv, kb, rl, kq);
 
-    RowsQ<HD, NT> q;
-    rows_query<HD, NT>(q, in, a.scale);
-    int seen[NT];       // keys before it are the row's
-    uint64_t bits[NT];  // and then those of n + its set bits
-#pragma unroll
-    for (int qt = 0; qt < NT; qt++) {
-        const int r = r0 + 16 * qt + rl, t = rows_div(min(r, R - 1), a.g_m);
-        seen[qt] = r >= R ? 0 : a.mode == ROWS_CAUSAL ? n + t + 1 : n;
-        bits[qt] = 0;
-        if (!ONE && a.mode == ROWS_TREE) {
-            const uint64_t m = a.mask[(int64_t)b * a.T + t] & (~0ull >> (64 - a.T));
-            bits[qt] = r < R ? m : 0;
-        }
+    RowsQ<HD, 1> q;
+    rows_query<HD, 1>(q, in, a.scale);
+    // Keys before `seen` are the lane's row's, and then those of n + the set bits.
+    const int t = rows_div(min(rl, R - 1), a.g_m), seen = rl >= R ? 0 : a.mode == ROWS_CAUSAL ? n + t + 1 : n;
+    uint64_t bits = 0;
+    if (!ONE && a.mode == ROWS_TREE) {
+        const uint64_t m = a.mask[(int64_t)b * a.T + t] & (~0ull >> (64 - a.T));
+        bits = rl < R ? m : 0;
     }
     if (!ONE && a.planes && split == 0 && wave == 0) {
-        const int tiles = (R + 15) / 16;
+        uint4 *p = a.planes + (int64_t)kvh * (HD / 32) * 2 * 64 + lane;
 #pragma unroll
-        for (int qt = 0; qt < NT; qt++) {
-            const int tile = r0 / 16 + qt;
-            if (tile >= tiles) break;
-            uint4 *p = a.planes + ((int64_t)kvh * tiles + tile) * (HD / 32) * 2 * 64 + lane;
-#pragma unroll
-            for (int c = 0; c < HD / 32; c++) {
-                p[(2 * c) * 64] = __builtin_bit_cast(uint4, q.h[qt][c]);
-                p[(2 * c + 1) * 64] = __builtin_bit_cast(uint4, q.l[qt][c]);
-            }
-            if (kq == 0) a.p2e[((int64_t)kvh * tiles + tile) * 16 + rl] = q.p2e[qt];
+        for (int c = 0; c < HD / 32; c++) {
+            p[(2 * c) * 64] = __builtin_bit_cast(uint4, q.h[0][c]);
+            p[(2 * c + 1) * 64] = __builtin_bit_cast(uint4, q.l[0][c]);
         }
+        if (kq == 0) a.p2e[(int64_t)kvh * 16 + rl] = q.p2e[0];
     }
-    RowsSum<HD, NT> sum;
-    rows_clear<HD, NT>(sum);
+    RowsSum<HD, 1> sum;
+    rows_clear<HD, 1>(sum);
     if (!ONE) __syncthreads();  // the flag is set
-    const int64_t row0 = ((int64_t)b * a.HKV + kvh) * R + r0;
+    const int64_t row0 = ((int64_t)b * a.HKV + kvh) * R;
     if constexpr (ONE) {
         // One unit ahead in three waves a SIMD; two ahead in two waves is no faster (122 us), and in three it
         // spills (170 us).
         auto put = [&](int, int key, const float (&s)[4]) {
-            if (rl < rows && key < kend)
+            if (rl < R && key < kend)
                 *(float4 *)(a.scores + (row0 + rl) * a.stride + key) =
                     make_float4(s[0] * q.p2e[0], s[1] * q.p2e[0], s[2] * q.p2e[0], s[3] * q.p2e[0]);
         };
@@ -143,7 +130,7 @@ __global__ __launch_bounds__(64 * NW, ONE && HD <= 128 ? 3 : 1) void k_attn_rows
             at(u + NW, kb);
             rows_load<HD, F16, KT>(nxt, kv, kb, rl, kq);  // (past the slice: zeros, no memory access)
             at(u, kb);
-            rows_unit<HD, F16, KT, NT, true, false>(cur, q, sum, kb, kq, seen4, put);
+            rows_unit<HD, F16, KT, 1, true, false>(cur, q, sum, kb, kq, seen4, put);
         }
     } else {
         auto put = [](int, int, const float (&)[4]) {};
@@ -154,20 +141,20 @@ __global__ __launch_bounds__(64 * NW, ONE && HD <= 128 ? 3 : 1) void k_attn_rows
             at(u + NW, kn);
             rows_load<HD, F16, KT>(nxt, kv, kn, rl, kq);
             if (kb[0] + S::UNIT <= full)
-                rows_unit<HD, F16, KT, NT, false, false>(cur, q, sum, kb, kq, [](int, int) { return 15u; }, put);
-            else if (rows_unit<HD, F16, KT, NT, true, true>(
+                rows_unit<HD, F16, KT, 1, false, false>(cur, q, sum, kb, kq, [](int, int) { return 15u; }, put);
+            else if (rows_unit<HD, F16, KT, 1, true, true>(
                          cur, q, sum, kb, kq,
-                         [&](int qt, int key) { return rows_below(key, seen[qt]) | rows_window(bits[qt], key - n); },
+                         [&](int, int key) { return rows_below(key, seen) | rows_window(bits, key - n); },
                          put))
                 nonfinite = 1;
         }
     }
-    rows_combine<HD, NT, NW>(L, sum, rows, wave, rl, kq, [&](int r, int d, float4 o, float m, float l) {
-        const int t = rows_div(r0 + r, a.g_m);
+    rows_combine<HD, 1, NW>(L, sum, R, wave, rl, kq, [&](int r, int d, float4 o, float m, float l) {
+        const int t = rows_div(r, a.g_m);
         if (!ONE && nonfinite)
             rows_add_nonfinite<HD, F16>(a, b, kvh, t, n, kbeg + max(full - kbeg, 0) / S::UNIT * S::UNIT, kend, d, o);
         if (!ONE && a.n_split == 1) {
-            *(float4 *)(a.out + rows_at(a, b, kvh, r0 + r) * HD + d) = rows_over(o, l);
+            *(float4 *)(a.out + rows_at(a, b, kvh, r) * HD + d) = rows_over(o, l);
             if (a.lse && d == 0) a.lse[row0 + r] = l == 0.f ? INFINITY : m + __log2f(l);
             return;
         }
@@ -183,21 +170,21 @@ __global__ __launch_bounds__(64 * NW, ONE && HD <= 128 ? 3 : 1) void k_attn_rows
 // operands' own layout in LDS (16 bytes a lane, so that no read or write meets a bank twice:
 // K [tile][chunk][lane], V hi and lo [tile pair][dim tile][lane]), and take all of it against
 // their own rows. Each key is converted once for 64 NT rows instead of once for 16 NT, and two
-// workgroups a CU fill each other's waits: k_attn_rows, one wave a SIMD, took 191 us where this takes
-// 95 (4 trees of 64 tokens, 32/8 heads, up to 8192 keys). What bounds it: the matrix cores are busy for 34 % of the
+// workgroups a CU fill each other's waits: waves that converted for themselves, one a SIMD, took 191 us where this
+// takes 95 (4 trees of 64 tokens, 32/8 heads, up to 8192 keys). What bounds it: the matrix cores are busy for 34 % of the
 // time and the vector ALU for 45 %, mostly in turn, as the two waves of a SIMD wait for their own chains.
 // Eight waves with two blocks in LDS convert half as much a row and were slower (103 us), and so were higher
 // priorities around the products (94 and 60 against 94 and 58 us).
-template <int HD, bool F16>
+template <int HD, bool F16, int NT_>
 struct TileShape {
-    static constexpr int NT = HD == 256 ? 1 : 2, NKT = HD == 256 ? 2 : 4, KEYS = 16 * NKT, ROWS = 64 * NT;
+    static constexpr int NT = NT_, NKT = HD == 256 ? 2 : 4, KEYS = 16 * NKT, ROWS = 64 * NT;
     static constexpr int WPT = 4 / NKT;  // waves that share a key tile's conversion
     static constexpr int NC = HD / 32, NDT = HD / 16, CW = NC / WPT, DW = NDT / WPT;  // chunks and dims of a lane's share
     static constexpr int VB = F16 ? 2 : 1, KW = F16 ? 4 : 2, VW = DW * VB / 4;
 };
 template <int HD, bool F16>
 struct TileLds {
-    using S = TileShape<HD, F16>;
+    using S = TileShape<HD, F16, 1>;
     uint4 k[S::NKT][S::NC][64];
     uint2 vh[S::NKT / 2][S::NDT][64][2];
     uint2 vl[F16 ? 1 : S::NKT / 2][F16 ? 1 : S::NDT][64][2];
@@ -205,15 +192,15 @@ struct TileLds {
     int nonfinite;
 };
 
-template <int HD, bool F16>
+template <int HD, bool F16, int NT_>
 __global__ __launch_bounds__(256, 2) void k_attn_tile(RowsArgs a) {
-    using S = TileShape<HD, F16>;
+    using S = TileShape<HD, F16, NT_>;
     constexpr int NT = S::NT, NKT = S::NKT, NC = S::NC, NDT = S::NDT;
     __shared__ TileLds<HD, F16> L;
     if (threadIdx.x == 0) L.nonfinite = 0;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int rl = lane & 15, kq = lane >> 4;
-    const int G = a.G, R = a.R;
+    const int R = a.R;
     const int split = blockIdx.x, kvh = rows_div(blockIdx.y, a.nrb_m), r0 = ((int)blockIdx.y - kvh * a.nrb) * S::ROWS, b = blockIdx.z;
     const int w0 = r0 + 16 * NT * wave;  // the wave's first row
     RowsIn<HD, NT> in;  // requested before the counts that the keys' addresses wait for
@@ -658,25 +645,33 @@ __global__ __launch_bounds__(64 * PW_UNITS * PW_ROWS) void k_prompt_weights(Rows
 
 // ---- host ----------------------------------------------------------------------------------------
 
-// Rows a KV head has of a sequence's tokens go to k_attn_rows, whose waves split the keys, while
-// one or two row tiles hold them, and past that to k_attn_tile, whose waves split the rows.
-static bool rows_tile(int R, int HD) { return R > (HD == 256 ? 16 : 32); }
-static int rows_blocks(int R, int HD) {
-    const int per = rows_tile(R, HD) ? (HD == 256 ? 64 : 128) : HD == 256 || R <= 16 ? 16 : 32;
-    return (R + per - 1) / per;
-}
-// Tiles of keys a unit.
-constexpr int rows_kt(int HD, int NT) { return HD == 256 || (HD == 128 && NT == 1) ? 1 : 2; }
-// A slice reads at least half as many bytes of keys and values as its rows' queries and partials take
-// (84 rows over 4096 keys of 32/8 heads: 128 keys a slice 27.5 us with the join, 192 25.3, 256 26.7, 384 30.8).
-static int rows_least(int R, int HD, int kv_f16) {
-    const int rows = std::min(R, HD == 256 ? 64 : 128), key = 2 * (kv_f16 ? 2 * HD : HD + HD / 16);
-    const int n = rows * (2 * HD + 4) * 4 / (2 * key);
-    return std::max(ROWS_MIN_KEYS, (n + 63) / 64 * 64);
-}
+// How the R rows that a KV head has of a sequence's tokens are shared out.
+struct RowsPlan {
+    bool tile;
+    int per, nrb, least, n_split;  // rows a workgroup, blocks of rows, keys a slice takes at least, slices
+};
 static int rows_splits(int items, int keys, int slots, int least) {
     const int most = std::min((keys + least - 1) / least, ROWS_MAX_SPLIT);
     return std::max(1, std::min(slots / std::max(items, 1), most));
+}
+
+// Up to 16 rows go to k_attn_rows, whose waves split the keys (8 caches of 16384 keys, 16 rows: 61 us, 85 by
+// k_attn_tile), more to k_attn_tile, whose waves split the rows (20 rows: 96 us, 130 by two row tiles a wave
+// there). Its waves take one row tile each, or two past 64 rows where every workgroup has more than 384
+// keys to go through: a key's conversion then serves twice the rows (64 tokens of 32/8 heads over 8 x 16384 keys 320 us,
+// 405 by one tile, over 8 x 4096 98 and 110), but a block takes longer (1 x 4096 37 and 33 us, 1 x 700 25 and 18).
+// A slice reads at least half as many bytes of keys and values as its rows' queries and partials take
+// (84 rows over 4096 keys, two tiles: 128 keys a slice 27.5 us with the join, 192 25.3, 256 26.7, 384 30.8).
+static RowsPlan rows_plan(int seqs, int R, int HD, int kv_f16, int keys, int n_cu) {  // seqs: caches x KV heads
+    RowsPlan p;
+    p.tile = R > 16;
+    const bool two = HD <= 128 && R > 64 && (int64_t)seqs * ((R + 127) / 128) * keys > (int64_t)384 * 2 * n_cu;
+    p.per = !p.tile ? 16 : two ? 128 : 64;
+    p.nrb = (R + p.per - 1) / p.per;
+    const int key = 2 * (kv_f16 ? 2 * HD : HD + HD / 16), n = std::min(R, p.per) * (2 * HD + 4) * 4 / (2 * key);
+    p.least = std::max(ROWS_MIN_KEYS, (n + 63) / 64 * 64);
+    p.n_split = rows_splits(seqs * p.nrb, keys, p.tile ? 2 * n_cu : n_cu, p.least);
+    return p;
 }
 
 bool attn_rows_supported(int H, int HKV, int HD) {
@@ -684,26 +679,20 @@ bool attn_rows_supported(int H, int HKV, int HD) {
 }
 
 // The arguments that follow from the others.
-static void rows_derive(RowsArgs &a, int HD, int kv_f16) {
-    a.least = rows_least(a.T * (a.H / a.HKV), HD, kv_f16);
-    a.G = a.H / a.HKV, a.R = a.T * a.G, a.nrb = rows_blocks(a.R, HD);
-    a.g_m = rows_magic(a.G), a.nrb_m = rows_magic(a.nrb), a.split_m = rows_magic(a.n_split);
+static void rows_derive(RowsArgs &a, int n_split, int nrb, int least) {
+    a.G = a.H / a.HKV, a.R = a.T * a.G, a.nrb = nrb, a.least = least, a.n_split = n_split;
+    a.g_m = rows_magic(a.G), a.nrb_m = rows_magic(nrb), a.split_m = rows_magic(n_split);
 }
 
+// 16-key tiles a unit of k_attn_rows.
+constexpr int rows_kt(int HD) { return HD == 64 ? 2 : 1; }
 template <int HD, bool F16>
-static hipError_t rows_launch(const RowsArgs &a, int B, bool one, hipStream_t s) {
-    const int R = a.R;
+static hipError_t rows_launch(const RowsArgs &a, const RowsPlan &p, int B, hipStream_t s) {
     const dim3 grid(a.n_split, a.HKV * a.nrb, B);
-    constexpr int NW = HD == 256 ? 4 : 8, K1 = rows_kt(HD, 1), K2 = rows_kt(HD, 2);
-    if (one) {
-        hipLaunchKernelGGL((k_attn_rows<HD, F16, K1, 1, 4, true>), grid, dim3(256), 0, s, a);
-    } else if (rows_tile(R, HD)) {
-        hipLaunchKernelGGL((k_attn_tile<HD, F16>), grid, dim3(256), 0, s, a);
-    } else if (HD == 256 || R <= 16) {
-        hipLaunchKernelGGL((k_attn_rows<HD, F16, K1, 1, NW, false>), grid, dim3(64 * NW), 0, s, a);
-    } else if constexpr (HD <= 128) {
-        hipLaunchKernelGGL((k_attn_rows<HD, F16, K2, 2, 4, false>), grid, dim3(256), 0, s, a);
-    }
+    constexpr int NW = HD == 256 ? 4 : 8;
+    if (!p.tile) hipLaunchKernelGGL((k_attn_rows<HD, F16, rows_kt(HD), NW, false>), grid, dim3(64 * NW), 0, s, a);
+    else if (p.per == 64) hipLaunchKernelGGL((k_attn_tile<HD, F16, 1>), grid, dim3(256), 0, s, a);
+    else if constexpr (HD <= 128) hipLaunchKernelGGL((k_attn_tile<HD, F16, 2>), grid, dim3(256), 0, s, a);
     return hipGetLastError();
 }
 template <int HD>
@@ -714,25 +703,23 @@ static hipError_t rows_launch_merge(const RowsArgs &a, int B, hipStream_t s) {
     else hipLaunchKernelGGL((k_rows_merge<HD, JOIN_SG>), grid(HD / 4 * JOIN_SG), dim3(256), 0, s, a, rows);
     return hipGetLastError();
 }
-static int tree_splits(int B, int T, int H, int HKV, int HD, int kv_f16, int n_ctx, int n_cu) {
-    const int R = T * (H / HKV);
-    return rows_splits(B * HKV * rows_blocks(R, HD), n_ctx, rows_tile(R, HD) ? 2 * n_cu : n_cu,
-                       rows_least(R, HD, kv_f16));
+static RowsPlan tree_plan(int B, int T, int H, int HKV, int HD, int kv_f16, int n_ctx, int n_cu) {
+    return rows_plan(B * HKV, T * (H / HKV), HD, kv_f16, n_ctx, n_cu);
 }
 size_t attn_tree_scratch_bytes(int B, int T, int H, int HKV, int HD, int kv_f16, int n_ctx, int n_cu) {
-    const int ns = tree_splits(B, T, H, HKV, HD, kv_f16, n_ctx, n_cu);
+    const int ns = tree_plan(B, T, H, HKV, HD, kv_f16, n_ctx, n_cu).n_split;
     return ns > 1 ? (size_t)B * T * H * ns * (HD + 4) * sizeof(float) : 0;
 }
 hipError_t launch_attn_tree(const float *q, int B, int T, int H, int HKV, int HD, KvLayer kv, int kv_f16, int n_ctx,
                             const int32_t *n_past, const uint64_t *mask, float scale, float *part, float *out, int n_cu,
                             hipStream_t s) {
+    const RowsPlan p = tree_plan(B, T, H, HKV, HD, kv_f16, n_ctx, n_cu);
     RowsArgs a{};
     a.q = q, a.kv = kv, a.n_ctx = n_ctx, a.H = H, a.HKV = HKV, a.T = T, a.n_keys = n_past, a.mask = mask;
     a.mode = ROWS_TREE, a.scale = scale, a.part = part, a.out = out;
-    a.n_split = tree_splits(B, T, H, HKV, HD, kv_f16, n_ctx, n_cu);
-    rows_derive(a, HD, kv_f16);
+    rows_derive(a, p.n_split, p.nrb, p.least);
     return rows_by_shape(HD, kv_f16, [&](auto hd, auto f16) {
-        const hipError_t e = rows_launch<decltype(hd)::value, decltype(f16)::value>(a, B, false, s);
+        const hipError_t e = rows_launch<decltype(hd)::value, decltype(f16)::value>(a, p, B, s);
         return e != hipSuccess || a.n_split == 1 ? e : rows_launch_merge<decltype(hd)::value>(a, B, s);
     });
 }
@@ -750,12 +737,12 @@ hipError_t launch_attn_one_weights(const float *q, int B, int H, int HKV, int HD
     RowsArgs a{};
     a.q = q, a.kv = kv, a.n_ctx = n_ctx, a.H = H, a.HKV = HKV, a.T = 1, a.n_keys = n_keys;
     a.mode = ROWS_ONE, a.scale = scale, a.out = out, a.stride = one_stride(n_ctx);
-    a.n_split = one_splits(B, HKV, n_ctx, n_cu);
     a.scores = (float *)scratch, a.part = a.scores + (int64_t)B * H * a.stride;
-    rows_derive(a, HD, kv_f16);
+    rows_derive(a, one_splits(B, HKV, n_ctx, n_cu), 1, ROWS_MIN_KEYS);
     return rows_by_shape(HD, kv_f16, [&](auto hd, auto f16) {
         constexpr int D = decltype(hd)::value;
-        const hipError_t e = rows_launch<D, decltype(f16)::value>(a, B, true, s);
+        hipLaunchKernelGGL((k_attn_rows<D, decltype(f16)::value, rows_kt(D), 4, true>), dim3(a.n_split, HKV, B), dim3(256), 0, s, a);
+        const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
         hipLaunchKernelGGL(k_one_weights<D>, dim3(1 + (n_ctx + 1023) / 1024, HKV, B), dim3(256), 0, s, a, acc,
                            acc_out);
@@ -764,14 +751,14 @@ hipError_t launch_attn_one_weights(const float *q, int B, int H, int HKV, int HD
 }
 
 struct PromptWeightsScratch {
-    int ns;
+    RowsPlan plan;
     size_t part, planes, p2e, lse;  // bytes
 };
 static PromptWeightsScratch prompt_scratch(int nq, int H, int HKV, int HD, int kv_f16, int n_keys, int n_cu) {
     const int R = nq * (H / HKV), tiles = (R + 15) / 16;
     PromptWeightsScratch p;
-    p.ns = rows_splits(HKV * rows_blocks(R, HD), n_keys, 2 * n_cu, rows_least(R, HD, kv_f16));
-    p.part = p.ns > 1 ? (size_t)nq * H * p.ns * (HD + 4) * sizeof(float) : 0;
+    p.plan = rows_plan(HKV, R, HD, kv_f16, n_keys, n_cu);
+    p.part = p.plan.n_split > 1 ? (size_t)nq * H * p.plan.n_split * (HD + 4) * sizeof(float) : 0;
     p.planes = (size_t)HKV * tiles * HD / 32 * 2 * 64 * sizeof(uint4);
     p.p2e = (size_t)HKV * tiles * 16 * sizeof(float);
     p.lse = (size_t)HKV * R * sizeof(float);
@@ -788,14 +775,14 @@ hipError_t launch_attn_prompt_weights(const float *q, int nq, int H, int HKV, in
     uint8_t *base = (uint8_t *)scratch;
     RowsArgs a{};
     a.q = q, a.kv = kv, a.n_ctx = n_ctx, a.H = H, a.HKV = HKV, a.T = nq, a.pos0 = pos0;
-    a.mode = ROWS_CAUSAL, a.scale = scale, a.out = out, a.n_split = p.ns;
+    a.mode = ROWS_CAUSAL, a.scale = scale, a.out = out;
     a.planes = (uint4 *)base, a.p2e = (float *)(base + p.planes), a.lse = (float *)(base + p.planes + p.p2e);
     a.part = (float *)(base + p.planes + p.p2e + p.lse);
-    rows_derive(a, HD, kv_f16);
+    rows_derive(a, p.plan.n_split, p.plan.nrb, p.plan.least);
     return rows_by_shape(HD, kv_f16, [&](auto hd, auto f16) {
         constexpr int D = decltype(hd)::value;
         constexpr bool F = decltype(f16)::value;
-        hipError_t e = rows_launch<D, F>(a, 1, false, s);
+        hipError_t e = rows_launch<D, F>(a, p.plan, 1, s);
         if (e == hipSuccess && a.n_split > 1) e = rows_launch_merge<D>(a, 1, s);
         if (e != hipSuccess) return e;
         constexpr int KT = D == 256 ? 1 : 2, per = PW_UNITS * 16 * KT;
