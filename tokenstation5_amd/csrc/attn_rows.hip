@@ -656,10 +656,13 @@ static int rows_splits(int items, int keys, int slots, int least) {
 }
 
 // Up to 16 rows go to k_attn_rows, whose waves split the keys (8 caches of 16384 keys, 16 rows: 61 us, 85 by
-// k_attn_tile), more to k_attn_tile, whose waves split the rows (20 rows: 96 us, 130 by two row tiles a wave
+// k_attn_tile), more to k_attn_tile, whose waves split the rows (20 rows: 80 us, 130 by two row tiles a wave
 // there). Its waves take one row tile each, or two past 64 rows where every workgroup has more than 384
 // keys to go through: a key's conversion then serves twice the rows (64 tokens of 32/8 heads over 8 x 16384 keys 320 us,
 // 405 by one tile, over 8 x 4096 98 and 110), but a block takes longer (1 x 4096 37 and 33 us, 1 x 700 25 and 18).
+// Two workgroups a CU, but three of up to 32 rows of a q8 cache (two of their waves have none, and the keys' conversion
+// bounds them: 20 rows over 8 x 16384 keys 80 us, 96 by two; f16 97 and 92, 64 rows over 8 x 4096 43 and 41, heads of
+// 64 over 8 x 4096 14.7 and 13.4).
 // A slice reads at least half as many bytes of keys and values as its rows' queries and partials take
 // (84 rows over 4096 keys, two tiles: 128 keys a slice 27.5 us with the join, 192 25.3, 256 26.7, 384 30.8).
 static RowsPlan rows_plan(int seqs, int R, int HD, int kv_f16, int keys, int n_cu) {  // seqs: caches x KV heads
@@ -670,7 +673,7 @@ static RowsPlan rows_plan(int seqs, int R, int HD, int kv_f16, int keys, int n_c
     p.nrb = (R + p.per - 1) / p.per;
     const int key = 2 * (kv_f16 ? 2 * HD : HD + HD / 16), n = std::min(R, p.per) * (2 * HD + 4) * 4 / (2 * key);
     p.least = std::max(ROWS_MIN_KEYS, (n + 63) / 64 * 64);
-    p.n_split = rows_splits(seqs * p.nrb, keys, p.tile ? 2 * n_cu : n_cu, p.least);
+    p.n_split = rows_splits(seqs * p.nrb, keys, (!p.tile ? 1 : R <= 32 && HD == 128 && !kv_f16 ? 3 : 2) * n_cu, p.least);
     return p;
 }
 
