@@ -663,16 +663,21 @@ static int rows_splits(int items, int keys, int slots, int least) {
 // Two workgroups a CU, but three of up to 32 rows of a q8 cache (two of their waves have none, and the keys' conversion
 // bounds them: 20 rows over 8 x 16384 keys 80 us, 96 by two; f16 97 and 92, 64 rows over 8 x 4096 43 and 41, heads of
 // 64 over 8 x 4096 14.7 and 13.4).
-// A slice reads at least half as many bytes of keys and values as its rows' queries and partials take
-// (84 rows over 4096 keys, two tiles: 128 keys a slice 27.5 us with the join, 192 25.3, 256 26.7, 384 30.8).
+// A slice reads at least half as many bytes of keys and values as its rows' queries and partials take, and 128 keys.
+// Where that is more than 64 keys and slices are more than the CUs, 64 keys more (64 rows over 4096 keys, 8 KV heads:
+// 192 keys a slice 19.9 us with the join, 128 21.9, 256 21.0; over 1500 keys 16.8, 15.1, 19.3); where it is not and
+// slices are at most half of the CUs, 64 (20 rows over 1500 keys 11.5 us, 12.9 by 128; over 3 x 1500 16.5 and 15.5).
 static RowsPlan rows_plan(int seqs, int R, int HD, int kv_f16, int keys, int n_cu) {  // seqs: caches x KV heads
     RowsPlan p;
     p.tile = R > 16;
     const bool two = HD <= 128 && R > 64 && (int64_t)seqs * ((R + 127) / 128) * keys > (int64_t)384 * 2 * n_cu;
     p.per = !p.tile ? 16 : two ? 128 : 64;
     p.nrb = (R + p.per - 1) / p.per;
-    const int key = 2 * (kv_f16 ? 2 * HD : HD + HD / 16), n = std::min(R, p.per) * (2 * HD + 4) * 4 / (2 * key);
-    p.least = std::max(ROWS_MIN_KEYS, (n + 63) / 64 * 64);
+    const int key = 2 * (kv_f16 ? 2 * HD : HD + HD / 16), worth = std::min(R, p.per) * (2 * HD + 4) * 4 / (2 * key);
+    p.least = std::max(ROWS_MIN_KEYS, (worth + 63) / 64 * 64);
+    const int64_t all = (int64_t)seqs * p.nrb * keys;
+    if (p.tile && worth > 64 && all > (int64_t)p.least * n_cu) p.least += 64;
+    if (p.tile && worth <= 64 && 2 * all <= (int64_t)ROWS_MIN_KEYS * n_cu) p.least = 64;
     p.n_split = rows_splits(seqs * p.nrb, keys, (!p.tile ? 1 : R <= 32 && HD == 128 && !kv_f16 ? 3 : 2) * n_cu, p.least);
     return p;
 }
