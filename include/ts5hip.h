@@ -184,7 +184,8 @@ int ts5hip_topk(ts5hip_ctx *ctx, const float *x, int n, int k, float *vals_dev, 
  * counts within f16's range (65504). TS5HIP_KV_F16: k, v f16, ks and vs null. B caches lie back to back.
  * Head dimension 64, 128 or 256, up to 16 query heads a KV head, n_ctx x head_dim x value bytes a KV head
  * below 2 GiB, n_head_kv up to 512, B up to 4096. q, out, cache values and bounds are 16-byte aligned. Counts on the device
- * (n_keys_dev, n_past_dev) are taken into 0..n_ctx. A query without a key gets zeros; one that is NaN
+ * (n_keys_dev, n_past_dev) are taken into 0..n_ctx. A query without a key (or whose scores are all
+ * minus infinity) gets zeros; one that is NaN
  * or reads NaN keys gets NaN; one that reads infinite values, infinities or NaN there. Scratch is the context's: it
  * grows on the first call of a size, and no two streams use it. ---- */
 

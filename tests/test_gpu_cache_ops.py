@@ -190,6 +190,63 @@ def test_tree_nonfinite_values_of_other_branches(ctx, kv, H, HKV, HD):
         assert np.all(np.isfinite(got[0, 9, :, 3:]))
 
 
+@pytest.mark.parametrize("kv", [Q8, F16])
+@pytest.mark.parametrize("HD", [64, 128])
+@pytest.mark.parametrize("T,past", [(64, 130), (37, 0), (61, 700)])
+def test_tree_two_row_tiles(ctx, kv, HD, T, past):
+    """A large cache and many rows (two row tiles a wave): slices, rows past the last, and values that are no numbers
+    in other branches and behind the tree."""
+    H, HKV, slots = 32, 2, 22000
+    rng = np.random.default_rng([101, HD, T, kv])
+    c = Cache(ctx, rng, kv, 1, HKV, slots, HD)
+    bad = [past + 4, past + 7]
+    for n in "kv":
+        raw = c.raw[n + "s"] if kv == Q8 else c.raw[n]
+        raw[0, :, bad[0]], raw[0, :, bad[1]], raw[0, :, past + T:] = np.nan, np.inf, np.nan
+    c.send()
+    q = rng.standard_normal((1, T, H, HD)).astype(np.float32)
+    mask = random_masks(rng, 1, T)
+    mask[0, [t for t in range(T) if t not in (4, 7)]] &= ~np.uint64(1 << 4 | 1 << 7)
+    got = run_tree(ctx, c, q, T, [past], mask, 0.1, H)
+    clean = [t for t in range(T) if t not in (4, 7)]
+    k, v, G, seen = c.values("k"), c.values("v"), H // HKV, tree_seen(mask[0], past, T)[clean]
+    for h in range(H):
+        want, _, tol, _ = attend(q[0, clean, h].astype(np.float64), k[0, h // G, :past + T], v[0, h // G, :past + T], seen, 0.1)
+        check_rows(got[0, clean, h], want, tol, (kv, h))
+    assert np.all(np.isnan(got[0, 4]))
+    # (q8: an infinite scale times its group's sum of q k. Where all four sums are negative the score is minus
+    # infinity and the weight 0, and a row that sees that key alone counts as one without a key.)
+    if kv == F16:
+        assert not np.any(np.isfinite(got[0, 7]))
+
+
+@pytest.mark.parametrize("kv", [Q8, F16])
+def test_prompt_weights_two_row_tiles(ctx, kv):
+    """A chunk long enough for two row tiles a wave."""
+    H, HKV, HD, nq, pos0, scale = 32, 2, 64, 530, 1101, 0.1
+    n, G = nq + pos0, H // HKV
+    rng = np.random.default_rng([103, kv])
+    c = Cache(ctx, rng, kv, 1, HKV, n, HD)
+    q = rng.standard_normal((nq, H, HD)).astype(np.float32)
+    out, acc = ctx.alloc(q.nbytes), ctx.to_device(np.zeros((1, HKV, n), np.float32))
+    ctx.attn_prompt_weights(ctx.to_device(q), nq, H, HKV, HD, *c.args, pos0, scale, out, acc, acc)
+    got, sums = out.download(np.float32, q.shape), acc.download(np.float32, (HKV, n))
+    k, v = c.values("k").astype(np.float64), c.values("v").astype(np.float64)
+    seen = np.arange(n)[None] <= pos0 + np.arange(nq)[:, None]
+    add, add_tol = np.zeros((HKV, n)), np.zeros((HKV, n))
+    for h in range(H):  # attend's formulas, with products of matrices
+        x, kk, vv = q[:, h].astype(np.float64), k[0, h // G], v[0, h // G]
+        s = np.where(seen, x @ kk.T * scale, -np.inf)
+        p = np.exp(s - s.max(1, keepdims=True))
+        p /= p.sum(1, keepdims=True)
+        ds = np.where(seen, 4 * 2.0 ** -22 * scale * (np.abs(x) @ np.abs(kk).T), 0).max(1, keepdims=True)
+        rel = 2 * ds + 2.0 ** -24 * (16 + 4 * np.sqrt(n))
+        check_rows(got[:, h], p @ vv, rel * (p @ np.abs(vv)) + 1e-30, (kv, h))
+        add[h // G] += p.sum(0)
+        add_tol[h // G] += (rel * p + 1e-30).sum(0)
+    check_sums(np.zeros((HKV, n), np.float32), sums, n, add, add_tol, nq * G, (kv,))
+
+
 def test_tree_counts_outside_the_cache(ctx):
     """Counts in device memory are taken into the cache: -5 as 0, one past the end as the last that fits."""
     rng = np.random.default_rng(6)
@@ -378,7 +435,7 @@ def test_prompt_weights_long(ctx):
 @pytest.mark.parametrize("H,HKV,HD", [(14, 2, 64), (2, 2, 128), (8, 2, 128), (32, 4, 128), (8, 4, 256), (16, 2, 256)])
 def test_prompt_weights_nonfinite_later_keys(ctx, kv, H, HKV, HD):
     """NaN keys and values of a later token of the chunk do not reach the queries before it: rows for every form
-    of the kernel (one and two row tiles, four and eight waves)."""
+    of the kernel (waves that split the keys, four or eight, and waves that split the rows)."""
     nq, pos0 = 20, 50
     rng = np.random.default_rng(22)
     c = Cache(ctx, rng, kv, 1, HKV, 70, HD)
