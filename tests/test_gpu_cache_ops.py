@@ -874,3 +874,48 @@ def test_calls_repeat_bit_for_bit(ctx):
         got = [d.download(np.uint32) for d in outs[:2] + sums]
         first = first or got
         assert all(np.array_equal(a, b) for a, b in zip(got, first))
+
+
+@pytest.mark.parametrize("kv", [Q8, F16])
+@pytest.mark.parametrize("H,HKV,HD", [(4, 2, 64), (32, 8, 128), (8, 4, 256)])
+@pytest.mark.parametrize("n", [1, 700])
+def test_weights_of_scores_that_are_all_minus_infinity(ctx, kv, H, HKV, HD, n):
+    """A head whose scores are all past fp32's lowest has no weights: zeros, and the sums of its KV head's keys are
+    those of the other heads. (Scores: a sum of HD products of 2e38 and a key below 0, of 0.8 at the mean, times 0.09.)"""
+    G, scale = H // HKV, 0.09
+    rng = np.random.default_rng([107, HD, n, kv])
+    c = Cache(ctx, rng, kv, 2, HKV, n, HD)
+    c.raw["k"] = -np.abs(c.raw["k"])
+    if kv == Q8:  # the second cache: infinite scales, the same for every head
+        c.raw["k"][1] = np.minimum(c.raw["k"][1], -1)
+        c.raw["ks"][1] = np.inf
+    c.send()
+    q = rng.standard_normal((2, H, HD)).astype(np.float32)
+    q[0, ::G] = 2e38
+    if kv == Q8:
+        q[1] = np.abs(q[1]) + np.float32(0.01)
+    none = np.zeros((2, H), bool)  # heads without a weight
+    none[0, ::G], none[1] = True, kv == Q8
+    acc = rng.random((2, HKV, n)).astype(np.float32)
+    want, tol = np.zeros((2, H, HD)), np.zeros((2, H, HD)) + 1e-30
+    add, add_tol = np.zeros((2, HKV, n)), np.zeros((2, HKV, n))
+    k, v = c.values("k"), c.values("v")
+    for b, h in np.argwhere(~none):
+        o, p, t, tp = attend(q[b, h][None].astype(np.float64), k[b, h // G], v[b, h // G], np.ones((1, n), bool), scale)
+        want[b, h], tol[b, h] = o[0], t[0]
+        add[b, h // G] += p[0]
+        add_tol[b, h // G] += tp[0]
+    out, d_acc = ctx.to_device(np.full_like(q, 9)), ctx.to_device(acc)
+    ctx.attn_decode_weights(ctx.to_device(q), 2, H, HKV, HD, *c.args, ctx.to_device(np.array([n, n], np.int32)), scale, out,
+                            d_acc, d_acc)
+    got, sums = out.download(np.float32, q.shape), d_acc.download(np.float32, acc.shape)
+    assert np.all(got[none] == 0)
+    check_rows(got, want, tol, (kv, HD))
+    for b in range(2):
+        check_sums(acc[b], sums[b], n, add[b], add_tol[b], G, (kv, HD, b))
+    # A prompt of one token over the first cache.
+    d_acc = ctx.to_device(acc)
+    ctx.attn_prompt_weights(ctx.to_device(q[0]), 1, H, HKV, HD, *c.args, n - 1, scale, out, d_acc, d_acc)
+    got, sums = out.download(np.float32, q.shape), d_acc.download(np.float32, acc.shape)
+    check_rows(got[0], want[0], tol[0], (kv, HD, "prompt"))
+    check_sums(acc[0], sums[0], n, add[0], add_tol[0], G, (kv, HD, "prompt"))

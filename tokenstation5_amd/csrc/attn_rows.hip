@@ -521,7 +521,7 @@ __global__ __launch_bounds__(256) void k_one_weights(RowsArgs a, const float *ac
             if (m[i] != -INFINITY || l[i] != l[i])  // (a slice of NaN scores has no maximum)
                 sum = fmaf(__builtin_amdgcn_exp2f(m[i] - M), l[i], sum);
         sum = row_sum_dpp(sum);
-        if (s0 == 0) lse[g] = M + __log2f(sum);
+        if (s0 == 0) lse[g] = sum == 0.f ? INFINITY : M + __log2f(sum);  // (every score minus infinity: no weights)
     }
     __syncthreads();
     float w[4] = {0.f, 0.f, 0.f, 0.f};
