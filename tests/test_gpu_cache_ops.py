@@ -919,3 +919,20 @@ def test_weights_of_scores_that_are_all_minus_infinity(ctx, kv, H, HKV, HD, n):
     got, sums = out.download(np.float32, q.shape), d_acc.download(np.float32, acc.shape)
     check_rows(got[0], want[0], tol[0], (kv, HD, "prompt"))
     check_sums(acc[0], sums[0], n, add[0], add_tol[0], G, (kv, HD, "prompt"))
+
+
+@pytest.mark.parametrize("count,same", [(2 ** 31 - 1, 300), (2 ** 31 - 3, 300), (-7, 0), (-2 ** 31, 0)])
+def test_sparse_counts_past_the_cache(ctx, count, same):
+    """A batch's count on the device is taken into the cache before the queries' places are added to it."""
+    H, HKV, HD, B, slots = 8, 2, 128, 5, 300
+    rng = np.random.default_rng(109)
+    c = Cache(ctx, rng, Q8, 1, HKV, slots, HD)
+    q = ctx.to_device(rng.standard_normal((B, H, HD)).astype(np.float32))
+    bounds = ctx.to_device(np.stack([bounds_want(c.values("k")[0, h], slots, 16) for h in range(HKV)]))
+    got = []
+    for n in (count, same):
+        out, picked = ctx.to_device(np.full((B, H, HD), 9, np.float32)), ctx.to_device(np.full((B, HKV, 4), 77, np.int32))
+        ctx.attn_sparse(q, B, H, HKV, HD, *c.args, ctx.to_device(np.array([n], np.int32)), 0, bounds, 16, 4, 0.1, out, picked)
+        got.append((out.download(np.float32), picked.download(np.int32)))
+    assert np.array_equal(got[0][1], got[1][1]) and np.array_equal(got[0][0], got[1][0])
+    assert np.any(got[1][0])

@@ -109,7 +109,8 @@ struct SparseArgs {
     float *out;
 };
 __device__ inline int sparse_count(const SparseArgs &a, int b) {
-    return max(0, min(a.per_batch ? a.n_keys[b] : a.n_keys[0] + b + 1, a.n_ctx));
+    const int n = max(0, min(a.n_keys[a.per_batch ? b : 0], a.n_ctx));  // (before b is added: no overflow)
+    return a.per_batch ? n : min(n + b + 1, a.n_ctx);
 }
 
 template <int CTRL>
