@@ -1,5 +1,7 @@
 """What the entry points around a KV cache (trees, key weights, eviction, block-sparse attention) refuse, on the
 CPU: their arguments are checked before their context, so a null context reaches every check and no GPU."""
+import ctypes
+
 import pytest
 
 from tokenstation5_amd import ts5hip
@@ -88,3 +90,20 @@ def test_bounds_bytes():
     assert f(1, 1, 64, 1, 128) == 256
     assert f(1, 1, 64, 2 ** 31 - 1, 128) == 2 ** 24 * 256
     assert [f(*a) for a in ((0, 1, 64, 1, 64), (1, 0, 64, 1, 64), (1, 1, 64, 0, 64), (1, 1, 64, 1, 8))] == [-1] * 4
+
+
+@pytest.mark.parametrize("H,HKV,HD", [(14, 2, 64), (5, 1, 128), (32, 8, 128), (6, 2, 256)])
+@pytest.mark.parametrize("nq,keys", [(1, 1), (5, 700), (37, 4096), (530, 1631)])
+def test_prompt_weights_scratch_is_aligned(H, HKV, HD, nq, keys):
+    """The parts of the prompt key weights' scratch begin on lines of their own, none inside another, whatever the rows."""
+    layout = L()._ZN6ts5hip26attn_prompt_weights_layoutEiiiiiiiPm
+    layout.argtypes, layout.restype = [ctypes.c_int] * 7 + [ctypes.POINTER(ctypes.c_size_t)], None
+    total = L()._ZN6ts5hip33attn_prompt_weights_scratch_bytesEiiiiiii
+    total.argtypes, total.restype = [ctypes.c_int] * 7, ctypes.c_size_t
+    for f16 in (0, 1):
+        at = (ctypes.c_size_t * 4)()
+        layout(nq, H, HKV, HD, f16, keys, 256, at)
+        assert all(x % 256 == 0 for x in at), list(at)
+        tiles = -(-nq * (H // HKV) // 16)
+        ends = [at[0] + HKV * tiles * (HD // 32) * 2 * 64 * 16, at[1] + HKV * tiles * 16 * 4, at[2] + H * nq * 4]
+        assert all(e <= b for e, b in zip(ends, list(at)[1:])) and at[3] <= total(nq, H, HKV, HD, f16, keys, 256)

@@ -760,21 +760,25 @@ hipError_t launch_attn_one_weights(const float *q, int B, int H, int HKV, int HD
 
 struct PromptWeightsScratch {
     RowsPlan plan;
-    size_t part, planes, p2e, lse;  // bytes
+    size_t planes, p2e, lse, part, bytes;  // where each begins, and the end
 };
 static PromptWeightsScratch prompt_scratch(int nq, int H, int HKV, int HD, int kv_f16, int n_keys, int n_cu) {
-    const int R = nq * (H / HKV), tiles = (R + 15) / 16;
+    const size_t R = (size_t)nq * (H / HKV), tiles = (R + 15) / 16;
     PromptWeightsScratch p;
-    p.plan = rows_plan(HKV, R, HD, kv_f16, n_keys, n_cu);
-    p.part = p.plan.n_split > 1 ? (size_t)nq * H * p.plan.n_split * (HD + 4) * sizeof(float) : 0;
-    p.planes = (size_t)HKV * tiles * HD / 32 * 2 * 64 * sizeof(uint4);
-    p.p2e = (size_t)HKV * tiles * 16 * sizeof(float);
-    p.lse = (size_t)HKV * R * sizeof(float);
+    p.plan = rows_plan(HKV, (int)R, HD, kv_f16, n_keys, n_cu);
+    p.planes = 0;
+    p.p2e = p.planes + align_up(HKV * tiles * HD / 32 * 2 * 64 * sizeof(uint4), 256);
+    p.lse = p.p2e + align_up(HKV * tiles * 16 * sizeof(float), 256);
+    p.part = p.lse + align_up(HKV * R * sizeof(float), 256);
+    p.bytes = p.part + (p.plan.n_split > 1 ? (size_t)nq * H * p.plan.n_split * (HD + 4) * sizeof(float) : 0);
     return p;
 }
 size_t attn_prompt_weights_scratch_bytes(int nq, int H, int HKV, int HD, int kv_f16, int n_keys, int n_cu) {
+    return prompt_scratch(nq, H, HKV, HD, kv_f16, n_keys, n_cu).bytes;
+}
+void attn_prompt_weights_layout(int nq, int H, int HKV, int HD, int kv_f16, int n_keys, int n_cu, size_t at[4]) {
     const PromptWeightsScratch p = prompt_scratch(nq, H, HKV, HD, kv_f16, n_keys, n_cu);
-    return p.part + p.planes + p.p2e + p.lse;
+    at[0] = p.planes, at[1] = p.p2e, at[2] = p.lse, at[3] = p.part;
 }
 hipError_t launch_attn_prompt_weights(const float *q, int nq, int H, int HKV, int HD, KvLayer kv, int kv_f16, int n_ctx,
                                       int pos0, float scale, void *scratch, float *out, const float *acc,
@@ -784,8 +788,8 @@ hipError_t launch_attn_prompt_weights(const float *q, int nq, int H, int HKV, in
     RowsArgs a{};
     a.q = q, a.kv = kv, a.n_ctx = n_ctx, a.H = H, a.HKV = HKV, a.T = nq, a.pos0 = pos0;
     a.mode = ROWS_CAUSAL, a.scale = scale, a.out = out;
-    a.planes = (uint4 *)base, a.p2e = (float *)(base + p.planes), a.lse = (float *)(base + p.planes + p.p2e);
-    a.part = (float *)(base + p.planes + p.p2e + p.lse);
+    a.planes = (uint4 *)(base + p.planes), a.p2e = (float *)(base + p.p2e), a.lse = (float *)(base + p.lse);
+    a.part = (float *)(base + p.part);
     rows_derive(a, p.plan.n_split, p.plan.nrb, p.plan.least);
     return rows_by_shape(HD, kv_f16, [&](auto hd, auto f16) {
         constexpr int D = decltype(hd)::value;

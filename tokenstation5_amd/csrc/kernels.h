@@ -189,6 +189,8 @@ hipError_t launch_attn_one_weights(const float *q, int B, int H, int HKV, int HD
                                    float *acc_out, int n_cu, hipStream_t s);
 // nq consecutive queries over one cache, causal, and the same sums.
 size_t attn_prompt_weights_scratch_bytes(int nq, int H, int HKV, int HD, int kv_f16, int n_keys, int n_cu);
+// Where in it the rows' planes, their 2^e, their log sums and the slices' partials begin.
+void attn_prompt_weights_layout(int nq, int H, int HKV, int HD, int kv_f16, int n_keys, int n_cu, size_t at[4]);
 hipError_t launch_attn_prompt_weights(const float *q, int nq, int H, int HKV, int HD, KvLayer kv, int kv_f16, int n_ctx,
                                       int pos0, float scale, void *scratch, float *out, const float *acc,
                                       float *acc_out, int n_cu, hipStream_t s);
