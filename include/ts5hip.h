@@ -228,7 +228,7 @@ int ts5hip_attn_prompt_weights(ts5hip_ctx *ctx, const float *q, int nq, int n_he
  * last), in slot order; all of them where there are no more than n_keep. Each KV head keeps its own. acc_out
  * [B][n_head_kv][n_ctx_out] gets their sums and zeros behind them; kept_dev [B][n_head_kv][n_keep] their slots
  * (-1 behind the last); n_out_dev [B] (may be null) the keys kept. Cache rows behind them stay as they are. The
- * outputs overlap none of the inputs. */
+ * outputs overlap none of the inputs (n_out_dev is not n_keys_dev) and not each other: TS5HIP_ERR_ARG. */
 int ts5hip_kv_evict(ts5hip_ctx *ctx, int B, int n_head_kv, int head_dim, int kv_type, const void *k, const void *ks,
                     const void *v, const void *vs, int n_ctx, const int32_t *n_keys_dev, const float *acc, int n_keep,
                     int n_first, int n_last, int n_ctx_out, void *k_out, void *ks_out, void *v_out, void *vs_out,

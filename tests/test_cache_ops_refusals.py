@@ -107,3 +107,12 @@ def test_prompt_weights_scratch_is_aligned(H, HKV, HD, nq, keys):
         tiles = -(-nq * (H // HKV) // 16)
         ends = [at[0] + HKV * tiles * (HD // 32) * 2 * 64 * 16, at[1] + HKV * tiles * 16 * 4, at[2] + H * nq * 4]
         assert all(e <= b for e, b in zip(ends, list(at)[1:])) and at[3] <= total(nq, H, HKV, HD, f16, keys, 256)
+
+
+@pytest.mark.parametrize("change", [dict(n_out=P), dict(n_keys=11 * P, n_out=11 * P), dict(n_keys=11 * P, n_out=11 * P + 4, B=3),
+                                    dict(n_out=3 * P + 4096), dict(n_out=5 * P), dict(n_out=10 * P), dict(n_out=6 * P + 64),
+                                    dict(n_keys=6 * P + 8), dict(n_keys=10 * P), dict(v_out=6 * P), dict(vs_out=7 * P + 512)])
+def test_evict_outputs_of_their_own(change):
+    """Counts written over the counts that other workgroups still read, and outputs over inputs or other outputs."""
+    assert call("evict", **change) == (ARG, "an eviction's outputs lie over its inputs or each other")
+    assert call("evict", n_keys=12 * P, n_out=11 * P) == (ARG, "ctx is null")

@@ -936,3 +936,20 @@ def test_sparse_counts_past_the_cache(ctx, count, same):
         got.append((out.download(np.float32), picked.download(np.int32)))
     assert np.array_equal(got[0][1], got[1][1]) and np.array_equal(got[0][0], got[1][0])
     assert np.any(got[1][0])
+
+
+@pytest.mark.parametrize("kv", [Q8, F16])
+def test_evict_refuses_slots_over_its_inputs(ctx, kv):
+    """The list of kept slots over the counts, the sums, a cache or another output (the call is not made)."""
+    rng = np.random.default_rng(113)
+    HKV, HD, n, keep = 2, 64, 96, 32
+    c, to = Cache(ctx, rng, kv, 1, HKV, n, HD), Cache(ctx, rng, kv, 1, HKV, keep, HD)
+    n_keys, acc = ctx.to_device(np.array([n], np.int32)), ctx.to_device(rng.random((1, HKV, n)).astype(np.float32))
+    acc_out, n_out, kept = ctx.alloc(HKV * keep * 4), ctx.alloc(4), ctx.alloc(HKV * keep * 4)
+    t = to.args[1:5]
+    for bad in (n_keys, acc, c.dev["k"], c.dev["v"], t[0], acc_out, n_out):
+        with pytest.raises(ts5hip.Ts5HipError) as e:
+            ctx.kv_evict(1, HKV, HD, *c.args, n_keys, acc, keep, 1, 4, keep, *t, acc_out, bad, n_out)
+        assert e.value.code == ts5hip.ERR_ARG
+    ctx.kv_evict(1, HKV, HD, *c.args, n_keys, acc, keep, 1, 4, keep, *t, acc_out, kept, n_out)
+    assert n_out.download(np.int32).tolist() == [keep] and n_keys.download(np.int32).tolist() == [n]

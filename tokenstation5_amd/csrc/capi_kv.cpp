@@ -54,9 +54,13 @@ KvLayer layer(const void *k, const void *ks, const void *v, const void *vs) {
     return KvLayer{(int8_t *)k, (uint16_t *)ks, (int8_t *)v, (uint16_t *)vs};
 }
 
-bool overlap(const void *a, size_t na, const void *b, size_t nb) {
-    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
-    return a && b && x < y + nb && y < x + na;
+struct Range {
+    const void *p;
+    size_t bytes;
+};
+bool overlap(const Range &a, const Range &b) {
+    const uintptr_t x = (uintptr_t)a.p, y = (uintptr_t)b.p;
+    return a.p && b.p && a.bytes && b.bytes && x < y + b.bytes && y < x + a.bytes;
 }
 
 }  // namespace
@@ -165,15 +169,19 @@ int ts5hip_kv_evict(ts5hip_ctx *ctx, int B, int n_head_kv, int head_dim, int kv_
     if (n_keep < 1 || n_keep > n_ctx_out || n_first < 0 || n_last < 0 || (int64_t)n_first + n_last > n_keep)
         return fail(ctx, TS5HIP_ERR_ARG, "keeping %d keys (the first %d, the last %d) in a cache of %d", n_keep, n_first,
                     n_last, n_ctx_out);
-    const size_t vb = kv_type == KV_Q8 ? 1 : 2, rows = (size_t)B * n_head_kv * n_ctx;
-    const size_t rows_out = (size_t)B * n_head_kv * n_ctx_out;
-    const size_t row = head_dim * vb, sc = kv_type == KV_Q8 ? head_dim / 32 * 2 : 0;  // bytes (f16: no scales)
-    const struct { const void *p; size_t row; } from[] = {{k, row}, {v, row}, {ks, sc}, {vs, sc}, {acc, 4}};
-    const struct { const void *p; size_t row; } to[] = {{k_out, row}, {v_out, row}, {ks_out, sc}, {vs_out, sc}, {acc_out, 4}};
-    for (const auto &f : from)
-        for (const auto &t : to)
-            if (f.row && t.row && overlap(f.p, rows * f.row, t.p, rows_out * t.row))
-                return fail(ctx, TS5HIP_ERR_ARG, "the kept keys need a cache (and sums) of their own");
+    const size_t heads = (size_t)B * n_head_kv, rows = heads * n_ctx, rows_out = heads * n_ctx_out;
+    const size_t row = head_dim * (kv_type == KV_Q8 ? 1 : 2), sc = kv_type == KV_Q8 ? head_dim / 32 * 2 : 0;  // bytes (f16: no scales)
+    const Range in[] = {{k, rows * row}, {v, rows * row}, {ks, rows * sc}, {vs, rows * sc}, {acc, rows * 4}, {n_keys_dev, (size_t)B * 4}};
+    const Range out[] = {{k_out, rows_out * row}, {v_out, rows_out * row}, {ks_out, rows_out * sc}, {vs_out, rows_out * sc},
+                         {acc_out, rows_out * 4}, {n_out_dev, (size_t)B * 4}, {kept_dev, heads * n_keep * 4}};
+    constexpr int N_IN = sizeof in / sizeof *in, N_OUT = sizeof out / sizeof *out;
+    for (int o = 0; o < N_OUT; o++) {
+        // kept_dev last, and only for a call that has a context: without one its address may be any.
+        if (o == N_OUT - 1 && !ctx) break;
+        for (int i = 0; i < N_IN + o; i++)
+            if (overlap(out[o], i < N_IN ? in[i] : out[i - N_IN]))
+                return fail(ctx, TS5HIP_ERR_ARG, "an eviction's outputs lie over its inputs or each other");
+    }
     if (!ctx) return fail(nullptr, TS5HIP_ERR_ARG, "ctx is null");
     const OnDevice on(ctx->device);
     TS5_HIP(ctx, launch_kv_evict(B, n_head_kv, head_dim, layer(k, ks, v, vs), kv_type == KV_F16, n_ctx, n_keys_dev, acc,

@@ -52,7 +52,7 @@ __global__ __launch_bounds__(256) void k_evict_copy(EvictArgs a) {
     const int m = min(evict_count(a, b), a.n_keep), rows = min(EVICT_ROWS, m - r0);
     if (tid < EVICT_ROWS && r0 + tid < a.n_ctx_out) {
         const int r = r0 + tid;
-        if (r < m) src[tid] = a.kept[head * a.n_keep + r];
+        if (r < m) src[tid] = max(0, min(a.kept[head * a.n_keep + r], a.n_ctx - 1));  // (inside the cache, whatever came between)
         a.acc_out[to + r] = r < m ? a.acc[from + src[tid]] : 0.f;
     }
     __syncthreads();
