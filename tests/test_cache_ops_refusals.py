@@ -116,3 +116,14 @@ def test_evict_outputs_of_their_own(change):
     """Counts written over the counts that other workgroups still read, and outputs over inputs or other outputs."""
     assert call("evict", **change) == (ARG, "an eviction's outputs lie over its inputs or each other")
     assert call("evict", n_keys=12 * P, n_out=11 * P) == (ARG, "ctx is null")
+
+
+@pytest.mark.parametrize("name,B", [("weights", 1), ("weights", 3), ("prompt", 1)])
+def test_sums_over_themselves(name, B):
+    """acc_out beside acc or acc itself, not a part of it: one thread would write what another has yet to read."""
+    more = dict(B=B) if name == "weights" else {}
+    size = B * 2 * 256 * 4
+    for at in (4, 1024, size - 4, -4, 4 - size):
+        assert call(name, acc=Q, acc_out=Q + at, **more) == (ARG, "acc_out is acc or does not overlap it")
+    for at in (0, size, -size):
+        assert call(name, acc=Q, acc_out=Q + at, **more) == (ARG, "ctx is null")

@@ -63,6 +63,14 @@ bool overlap(const Range &a, const Range &b) {
     return a.p && b.p && a.bytes && b.bytes && x < y + b.bytes && y < x + a.bytes;
 }
 
+// The sums of key weights, [B][n_head_kv][n_ctx], before and after.
+int check_sums(ts5hip_ctx *ctx, int B, int n_head_kv, int n_ctx, const float *acc, const float *acc_out) {
+    const size_t bytes = (size_t)B * n_head_kv * n_ctx * 4;
+    if (acc != acc_out && overlap({acc, bytes}, {acc_out, bytes}))
+        return fail(ctx, TS5HIP_ERR_ARG, "acc_out is acc or does not overlap it");
+    return TS5HIP_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -126,6 +134,7 @@ int ts5hip_attn_decode_weights(ts5hip_ctx *ctx, const float *q, int B, int n_hea
     if (int rc = check_heads(ctx, n_head, n_head_kv, head_dim)) return rc;
     if (int rc = check_cache(ctx, B, n_head_kv, head_dim, kv_type, k, ks, v, vs, n_ctx, true)) return rc;
     if (!aligned(q, 16) || !aligned(out, 16)) return fail(ctx, TS5HIP_ERR_ARG, "q and out need 16-byte alignment");
+    if (int rc = check_sums(ctx, B, n_head_kv, n_ctx, acc, acc_out)) return rc;
     if (!ctx) return fail(nullptr, TS5HIP_ERR_ARG, "ctx is null");
     const OnDevice on(ctx->device);
     if (int rc = ensure_scratch(ctx, attn_one_weights_scratch_bytes(B, n_head, n_head_kv, head_dim, n_ctx, ctx->n_cu)))
@@ -147,6 +156,7 @@ int ts5hip_attn_prompt_weights(ts5hip_ctx *ctx, const float *q, int nq, int n_he
     if ((int64_t)n_head * nq > 960000)  // (the grid's rows of 16)
         return fail(ctx, TS5HIP_ERR_UNSUPPORTED, "%d queries of %d heads (960000 in all)", nq, n_head);
     if (!aligned(q, 16) || !aligned(out, 16)) return fail(ctx, TS5HIP_ERR_ARG, "q and out need 16-byte alignment");
+    if (int rc = check_sums(ctx, 1, n_head_kv, n_ctx, acc, acc_out)) return rc;
     if (!ctx) return fail(nullptr, TS5HIP_ERR_ARG, "ctx is null");
     const OnDevice on(ctx->device);
     if (int rc = ensure_scratch(ctx, attn_prompt_weights_scratch_bytes(nq, n_head, n_head_kv, head_dim, kv_type == KV_F16,
