@@ -336,8 +336,11 @@ __device__ inline uint32_t rows_window(uint64_t x, int at) {
 }
 
 // One unit into the sums. With MASK, seen(qt, key) has a bit for each of keys key .. + 3 that a
-// row takes (branch-free: a branch here let the compiler overwrite scores);
-// with SAN infinite and NaN values are left out (the product with a row that does not
+// row takes: bits, and no `a || b ? score : -inf` of a key at a time. The compiler (LLVM 22 of ROCm 7.2.0,
+// structurizecfg, whatever the flags) moves an element of a product's vector, which costs nothing, out of the block that
+// such a branch guards, and lanes that come to the block by b, not by a, get -inf: the score's register took b's
+// shift and then -inf, and the block that had to bring the score back was empty (f16 scores are elements; q8's are sums).
+// With SAN infinite and NaN values are left out (the product with a row that does not
 // take their key would be NaN), and the unit says that it had some: they are added
 // where the rows are written.
 template <int HD, bool F16, int KT, int NT, bool MASK, bool SAN, class Seen, class Put>
