@@ -46,7 +46,8 @@ __global__ __launch_bounds__(64) void k_rope_kv(const float *__restrict__ qkv, i
                                                 const int32_t *__restrict__ at, int n_pos) {
     __shared__ float v[256];
     const int hh = blockIdx.x, t = blockIdx.y, i = threadIdx.x;
-    const int pos = pos0p[0] + t, turn = AT ? at[t] : pos;
+    // (a sum past 2^31 wraps to a slot below 0: out of the cache)
+    const int pos = (int)((uint32_t)pos0p[0] + (uint32_t)t), turn = AT ? at[t] : pos;
     if (AT && (turn < 0 || turn >= n_pos || pos < 0 || pos >= n_ctx)) return;
     const float *src = qkv + (int64_t)t * qkv_stride + (int64_t)hh * HD;
     const bool is_q = hh < H, is_k = !is_q && hh < H + HKV;
