@@ -953,3 +953,100 @@ def test_evict_refuses_slots_over_its_inputs(ctx, kv):
         assert e.value.code == ts5hip.ERR_ARG
     ctx.kv_evict(1, HKV, HD, *c.args, n_keys, acc, keep, 1, 4, keep, *t, acc_out, kept, n_out)
     assert n_out.download(np.int32).tolist() == [keep] and n_keys.download(np.int32).tolist() == [n]
+
+
+@pytest.mark.parametrize("slot0", [-3, 29, 2 ** 31 - 3, -2 ** 31])
+def test_append_at_slots_past_the_cache(ctx, slot0):
+    """Tokens whose slots are not in the cache are left out, those of the same call that are in it are not, near 2^31 too."""
+    H, HKV, HD, T, slots = 4, 2, 64, 7, 32
+    rng = np.random.default_rng([127, slot0 % 97])
+    qkv, pos = rng.standard_normal((T, (H + 2 * HKV) * HD)).astype(np.float32), np.arange(5, 5 + T, dtype=np.int32)
+    cs, c = ctx.rope_table(HD, 64, 10000.0), Cache(ctx, rng, Q8, 1, HKV, slots, HD)
+    q_out = ctx.to_device(np.full((T, H * HD), 7, np.float32))
+    kvt, k, ks, v, vs, _ = c.args
+    ctx.rope_kv_append_at(ctx.to_device(qkv), T, ctx.to_device(pos), ctx.to_device(np.array([slot0], np.int32)), H, HKV, HD,
+                          HD, 0, cs, 64, slots, kvt, q_out, k, ks, v, vs)
+    got, got_q = c.fetch(), q_out.download(np.float32, (T, H * HD))
+    taken = [t for t in range(T) if 0 <= slot0 + t < slots]
+    for t in range(T):
+        assert (t in taken) != bool(np.all(got_q[t] == 7)), t
+    for s in range(slots):
+        same = all(np.array_equal(got[n][:, :, s], c.raw[n][:, :, s]) for n in got)
+        assert same != (s - slot0 in taken), s
+    for t in taken:  # as at a slot in the middle
+        one = Cache(ctx, rng, Q8, 1, HKV, slots, HD)
+        ctx.rope_kv_append_at(ctx.to_device(qkv[t]), 1, ctx.to_device(pos[t:t + 1]), ctx.to_device(np.array([9], np.int32)), H,
+                              HKV, HD, HD, 0, cs, 64, slots, kvt, q_out, *one.args[1:5])
+        o = one.fetch()
+        assert all(np.array_equal(o[n][:, :, 9], got[n][:, :, slot0 + t]) for n in o), t
+
+
+@pytest.mark.parametrize("kv", [Q8, F16])
+@pytest.mark.parametrize("HKV,HD,block,n", [(2, 64, 16, 203), (2, 128, 32, 320), (1, 256, 64, 130)])
+def test_bounds_that_attention_reads(ctx, kv, HKV, HD, block, n):
+    """The bounds that the library writes, from a buffer of NaN: of the whole blocks of a cache, then of each key that is
+    appended, its block's. The blocks picked and the outputs are those of bounds computed here, and the last block
+    is read with its bounds not there (a NaN block would rank first, and a block too many would show)."""
+    H, n_pick, slots, steps = 4 * HKV, 3, 512, 2 * block
+    rng = np.random.default_rng([131, HD, kv])
+    c = Cache(ctx, rng, kv, 1, HKV, slots, HD)
+    cs = ctx.rope_table(HD, slots, 10000.0)
+    nb = -(-slots // block)
+    bounds = ctx.to_device(np.full((HKV, nb, 2, HD), np.nan, np.float16))
+    kvt, k, ks, v, vs, _ = c.args
+    whole = n // block * block
+
+    def counts(m):
+        return ctx.to_device(np.array([m], np.int32))
+
+    def check(m, what):
+        c.raw = c.fetch()
+        want = np.stack([bounds_want(c.values("k")[0, h], slots, block) for h in range(HKV)])
+        q = ctx.to_device(rng.standard_normal((1, H, HD)).astype(np.float32))
+        got = []
+        for b in (bounds, ctx.to_device(want)):
+            out, picked = ctx.to_device(np.full((H, HD), 9, np.float32)), ctx.to_device(np.full((HKV, n_pick), 77, np.int32))
+            ctx.attn_sparse(q, 1, H, HKV, HD, *c.args, counts(m), 1, b, block, n_pick, 0.1, out, picked)
+            got.append((out.download(np.float32), picked.download(np.int32)))
+        assert np.array_equal(got[0][1], got[1][1]) and np.array_equal(got[0][0], got[1][0]), what
+        assert got[0][1][-1] == -(-m // block) - 1 and np.all(np.isfinite(got[0][0])), what
+
+    ctx.kv_block_bounds(1, HKV, HD, kv, k, ks, slots, counts(whole), slots, block, bounds)
+    check(n, "whole blocks")  # (where n ends inside a block, that block's bounds are NaN)
+    check_sparse(ctx, c, rng.standard_normal((1, H, HD)).astype(np.float32), H, [n], 1, block, n_pick, 0.1, (kv, HD))
+    ctx.kv_block_bounds(1, HKV, HD, kv, k, ks, slots, counts(n), 1, block, bounds)
+    q_out = ctx.alloc(H * HD * 4)
+    for i in range(steps):
+        qkv = ctx.to_device(rng.standard_normal((1, (H + 2 * HKV) * HD)).astype(np.float32))
+        ctx.rope_kv_append_at(qkv, 1, counts(n + i), counts(n + i), H, HKV, HD, HD, 0, cs, slots, slots, kvt, q_out, k, ks, v, vs)
+        ctx.kv_block_bounds(1, HKV, HD, kv, k, ks, slots, counts(n + i + 1), 1, block, bounds)
+        if i % 7 == 0 or i + 1 == steps:
+            check(n + i + 1, i)
+
+
+@pytest.mark.parametrize("kv", [Q8, F16])
+def test_counts_outside_the_cache(ctx, kv):
+    """Counts below 0 and past the slots in device memory: none, and as many as there are, for every entry point."""
+    H, HKV, HD, slots, block = 8, 2, 128, 150, 32
+    rng = np.random.default_rng([137, kv])
+    c = Cache(ctx, rng, kv, 3, HKV, slots, HD)
+    q = ctx.to_device(rng.standard_normal((3, H, HD)).astype(np.float32))
+    acc = ctx.to_device(rng.random((3, HKV, slots)).astype(np.float32))
+    kvt, k, ks, v, vs, _ = c.args
+    nb = -(-slots // block)
+    got = []
+    for counts in ([-5, 2 ** 31 - 1, slots + 1], [0, slots, slots]):
+        n = ctx.to_device(np.array(counts, np.int32))
+        out, sums = ctx.to_device(np.full((3, H, HD), 9, np.float32)), ctx.to_device(np.full((3, HKV, slots), 9, np.float32))
+        ctx.attn_decode_weights(q, 3, H, HKV, HD, *c.args, n, 0.1, out, acc, sums)
+        bounds = ctx.to_device(np.full((3, HKV, nb, 2, HD), 7, np.float16))
+        ctx.kv_block_bounds(3, HKV, HD, kv, k, ks, slots, n, slots, block, bounds)
+        sparse, picked = ctx.to_device(np.full((3, H, HD), 9, np.float32)), ctx.to_device(np.full((3, HKV, 3), 77, np.int32))
+        ctx.attn_sparse(q, 3, H, HKV, HD, *c.args, n, 1, bounds, block, 3, 0.1, sparse, picked)
+        to = Cache(ctx, np.random.default_rng(1), kv, 3, HKV, 60, HD)
+        to_acc, kept, n_out = ctx.alloc(3 * HKV * 60 * 4), ctx.alloc(3 * HKV * 50 * 4), ctx.alloc(12)
+        ctx.kv_evict(3, HKV, HD, *c.args, n, acc, 50, 2, 9, 60, *to.args[1:5], to_acc, kept, n_out)
+        parts = [d.download(np.uint32) for d in (out, sums, bounds, sparse, picked, to_acc, kept, n_out)]
+        got.append(parts + list(to.fetch().values()))
+    assert all(np.array_equal(a, b) for a, b in zip(*got))
+    assert got[0][7].tolist() == [0, 50, 50] and not np.any(got[0][0].reshape(3, -1)[0])
