@@ -220,30 +220,22 @@ __device__ inline void rows_clear(RowsSum<HD, NT> &a) {
     }
 }
 
-// S^T of a unit: s[t][qt][i] (times 2^-e) of key 4 kq + i of tile t, row 16 qt + rl.
-template <int HD, bool F16, int KT, int NT>
-__device__ inline void rows_scores(const RowsUnit<HD, F16, KT> &u, const RowsQ<HD, NT> &q,
-                                   float (&s)[KT][NT][4]) {
+// S^T of a unit: s[t][i] (times 2^-e) of key 4 kq + i of tile t, row rl.
+template <int HD, bool F16, int KT>
+__device__ inline void rows_scores(const RowsUnit<HD, F16, KT> &u, const RowsQ<HD, 1> &q, float (&s)[KT][4]) {
     using S = RowsShape<HD, F16, KT>;
 #pragma unroll
     for (int t = 0; t < KT; t++) {
         if constexpr (F16) {
-            ar_f4 R[NT];
-#pragma unroll
-            for (int qt = 0; qt < NT; qt++) R[qt] = ar_f4{0.f, 0.f, 0.f, 0.f};
+            ar_f4 R = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int c = 0; c < S::NC; c++) {
                 const ar_h8 ka = rows_values<S::KW>(u.k[t][c]);
-#pragma unroll
-                for (int qt = 0; qt < NT; qt++) {
-                    R[qt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q.h[qt][c], R[qt], 0, 0, 0);
-                    R[qt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q.l[qt][c], R[qt], 0, 0, 0);
-                }
+                R = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q.h[0][c], R, 0, 0, 0);
+                R = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q.l[0][c], R, 0, 0, 0);
             }
 #pragma unroll
-            for (int qt = 0; qt < NT; qt++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) s[t][qt][i] = R[qt][i];
+            for (int i = 0; i < 4; i++) s[t][i] = R[i];
         } else {
 #pragma unroll
             for (int c = 0; c < S::NC; c++) {
@@ -251,14 +243,10 @@ __device__ inline void rows_scores(const RowsUnit<HD, F16, KT> &u, const RowsQ<H
                 float ks[4];
 #pragma unroll
                 for (int i = 0; i < 4; i++) ks[i] = h2f((u.ks[t][(i * S::NC + c) / 2] >> (16 * (c & 1))) & 0xffff);
+                ar_f4 R = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q.h[0][c], ar_f4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                R = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q.l[0][c], R, 0, 0, 0);
 #pragma unroll
-                for (int qt = 0; qt < NT; qt++) {
-                    ar_f4 R = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q.h[qt][c], ar_f4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-                    R = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q.l[qt][c], R, 0, 0, 0);
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        s[t][qt][i] = c == 0 ? ks[i] * R[i] : fmaf(ks[i], R[i], s[t][qt][i]);
-                }
+                for (int i = 0; i < 4; i++) s[t][i] = c == 0 ? ks[i] * R[i] : fmaf(ks[i], R[i], s[t][i]);
             }
         }
     }
@@ -335,7 +323,7 @@ __device__ inline uint32_t rows_window(uint64_t x, int at) {
     return at >= 64 ? 0u : (uint32_t)(at >= 0 ? r : l) & 15u;
 }
 
-// One unit into the sums. With MASK, seen(qt, key) has a bit for each of keys key .. + 3 that a
+// One unit into the sums. With MASK, seen(key) has a bit for each of keys key .. + 3 that a
 // row takes: bits, and no `a || b ? score : -inf` of a key at a time. The compiler (LLVM 22 of ROCm 7.2.0,
 // structurizecfg, whatever the flags) moves an element of a product's vector, which costs nothing, out of the block that
 // such a branch guards, and lanes that come to the block by b, not by a, get -inf: the score's register took b's
@@ -343,43 +331,39 @@ __device__ inline uint32_t rows_window(uint64_t x, int at) {
 // With SAN infinite and NaN values are left out (the product with a row that does not
 // take their key would be NaN), and the unit says that it had some: they are added
 // where the rows are written.
-template <int HD, bool F16, int KT, int NT, bool MASK, bool SAN, class Seen, class Put>
-__device__ inline bool rows_unit(const RowsUnit<HD, F16, KT> &u, const RowsQ<HD, NT> &q, RowsSum<HD, NT> &a,
+template <int HD, bool F16, int KT, bool MASK, bool SAN, class Seen, class Put>
+__device__ inline bool rows_unit(const RowsUnit<HD, F16, KT> &u, const RowsQ<HD, 1> &q, RowsSum<HD, 1> &a,
                                  const int (&kb)[KT], int kq, Seen seen, Put put) {
     using S = RowsShape<HD, F16, KT>;
     using Op = RowsOp<KT>;
-    float s[KT][NT][4];
-    rows_scores<HD, F16, KT, NT>(u, q, s);
-    typename Op::T ph[NT], pl[NT];
+    float s[KT][4];
+    rows_scores<HD, F16, KT>(u, q, s);
+    float mx = -INFINITY;
 #pragma unroll
-    for (int qt = 0; qt < NT; qt++) {
-        float mx = -INFINITY;
+    for (int t = 0; t < KT; t++) {
+        const uint32_t take = MASK ? seen(kb[t] + 4 * kq) : 15u;
 #pragma unroll
-        for (int t = 0; t < KT; t++) {
-            const uint32_t take = MASK ? seen(qt, kb[t] + 4 * kq) : 15u;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if constexpr (MASK) s[t][qt][i] = take & 1u << i ? s[t][qt][i] : -INFINITY;
-                mx = fmaxf(mx, s[t][qt][i]);
-            }
+        for (int i = 0; i < 4; i++) {
+            if constexpr (MASK) s[t][i] = take & 1u << i ? s[t][i] : -INFINITY;
+            mx = fmaxf(mx, s[t][i]);
         }
-#pragma unroll
-        for (int t = 0; t < KT; t++) put(qt, kb[t] + 4 * kq, s[t][qt]);
-        const float m0 = rows_reference(a, qt, max_xor32(max_xor16(mx)) * q.p2e[qt]);
-        float sum = 0.f;
-        uint32_t hi[2 * KT], lo[2 * KT];
-#pragma unroll
-        for (int t = 0; t < KT; t++)
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const float p0 = __builtin_amdgcn_exp2f(fmaf(s[t][qt][2 * i], q.p2e[qt], -m0));
-                const float p1 = __builtin_amdgcn_exp2f(fmaf(s[t][qt][2 * i + 1], q.p2e[qt], -m0));
-                sum += p0 + p1;
-                rows_split(p0, p1, hi[2 * t + i], lo[2 * t + i]);
-            }
-        ph[qt] = Op::of(hi), pl[qt] = Op::of(lo);
-        a.l[qt] += sum;  // (the lane's share: its four keys of each tile)
     }
+#pragma unroll
+    for (int t = 0; t < KT; t++) put(kb[t] + 4 * kq, s[t]);
+    const float m0 = rows_reference(a, 0, max_xor32(max_xor16(mx)) * q.p2e[0]);
+    float sum = 0.f;
+    uint32_t whi[2 * KT], wlo[2 * KT];
+#pragma unroll
+    for (int t = 0; t < KT; t++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[t][2 * i], q.p2e[0], -m0));
+            const float p1 = __builtin_amdgcn_exp2f(fmaf(s[t][2 * i + 1], q.p2e[0], -m0));
+            sum += p0 + p1;
+            rows_split(p0, p1, whi[2 * t + i], wlo[2 * t + i]);
+        }
+    const typename Op::T ph = Op::of(whi), pl = Op::of(wlo);
+    a.l[0] += sum;  // (the lane's share: its four keys of each tile)
     RowsScale<HD, F16, KT> sc;
     if constexpr (!F16) {
 #pragma unroll
@@ -416,12 +400,9 @@ __device__ inline bool rows_unit(const RowsUnit<HD, F16, KT> &u, const RowsQ<HD,
                 }
             }
             const typename Op::T vh = Op::of(hi), vl = Op::of(lo);
-#pragma unroll
-            for (int qt = 0; qt < NT; qt++) {
-                a.o[qt][dt] = Op::mfma(vh, ph[qt], a.o[qt][dt]);
-                if constexpr (!F16) a.o[qt][dt] = Op::mfma(vl, ph[qt], a.o[qt][dt]);
-                a.o[qt][dt] = Op::mfma(vh, pl[qt], a.o[qt][dt]);
-            }
+            a.o[0][dt] = Op::mfma(vh, ph, a.o[0][dt]);
+            if constexpr (!F16) a.o[0][dt] = Op::mfma(vl, ph, a.o[0][dt]);
+            a.o[0][dt] = Op::mfma(vh, pl, a.o[0][dt]);
         }
     };
     if (!SAN || !bad) products(std::false_type{});
@@ -438,51 +419,47 @@ __device__ inline float rows_nonfinite(const KvLayer &kv, int64_t slot, int d) {
     return (__builtin_bit_cast(uint16_t, h) & 0x7c00) == 0x7c00 ? (float)h : 0.f;
 }
 
-// The waves' sums of the workgroup's 16 NT rows, combined: emit(row, d, o, m, l) once
+// The waves' sums of the workgroup's 16 rows, combined: emit(row, d, o, m, l) once
 // for each row below `rows` and 4 dims from d on. Every thread calls it.
 template <int HD, int NW>
 struct RowsLds {
     __align__(16) float o[NW][16][HD + 4];
     float m[NW][16], l[NW][16];
 };
-template <int HD, int NT, int NW, class Emit>
-__device__ inline void rows_combine(RowsLds<HD, NW> &L, const RowsSum<HD, NT> &a, int rows, int wave, int rl, int kq,
+template <int HD, int NW, class Emit>
+__device__ inline void rows_combine(RowsLds<HD, NW> &L, const RowsSum<HD, 1> &a, int rows, int wave, int rl, int kq,
                                     Emit emit) {
     constexpr int NDT = HD / 16;
+    const int nr = min(rows, 16);
+    __syncthreads();
+    const float sum = add_xor32(add_xor16(a.l[0]));
+    if (rl < nr) {
+        if (kq == 0) L.m[wave][rl] = a.m[0], L.l[wave][rl] = sum;
 #pragma unroll
-    for (int qt = 0; qt < NT; qt++) {
-        const int nr = min(rows - 16 * qt, 16);  // (uniform: every thread leaves together)
-        if (nr <= 0) return;
-        __syncthreads();
-        const float sum = add_xor32(add_xor16(a.l[qt]));
-        if (rl < nr) {
-            if (kq == 0) L.m[wave][rl] = a.m[qt], L.l[wave][rl] = sum;
+        for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+            for (int d = 0; d < NDT; d += 4)
+                *(float4 *)&L.o[wave][rl][NDT * (4 * kq + i) + d] =
+                    make_float4(a.o[0][d][i], a.o[0][d + 1][i], a.o[0][d + 2][i], a.o[0][d + 3][i]);
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < nr * (HD / 4); e += 64 * NW) {
+        const int r = e / (HD / 4), d = 4 * (e % (HD / 4));
+        float M = L.m[0][r];
 #pragma unroll
-                for (int d = 0; d < NDT; d += 4)
-                    *(float4 *)&L.o[wave][rl][NDT * (4 * kq + i) + d] =
-                        make_float4(a.o[qt][d][i], a.o[qt][d + 1][i], a.o[qt][d + 2][i], a.o[qt][d + 3][i]);
+        for (int w = 1; w < NW; w++) M = fmaxf(M, L.m[w][r]);
+        float l = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+            const float lw = L.l[w][r];
+            const float x = lw != lw ? lw : L.m[w][r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(L.m[w][r] - M);
+            if (x == 0.f) continue;  // (a wave with no key of the row; NaN scores have no maximum)
+            const float4 p = *(const float4 *)&L.o[w][r][d];
+            l = fmaf(x, lw, l);
+            o.x = fmaf(x, p.x, o.x), o.y = fmaf(x, p.y, o.y), o.z = fmaf(x, p.z, o.z), o.w = fmaf(x, p.w, o.w);
         }
-        __syncthreads();
-        for (int e = threadIdx.x; e < nr * (HD / 4); e += 64 * NW) {
-            const int r = e / (HD / 4), d = 4 * (e % (HD / 4));
-            float M = L.m[0][r];
-#pragma unroll
-            for (int w = 1; w < NW; w++) M = fmaxf(M, L.m[w][r]);
-            float l = 0.f;
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int w = 0; w < NW; w++) {
-                const float lw = L.l[w][r];
-                const float x = lw != lw ? lw : L.m[w][r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(L.m[w][r] - M);
-                if (x == 0.f) continue;  // (a wave with no key of the row; NaN scores have no maximum)
-                const float4 p = *(const float4 *)&L.o[w][r][d];
-                l = fmaf(x, lw, l);
-                o.x = fmaf(x, p.x, o.x), o.y = fmaf(x, p.y, o.y), o.z = fmaf(x, p.z, o.z), o.w = fmaf(x, p.w, o.w);
-            }
-            emit(16 * qt + r, d, o, M, l);
-        }
+        emit(r, d, o, M, l);
     }
 }
 

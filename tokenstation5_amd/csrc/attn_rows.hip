@@ -119,21 +119,21 @@ __global__ __launch_bounds__(64 * NW, ONE && HD <= 128 ? 3 : 1) void k_attn_rows
     if constexpr (ONE) {
         // One unit ahead in three waves a SIMD; two ahead in two waves is no faster (122 us), and in three it
         // spills (170 us).
-        auto put = [&](int, int key, const float (&s)[4]) {
+        auto put = [&](int key, const float (&s)[4]) {
             if (rl < R && key < kend)
                 *(float4 *)(a.scores + (row0 + rl) * a.stride + key) =
                     make_float4(s[0] * q.p2e[0], s[1] * q.p2e[0], s[2] * q.p2e[0], s[3] * q.p2e[0]);
         };
-        auto seen4 = [&](int, int key) { return rows_below(key, kend); };
+        auto seen4 = [&](int key) { return rows_below(key, kend); };
         for (int u = wave; u < units; u += NW) {
             const RowsUnit<HD, F16, KT> cur = nxt;
             at(u + NW, kb);
             rows_load<HD, F16, KT>(nxt, kv, kb, rl, kq);  // (past the slice: zeros, no memory access)
             at(u, kb);
-            rows_unit<HD, F16, KT, 1, true, false>(cur, q, sum, kb, kq, seen4, put);
+            rows_unit<HD, F16, KT, true, false>(cur, q, sum, kb, kq, seen4, put);
         }
     } else {
-        auto put = [](int, int, const float (&)[4]) {};
+        auto put = [](int, const float (&)[4]) {};
         for (int u = wave; u < units; u += NW) {
             const RowsUnit<HD, F16, KT> cur = nxt;
             int kn[KT];
@@ -141,15 +141,15 @@ __global__ __launch_bounds__(64 * NW, ONE && HD <= 128 ? 3 : 1) void k_attn_rows
             at(u + NW, kn);
             rows_load<HD, F16, KT>(nxt, kv, kn, rl, kq);
             if (kb[0] + S::UNIT <= full)
-                rows_unit<HD, F16, KT, 1, false, false>(cur, q, sum, kb, kq, [](int, int) { return 15u; }, put);
-            else if (rows_unit<HD, F16, KT, 1, true, true>(
+                rows_unit<HD, F16, KT, false, false>(cur, q, sum, kb, kq, [](int) { return 15u; }, put);
+            else if (rows_unit<HD, F16, KT, true, true>(
                          cur, q, sum, kb, kq,
-                         [&](int, int key) { return rows_below(key, seen) | rows_window(bits, key - n); },
+                         [&](int key) { return rows_below(key, seen) | rows_window(bits, key - n); },
                          put))
                 nonfinite = 1;
         }
     }
-    rows_combine<HD, 1, NW>(L, sum, R, wave, rl, kq, [&](int r, int d, float4 o, float m, float l) {
+    rows_combine<HD, NW>(L, sum, R, wave, rl, kq, [&](int r, int d, float4 o, float m, float l) {
         const int t = rows_div(r, a.g_m);
         if (!ONE && nonfinite)
             rows_add_nonfinite<HD, F16>(a, b, kvh, t, n, kbeg + max(full - kbeg, 0) / S::UNIT * S::UNIT, kend, d, o);

@@ -97,7 +97,7 @@ hipError_t launch_block_bounds(int B, int HKV, int HD, KvLayer kv, int kv_f16, i
 struct SparseArgs {
     const float *q;  // [B][H * HD]
     KvLayer kv;
-    int n_ctx, H, HKV, B, per_batch, block, n_pick, n_split;
+    int n_ctx, H, HKV, per_batch, block, n_pick, n_split;
     const int32_t *n_keys;
     const _Float16 *bounds;  // [caches][HKV][n_blocks][2][HD]
     int n_blocks;
@@ -253,15 +253,15 @@ __global__ __launch_bounds__(64 * NW) void k_attn_picked(SparseArgs a) {
         for (int t = 0; t < KT; t++) kb[t] = kn[t];
         at(u + NW, kn);
         rows_load<HD, F16, KT>(nxt, kv, kn, rl, kq);
-        rows_unit<HD, F16, KT, 1, true, false>(cur, q, sum, kb, kq, [&](int, int key) { return rows_below(key, n); },
-                                               [](int, int, const float (&)[4]) {});
+        rows_unit<HD, F16, KT, true, false>(cur, q, sum, kb, kq, [&](int key) { return rows_below(key, n); },
+                                               [](int, const float (&)[4]) {});
     }
     // For the last workgroup, which may run on another XCD, the partials go past this one's L2, and only when they
     // are out does the workgroup count itself in.
     const int used = (units + per - 1) / per;
     const int64_t row0 = ((int64_t)b * a.HKV + kvh) * G;
     const __amdgpu_buffer_rsrc_t part = slice_rsrc(a.part + row0 * a.n_split * (HD + 4), (uint32_t)(G * a.n_split * (HD + 4) * 4));
-    rows_combine<HD, 1, NW>(L, sum, G, wave, rl, kq, [&](int r, int d, float4 o, float m, float l) {
+    rows_combine<HD, NW>(L, sum, G, wave, rl, kq, [&](int r, int d, float4 o, float m, float l) {
         if (FUSED && used == 1) {
             *(float4 *)(a.out + (row0 + r) * HD + d) = rows_over(o, l);
             return;
@@ -337,7 +337,7 @@ hipError_t launch_attn_sparse(const float *q, int B, int H, int HKV, int HD, KvL
     const SparseScratch p = sparse_scratch(B, H, HKV, HD, n_ctx, block, n_pick, n_cu);
     uint8_t *base = (uint8_t *)scratch;
     SparseArgs a{};
-    a.q = q, a.kv = kv, a.n_ctx = n_ctx, a.H = H, a.HKV = HKV, a.B = B, a.per_batch = per_batch, a.block = block;
+    a.q = q, a.kv = kv, a.n_ctx = n_ctx, a.H = H, a.HKV = HKV, a.per_batch = per_batch, a.block = block;
     a.n_pick = picked ? n_pick : std::min(n_pick, p.n_blocks), a.n_split = p.n_split, a.n_keys = n_keys, a.bounds = (const _Float16 *)bounds;
     a.n_blocks = p.n_blocks, a.scale = scale, a.out = out;
     a.scores = (double *)base, a.picked = picked ? picked : (int32_t *)(base + p.scores);
