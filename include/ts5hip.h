@@ -184,10 +184,10 @@ int ts5hip_topk(ts5hip_ctx *ctx, const float *x, int n, int k, float *vals_dev, 
  * counts within f16's range (65504). TS5HIP_KV_F16: k, v f16, ks and vs null. B caches lie back to back.
  * Head dimension 64, 128 or 256, up to 16 query heads a KV head, n_ctx x head_dim x value bytes a KV head
  * below 2 GiB, n_head_kv up to 512, B up to 4096. q, out, cache values and bounds are 16-byte aligned. Counts on the device
- * (n_keys_dev, n_past_dev) are taken into 0..n_ctx. A query without a key (or whose scores are all
- * minus infinity) gets zeros; one that is NaN
- * or reads NaN keys gets NaN; one that reads infinite values, infinities or NaN there. Scratch is the context's: it
- * grows on the first call of a size, and no two streams use it. ---- */
+ * (n_keys_dev) are taken into 0..n_ctx, n_past_dev into 0..n_ctx - n_tree. A query without a key (or whose scores are
+ * all minus infinity, in fp32) gets zeros and adds no key weights; one that is NaN or reads NaN keys gets NaN, and so may
+ * one that reads infinite f16 keys; one that reads infinite values, infinities or NaN there. Scratch is the
+ * context's: it grows on the first call of a size, and no two streams use it. ---- */
 
 /* ts5hip_rope_kv_append with each token's RoPE position pos_dev[t] (0..n_pos - 1, the rows of rope_cs) apart
  * from its cache slot *slot0_dev + t: the drafts of a tree that share a depth share a position, and an
@@ -214,7 +214,7 @@ int ts5hip_kv_path(ts5hip_ctx *ctx, int B, int n_head_kv, int head_dim, int kv_t
 /* ts5hip_attn_decode of one query per cache (n_keys_dev[b] keys each) that also adds up what each key was
  * worth: acc_out[b][h][j] = acc[b][h][j] + the softmax weights of key j over KV head h's query heads, for
  * j < n_keys_dev[b]; later entries stay as they are. acc, acc_out: [B][n_head_kv][n_ctx], the same
- * array or not overlapping. */
+ * array or not overlapping (else TS5HIP_ERR_ARG). */
 int ts5hip_attn_decode_weights(ts5hip_ctx *ctx, const float *q, int B, int n_head, int n_head_kv, int head_dim,
                                int kv_type, const void *k, const void *ks, const void *v, const void *vs, int n_ctx,
                                const int32_t *n_keys_dev, float scale, float *out, const float *acc, float *acc_out);

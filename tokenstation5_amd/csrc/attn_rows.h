@@ -13,6 +13,8 @@
 //    columns. The reference is a running maximum less 7, so that weights go past
 //    128 and their lo plane stays out of the fp16 subnormals; it follows the true
 //    maximum only once that is 4 above it (weights to 2^11), so that the sums are rarely scaled.
+//    A weight's planes end at 2^-24: beside its relative 2^-22 it is off by up to 2^-32 of the row's largest, which
+//    shows only in a dim where the large weights all meet values of 0.
 //  * O^T (dims x rows) += V^T . P^T. The D layout of S^T (lane: keys 4 kq .. + 3 of
 //    each tile) is the B layout of P^T, so P stays in registers as hi + lo. For V^T
 //    the lane in MFMA row m = lane & 15 and key group kq = lane >> 4 loads keys 4 kq ..

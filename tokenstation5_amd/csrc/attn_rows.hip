@@ -483,8 +483,9 @@ __global__ __launch_bounds__(256) void k_rows_merge(RowsArgs a, int64_t rows) {
 }
 
 // One query a cache: the join (the first workgroup of a KV head) and acc_out = acc + the group's
-// weights 2^(score - lse). HBM bounds it: scores read, sums read and written, 60 MB in 14 us. grid (1 + key blocks of
-// 1024, HKV, B).
+// weights 2^(score - lse). Scores read, sums read and written: 44 MB in 15 us (16 of 12288 to 16384 keys), 3 TB/s, so
+// latency more than HBM: the slices' sums, then the scores (requested before those: the same time). grid (1 + key
+// blocks of 1024, HKV, B).
 template <int HD>
 __global__ __launch_bounds__(256) void k_one_weights(RowsArgs a, const float *acc, float *acc_out) {
     __shared__ RowsJoin J;
@@ -667,6 +668,12 @@ static int rows_splits(int items, int keys, int slots, int least) {
 // Where that is more than 64 keys and slices are more than the CUs, 64 keys more (64 rows over 4096 keys, 8 KV heads:
 // 192 keys a slice 19.9 us with the join, 128 21.9, 256 21.0; over 1500 keys 16.8, 15.1, 19.3); where it is not and
 // slices are at most half of the CUs, 64 (20 rows over 1500 keys 11.5 us, 12.9 by 128; over 3 x 1500 16.5 and 15.5).
+// The same rules hold where they were not found, whole calls in us, two row tiles and one: f16, 32/8 heads of 128, 64
+// tokens over 8 x 16384 keys 263 and 316, 8 x 4096 90 and 97 (32 tokens 62 and 56: the rule's worst), 1 x 4096 33 and 29;
+// f16, 14/2 heads of 64, 64 tokens over 8 x 16384 80 and 86, 1 x 4096 17.2 and 16.0. Three workgroups a CU and two:
+// 8/4 heads of 256, 16 to 64 tokens over 8 x 4096, q8 48 to 89 and 38 to 72, f16 44 to 85 and 37 to 60.
+// `keys` is a tree's capacity, not its length, which is in device memory: a cache that is far from full is cut into longer
+// slices than its keys are worth.
 static RowsPlan rows_plan(int seqs, int R, int HD, int kv_f16, int keys, int n_cu) {  // seqs: caches x KV heads
     RowsPlan p;
     p.tile = R > 16;

@@ -123,7 +123,7 @@ __device__ inline double dpp_f64(double x) {
 
 // HD / 8 lanes a block, 8 dims and four blocks a lane; a head's four sums over the lanes go together:
 // two exchanges within a quad leave each of its lanes the quad's sum of one block, and only that goes
-// on to the other quads. 16 queries over 29000 blocks of 8 heads of 128 (59 MB): 16 us, the bytes and
+// on to the other quads. 16 queries over 14464 blocks in all of 8 heads of 128 (59 MB): 16 us, the bytes and
 // the fp64 multiply-adds about even (30 us with a head's sum over all lanes by itself and q
 // converted for each block). grid (ceil(n_blocks / blocks a workgroup), HKV, B).
 template <int HD>

@@ -153,7 +153,7 @@ int ts5hip_attn_prompt_weights(ts5hip_ctx *ctx, const float *q, int nq, int n_he
     if (int rc = check_cache(ctx, 1, n_head_kv, head_dim, kv_type, k, ks, v, vs, n_ctx, true)) return rc;
     if (nq < 1 || nq > 4096 || pos0 < 0 || (int64_t)pos0 + nq > n_ctx)
         return fail(ctx, TS5HIP_ERR_ARG, "%d queries (1..4096) at %d in a cache of %d", nq, pos0, n_ctx);
-    if ((int64_t)n_head * nq > 960000)  // (the grid's rows of 16)
+    if ((int64_t)n_head * nq > 960000)  // (blocks of 16 rows or more along the grid's y)
         return fail(ctx, TS5HIP_ERR_UNSUPPORTED, "%d queries of %d heads (960000 in all)", nq, n_head);
     if (!aligned(q, 16) || !aligned(out, 16)) return fail(ctx, TS5HIP_ERR_ARG, "q and out need 16-byte alignment");
     if (int rc = check_sums(ctx, 1, n_head_kv, n_ctx, acc, acc_out)) return rc;

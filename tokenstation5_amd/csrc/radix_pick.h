@@ -1,7 +1,8 @@
 // The k largest of n keys for one workgroup of 1024 threads, ties to the lowest index, as ascending
 // indices: a radix descent from the top digit to the k-th largest key, then the keys above it and the
 // first ones equal to it. 12 bits a pass: one pass spreads an fp32 key's exponent and 3 bits
-// over the bins, so that its LDS additions rarely meet, and few keys are left for the next;
+// over the bins, so that its LDS additions rarely meet, and few keys are left for the next (an fp64 key's first digit
+// is its sign and exponent alone, which scores of one query share: that pass settles little and its additions meet);
 // it ends once a bin is taken whole. The keys are staged in LDS, sixteen requests at a time, and a
 // thread takes an odd number of neighbours there (an odd stride meets no bank twice), so that the
 // last pass is counts and bit masks of its own keys instead of ballots; the picked
