@@ -253,6 +253,59 @@ int ts5hip_attn_sparse(ts5hip_ctx *ctx, const float *q, int B, int n_head, int n
                        const int32_t *n_keys_dev, int kv_per_batch, const void *bounds, int block, int n_pick,
                        float scale, float *out, int32_t *picked_dev);
 
+/* ---- caches in pages, and drafts judged by probabilities: device pointers, asynchronous on the context's stream, as
+ * above. No counterpart in the reference (one sequence, one cache of n_ctx slots; drafts kept where the sample equals them).
+ *
+ * A pool has n_pages pages of `page` slots (16, 32, 64, 128 or 256), back to back, each laid out as a cache of `page` slots:
+ * TS5HIP_KV_Q8: k, v int8 [n_pages][n_head_kv][page][head_dim], ks, vs f16 [..][head_dim / 32]; TS5HIP_KV_F16: k, v f16, ks
+ * and vs null. Position p of sequence s is slot p % page of page table_dev[s * n_table + p / page]; sequences may share
+ * pages. An entry outside 0..n_pages-1 is no page: tokens there are not written or read back, and their keys are no query's.
+ * Head dimension 64, 128 or 256, n_head_kv up to 512, n_table x page up to 2^30; float arrays, cache values and read-back rows are
+ * 16-byte aligned. Scratch is the context's, as above. ---- */
+
+/* ts5hip_rope_kv_append into pages: token t (of 1..65535) belongs to position pos_dev[t] (which is its RoPE position too, a
+ * row of rope_cs: 0..n_pos - 1) of sequence seq_dev[t] (0..n_seq - 1). A token without a place (padding: -1) is left out,
+ * its row of q_out too. No two tokens of a call have one place: what it held then would be parts of both. q_out does not
+ * overlap qkv. */
+int ts5hip_rope_kv_append_paged(ts5hip_ctx *ctx, const float *qkv, int ntok, const int32_t *seq_dev, const int32_t *pos_dev,
+                                int n_head, int n_head_kv, int head_dim, int n_rot, int neox, const float *rope_cs,
+                                int n_pos, const float *bias, const float *q_norm, const float *k_norm, float eps,
+                                float *q_out, int kv_type, void *k, void *ks, void *v, void *vs, int n_pages, int page,
+                                const int32_t *table_dev, int n_seq, int n_table);
+/* The cached K and V of ntok (1..2^24) tokens, token t position pos_dev[t] of sequence seq_dev[t], as the values they stand
+ * for: k_out, v_out [ntok][n_head_kv * head_dim], out_type TS5HIP_F32 (exact) or TS5HIP_F16 (rounded once). Rows of tokens
+ * without a place stay as they are. The outputs overlap neither the pool nor each other. */
+int ts5hip_kv_read_paged(ts5hip_ctx *ctx, int ntok, const int32_t *seq_dev, const int32_t *pos_dev, int n_head_kv,
+                         int head_dim, int kv_type, const void *k, const void *ks, const void *v, const void *vs,
+                         int n_pages, int page, const int32_t *table_dev, int n_seq, int n_table, int out_type,
+                         void *k_out, void *v_out);
+/* Attention of the n_new (1..16) newest tokens of each of B (1..4096) sequences over its pages: n_keys_dev[b] counts the
+ * sequence's keys, those tokens' included (it is taken into 0..n_table x page), and token t reads keys below L = n_keys_dev[b]
+ * - n_new + t + 1; with window > 0 only the last `window` of them. table_dev [B][n_table]; q, out [B][n_new][n_head *
+ * head_dim], not overlapping; up to 16 query heads a KV head; B x n_table x page up to 2^34. A query without a key (or whose
+ * scores are all minus infinity, in fp32) gets zeros; infinities and NaN of keys and values that it does not read do not
+ * reach it, of those that it reads they do. */
+int ts5hip_attn_paged(ts5hip_ctx *ctx, const float *q, int B, int n_new, int n_head, int n_head_kv, int head_dim,
+                      int kv_type, const void *k, const void *ks, const void *v, const void *vs, int n_pages, int page,
+                      const int32_t *table_dev, int n_table, const int32_t *n_keys_dev, int window, float scale, float *out);
+/* Drafted tokens judged by probabilities. logits: the target's rows [B][n_draft + 1][ld], row i those after the pending token
+ * and i drafts; draft_logits: the draft model's [B][n_draft][ld_draft] that the drafts were drawn from, or null for drafts
+ * that were certain (prompt lookup, a draft model's best token); of a row the first n_vocab (up to 2^20) entries count, minus
+ * infinity is probability 0. p = softmax(logits / temperature_dev[b]), q likewise of draft_logits, or 1 at the draft. Of sequence
+ * b's first n_draft_dev[b] (null: all n_draft, 0..63) drafts x_i = drafts_dev[b * n_draft + i], the first ones with
+ * uniform[i] q(x_i) < p(x_i) are kept; then one token is drawn by uniform[n_draft]: from max(p - q, 0) of the draft that was
+ * not kept (from p where that is 0 everywhere), or from the last row's p, as the first index whose cumulative weight is past
+ * uniform x their sum. uniform_dev [B][n_draft + 1] in [0, 1). At temperature 0 (or below, or NaN) drafts are kept while they
+ * are the row's first maximum, and the next token is that. tokens_dev [B][n_draft + 1]: the kept drafts, the next token, -1
+ * behind; n_tokens_dev [B]: how many; logp_dev [B][n_draft + 1] (may be null): log p of each (0 at temperature 0 and behind).
+ * A draft outside 0..n_vocab-1 is not kept. A row with a NaN or plus infinity, or all minus infinity, is no distribution: a draft's
+ * row counts as q = 0 and its draft is not kept; a sequence whose next token would come from one has none (-1, not counted).
+ * Computed in fp64. B up to 4096; the outputs overlap no input and not each other. */
+int ts5hip_verify_drafts(ts5hip_ctx *ctx, const float *logits, int64_t ld, const float *draft_logits, int64_t ld_draft,
+                         int n_vocab, int B, int n_draft, const int32_t *drafts_dev, const int32_t *n_draft_dev,
+                         const float *temperature_dev, const float *uniform_dev, int32_t *tokens_dev,
+                         int32_t *n_tokens_dev, float *logp_dev);
+
 /* ---- the sampler: Engine::sample (engine/src/engine.cpp:16-46) on host, std::mt19937_64 ---- */
 ts5hip_sampler *ts5hip_sampler_new(uint64_t seed);
 void ts5hip_sampler_free(ts5hip_sampler *s);

@@ -171,7 +171,8 @@ __device__ inline void rows_request(RowsIn<HD, NT> &in, int kq, Row row) {
             in.x[qt][c][0] = *(const float4 *)(p + 32 * c), in.x[qt][c][1] = *(const float4 *)(p + 32 * c + 4);
     }
 }
-template <int HD, int NT>
+// With WIDE, rows whose largest value is past fp32's range once it is scaled keep their 2^e all the same.
+template <int HD, int NT, bool WIDE = false>
 __device__ inline void rows_query(RowsQ<HD, NT> &q, const RowsIn<HD, NT> &in, float scale) {
     constexpr int NC = HD / 32;
     const float by = scale * AR_LOG2E;
@@ -187,8 +188,11 @@ __device__ inline void rows_query(RowsQ<HD, NT> &q, const RowsIn<HD, NT> &in, fl
                 asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(amax) : "v"(x.x), "v"(x.y));
                 asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(amax) : "v"(x.z), "v"(x.w));
             }
-        amax = max_xor32(max_xor16(amax)) * fabsf(by);
-        const int e = amax > 0.f ? max(ilogbf(amax) - 13, -100) : 0;
+        amax = max_xor32(max_xor16(amax));
+        const float most = amax;
+        amax *= fabsf(by);
+        int e = amax > 0.f ? max(ilogbf(amax) - 13, -100) : 0;
+        if (WIDE && amax == INFINITY && most < INFINITY && fabsf(by) < INFINITY) e = ilogbf(most) + ilogbf(by) - 12;
         const float sc = in.ok[qt] ? ldexpf(by, -e) : 0.f;  // (one rounding of q * by: the rest is a power of 2)
         q.p2e[qt] = ldexpf(1.0f, e);
 #pragma unroll

@@ -1,7 +1,7 @@
 // The entry points of include/ts5hip.h around a KV cache beyond decode, verify and prompt
 // attention: trees of drafts, accumulated key weights and eviction, block-sparse
 // attention. Host checks here, the context's last (so that arguments can be checked without a
-// GPU); kernels through kernels.h.
+// GPU); kernels through kernels.h. And around caches in pages and drafts judged by probabilities.
 #include <algorithm>
 
 #include "common_host.h"
@@ -61,6 +61,35 @@ struct Range {
 bool overlap(const Range &a, const Range &b) {
     const uintptr_t x = (uintptr_t)a.p, y = (uintptr_t)b.p;
     return a.p && b.p && a.bytes && b.bytes && x < y + b.bytes && y < x + a.bytes;
+}
+
+// No output lies over an input or over another output.
+template <int N_OUT, int N_IN>
+int check_apart(ts5hip_ctx *ctx, const Range (&out)[N_OUT], const Range (&in)[N_IN]) {
+    for (int o = 0; o < N_OUT; o++)
+        for (int i = 0; i < N_IN + o; i++)
+            if (overlap(out[o], i < N_IN ? in[i] : out[i - N_IN]))
+                return fail(ctx, TS5HIP_ERR_ARG, "outputs lie over inputs or each other");
+    return TS5HIP_OK;
+}
+
+// A pool of pages and the tables of n_seq sequences.
+int check_pool(ts5hip_ctx *ctx, int n_head_kv, int head_dim, int kv_type, const void *k, const void *ks, const void *v,
+               const void *vs, int n_pages, int page, const int32_t *table_dev, int n_seq, int n_table) {
+    if (!table_dev) return fail(ctx, TS5HIP_ERR_ARG, "null argument");
+    if (page != 16 && page != 32 && page != 64 && page != 128 && page != 256)
+        return fail(ctx, TS5HIP_ERR_UNSUPPORTED, "pages of %d slots (16, 32, 64, 128 or 256)", page);
+    if (int rc = check_cache(ctx, 1, n_head_kv, head_dim, kv_type, k, ks, v, vs, page, true)) return rc;
+    if (n_pages < 1 || n_seq < 1 || n_table < 1 || (int64_t)n_table * page > 1 << 30)
+        return fail(ctx, TS5HIP_ERR_ARG, "%d pages, tables of %d pages of %d sequences", n_pages, n_table, n_seq);
+    return TS5HIP_OK;
+}
+// Bytes of a pool's values (K or V) and of their scales.
+size_t pool_values(int n_pages, int page, int n_head_kv, int head_dim, int kv_type) {
+    return (size_t)n_pages * page * n_head_kv * head_dim * (kv_type == KV_Q8 ? 1 : 2);
+}
+size_t pool_scales(int n_pages, int page, int n_head_kv, int head_dim) {
+    return (size_t)n_pages * page * n_head_kv * (head_dim / 32) * 2;
 }
 
 // The sums of key weights, [B][n_head_kv][n_ctx], before and after.
@@ -243,6 +272,104 @@ int ts5hip_attn_sparse(ts5hip_ctx *ctx, const float *q, int B, int n_head, int n
     TS5_HIP(ctx, launch_attn_sparse(q, B, n_head, n_head_kv, head_dim, layer(k, ks, v, vs), kv_type == KV_F16, n_ctx,
                                     n_keys_dev, kv_per_batch != 0, bounds, block, n_pick, scale, ctx->scratch,
                                     ctx->counters, out, picked_dev, ctx->n_cu, ctx->stream));
+    return TS5HIP_OK;
+}
+
+int ts5hip_rope_kv_append_paged(ts5hip_ctx *ctx, const float *qkv, int ntok, const int32_t *seq_dev, const int32_t *pos_dev,
+                                int n_head, int n_head_kv, int head_dim, int n_rot, int neox, const float *rope_cs,
+                                int n_pos, const float *bias, const float *q_norm, const float *k_norm, float eps,
+                                float *q_out, int kv_type, void *k, void *ks, void *v, void *vs, int n_pages, int page,
+                                const int32_t *table_dev, int n_seq, int n_table) {
+    if (!qkv || !seq_dev || !pos_dev || !rope_cs || !q_out) return fail(ctx, TS5HIP_ERR_ARG, "null argument");
+    if (int rc = check_pool(ctx, n_head_kv, head_dim, kv_type, k, ks, v, vs, n_pages, page, table_dev, n_seq, n_table))
+        return rc;
+    if (n_head < 1 || n_head % n_head_kv || n_head > 65535 - 2 * n_head_kv || n_rot < 0 || n_rot > head_dim || n_rot % 2)
+        return fail(ctx, TS5HIP_ERR_UNSUPPORTED, "rope/kv for %d/%d heads of %d (n_rot %d)", n_head, n_head_kv,
+                    head_dim, n_rot);
+    if (ntok < 1 || ntok > 65535 || n_pos < 1) return fail(ctx, TS5HIP_ERR_ARG, "%d tokens, %d positions", ntok, n_pos);
+    if (!aligned(qkv, 16) || !aligned(q_out, 16) || !aligned(bias, 16) || !aligned(q_norm, 16) || !aligned(k_norm, 16) ||
+        !aligned(rope_cs, 16))
+        return fail(ctx, TS5HIP_ERR_ARG, "q, k, v, biases, norms and angles need 16-byte alignment");
+    const size_t heads = (size_t)ntok * head_dim * 4;
+    if (int rc = check_apart(ctx, {{q_out, heads * n_head}}, {{qkv, heads * (n_head + 2 * n_head_kv)}})) return rc;
+    if (!ctx) return fail(nullptr, TS5HIP_ERR_ARG, "ctx is null");
+    const OnDevice on(ctx->device);
+    TS5_HIP(ctx, launch_append_paged(qkv, ntok, seq_dev, pos_dev, n_head, n_head_kv, head_dim, bias, q_norm, k_norm, eps,
+                                     rope_cs, n_pos, n_rot, neox, q_out, layer(k, ks, v, vs), kv_type == KV_F16, n_pages,
+                                     page, table_dev, n_seq, n_table, ctx->stream));
+    return TS5HIP_OK;
+}
+
+int ts5hip_kv_read_paged(ts5hip_ctx *ctx, int ntok, const int32_t *seq_dev, const int32_t *pos_dev, int n_head_kv,
+                         int head_dim, int kv_type, const void *k, const void *ks, const void *v, const void *vs,
+                         int n_pages, int page, const int32_t *table_dev, int n_seq, int n_table, int out_type,
+                         void *k_out, void *v_out) {
+    if (!seq_dev || !pos_dev || !k_out || !v_out) return fail(ctx, TS5HIP_ERR_ARG, "null argument");
+    if (int rc = check_pool(ctx, n_head_kv, head_dim, kv_type, k, ks, v, vs, n_pages, page, table_dev, n_seq, n_table))
+        return rc;
+    if (ntok < 1 || ntok > 1 << 24) return fail(ctx, TS5HIP_ERR_ARG, "%d tokens (1..2^24)", ntok);
+    if (out_type != TS5HIP_F32 && out_type != TS5HIP_F16)
+        return fail(ctx, TS5HIP_ERR_UNSUPPORTED, "rows of type %d (f32 or f16)", out_type);
+    if (!aligned(k_out, 16) || !aligned(v_out, 16)) return fail(ctx, TS5HIP_ERR_ARG, "rows need 16-byte alignment");
+    const size_t rows = (size_t)ntok * n_head_kv * head_dim * (out_type == TS5HIP_F32 ? 4 : 2);
+    const size_t pool = pool_values(n_pages, page, n_head_kv, head_dim, kv_type);
+    const size_t scales = kv_type == KV_Q8 ? pool_scales(n_pages, page, n_head_kv, head_dim) : 0;
+    if (int rc = check_apart(ctx, {{k_out, rows}, {v_out, rows}}, {{k, pool}, {v, pool}, {ks, scales}, {vs, scales}})) return rc;
+    if (!ctx) return fail(nullptr, TS5HIP_ERR_ARG, "ctx is null");
+    const OnDevice on(ctx->device);
+    TS5_HIP(ctx, launch_read_paged(ntok, seq_dev, pos_dev, n_head_kv, head_dim, layer(k, ks, v, vs), kv_type == KV_F16,
+                                   n_pages, page, table_dev, n_seq, n_table, out_type == TS5HIP_F16, k_out, v_out,
+                                   ctx->stream));
+    return TS5HIP_OK;
+}
+
+int ts5hip_attn_paged(ts5hip_ctx *ctx, const float *q, int B, int n_new, int n_head, int n_head_kv, int head_dim,
+                      int kv_type, const void *k, const void *ks, const void *v, const void *vs, int n_pages, int page,
+                      const int32_t *table_dev, int n_table, const int32_t *n_keys_dev, int window, float scale,
+                      float *out) {
+    if (!q || !n_keys_dev || !out) return fail(ctx, TS5HIP_ERR_ARG, "null argument");
+    if (int rc = check_heads(ctx, n_head, n_head_kv, head_dim)) return rc;
+    if (int rc = check_pool(ctx, n_head_kv, head_dim, kv_type, k, ks, v, vs, n_pages, page, table_dev, B, n_table)) return rc;
+    if (B > 4096 || (int64_t)B * n_table * page > (int64_t)1 << 34)
+        return fail(ctx, TS5HIP_ERR_ARG, "%d sequences of up to %lld keys", B, (long long)n_table * page);
+    if (n_new < 1 || n_new > ATTN_MAX_NEW || window < 0)
+        return fail(ctx, TS5HIP_ERR_ARG, "%d new tokens (1..%d), window %d", n_new, ATTN_MAX_NEW, window);
+    if (!aligned(q, 16) || !aligned(out, 16)) return fail(ctx, TS5HIP_ERR_ARG, "q and out need 16-byte alignment");
+    const size_t rows = (size_t)B * n_new * n_head * head_dim * 4;
+    if (int rc = check_apart(ctx, {{out, rows}}, {{q, rows}})) return rc;
+    if (!ctx) return fail(nullptr, TS5HIP_ERR_ARG, "ctx is null");
+    const OnDevice on(ctx->device);
+    if (int rc = ensure_scratch(ctx, attn_paged_scratch_bytes(B, n_new, n_head, n_head_kv, head_dim, ctx->n_cu))) return rc;
+    TS5_HIP(ctx, launch_attn_paged(q, B, n_new, n_head, n_head_kv, head_dim, layer(k, ks, v, vs), kv_type == KV_F16,
+                                   n_pages, page, table_dev, n_table, n_keys_dev, window, scale, ctx->scratch,
+                                   ctx->counters, out, ctx->n_cu, ctx->stream));
+    return TS5HIP_OK;
+}
+
+int ts5hip_verify_drafts(ts5hip_ctx *ctx, const float *logits, int64_t ld, const float *draft_logits, int64_t ld_draft,
+                         int n_vocab, int B, int n_draft, const int32_t *drafts_dev, const int32_t *n_draft_dev,
+                         const float *temperature_dev, const float *uniform_dev, int32_t *tokens_dev,
+                         int32_t *n_tokens_dev, float *logp_dev) {
+    if (!logits || !temperature_dev || !uniform_dev || !tokens_dev || !n_tokens_dev || (n_draft > 0 && !drafts_dev))
+        return fail(ctx, TS5HIP_ERR_ARG, "null argument");
+    if (n_vocab < 1 || n_vocab > verify_max_vocab() || ld < n_vocab || (draft_logits && ld_draft < n_vocab))
+        return fail(ctx, TS5HIP_ERR_ARG, "%d entries (1..%d) of rows of %lld and %lld", n_vocab, verify_max_vocab(),
+                    (long long)ld, (long long)ld_draft);
+    if (B < 1 || B > 4096 || n_draft < 0 || n_draft > verify_max_drafts())
+        return fail(ctx, TS5HIP_ERR_ARG, "%d sequences of %d drafts (0..%d)", B, n_draft, verify_max_drafts());
+    const size_t rows = (size_t)B * (n_draft + 1), drafts = (size_t)B * n_draft;
+    if (ld > (int64_t)1 << 40 || (draft_logits && ld_draft > (int64_t)1 << 40))
+        return fail(ctx, TS5HIP_ERR_ARG, "rows of %lld and %lld entries", (long long)ld, (long long)ld_draft);
+    if (int rc = check_apart(ctx, {{tokens_dev, rows * 4}, {n_tokens_dev, (size_t)B * 4}, {logp_dev, rows * 4}},
+                             {{logits, rows * (size_t)ld * 4}, {draft_logits, drafts * (size_t)ld_draft * 4}, {drafts_dev, drafts * 4},
+                              {n_draft_dev, (size_t)B * 4}, {temperature_dev, (size_t)B * 4}, {uniform_dev, rows * 4}}))
+        return rc;
+    if (!ctx) return fail(nullptr, TS5HIP_ERR_ARG, "ctx is null");
+    const OnDevice on(ctx->device);
+    if (int rc = ensure_scratch(ctx, verify_scratch_bytes(n_vocab, B, n_draft))) return rc;
+    TS5_HIP(ctx, launch_verify(logits, ld, n_draft ? draft_logits : nullptr, ld_draft, n_vocab, B, n_draft, drafts_dev,
+                               n_draft_dev, temperature_dev, uniform_dev, ctx->scratch, ctx->counters, tokens_dev,
+                               n_tokens_dev, logp_dev, ctx->stream));
     return TS5HIP_OK;
 }
 

@@ -214,6 +214,30 @@ constexpr int KV_PATH_MAX = 64;  // rows of a path
 hipError_t launch_kv_path(int B, int HKV, int HD, KvLayer kv, int kv_f16, int n_ctx, const int32_t *slots, int n,
                           const int32_t *slot0, hipStream_t s);
 
+// A pool of pages of `page` slots (a power of 2), each a cache of that many slots, and the sequences' tables of them.
+// kv_paged.hip
+hipError_t launch_append_paged(const float *qkv, int ntok, const int32_t *seq, const int32_t *pos, int H, int HKV, int HD,
+                               const float *bias, const float *q_norm, const float *k_norm, float eps,
+                               const float *rope_cs, int n_pos, int n_rot, int neox, float *q_out, KvLayer kv, int kv_f16,
+                               int n_pages, int page, const int32_t *table, int n_seq, int n_table, hipStream_t s);
+hipError_t launch_read_paged(int ntok, const int32_t *seq, const int32_t *pos, int HKV, int HD, KvLayer kv, int kv_f16,
+                             int n_pages, int page, const int32_t *table, int n_seq, int n_table, int out16, void *k_out,
+                             void *v_out, hipStream_t s);
+// attn_paged.hip: T new tokens of each of B sequences; counters: 4096 of them, CTR_STRIDE ints apart, zero before and after.
+size_t attn_paged_scratch_bytes(int B, int T, int H, int HKV, int HD, int n_cu);
+hipError_t launch_attn_paged(const float *q, int B, int T, int H, int HKV, int HD, KvLayer kv, int kv_f16, int n_pages,
+                             int page, const int32_t *table, int n_table, const int32_t *n_keys, int window, float scale,
+                             void *scratch, int *counters, float *out, int n_cu, hipStream_t s);
+
+// verify.hip: T drafts of each of B sequences (T <= verify_max_drafts()) over rows of V <= verify_max_vocab() logits;
+// counters: B of them, CTR_STRIDE ints apart, zero before and after.
+int verify_max_vocab();
+int verify_max_drafts();
+size_t verify_scratch_bytes(int V, int B, int T);
+hipError_t launch_verify(const float *logits, int64_t ld, const float *draft, int64_t ld_draft, int V, int B, int T,
+                         const int32_t *drafts, const int32_t *n_draft, const float *temp, const float *uni, void *scratch,
+                         int *counters, int32_t *tokens, int32_t *n_tokens, float *logp, hipStream_t s);
+
 // sample.hip
 size_t argmax_scratch_bytes(int rows);
 // out[r] = argmax of row r; with seq (one row): seq[*pos + 1] = id, ++*pos.

@@ -97,6 +97,13 @@ _SIGS = {
     "ts5hip_kv_block_bounds": (_i32, [_vp, _i32, _i32, _i32, _i32, _vp, _vp, _i32, _vp, _i32, _i32, _vp]),
     "ts5hip_attn_sparse": (_i32, [_vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _vp, _i32, _vp, _i32,
                                   _i32, _f32, _vp, _vp]),
+    "ts5hip_rope_kv_append_paged": (_i32, [_vp, _vp, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _i32, _vp, _vp, _vp,
+                                           _f32, _vp, _i32, _vp, _vp, _vp, _vp, _i32, _i32, _vp, _i32, _i32]),
+    "ts5hip_kv_read_paged": (_i32, [_vp, _i32, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _i32, _vp, _i32, _i32,
+                                    _i32, _vp, _vp]),
+    "ts5hip_attn_paged": (_i32, [_vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _i32, _vp, _i32, _vp,
+                                 _i32, _f32, _vp]),
+    "ts5hip_verify_drafts": (_i32, [_vp, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "ts5hip_argmax": (_i32, [_vp, _vp, _i32, _i32, _vp]),
     "ts5hip_topk": (_i32, [_vp, _vp, _i32, _i32, _vp, _vp]),
     "ts5hip_sampler_new": (_vp, [_u64]),
@@ -407,6 +414,31 @@ class Context:
         self.check(lib().ts5hip_attn_sparse(self.h, _ptr(q), B, H, HKV, HD, kv, _ptr(k), _ptr(ks), _ptr(v), _ptr(vs),
                                             n_ctx, _ptr(n_keys_dev), int(kv_per_batch), _ptr(bounds), block, n_pick,
                                             scale, _ptr(out), _ptr(picked_dev)))
+
+    def rope_kv_append_paged(self, qkv, ntok, seq_dev, pos_dev, H, HKV, HD, n_rot, neox, rope_cs, n_pos, q_out, kv, k, ks, v,
+                             vs, n_pages, page, table_dev, n_seq, n_table, bias=None, q_norm=None, k_norm=None, eps=1e-6):
+        self.check(lib().ts5hip_rope_kv_append_paged(self.h, _ptr(qkv), ntok, _ptr(seq_dev), _ptr(pos_dev), H, HKV, HD,
+                                                     n_rot, int(neox), _ptr(rope_cs), n_pos, _ptr(bias), _ptr(q_norm),
+                                                     _ptr(k_norm), eps, _ptr(q_out), kv, _ptr(k), _ptr(ks), _ptr(v),
+                                                     _ptr(vs), n_pages, page, _ptr(table_dev), n_seq, n_table))
+
+    def kv_read_paged(self, ntok, seq_dev, pos_dev, HKV, HD, kv, k, ks, v, vs, n_pages, page, table_dev, n_seq, n_table,
+                      out_type, k_out, v_out):
+        self.check(lib().ts5hip_kv_read_paged(self.h, ntok, _ptr(seq_dev), _ptr(pos_dev), HKV, HD, kv, _ptr(k), _ptr(ks),
+                                              _ptr(v), _ptr(vs), n_pages, page, _ptr(table_dev), n_seq, n_table, out_type,
+                                              _ptr(k_out), _ptr(v_out)))
+
+    def attn_paged(self, q, B, n_new, H, HKV, HD, kv, k, ks, v, vs, n_pages, page, table_dev, n_table, n_keys_dev, window,
+                   scale, out):
+        self.check(lib().ts5hip_attn_paged(self.h, _ptr(q), B, n_new, H, HKV, HD, kv, _ptr(k), _ptr(ks), _ptr(v), _ptr(vs),
+                                           n_pages, page, _ptr(table_dev), n_table, _ptr(n_keys_dev), window, scale,
+                                           _ptr(out)))
+
+    def verify_drafts(self, logits, ld, draft_logits, ld_draft, n_vocab, B, n_draft, drafts_dev, n_draft_dev,
+                      temperature_dev, uniform_dev, tokens_dev, n_tokens_dev, logp_dev=None):
+        self.check(lib().ts5hip_verify_drafts(self.h, _ptr(logits), ld, _ptr(draft_logits), ld_draft, n_vocab, B, n_draft,
+                                              _ptr(drafts_dev), _ptr(n_draft_dev), _ptr(temperature_dev),
+                                              _ptr(uniform_dev), _ptr(tokens_dev), _ptr(n_tokens_dev), _ptr(logp_dev)))
 
     def argmax(self, x, n, rows, out):
         self.check(lib().ts5hip_argmax(self.h, _ptr(x), n, rows, _ptr(out)))
