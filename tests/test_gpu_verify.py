@@ -214,6 +214,21 @@ def test_temperatures(ctx):
 
 
 @pytest.mark.parametrize("model", [False, True])
+def test_numbers_outside_0_to_1(ctx, model):
+    """Numbers that are no probabilities draw some entry of the row all the same, one with a weight."""
+    rng = np.random.default_rng(71)
+    logits, draft, drafts, temp, uni = inputs(rng, 8, 2, 5000, model)
+    logits[:4] = np.where(np.arange(5000) == 4321, 3.0, -np.inf)
+    drafts[:4] = 4321
+    uni[:] = [[np.nan] * 3, [1, 1, 1], [2, -1, 5], [np.inf, 0.5, -np.inf]] * 2
+    tokens, n, logp = run(ctx, logits, draft, drafts, None, temp, uni)
+    assert np.all((n >= 1) & (n <= 3))
+    for b in range(8):
+        assert np.all((tokens[b, :n[b]] >= 0) & (tokens[b, :n[b]] < 5000)) and np.all(tokens[b, n[b]:] == -1)
+        assert b >= 4 or np.all(tokens[b, :n[b]] == 4321)
+
+
+@pytest.mark.parametrize("model", [False, True])
 def test_the_tokens_have_the_targets_distribution(ctx, model):
     """The first token of 3 x 4096 sequences with drafts from another distribution: its counts are within 5 standard
     deviations of the target's probabilities."""

@@ -6,9 +6,10 @@
 // All of it in fp64: a token is the first past a bound, and with fp32 weights about one draw in a thousand over 150000
 // entries would be another one. Two launches:
 //  k_verify_rows  the maximum of each slice of each row and the sum of its weights 2^((l - maximum) log2(e) / T);
-//  k_verify_pick  every workgroup of a sequence joins its rows' slices and judges the drafts (cheaper than a third
-//                 launch), sums one slice's weights of the row the token is drawn from, and the last one to finish finds
-//                 the slice and the entry.
+//  k_verify_pick  joins the rows' slices, judges the drafts, and finds the slice and then the entry that the token is. Where
+//                 that is drawn from p - q of two rows, a workgroup a slice judges (cheaper than a third launch) and sums
+//                 that slice's weights, and the last one to finish goes on; else one workgroup does it all, from
+//                 the sums there are (a draft's own entry is kept out of them, so that p without it is exact).
 #include <algorithm>
 #include <climits>
 
@@ -17,11 +18,11 @@
 
 namespace ts5hip {
 
-constexpr int VF_NT = 256, VF_SLICE = 4096, VF_PER = VF_SLICE / VF_NT;  // 16 entries a thread, 4 neighbours at a time
+constexpr int VF_SLICE = 4096, VF_NT = 256, VP_NT = 512;  // entries of a slice, threads of k_verify_rows, of k_verify_pick
 constexpr double VF_LOG2E = 1.4426950408889634;
 
 struct VerifyPart {
-    double sum;   // of the weights, over the slice's own maximum's
+    double sum;   // of the weights over the slice's own maximum's, less the row's draft
     float top;    // -inf: every entry is; NaN: no distribution (a NaN or plus infinity)
     int32_t best; // the first entry at the maximum
 };
@@ -41,37 +42,75 @@ struct VerifyArgs {
 __device__ inline int vf_drafts(const VerifyArgs &a, int b) { return a.n_draft ? max(0, min(a.n_draft[b], a.T)) : a.T; }
 __device__ inline bool vf_greedy(float t) { return !(t > 0.f); }
 
-// 2^x, x <= 0: x = k + f with |f| <= 1/2, the series of 2^f to its 13th term (under 2^-53), and k to the exponent.
+// 2^x, x <= 0 (minus infinity: 0): x = k + f with |f| <= 1/2, the polynomial of degree 10 that meets 2^f at the zeros of
+// the 11th Chebyshev polynomial (off by 3.2e-16 at most), and k to the exponent.
 __device__ inline double vf_exp2(double x) {
     x = fmax(x, -2000.0);  // (0; and where x is a product, a fused x - k would be its rounding error, of any size)
-    const double k = __builtin_rint(x), f = (x - k) * 0.6931471805599453;
-    double p = 1.0 / 6227020800.0;
-    p = fma(p, f, 1.0 / 479001600.0);
-    p = fma(p, f, 1.0 / 39916800.0);
-    p = fma(p, f, 1.0 / 3628800.0);
-    p = fma(p, f, 1.0 / 362880.0);
-    p = fma(p, f, 1.0 / 40320.0);
-    p = fma(p, f, 1.0 / 5040.0);
-    p = fma(p, f, 1.0 / 720.0);
-    p = fma(p, f, 1.0 / 120.0);
-    p = fma(p, f, 1.0 / 24.0);
-    p = fma(p, f, 1.0 / 6.0);
-    p = fma(p, f, 0.5);
-    p = fma(p, f, 1.0);
+    const double k = __builtin_rint(x), f = x - k;
+    double p = 7.072585949269223e-09;
+    p = fma(p, f, 1.0208690299958306e-07);
+    p = fma(p, f, 1.321544258792169e-06);
+    p = fma(p, f, 1.5252657260200837e-05);
+    p = fma(p, f, 0.0001540353044173605);
+    p = fma(p, f, 0.0013333558230164974);
+    p = fma(p, f, 0.009618129107606888);
+    p = fma(p, f, 0.05550410866444772);
+    p = fma(p, f, 0.24022650695910097);
+    p = fma(p, f, 0.69314718055995);
     p = fma(p, f, 1.0);
     return ldexp(p, (int)k);
 }
-// The weight of logit l where the maximum is m; by = log2(e) / T.
-__device__ inline double vf_weight(float l, float m, double by) {
-    return l == -INFINITY ? 0.0 : vf_exp2(((double)l - (double)m) * by);
+// The weight of logit l where the maximum is m (finite). by = log2(e) / T, above 0, so that minus infinity weighs 0.
+__device__ inline double vf_weight(float l, float m, double by) { return vf_exp2(((double)l - (double)m) * by); }
+__device__ inline double vf_by(float temp) { return fmax(VF_LOG2E / (double)temp, 1e-300); }
+
+// Lanes moved by DPP, a double as two halves; a lane without a source gets 0.
+template <int CTRL, int ROW_MASK, int BANK_MASK>
+__device__ inline double vf_dpp(double x) {
+    const uint64_t u = (uint64_t)__double_as_longlong(x);
+    const uint32_t l = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROW_MASK, BANK_MASK, true);
+    const uint32_t h = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROW_MASK, BANK_MASK, true);
+    return __longlong_as_double((long long)((uint64_t)h << 32 | l));
+}
+// The sum over each 16-lane row, in every lane of it.
+__device__ inline double vf_row_sum(double x) {
+    x += vf_dpp<0xB1, 0xF, 0xF>(x);   // quad_perm [1,0,3,2]
+    x += vf_dpp<0x4E, 0xF, 0xF>(x);   // quad_perm [2,3,0,1]
+    x += vf_dpp<0x141, 0xF, 0xF>(x);  // row_half_mirror
+    return x + vf_dpp<0x140, 0xF, 0xF>(x);  // row_mirror
+}
+// Inclusive sums over the wave's lanes.
+__device__ inline double vf_scan(double x) {
+    x += vf_dpp<0x111, 0xF, 0xF>(x);  // row_shr:1
+    x += vf_dpp<0x112, 0xF, 0xF>(x);  // row_shr:2
+    x += vf_dpp<0x114, 0xF, 0xE>(x);  // row_shr:4
+    x += vf_dpp<0x118, 0xF, 0xC>(x);  // row_shr:8
+    x += vf_dpp<0x142, 0xA, 0xF>(x);  // row_bcast:15 into rows 1 and 3
+    return x + vf_dpp<0x143, 0xC, 0xF>(x);  // row_bcast:31 into rows 2 and 3
+}
+__device__ inline double vf_lane(double x, int lane) {
+    const uint64_t u = (uint64_t)__double_as_longlong(x);
+    const uint32_t l = __builtin_amdgcn_readlane((int)(uint32_t)u, lane), h = __builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
+    return __longlong_as_double((long long)((uint64_t)h << 32 | l));
+}
+// The least over each 16-lane row, over the wave: in every lane.
+template <int CTRL, int ROW_MASK>
+__device__ inline int vf_dpp_min(int x) { return min(x, __builtin_amdgcn_update_dpp(x, x, CTRL, ROW_MASK, 0xF, false)); }
+__device__ inline int vf_row_min(int x) {
+    return vf_dpp_min<0x140, 0xF>(vf_dpp_min<0x141, 0xF>(vf_dpp_min<0x4E, 0xF>(vf_dpp_min<0xB1, 0xF>(x))));
+}
+__device__ inline int vf_wave_min(int x) {
+    x = vf_dpp_min<0x143, 0xC>(vf_dpp_min<0x142, 0xA>(vf_row_min(x)));
+    return __builtin_amdgcn_readlane(x, 63);
 }
 
 typedef float vf_f4 __attribute__((ext_vector_type(4), aligned(4)));  // rows begin anywhere
-// The thread's entries of a slice: x[4 j + i] is entry s0 + 4 (256 j + thread) + i; past the row: minus infinity.
-__device__ inline void vf_load(const float *row, int s0, int V, float (&x)[VF_PER]) {
+// A thread's entries of a slice, of NT threads: x[4 j + i] is entry s0 + 4 (NT j + thread) + i; past the row: minus infinity.
+template <int NT>
+__device__ inline void vf_load(const float *row, int s0, int V, float (&x)[VF_SLICE / NT]) {
 #pragma unroll
-    for (int j = 0; j < VF_PER / 4; j++) {
-        const int e = s0 + 4 * (VF_NT * j + (int)threadIdx.x);
+    for (int j = 0; j < VF_SLICE / NT / 4; j++) {
+        const int e = s0 + 4 * (NT * j + (int)threadIdx.x);
         if (e + 4 <= V) {
             const vf_f4 v = *(const vf_f4 *)(row + e);
 #pragma unroll
@@ -82,20 +121,25 @@ __device__ inline void vf_load(const float *row, int s0, int V, float (&x)[VF_PE
         }
     }
 }
-__device__ inline int vf_index(int s0, int k) { return s0 + 4 * (VF_NT * (k / 4) + (int)threadIdx.x) + k % 4; }
+template <int NT>
+__device__ inline int vf_index(int s0, int k) { return s0 + 4 * (NT * (k / 4) + (int)threadIdx.x) + k % 4; }
 
-// Sum over the workgroup, in thread 0.
-__device__ inline double vf_block_sum(double v, double *lds) {
+// Sum over the workgroup, in every thread.
+template <int NT>
+__device__ inline double vf_block_sum(double v, double (&lds)[NT / WAVE]) {
+    v = vf_scan(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 63) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    double s = 0.0;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, WAVE);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return lds[0] + lds[1] + lds[2] + lds[3];
+    for (int w = 0; w < NT / WAVE; w++) s += lds[w];
+    return s;
 }
 
 // grid (slices, 2 T + 1 or T + 1 rows, B)
 __global__ __launch_bounds__(VF_NT) void k_verify_rows(VerifyArgs a) {
+    constexpr int PER = VF_SLICE / VF_NT;
     __shared__ double sums[4];
     __shared__ float tops[4];
     __shared__ int bests[4];
@@ -106,13 +150,15 @@ __global__ __launch_bounds__(VF_NT) void k_verify_rows(VerifyArgs a) {
     if (target ? r > nd : r - a.T - 1 >= nd || vf_greedy(temp)) return;  // not one of the sequence's rows
     const float *row = target ? a.logits + ((int64_t)b * (a.T + 1) + r) * a.ld
                               : a.draft + ((int64_t)b * a.T + r - a.T - 1) * a.ld_draft;
-    float x[VF_PER];
-    vf_load(row, s0, a.V, x);
+    float x[PER];
+    vf_load<VF_NT>(row, s0, a.V, x);
+    const int d = r < nd ? a.drafts[(int64_t)b * a.T + r] : -1;
     if (threadIdx.x == 0) bad = 0;
     float top = -INFINITY;
     bool no = false;
 #pragma unroll
-    for (int k = 0; k < VF_PER; k++) top = fmaxf(top, x[k]), no |= !(x[k] < INFINITY);
+    for (int k = 0; k < PER; k++) top = fmaxf(top, x[k]), no |= x[k] != x[k];
+    no |= top == INFINITY;
     top = wave_max_dpp(top);
     if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
     __syncthreads();
@@ -120,18 +166,23 @@ __global__ __launch_bounds__(VF_NT) void k_verify_rows(VerifyArgs a) {
     if (no) bad = 1;
     int best = INT_MAX;
 #pragma unroll
-    for (int k = VF_PER - 1; k >= 0; k--)
-        if (x[k] == top) best = min(best, vf_index(s0, k));
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) best = min(best, __shfl_xor(best, o, WAVE));
+    for (int k = PER - 1; k >= 0; k--) best = x[k] == top ? vf_index<VF_NT>(s0, k) : best;  // (ascending with k)
+    best = vf_wave_min(best);
     if ((threadIdx.x & 63) == 0) bests[threadIdx.x >> 6] = best;
     double sum = 0.0;
     if (!vf_greedy(temp) && top != -INFINITY) {
-        const double by = VF_LOG2E / (double)temp;
+        const double by = vf_by(temp);
+        double w[PER];
 #pragma unroll
-        for (int k = 0; k < VF_PER; k++) sum += vf_weight(x[k], top, by);
+        for (int k = 0; k < PER; k++) w[k] = vf_weight(x[k], top, by);
+        if ((uint32_t)(d - s0) < (uint32_t)VF_SLICE) {
+#pragma unroll
+            for (int k = 0; k < PER; k++) w[k] = vf_index<VF_NT>(s0, k) == d ? 0.0 : w[k];
+        }
+#pragma unroll
+        for (int k = 0; k < PER; k++) sum += w[k];
     }
-    sum = vf_block_sum(sum, sums);
+    sum = vf_block_sum<VF_NT>(sum, sums);
     if (threadIdx.x == 0) {
         VerifyPart p;
         p.sum = sum, p.top = bad ? NAN : top, p.best = min(min(bests[0], bests[1]), min(bests[2], bests[3]));
@@ -139,58 +190,67 @@ __global__ __launch_bounds__(VF_NT) void k_verify_rows(VerifyArgs a) {
     }
 }
 
-// A row's slices as one, by a wave: in every lane.
+// A row's slices as one, by 16 lanes: in every one of them.
 __device__ inline VerifyPart vf_join(const VerifyPart *p, int ns, double by) {
-    const int lane = threadIdx.x & 63;
-    VerifyPart s;
-    s.top = -INFINITY, s.sum = 0.0, s.best = INT_MAX;
-    bool no = false;
-    for (int i = lane; i < ns; i += WAVE) {  // (ascending: the first of equal maxima stays)
-        const VerifyPart x = p[i];
-        no |= x.top != x.top;
-        if (x.top > s.top) {
-            s.sum = x.sum + (s.top == -INFINITY ? 0.0 : s.sum * vf_exp2(((double)s.top - (double)x.top) * by));
-            s.top = x.top, s.best = x.best;
-        } else if (x.top > -INFINITY) {
-            s.sum += x.sum * vf_exp2(((double)x.top - (double)s.top) * by);
+    constexpr int AHEAD = 4;
+    const int lane = threadIdx.x & 15;
+    float top = -INFINITY;
+    double sum = 0.0;
+    int best = INT_MAX, no = 0;
+    for (int i0 = lane; i0 < ns; i0 += 16 * AHEAD) {  // (ascending: the first of equal maxima stays)
+        VerifyPart x[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; k++) x[k] = p[min(i0 + 16 * k, ns - 1)];
+#pragma unroll
+        for (int k = 0; k < AHEAD; k++) {
+            if (i0 + 16 * k >= ns) break;
+            no |= x[k].top != x[k].top;
+            if (x[k].top > top) {
+                sum = x[k].sum + (top == -INFINITY ? 0.0 : sum * vf_weight(top, x[k].top, by));
+                top = x[k].top, best = x[k].best;
+            } else if (x[k].top > -INFINITY) {
+                sum += x[k].sum * vf_weight(x[k].top, top, by);
+            }
         }
     }
-    const float top = wave_max_dpp(s.top);
-    s.sum = s.top == -INFINITY ? 0.0 : s.sum * vf_exp2(((double)s.top - (double)top) * by);
-    if (s.top != top) s.best = INT_MAX;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        s.sum += __shfl_xor(s.sum, o, WAVE);
-        s.best = min(s.best, __shfl_xor(s.best, o, WAVE));
-    }
-    s.top = __builtin_amdgcn_ballot_w64(no) ? NAN : top;
+    VerifyPart s;
+    s.top = row_max_dpp(top);
+    sum = top == -INFINITY ? 0.0 : sum * vf_weight(top, s.top, by);
+    s.sum = vf_row_sum(sum), s.best = vf_row_min(top == s.top ? best : INT_MAX);
+    if (vf_row_min(-no)) s.top = NAN;
     return s;
 }
 __device__ inline bool vf_has(const VerifyPart &p) { return p.top > -INFINITY; }  // (not NaN: a distribution)
 
-// grid (slices, B)
+// grid (slices with a draft model, else 1, B). Its time is a chain: the counts and drafts, the drafts' logits and the slices'
+// sums, the slice, its weights.
 constexpr int VF_MAX_DRAFTS = 63, VF_MAX_SLICES = 256;
-__global__ __launch_bounds__(VF_NT) void k_verify_pick(VerifyArgs a) {
+__global__ __launch_bounds__(VP_NT) void k_verify_pick(VerifyArgs a) {
     __shared__ VerifyPart rows[2 * VF_MAX_DRAFTS + 1];
-    __shared__ double lds[4];
-    __shared__ int kept;
-    const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, nd = vf_drafts(a, b);
+    __shared__ double lds[VP_NT / WAVE];
+    __shared__ int drafts[VF_MAX_DRAFTS + 1], kept;
+    __shared__ float draft_l[VF_MAX_DRAFTS + 1];  // their logits
+    constexpr int PER = VF_SLICE / VP_NT, NW = VP_NT / WAVE;
+    const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const float temp = a.temp[b];
+    const int nd = vf_drafts(a, b);
+    const float u_draw = a.uni[(int64_t)b * (a.T + 1) + a.T];
     const bool greedy = vf_greedy(temp), model = a.draft && !greedy;
-    const double by = greedy ? 0.0 : VF_LOG2E / (double)temp;
-    // Thread t < nd: draft t and its logits.
-    const int32_t d = tid < nd ? a.drafts[(int64_t)b * a.T + tid] : -1;
-    const bool inside = (uint32_t)d < (uint32_t)a.V;
+    const double by = greedy ? 1.0 : vf_by(temp);
     const float *target = a.logits + (int64_t)b * (a.T + 1) * a.ld, *draft = a.draft + (int64_t)b * a.T * a.ld_draft;
-    const float lp = inside ? target[tid * a.ld + d] : -INFINITY, lq = inside && model ? draft[tid * a.ld_draft + d] : 0.f;
-    const float r = tid < nd ? a.uni[(int64_t)b * (a.T + 1) + tid] : 0.f;
+    // Thread t < nd: draft t, its number and its logits.
+    const int32_t d = tid < a.T ? a.drafts[(int64_t)b * a.T + tid] : -1;
+    const float r = a.uni[(int64_t)b * (a.T + 1) + min(tid, a.T)];
+    const bool inside = (uint32_t)d < (uint32_t)a.V;
+    const float lp = inside ? target[tid * a.ld + d] : -INFINITY, lq = inside && a.draft ? draft[tid * a.ld_draft + d] : -INFINITY;
+    if (tid < nd) drafts[tid] = d, draft_l[tid] = lp;
     const VerifyPart *parts = a.parts + (int64_t)b * (2 * a.T + 1) * a.ns;
-    for (int i = wave; i < nd + 1 + (model ? nd : 0); i += VF_NT / WAVE) {
+    for (int i = tid / 16; i < nd + 1 + (model ? nd : 0); i += VP_NT / 16) {
         const VerifyPart p = vf_join(parts + (int64_t)(i <= nd ? i : a.T + i - nd) * a.ns, a.ns, by);
-        if (lane == 0) rows[i] = p;
+        if (tid % 16 == 0) rows[i] = p;
     }
     __syncthreads();
-    float logp = 0.f;
+    double wp = 0.0, sp = 1.0;  // the draft's weight and its row's sum
     if (wave == 0) {
         bool ok = false;
         if (tid < nd && vf_has(rows[tid])) {
@@ -198,11 +258,13 @@ __global__ __launch_bounds__(VF_NT) void k_verify_pick(VerifyArgs a) {
             if (greedy) {
                 ok = d == p.best;
             } else if (inside) {
-                const double w = vf_weight(lp, p.top, by) / p.sum;
-                const VerifyPart &q = rows[nd + 1 + (model ? tid : 0)];
-                const double wq = !model ? 1.0 : vf_has(q) ? vf_weight(lq, q.top, by) / q.sum : NAN;
-                ok = (double)r * wq < w;
-                logp = (float)(((double)lp - (double)p.top) / (double)temp - log(p.sum));
+                wp = vf_weight(lp, p.top, by), sp = p.sum + wp;
+                double q = 1.0;
+                if (model) {
+                    const VerifyPart &y = rows[nd + 1 + tid];
+                    q = vf_has(y) ? vf_weight(lq, y.top, by) / y.sum : NAN;
+                }
+                ok = (double)r * q < wp / sp;
             }
         }
         const uint64_t no = __builtin_amdgcn_ballot_w64(!ok);
@@ -215,7 +277,7 @@ __global__ __launch_bounds__(VF_NT) void k_verify_pick(VerifyArgs a) {
     if (blockIdx.x == 0) {  // the kept ones, and nothing behind the next
         if (tid < m) {
             tokens[tid] = d;
-            if (logps) logps[tid] = logp;
+            if (logps) logps[tid] = greedy ? 0.f : (float)(((double)lp - (double)rows[tid].top) / (double)temp - log(sp));
         }
         if (tid > m && tid <= a.T) {
             tokens[tid] = -1;
@@ -231,127 +293,121 @@ __global__ __launch_bounds__(VF_NT) void k_verify_pick(VerifyArgs a) {
         }
         return;
     }
-    // The token's weights: p, less q where the draft was not kept.
-    const float *row = target + (int64_t)m * a.ld, *qrow = model && m < nd ? draft + (int64_t)m * a.ld_draft : nullptr;
+    // The token's weights: p of row m, less q where that row's draft was not kept.
+    const int dm = m < nd ? drafts[m] : -1;
     const VerifyPart q = rows[model && m < nd ? nd + 1 + m : 0];
-    const bool by_q = qrow && vf_has(q);
-    const int certain = !model && m < nd ? a.drafts[(int64_t)b * a.T + m] : -1;
-    const double inv_p = 1.0 / p.sum, inv_q = by_q ? 1.0 / q.sum : 0.0;
-    double w[VF_PER];
-    auto weights = [&](int s0, bool plain) {
-        float x[VF_PER];
-        vf_load(row, s0, a.V, x);
+    const bool by_q = model && m < nd && vf_has(q);
+    if (!by_q && blockIdx.x > 0) return;
+    const float *row = target + (int64_t)m * a.ld, *qrow = draft + (int64_t)m * a.ld_draft;
+    const float lm = m < nd ? draft_l[m] : -INFINITY;
+    const double wm = vf_weight(lm, p.top, by), sum_p = p.sum + wm, inv_p = 1.0 / sum_p;
+    int certain = !model ? dm : -1;  // (its entry is not drawn)
+    double w[PER];
+    auto weights = [&](int s0, bool less) {
+        float x[PER];
+        vf_load<VP_NT>(row, s0, a.V, x);
+        if (less) {
+            float y[PER];
+            vf_load<VP_NT>(qrow, s0, a.V, y);
+            const double inv_q = 1.0 / q.sum;
 #pragma unroll
-        for (int k = 0; k < VF_PER; k++) w[k] = vf_weight(x[k], p.top, by) * inv_p;
-        if (plain) return;
-        if (by_q) {
-            vf_load(qrow, s0, a.V, x);
+            for (int k = 0; k < PER; k++)
+                w[k] = fmax(vf_weight(x[k], p.top, by) * inv_p - vf_weight(y[k], q.top, by) * inv_q, 0.0);
+        } else {
 #pragma unroll
-            for (int k = 0; k < VF_PER; k++) w[k] = fmax(w[k] - vf_weight(x[k], q.top, by) * inv_q, 0.0);
+            for (int k = 0; k < PER; k++) {
+                w[k] = vf_weight(x[k], p.top, by);
+                w[k] = vf_index<VP_NT>(s0, k) == certain ? 0.0 : w[k];
+            }
         }
-#pragma unroll
-        for (int k = 0; k < VF_PER; k++)
-            if (vf_index(s0, k) == certain) w[k] = 0.0;
     };
-    auto sum_of = [&]() {
+    double mine = 0.0;  // thread i: the weights of slice i
+    if (by_q) {
+        weights(blockIdx.x * VF_SLICE, true);
         double s = 0.0;
 #pragma unroll
-        for (int k = 0; k < VF_PER; k++) s += w[k];
-        return vf_block_sum(s, lds);
+        for (int k = 0; k < PER; k++) s += w[k];
+        s = vf_block_sum<VP_NT>(s, lds);
+        double *sums = a.sums + (int64_t)b * a.sums_stride;
+        __shared__ int last;
+        if (tid == 0) {
+            __hip_atomic_store(sums + blockIdx.x, s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            wait_stores();
+            int *c = a.counters + b * CTR_STRIDE;
+            last = atomicAdd(c, 1) == a.ns - 1;
+            if (last) st_dev(c, 0);
+        }
+        __syncthreads();
+        if (!last) return;
+        if (tid < a.ns) mine = __hip_atomic_load(sums + tid, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    const bool less = by_q && vf_block_sum<VP_NT>(mine, lds) > 0.0;  // (else p and q are equal up to rounding)
+    if (!less) {
+        mine = 0.0;
+        if (tid < a.ns) {
+            const VerifyPart x = parts[(int64_t)m * a.ns + tid];
+            if (x.top > -INFINITY) mine = x.sum * vf_weight(x.top, p.top, by);
+        }
+        // The draft's own entry: not drawn where it was certain, unless there is no other (a number that is not below 1).
+        if (!model && !(vf_block_sum<VP_NT>(mine, lds) > 0.0)) certain = -1;
+        if (certain < 0 && (uint32_t)dm < (uint32_t)a.V && dm / VF_SLICE == tid) mine += wm;
+    }
+    // The slice: the first whose cumulative sum passes u of all; roundings may leave none: the last with a weight.
+    __shared__ double before;
+    __shared__ int firsts[NW], lasts[NW];
+    double incl = vf_scan(mine);
+    __syncthreads();
+    if (lane == 63) lds[wave] = incl;
+    __syncthreads();
+    double base = 0.0, all = 0.0;
+#pragma unroll
+    for (int v = 0; v < NW; v++) base += v < wave ? lds[v] : 0.0, all += lds[v];
+    incl += base;
+    const double bound = (double)u_draw * all;
+    auto pick = [&](int first, int last) {  // the least `first` there is, or the largest `last`
+        first = vf_wave_min(first), last = -vf_wave_min(-last);
+        if (lane == 0) firsts[wave] = first, lasts[wave] = last;
+        __syncthreads();
+        int f = INT_MAX, l = 0;
+#pragma unroll
+        for (int v = 0; v < NW; v++) f = min(f, firsts[v]), l = max(l, lasts[v]);
+        return f != INT_MAX ? f : l;
     };
-    weights(blockIdx.x * VF_SLICE, false);
-    const double mine = sum_of();
-    double *sums = a.sums + (int64_t)b * a.sums_stride;
-    __shared__ int last;
-    if (tid == 0) {
-        __hip_atomic_store(sums + blockIdx.x, mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        wait_stores();
-        int *c = a.counters + b * CTR_STRIDE;
-        last = atomicAdd(c, 1) == a.ns - 1;
-        if (last) st_dev(c, 0);
+    const int slice = pick(mine > 0.0 && incl > bound ? tid : INT_MAX, mine > 0.0 ? tid : 0), s0 = slice * VF_SLICE;
+    if (tid == slice) before = incl - mine;
+    weights(s0, less);
+    // Cumulative weights in the entries' order: groups j of 4 VP_NT, waves, lanes, four neighbours.
+    __shared__ double tot[PER / 4][NW];
+    double run[PER / 4];
+#pragma unroll
+    for (int j = 0; j < PER / 4; j++) {
+        run[j] = vf_scan((w[4 * j] + w[4 * j + 1]) + (w[4 * j + 2] + w[4 * j + 3]));
+        if (lane == 63) tot[j][wave] = run[j];
     }
     __syncthreads();
-    if (!last) return;
-    // The slice: the first whose cumulative sum passes u of all.
-    __shared__ double slice[VF_MAX_SLICES];
-    __shared__ double bound, before;
-    __shared__ int chosen, entry, plain;
-    if (tid < a.ns) slice[tid] = __hip_atomic_load(sums + tid, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __syncthreads();
-    if (tid == 0) {
-        double all = 0.0;
-        for (int i = 0; i < a.ns; i++) all += slice[i];
-        plain = !(all > 0.0);  // (p and q equal up to rounding: the draft's row says nothing)
-        if (plain) {
-            all = 0.0;
-            for (int i = 0; i < a.ns; i++) {
-                const VerifyPart x = parts[(int64_t)m * a.ns + i];
-                slice[i] = x.top == -INFINITY ? 0.0 : x.sum * vf_exp2(((double)x.top - (double)p.top) * by) * inv_p;
-                all += slice[i];
-            }
-        }
-        const double u = (double)a.uni[(int64_t)b * (a.T + 1) + a.T] * all;
-        double run = 0.0;
-        int at = -1;
-        for (int i = 0; i < a.ns; i++) {
-            if (slice[i] > 0.0) at = i, before = run;
-            run += slice[i];
-            if (run > u) break;
-        }
-        chosen = at, bound = u, entry = INT_MAX;
-    }
-    __syncthreads();
-    const int s0 = chosen * VF_SLICE;
-    weights(s0, plain);
-    // Cumulative weights in the entries' order: groups j of 1024, waves, lanes, four neighbours.
-    __shared__ double tot[VF_PER / 4][VF_NT / WAVE];
-    double incl[VF_PER / 4];
+    base = before;
+    int found = INT_MAX, positive = 0;
 #pragma unroll
-    for (int j = 0; j < VF_PER / 4; j++) {
-        double s = (w[4 * j] + w[4 * j + 1]) + (w[4 * j + 2] + w[4 * j + 3]);
+    for (int j = 0; j < PER / 4; j++) {
+        double c = base;
 #pragma unroll
-        for (int o = 1; o < WAVE; o <<= 1) {
-            const double y = __shfl_up(s, o, WAVE);
-            if (lane >= o) s += y;
-        }
-        incl[j] = s;
-        if (lane == 63) tot[j][wave] = s;
-    }
-    __syncthreads();
-    const double u = bound;
-    double base = before;
-    int found = INT_MAX, positive = -1;
-#pragma unroll
-    for (int j = 0; j < VF_PER / 4; j++) {
-#pragma unroll
-        for (int v = 0; v < VF_NT / WAVE; v++) {
-            if (v == wave) {
-                const double prev = __shfl_up(incl[j], 1, WAVE);
-                double c = base + (lane ? prev : 0.0);
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    c += w[4 * j + i];
-                    const int e = vf_index(s0, 4 * j + i);
-                    if (w[4 * j + i] > 0.0) {
-                        positive = e;
-                        if (c > u) found = min(found, e);
-                    }
-                }
-            }
+        for (int v = 0; v < NW; v++) {
+            c += v < wave ? tot[j][v] : 0.0;
             base += tot[j][v];
         }
+        c += vf_dpp<0x138, 0xF, 0xF>(run[j]);  // wave_shr:1
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            c += w[4 * j + i];
+            const int e = vf_index<VP_NT>(s0, 4 * j + i);
+            positive = w[4 * j + i] > 0.0 ? e : positive;
+            found = w[4 * j + i] > 0.0 && c > bound ? min(found, e) : found;
+        }
     }
-    // Roundings may leave no entry past the bound: then the slice's last with a weight.
-    __shared__ int backup;
-    if (tid == 0) backup = -1;
-    __syncthreads();
-    if (found != INT_MAX) atomicMin(&entry, found);
-    if (positive >= 0) atomicMax(&backup, positive);
-    __syncthreads();
+    const int e = pick(found, positive);
     if (tid == 0) {
-        const int e = entry != INT_MAX ? entry : backup;
         tokens[m] = e, a.n_tokens[b] = m + 1;
-        if (logps) logps[m] = (float)(((double)row[e] - (double)p.top) / (double)temp - log(p.sum));
+        if (logps) logps[m] = (float)(((double)row[e] - (double)p.top) / (double)temp - log(sum_p));
     }
 }
 
@@ -383,7 +439,7 @@ hipError_t launch_verify(const float *logits, int64_t ld, const float *draft, in
     a.parts = (VerifyPart *)scratch, a.sums = (double *)((uint8_t *)scratch + p.parts), a.sums_stride = p.stride;
     a.counters = counters, a.tokens = tokens, a.n_tokens = n_tokens, a.logp = logp;
     hipLaunchKernelGGL(k_verify_rows, dim3(p.ns, T + 1 + (draft ? T : 0), B), dim3(VF_NT), 0, s, a);
-    hipLaunchKernelGGL(k_verify_pick, dim3(p.ns, B), dim3(VF_NT), 0, s, a);
+    hipLaunchKernelGGL(k_verify_pick, dim3(draft ? p.ns : 1, B), dim3(VP_NT), 0, s, a);
     return hipGetLastError();
 }
 
