@@ -16,14 +16,14 @@ struct PagedArgs {
     KvLayer kv;            // [n_pages][HKV][page][HD]
     const int32_t *table;  // [B][n_table]
     int n_table, n_pages, lp;  // lp: log2 of the page
-    int B, T, H, HKV, G, R, RT, window;  // R = T G rows a KV head in tiles of RT (16, or fewer in all)
+    int B, T, H, HKV, G, R, RT, window;  // R = T G rows a KV head, in blocks of RT
     int cap;                // slices of all sequences, at most
     uint64_t g_m, hkv_m;    // rows_magic of G, HKV
     const int32_t *n_keys;  // [B]
     float scale;
-    float *part;   // [HKV][row tile][cap][RT][HD + 4]: m, l, -, -, O
+    float *part;   // [HKV][row block][cap][RT][HD + 4]: m, l, -, -, O
     int2 *plan;    // [B] each sequence's first slice and how many it has
-    int *counters; // [B * HKV * row tiles], CTR_STRIDE ints apart, zero between launches
+    int *counters; // [B * HKV * row blocks], CTR_STRIDE ints apart, zero between launches
     float *out;    // [B][T][H * HD]
 };
 
@@ -94,20 +94,27 @@ __device__ inline PagedSlice paged_slice(const PagedArgs &a, int j) {
     return s;
 }
 
-// A tile's 16 keys from `key` on, those below `end`, as bounded buffers: what is past them reads zeros. No page: all of it.
+// Where the wave finds a tile of 16 keys: those from `key` on and below `end`, as bounded buffers (what is past them reads
+// zeros); no page: all of it.
 template <int HD, bool F16>
 __device__ inline RowsKv paged_tile(const PagedArgs &a, int kvh, int page, int key, int end) {
     const bool ok = (uint32_t)page < (uint32_t)a.n_pages;
-    const int n = ok ? max(0, min(end - key, 16)) : 0;
+    // (readfirstlane: the compiler takes min and max as one vector instruction, and then each load as a loop over lanes that
+    // might have buffers of their own)
+    const int n = ok ? __builtin_amdgcn_readfirstlane(max(0, min(end - key, 16))) : 0;
     const int64_t slot = (((int64_t)(ok ? page : 0) * a.HKV + kvh) << a.lp) + (key & ((1 << a.lp) - 1));
     return rows_kv<HD, F16>(a.kv, slot, n);
 }
 template <int HD, bool F16, int KT>
-__device__ inline void paged_load(RowsUnit<HD, F16, KT> &u, int t, const RowsKv &kv, int rl, int kq) {
+__device__ inline void paged_load_k(RowsUnit<HD, F16, KT> &u, int t, const RowsKv &kv, int rl, int kq) {
     using S = RowsShape<HD, F16, KT>;
 #pragma unroll
     for (int c = 0; c < S::NC; c++) rows_words<S::KW>(kv.k, ((uint32_t)rl * HD + 32 * c + 8 * kq) * S::VB, u.k[t][c]);
     if constexpr (!F16) rows_words<2 * S::NC>(kv.ks, (uint32_t)(4 * kq) * S::NC * 2, u.ks[t]);
+}
+template <int HD, bool F16, int KT>
+__device__ inline void paged_load_v(RowsUnit<HD, F16, KT> &u, int t, const RowsKv &kv, int rl, int kq) {
+    using S = RowsShape<HD, F16, KT>;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const uint32_t key = (uint32_t)(4 * kq + i);
@@ -147,6 +154,98 @@ __device__ inline bool paged_clean(RowsUnit<HD, F16, KT> &u) {
     return __builtin_amdgcn_ballot_w64(any != 0) != 0;
 }
 
+// One unit into the sums of NT row tiles, its keys and values converted once. Without `whole`, seen(qt, key) has a bit for each of
+// keys key .. + 3 that the lane's row of tile qt takes. keys_done() comes where the unit's keys are used up.
+template <int HD, bool F16, int KT, int NT, class Seen, class Done>
+__device__ inline void paged_unit(const RowsUnit<HD, F16, KT> &u, const RowsQ<HD, NT> &q, RowsSum<HD, NT> &a,
+                                  const int (&kb)[KT], int kq, bool whole, Seen seen, Done keys_done) {
+    using S = RowsShape<HD, F16, KT>;
+    using Op = RowsOp<KT>;
+    float s[NT][KT][4];
+#pragma unroll
+    for (int t = 0; t < KT; t++) {
+        ar_f4 R[NT];
+#pragma unroll
+        for (int c = 0; c < S::NC; c++) {
+            const ar_h8 ka = rows_values<S::KW>(u.k[t][c]);
+            float ks[4];
+            if constexpr (!F16)
+#pragma unroll
+                for (int i = 0; i < 4; i++) ks[i] = h2f((u.ks[t][(i * S::NC + c) / 2] >> (16 * (c & 1))) & 0xffff);
+#pragma unroll
+            for (int qt = 0; qt < NT; qt++) {
+                if (!F16 || c == 0) R[qt] = ar_f4{0.f, 0.f, 0.f, 0.f};
+                R[qt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q.h[qt][c], R[qt], 0, 0, 0);
+            }
+#pragma unroll
+            for (int qt = 0; qt < NT; qt++) R[qt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q.l[qt][c], R[qt], 0, 0, 0);
+            if constexpr (!F16)
+#pragma unroll
+                for (int qt = 0; qt < NT; qt++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) s[qt][t][i] = c == 0 ? ks[i] * R[qt][i] : fmaf(ks[i], R[qt][i], s[qt][t][i]);
+        }
+        if constexpr (F16)
+#pragma unroll
+            for (int qt = 0; qt < NT; qt++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) s[qt][t][i] = R[qt][i];
+    }
+    keys_done();
+    typename Op::T ph[NT], pl[NT];
+#pragma unroll
+    for (int qt = 0; qt < NT; qt++) {
+        if (!whole) {
+#pragma unroll
+            for (int t = 0; t < KT; t++) {
+                const uint32_t take = seen(qt, kb[t] + 4 * kq);
+#pragma unroll
+                for (int i = 0; i < 4; i++) s[qt][t][i] = take & 1u << i ? s[qt][t][i] : -INFINITY;
+            }
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < KT; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) mx = fmaxf(mx, s[qt][t][i]);
+        const float m0 = rows_reference(a, qt, max_xor32(max_xor16(mx)) * q.p2e[qt]);
+        float sum = 0.f;
+        uint32_t hi[2 * KT], lo[2 * KT];
+#pragma unroll
+        for (int t = 0; t < KT; t++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const float p0 = __builtin_amdgcn_exp2f(fmaf(s[qt][t][2 * i], q.p2e[qt], -m0));
+                const float p1 = __builtin_amdgcn_exp2f(fmaf(s[qt][t][2 * i + 1], q.p2e[qt], -m0));
+                sum += p0 + p1;
+                rows_split(p0, p1, hi[2 * t + i], lo[2 * t + i]);
+            }
+        a.l[qt] += sum;  // (the lane's share: its four keys of each tile)
+        ph[qt] = Op::of(hi), pl[qt] = Op::of(lo);
+    }
+    RowsScale<HD, F16, KT> sc;
+    if constexpr (!F16) {
+#pragma unroll
+        for (int t = 0; t < KT; t++)
+#pragma unroll
+            for (int p = 0; p < 2; p++)
+                sc.s[t][p] = __builtin_bit_cast(ar_h2, (uint32_t)u.vs[t][2 * p] | (uint32_t)u.vs[t][2 * p + 1] << 16);
+    }
+#pragma unroll
+    for (int dt = 0; dt < S::NDT; dt++) {
+        uint32_t hi[2 * KT], lo[2 * KT];
+        rows_value_tile<HD, F16, KT>(u, sc, dt, hi, lo);
+        const typename Op::T vh = Op::of(hi), vl = Op::of(lo);
+#pragma unroll
+        for (int qt = 0; qt < NT; qt++) a.o[qt][dt] = Op::mfma(vh, ph[qt], a.o[qt][dt]);
+        if constexpr (!F16)
+#pragma unroll
+            for (int qt = 0; qt < NT; qt++) a.o[qt][dt] = Op::mfma(vl, ph[qt], a.o[qt][dt]);
+#pragma unroll
+        for (int qt = 0; qt < NT; qt++) a.o[qt][dt] = Op::mfma(vh, pl[qt], a.o[qt][dt]);
+    }
+}
+
 // A row's output.
 template <int HD>
 __device__ inline float *paged_out(const PagedArgs &a, int b, int kvh, int r) {
@@ -154,88 +253,134 @@ __device__ inline float *paged_out(const PagedArgs &a, int b, int kvh, int r) {
     return a.out + (((int64_t)b * a.T + t) * a.H + kvh * a.G + r - t * a.G) * HD;
 }
 
-// grid (cap * HKV, row tiles): one slice of one sequence's keys for up to 16 rows of a KV head; the waves take its units
-// in turn, each one's next requested before this one is used. With FUSED the last of a sequence's slices joins them.
-template <int HD, bool F16, int KT, int NW, int LEAST, bool FUSED>
-__global__ __launch_bounds__(64 * NW, HD <= 128 ? 2 : 1) void k_attn_paged(PagedArgs a) {
-    using S = RowsShape<HD, F16, KT>;
-    __shared__ RowsLds<HD, NW> L;
+// What a kernel is made for: NT row tiles a wave, NS units in its registers (one used, the others on their way; with one,
+// the next one's keys are requested once its keys are used and its values once all is), EDGE: rows that do not take the
+// same keys (several tokens, a window).
+template <int HD_, bool F16_, int NT_, int NS_, bool EDGE_>
+struct PagedForm {
+    static constexpr int HD = HD_, NT = NT_, NS = NS_, KT = HD == 64 ? 2 : 1, NW = 4, UNIT = 16 * KT, LEAST = 8 / KT;
+    static constexpr bool F16 = F16_, EDGE = EDGE_;
+};
+
+// grid (cap * HKV, row blocks): one slice of one sequence's keys for up to 16 NT rows of a KV head; the waves take its units
+// in turn. With FUSED the last of a sequence's slices joins them.
+template <class P, bool FUSED>
+__global__ __launch_bounds__(64 * P::NW, P::HD <= 128 ? 2 : 1) void k_attn_paged(PagedArgs a) {
+    constexpr int HD = P::HD, NT = P::NT, NS = P::NS, KT = P::KT, NW = P::NW, UNIT = P::UNIT;
+    constexpr bool F16 = P::F16, EDGE = P::EDGE;
+    __shared__ union {
+        RowsLds<HD, NW> parts;
+        RowsJoin join;
+    } L;
     __shared__ int nonfinite;  // a unit that not every row takes whole had infinite or NaN values: they are added at the end
-    if (threadIdx.x == 0) nonfinite = 0;
+    if (EDGE && threadIdx.x == 0) nonfinite = 0;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int rl = lane & 15, kq = lane >> 4;
     const int j = rows_div(blockIdx.x, a.hkv_m), kvh = (int)blockIdx.x - j * a.HKV;
-    const PagedSlice sl = paged_slice<S::UNIT, NW, LEAST>(a, j);
+    const PagedSlice sl = paged_slice<UNIT, NW, P::LEAST>(a, j);
     if (sl.b < 0) return;
-    const int b = sl.b, r0 = blockIdx.y * 16, rows = min(a.R - r0, 16);
-    RowsIn<HD, 1> in;
-    rows_request<HD, 1>(in, kq, [&](int, bool &ok) {
-        const int r = r0 + min(rl, rows - 1), t = rows_div(r, a.g_m);
-        ok = rl < rows;
+    const int b = sl.b, r0 = blockIdx.y * a.RT, rows = min(a.R - r0, a.RT);
+    RowsIn<HD, NT> in;
+    rows_request<HD, NT>(in, kq, [&](int qt, bool &ok) {
+        const int r = r0 + min(16 * qt + rl, rows - 1), t = rows_div(r, a.g_m);
+        ok = 16 * qt + rl < rows;
         return a.q + (((int64_t)b * a.T + t) * a.H + kvh * a.G + r - t * a.G) * HD;
     });
     const PagedSpan sp = paged_span(a, a.n_keys[b]);
-    const int units = paged_units(sp, S::UNIT), u0 = sl.at * sl.per, u1 = min(units, u0 + sl.per);
+    const int units = paged_units(sp, UNIT), u0 = sl.at * sl.per, u1 = min(units, u0 + sl.per);
     if (!FUSED && kvh == 0 && blockIdx.y == 0 && sl.at == 0 && threadIdx.x == 0) a.plan[b] = make_int2(j, sl.used);
 
-    // Pages of the wave's next 64 units, one a lane.
+    // The wave's i-th unit: u0 + wave + i NW. Its pages are looked up one request before they are needed.
     const int32_t *table = a.table + (int64_t)b * a.n_table;
+    const int mine = max(0, (u1 - u0 - wave + NW - 1) / NW);
+    auto key_of = [&](int i, int t) { return sp.first + (u0 + wave + i * NW) * UNIT + 16 * t; };
     int pages[KT];
-    auto look = [&](int u) {
+    auto look = [&](int i) {
 #pragma unroll
         for (int t = 0; t < KT; t++) {
-            const int i = (sp.first + (u + lane * NW) * S::UNIT + 16 * t) >> a.lp;
-            pages[t] = i < a.n_table ? table[i] : -1;
+            const int at = key_of(i, t) >> a.lp;
+            pages[t] = table[min(at, a.n_table - 1)];
+            if (i >= mine || at >= a.n_table) pages[t] = -1;
         }
     };
-    RowsUnit<HD, F16, KT> nxt;
-    int kb[KT], kn[KT];
-    auto request = [&](int u, int i) {  // unit u, the wave's i-th
+    RowsUnit<HD, F16, KT> set[NS];
+    uint32_t has[NS];  // bit t: tile t has a page
+    auto tile = [&](int i, int t) { return paged_tile<HD, F16>(a, kvh, pages[t], key_of(i, t), sp.end); };
+    auto request_k = [&](RowsUnit<HD, F16, KT> &u, int i) {
+#pragma unroll
+        for (int t = 0; t < KT; t++) paged_load_k<HD, F16, KT>(u, t, tile(i, t), rl, kq);
+    };
+    auto request_v = [&](RowsUnit<HD, F16, KT> &u, uint32_t &h, int i) {
+        h = 0;
 #pragma unroll
         for (int t = 0; t < KT; t++) {
-            const int key = sp.first + u * S::UNIT + 16 * t, page = __builtin_amdgcn_readlane(pages[t], i & 63);
-            const bool ok = u < u1 && (uint32_t)page < (uint32_t)a.n_pages;
-            paged_load<HD, F16, KT>(nxt, t, paged_tile<HD, F16>(a, kvh, ok ? page : -1, key, sp.end), rl, kq);
-            kn[t] = ok ? key : 0x7fffff00;  // (no page: no row takes its keys)
+            paged_load_v<HD, F16, KT>(u, t, tile(i, t), rl, kq);
+            h |= (uint32_t)pages[t] < (uint32_t)a.n_pages ? 1u << t : 0u;
         }
+        look(i + 1);
     };
-    look(u0 + wave);
-    request(u0 + wave, 0);
+    look(0);
+#pragma unroll
+    for (int s = 0; s < NS; s++) request_k(set[s], s), request_v(set[s], has[s], s);
 
-    RowsQ<HD, 1> q;
-    rows_query<HD, 1, true>(q, in, a.scale);
-    // The lane's row takes keys [from, to); every row of the tile those of [all0, all1).
-    const int t0 = rows_div(r0, a.g_m), t1 = rows_div(r0 + rows - 1, a.g_m), t = rows_div(r0 + min(rl, rows - 1), a.g_m);
-    auto last = [&](int tt) { return sp.end - a.T + tt + 1; };
-    const int to = rl < rows ? last(t) : 0, from = a.window ? max(0, last(t) - a.window) : 0;
-    const int all1 = last(t0), all0 = a.window ? max(0, last(t1) - a.window) : 0;
-    auto clean = [&](int key) { return key >= all0 && key + S::UNIT <= all1; };
-    RowsSum<HD, 1> sum;
-    rows_clear<HD, 1>(sum);
-    __syncthreads();  // the flag is set
-    for (int u = u0 + wave, i = 1; u < u1; u += NW, i++) {
-        RowsUnit<HD, F16, KT> cur = nxt;
-        bool whole = clean(sp.first + u * S::UNIT);
+    RowsQ<HD, NT> q;
+    rows_query<HD, NT, true>(q, in, a.scale);
+    // Token t's rows take keys [first(t), last(t)); every row of the workgroup those of [all0, all1).
+    auto last = [&](int t) { return sp.end - a.T + t + 1; };
+    auto first = [&](int t) { return a.window ? max(0, last(t) - a.window) : 0; };
+    const int all1 = last(rows_div(r0, a.g_m)), all0 = first(rows_div(r0 + rows - 1, a.g_m));
+    int from[NT], to[NT];
 #pragma unroll
-        for (int t = 0; t < KT; t++) kb[t] = kn[t], whole &= kn[t] != 0x7fffff00;
-        if ((i & 63) == 0) look(u + NW);
-        request(u + NW, i);
-        if (!whole && paged_clean<HD, F16, KT>(cur)) nonfinite = 1;
-        rows_unit<HD, F16, KT, true, false>(
-            cur, q, sum, kb, kq, [&](int key) { return rows_below(key, to) & ~rows_below(key, from); },
-            [](int, const float (&)[4]) {});
+    for (int qt = 0; qt < NT; qt++) {
+        const int t = rows_div(r0 + min(16 * qt + rl, rows - 1), a.g_m);
+        to[qt] = 16 * qt + rl < rows ? last(t) : 0, from[qt] = first(t);
     }
+    auto inside = [&](int key) { return key >= all0 && key + UNIT <= all1; };
+    RowsSum<HD, NT> sum;
+    rows_clear<HD, NT>(sum);
+    if (EDGE) __syncthreads();  // the flag is set
+    auto step = [&](RowsUnit<HD, F16, KT> &u, uint32_t h, int i, auto keys_done) {
+        const bool whole = inside(key_of(i, 0)) && h == (1u << KT) - 1;
+        int kb[KT];
+#pragma unroll
+        for (int t = 0; t < KT; t++) kb[t] = h >> t & 1 ? key_of(i, t) : 0x7fffff00;  // (no page: no row takes its keys)
+        if constexpr (EDGE)
+            if (!whole && paged_clean<HD, F16, KT>(u)) nonfinite = 1;
+        paged_unit<HD, F16, KT, NT>(
+            u, q, sum, kb, kq, whole,
+            [&](int qt, int key) {
+                const uint32_t x = rows_below(key, to[qt]);
+                return EDGE ? x & ~rows_below(key, from[qt]) : x;
+            },
+            keys_done);
+    };
+    // (no exit between the steps: the waits for one unit's loads leave the later ones in flight)
+    int i = 0;
+    for (; i + NS <= mine; i += NS)
+#pragma unroll
+        for (int s = 0; s < NS; s++) {
+            step(set[s], has[s], i + s, [&] {
+                if (NS == 1) request_k(set[s], i + s + NS);
+            });
+            if (NS > 1) request_k(set[s], i + s + NS);
+            request_v(set[s], has[s], i + s + NS);
+        }
+#pragma unroll
+    for (int s = 0; s < NS - 1; s++)
+        if (i + s < mine) step(set[s], has[s], i + s, [] {});
+
     // The infinite and NaN values that were left out, of the keys that row r takes.
     auto add_nonfinite = [&](int r, int d, float4 &o) {
-        const int end = last(rows_div(r0 + r, a.g_m)), begin = a.window ? max(0, end - a.window) : 0;
+        const int t = rows_div(r0 + r, a.g_m);
         for (int u = u0; u < u1; u++) {
-            bool whole = clean(sp.first + u * S::UNIT);
-            for (int key = sp.first + u * S::UNIT; key < sp.first + (u + 1) * S::UNIT; key++) {
-                const int i = key >> a.lp, page = i < a.n_table ? table[i] : -1;
-                if ((uint32_t)page >= (uint32_t)a.n_pages) whole = false;
+            const int k0 = sp.first + u * UNIT;
+            bool whole = inside(k0);
+            for (int key = k0; key < k0 + UNIT; key += 16) {
+                const int at = key >> a.lp;
+                if (at >= a.n_table || (uint32_t)table[at] >= (uint32_t)a.n_pages) whole = false;
             }
             if (whole) continue;
-            for (int key = max(begin, sp.first + u * S::UNIT); key < min(end, sp.first + (u + 1) * S::UNIT); key++) {
+            for (int key = max(first(t), k0); key < min(last(t), k0 + UNIT); key++) {
                 const int page = table[key >> a.lp];
                 if ((uint32_t)page >= (uint32_t)a.n_pages) continue;
                 const int64_t slot = (((int64_t)page * a.HKV + kvh) << a.lp) + (key & ((1 << a.lp) - 1));
@@ -249,19 +394,27 @@ __global__ __launch_bounds__(64 * NW, HD <= 128 ? 2 : 1) void k_attn_paged(Paged
     float *parts = a.part + ((int64_t)(kvh * gridDim.y + blockIdx.y) * a.cap + j - sl.at) * a.RT * (HD + 4);  // the sequence's
     const uint32_t stride = (uint32_t)a.RT * (HD + 4) * 4;  // bytes from a slice to the next
     const __amdgpu_buffer_rsrc_t part = slice_rsrc(parts, (uint32_t)sl.used * stride);
-    rows_combine<HD, NW>(L, sum, rows, wave, rl, kq, [&](int r, int d, float4 o, float m, float l) {
-        if (nonfinite) add_nonfinite(r, d, o);
-        if (sl.used == 1) {
-            *(float4 *)(paged_out<HD>(a, b, kvh, r0 + r) + d) = rows_over(o, l);
-            return;
-        }
-        const uint32_t at = (uint32_t)sl.at * stride + (uint32_t)r * (HD + 4) * 4;
-        constexpr int POLICY = FUSED ? BUF_SC1 : 0;
-        if (d == 0) __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, make_float2(m, l)), part, at, 0, POLICY);
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), part, at + 16 + 4 * d, 0, POLICY);
-    });
+#pragma unroll
+    for (int qt = 0; qt < NT; qt++) {
+        RowsSum<HD, 1> one;
+        one.m[0] = sum.m[qt], one.l[0] = sum.l[qt];
+#pragma unroll
+        for (int dt = 0; dt < HD / 16; dt++) one.o[0][dt] = sum.o[qt][dt];
+        if (16 * qt >= rows) break;
+        rows_combine<HD, NW>(L.parts, one, rows - 16 * qt, wave, rl, kq, [&](int r, int d, float4 o, float m, float l) {
+            r += 16 * qt;
+            if (EDGE && nonfinite) add_nonfinite(r, d, o);
+            if (sl.used == 1) {
+                *(float4 *)(paged_out<HD>(a, b, kvh, r0 + r) + d) = rows_over(o, l);
+                return;
+            }
+            const uint32_t at = (uint32_t)sl.at * stride + (uint32_t)r * (HD + 4) * 4;
+            constexpr int POLICY = FUSED ? BUF_SC1 : 0;
+            if (d == 0) __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, make_float2(m, l)), part, at, 0, POLICY);
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), part, at + 16 + 4 * d, 0, POLICY);
+        });
+    }
     if (!FUSED || sl.used == 1) return;
-    __shared__ RowsJoin J;
     __shared__ int is_last;
     wait_stores();
     __syncthreads();
@@ -272,19 +425,23 @@ __global__ __launch_bounds__(64 * NW, HD <= 128 ? 2 : 1) void k_attn_paged(Paged
     }
     __syncthreads();
     if (!is_last) return;
-    constexpr int TPR = HD / 4 * JOIN_SG;
     static_assert(64 * NW == 256, "rows_join's threads");
-    for (int g0 = 0; g0 < rows; g0 += 256 / TPR) {
-        const int g = g0 + (int)threadIdx.x / TPR;
-        float M, l;
-        const float4 o = rows_join<HD, JOIN_SG>(J, sl.used, M, l, [&](int s, int d, float2 &ml, float4 &x) {
-            const uint32_t at = (uint32_t)s * stride + (uint32_t)min(g, rows - 1) * (HD + 4) * 4;
-            ml = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(part, at, 0, BUF_SC1));
-            x = __builtin_bit_cast(float4, __builtin_amdgcn_raw_buffer_load_b128(part, at + 16 + 4 * d, 0, BUF_SC1));
-        });
-        if (g < rows && threadIdx.x % TPR < HD / 4)
-            *(float4 *)(paged_out<HD>(a, b, kvh, r0 + g) + 4 * (threadIdx.x % TPR)) = rows_over(o, l);
-    }
+    auto join = [&](auto sg) {  // rows at a time: few slices leave each to a quarter of the threads
+        constexpr int SG = decltype(sg)::value, TPR = HD / 4 * SG;
+        for (int g0 = 0; g0 < rows; g0 += 256 / TPR) {
+            const int g = g0 + (int)threadIdx.x / TPR;
+            float M, l;
+            const float4 o = rows_join<HD, SG>(L.join, sl.used, M, l, [&](int s, int d, float2 &ml, float4 &x) {
+                const uint32_t at = (uint32_t)s * stride + (uint32_t)min(g, rows - 1) * (HD + 4) * 4;
+                ml = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(part, at, 0, BUF_SC1));
+                x = __builtin_bit_cast(float4, __builtin_amdgcn_raw_buffer_load_b128(part, at + 16 + 4 * d, 0, BUF_SC1));
+            });
+            if (g < rows && threadIdx.x % TPR < HD / 4)
+                *(float4 *)(paged_out<HD>(a, b, kvh, r0 + g) + 4 * (threadIdx.x % TPR)) = rows_over(o, l);
+        }
+    };
+    if (sl.used <= 8) join(std::integral_constant<int, 1>{});
+    else join(std::integral_constant<int, JOIN_SG>{});
 }
 
 // The slices' join where few sequences have many: 256 / (HD / 4 x SG) rows a workgroup.
@@ -295,10 +452,10 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedArgs a, int64_t rows) 
     const int64_t row = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR, at = min(row, rows - 1);
     const int b = (int)(at / ((int64_t)a.HKV * a.R)), kvh = (int)(at / a.R % a.HKV), r = (int)(at % a.R);
     const int2 plan = a.plan[b];
-    const int tiles = (a.R + 15) / 16;
+    const int blocks = (a.R + a.RT - 1) / a.RT;
     float M, l;
     const float4 o = rows_join<HD, JOIN_SG>(J, plan.y == 1 ? 0 : plan.y, M, l, [&](int s, int d, float2 &ml, float4 &x) {
-        const float *p = a.part + (((int64_t)(kvh * tiles + r / 16) * a.cap + plan.x + s) * a.RT + r % 16) * (HD + 4);
+        const float *p = a.part + (((int64_t)(kvh * blocks + r / a.RT) * a.cap + plan.x + s) * a.RT + r % a.RT) * (HD + 4);
         ml = *(const float2 *)p, x = *(const float4 *)(p + 4 + d);
     });
     if (plan.y == 1 || row >= rows || threadIdx.x % TPR >= HD / 4) return;
@@ -308,17 +465,19 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedArgs a, int64_t rows) 
 // ---- host ----------------------------------------------------------------------------------------
 
 struct PagedPlan {
-    int cap, tiles;
+    int nt, rt, blocks, cap;  // row tiles a wave, rows a workgroup, blocks of them
     bool fused;
     size_t part, plan;
 };
 static PagedPlan paged_plan(int B, int T, int H, int HKV, int HD, int n_cu) {
     PagedPlan p;
     const int R = T * (H / HKV);
-    p.tiles = (R + 15) / 16;
-    p.cap = std::max(2 * B, 3 * n_cu / std::max(1, HKV * p.tiles));
-    p.fused = (int64_t)B * HKV * p.tiles <= 4096;
-    p.part = align_up((size_t)p.cap * HKV * p.tiles * std::min(R, 16) * (HD + 4) * sizeof(float), 256);
+    p.nt = R > 16 && HD <= 128 ? 2 : 1;
+    p.rt = std::min(R, 16 * p.nt);
+    p.blocks = (R + p.rt - 1) / p.rt;
+    p.cap = std::max(2 * B, (HD <= 128 ? 2 : 1) * n_cu / std::max(1, HKV * p.blocks));
+    p.fused = (int64_t)B * HKV * p.blocks <= 4096 && p.cap <= 16 * B;
+    p.part = align_up((size_t)p.cap * HKV * p.blocks * p.rt * (HD + 4) * sizeof(float), 256);
     p.plan = (size_t)B * sizeof(int2);
     return p;
 }
@@ -326,28 +485,35 @@ size_t attn_paged_scratch_bytes(int B, int T, int H, int HKV, int HD, int n_cu) 
     const PagedPlan p = paged_plan(B, T, H, HKV, HD, n_cu);
     return p.part + p.plan;
 }
+template <class P>
+static hipError_t paged_launch(const PagedArgs &a, const PagedPlan &p, hipStream_t s) {
+    const dim3 grid(p.cap * a.HKV, p.blocks), block(64 * P::NW);
+    if (p.fused) {
+        hipLaunchKernelGGL((k_attn_paged<P, true>), grid, block, 0, s, a);
+        return hipGetLastError();
+    }
+    hipLaunchKernelGGL((k_attn_paged<P, false>), grid, block, 0, s, a);
+    const int64_t rows = (int64_t)a.B * a.HKV * a.R;
+    constexpr int RPW = 256 / (P::HD / 4 * JOIN_SG);
+    hipLaunchKernelGGL(k_paged_merge<P::HD>, dim3((unsigned)((rows + RPW - 1) / RPW)), dim3(256), 0, s, a, rows);
+    return hipGetLastError();
+}
 hipError_t launch_attn_paged(const float *q, int B, int T, int H, int HKV, int HD, KvLayer kv, int kv_f16, int n_pages,
                              int page, const int32_t *table, int n_table, const int32_t *n_keys, int window, float scale,
                              void *scratch, int *counters, float *out, int n_cu, hipStream_t s) {
     const PagedPlan p = paged_plan(B, T, H, HKV, HD, n_cu);
     PagedArgs a{};
     a.q = q, a.kv = kv, a.table = table, a.n_table = n_table, a.n_pages = n_pages, a.lp = __builtin_ctz(page);
-    a.B = B, a.T = T, a.H = H, a.HKV = HKV, a.G = H / HKV, a.R = T * a.G, a.RT = std::min(a.R, 16), a.window = std::min(window, 1 << 30), a.cap = p.cap;
-    a.g_m = rows_magic(a.G), a.hkv_m = rows_magic(HKV), a.n_keys = n_keys, a.scale = scale;
+    a.B = B, a.T = T, a.H = H, a.HKV = HKV, a.G = H / HKV, a.R = T * a.G, a.RT = p.rt, a.window = std::min(window, 1 << 30);
+    a.cap = p.cap, a.g_m = rows_magic(a.G), a.hkv_m = rows_magic(HKV), a.n_keys = n_keys, a.scale = scale;
     a.part = (float *)scratch, a.plan = (int2 *)((uint8_t *)scratch + p.part), a.counters = counters, a.out = out;
     return rows_by_shape(HD, kv_f16, [&](auto hd, auto f16) {
-        constexpr int D = decltype(hd)::value, KT = D == 64 ? 2 : 1, NW = 4, LEAST = 8 / KT;
+        constexpr int D = decltype(hd)::value;
         constexpr bool F = decltype(f16)::value;
-        const dim3 grid(p.cap * HKV, p.tiles);
-        if (p.fused) {
-            hipLaunchKernelGGL((k_attn_paged<D, F, KT, NW, LEAST, true>), grid, dim3(64 * NW), 0, s, a);
-            return hipGetLastError();
-        }
-        hipLaunchKernelGGL((k_attn_paged<D, F, KT, NW, LEAST, false>), grid, dim3(64 * NW), 0, s, a);
-        const int64_t rows = (int64_t)B * HKV * a.R;
-        constexpr int RPW = 256 / (D / 4 * JOIN_SG);
-        hipLaunchKernelGGL(k_paged_merge<D>, dim3((unsigned)((rows + RPW - 1) / RPW)), dim3(256), 0, s, a, rows);
-        return hipGetLastError();
+        if constexpr (D <= 128)
+            if (p.nt == 2) return paged_launch<PagedForm<D, F, 2, D == 64 ? 2 : 1, true>>(a, p, s);
+        if (T > 1 || window) return paged_launch<PagedForm<D, F, 1, 2, true>>(a, p, s);
+        return paged_launch<PagedForm<D, F, 1, D == 256 ? 2 : 3, false>>(a, p, s);
     });
 }
 
