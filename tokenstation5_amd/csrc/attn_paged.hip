@@ -156,8 +156,9 @@ __device__ inline bool paged_clean(RowsUnit<HD, F16, KT> &u) {
 
 // One unit into the sums of NT row tiles, its keys and values converted once. Without `whole`, seen(qt, key) has a bit for each of
 // keys key .. + 3 that the lane's row of tile qt takes. keys_done() comes where the unit's keys are used up.
-template <int HD, bool F16, int KT, int NT, class Seen, class Done>
-__device__ inline void paged_unit(const RowsUnit<HD, F16, KT> &u, const RowsQ<HD, NT> &q, RowsSum<HD, NT> &a,
+// low(qt, c) is the low plane of chunk c of row tile qt.
+template <int HD, bool F16, int KT, int NT, class Low, class Seen, class Done>
+__device__ inline void paged_unit(const RowsUnit<HD, F16, KT> &u, const RowsQ<HD, NT> &q, Low low, RowsSum<HD, NT> &a,
                                   const int (&kb)[KT], int kq, bool whole, Seen seen, Done keys_done) {
     using S = RowsShape<HD, F16, KT>;
     using Op = RowsOp<KT>;
@@ -178,7 +179,7 @@ __device__ inline void paged_unit(const RowsUnit<HD, F16, KT> &u, const RowsQ<HD
                 R[qt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q.h[qt][c], R[qt], 0, 0, 0);
             }
 #pragma unroll
-            for (int qt = 0; qt < NT; qt++) R[qt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q.l[qt][c], R[qt], 0, 0, 0);
+            for (int qt = 0; qt < NT; qt++) R[qt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, low(qt, c), R[qt], 0, 0, 0);
             if constexpr (!F16)
 #pragma unroll
                 for (int qt = 0; qt < NT; qt++)
@@ -256,19 +257,21 @@ __device__ inline float *paged_out(const PagedArgs &a, int b, int kvh, int r) {
 // What a kernel is made for: NT row tiles a wave, NS units in its registers (one used, the others on their way; with one,
 // the next one's keys are requested once its keys are used and its values once all is), EDGE: rows that do not take the
 // same keys (several tokens, a window).
-template <int HD_, bool F16_, int NT_, int NS_, bool EDGE_>
+// FUSED: the last of a sequence's slices joins them.
+template <int HD_, bool F16_, int NT_, int NS_, int NW_, bool EDGE_, bool FUSED_>
 struct PagedForm {
-    static constexpr int HD = HD_, NT = NT_, NS = NS_, KT = HD == 64 ? 2 : 1, NW = 4, UNIT = 16 * KT, LEAST = 8 / KT;
-    static constexpr bool F16 = F16_, EDGE = EDGE_;
+    static constexpr int HD = HD_, NT = NT_, NS = NS_, KT = HD == 64 ? 2 : 1, NW = NW_, UNIT = 16 * KT, LEAST = 8 / KT;
+    static constexpr bool F16 = F16_, EDGE = EDGE_, FUSED = FUSED_;
 };
 
 // grid (cap * HKV, row blocks): one slice of one sequence's keys for up to 16 NT rows of a KV head; the waves take its units
-// in turn. With FUSED the last of a sequence's slices joins them.
-template <class P, bool FUSED>
+// in turn.
+template <class P>
 __global__ __launch_bounds__(64 * P::NW, P::HD <= 128 ? 2 : 1) void k_attn_paged(PagedArgs a) {
     constexpr int HD = P::HD, NT = P::NT, NS = P::NS, KT = P::KT, NW = P::NW, UNIT = P::UNIT;
-    constexpr bool F16 = P::F16, EDGE = P::EDGE;
+    constexpr bool F16 = P::F16, EDGE = P::EDGE, FUSED = P::FUSED, LOW = NT > 1;  // LOW: the rows' low planes are in LDS
     __shared__ union {
+        uint4 low[LOW ? NT : 1][HD / 32][64];
         RowsLds<HD, NW> parts;
         RowsJoin join;
     } L;
@@ -338,16 +341,24 @@ __global__ __launch_bounds__(64 * P::NW, P::HD <= 128 ? 2 : 1) void k_attn_paged
     auto inside = [&](int key) { return key >= all0 && key + UNIT <= all1; };
     RowsSum<HD, NT> sum;
     rows_clear<HD, NT>(sum);
-    if (EDGE) __syncthreads();  // the flag is set
+    if (LOW && wave == 0) {
+#pragma unroll
+        for (int qt = 0; qt < NT; qt++)
+#pragma unroll
+            for (int c = 0; c < HD / 32; c++) L.low[LOW ? qt : 0][c][lane] = __builtin_bit_cast(uint4, q.l[qt][c]);
+    }
+    if (EDGE) __syncthreads();  // the flag is set, the low planes are there
+    auto low = [&](int qt, int c) { return LOW ? __builtin_bit_cast(ar_h8, L.low[LOW ? qt : 0][c][lane]) : q.l[qt][c]; };
     auto step = [&](RowsUnit<HD, F16, KT> &u, uint32_t h, int i, auto keys_done) {
         const bool whole = inside(key_of(i, 0)) && h == (1u << KT) - 1;
         int kb[KT];
 #pragma unroll
         for (int t = 0; t < KT; t++) kb[t] = h >> t & 1 ? key_of(i, t) : 0x7fffff00;  // (no page: no row takes its keys)
+        if constexpr (LOW) asm volatile("" ::: "memory");  // (the low planes are read again: registers are what LDS saves)
         if constexpr (EDGE)
             if (!whole && paged_clean<HD, F16, KT>(u)) nonfinite = 1;
         paged_unit<HD, F16, KT, NT>(
-            u, q, sum, kb, kq, whole,
+            u, q, low, sum, kb, kq, whole,
             [&](int qt, int key) {
                 const uint32_t x = rows_below(key, to[qt]);
                 return EDGE ? x & ~rows_below(key, from[qt]) : x;
@@ -414,7 +425,8 @@ __global__ __launch_bounds__(64 * P::NW, P::HD <= 128 ? 2 : 1) void k_attn_paged
             __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), part, at + 16 + 4 * d, 0, POLICY);
         });
     }
-    if (!FUSED || sl.used == 1) return;
+    if constexpr (FUSED) {
+    if (sl.used == 1) return;
     __shared__ int is_last;
     wait_stores();
     __syncthreads();
@@ -442,6 +454,7 @@ __global__ __launch_bounds__(64 * P::NW, P::HD <= 128 ? 2 : 1) void k_attn_paged
     };
     if (sl.used <= 8) join(std::integral_constant<int, 1>{});
     else join(std::integral_constant<int, JOIN_SG>{});
+    }
 }
 
 // The slices' join where few sequences have many: 256 / (HD / 4 x SG) rows a workgroup.
@@ -465,7 +478,7 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedArgs a, int64_t rows) 
 // ---- host ----------------------------------------------------------------------------------------
 
 struct PagedPlan {
-    int nt, rt, blocks, cap;  // row tiles a wave, rows a workgroup, blocks of them
+    int nt, rt, blocks, nw, cap;  // row tiles a wave, rows a workgroup, blocks of them, waves a workgroup, slices in all
     bool fused;
     size_t part, plan;
 };
@@ -475,8 +488,10 @@ static PagedPlan paged_plan(int B, int T, int H, int HKV, int HD, int n_cu) {
     p.nt = R > 16 && HD <= 128 ? 2 : 1;
     p.rt = std::min(R, 16 * p.nt);
     p.blocks = (R + p.rt - 1) / p.rt;
-    p.cap = std::max(2 * B, (HD <= 128 ? 2 : 1) * n_cu / std::max(1, HKV * p.blocks));
-    p.fused = (int64_t)B * HKV * p.blocks <= 4096 && p.cap <= 16 * B;
+    const int items = B * HKV * p.blocks, slots = (HD <= 128 ? 2 : 1) * n_cu;
+    p.fused = items <= 4096 && R <= 16 && 16 * items >= slots;
+    p.nw = !p.fused && HD <= 128 ? 8 : 4;
+    p.cap = std::max(2 * B, slots * 4 / p.nw / std::max(1, HKV * p.blocks));
     p.part = align_up((size_t)p.cap * HKV * p.blocks * p.rt * (HD + 4) * sizeof(float), 256);
     p.plan = (size_t)B * sizeof(int2);
     return p;
@@ -487,12 +502,8 @@ size_t attn_paged_scratch_bytes(int B, int T, int H, int HKV, int HD, int n_cu) 
 }
 template <class P>
 static hipError_t paged_launch(const PagedArgs &a, const PagedPlan &p, hipStream_t s) {
-    const dim3 grid(p.cap * a.HKV, p.blocks), block(64 * P::NW);
-    if (p.fused) {
-        hipLaunchKernelGGL((k_attn_paged<P, true>), grid, block, 0, s, a);
-        return hipGetLastError();
-    }
-    hipLaunchKernelGGL((k_attn_paged<P, false>), grid, block, 0, s, a);
+    hipLaunchKernelGGL(k_attn_paged<P>, dim3(p.cap * a.HKV, p.blocks), dim3(64 * P::NW), 0, s, a);
+    if (P::FUSED) return hipGetLastError();
     const int64_t rows = (int64_t)a.B * a.HKV * a.R;
     constexpr int RPW = 256 / (P::HD / 4 * JOIN_SG);
     hipLaunchKernelGGL(k_paged_merge<P::HD>, dim3((unsigned)((rows + RPW - 1) / RPW)), dim3(256), 0, s, a, rows);
@@ -510,10 +521,15 @@ hipError_t launch_attn_paged(const float *q, int B, int T, int H, int HKV, int H
     return rows_by_shape(HD, kv_f16, [&](auto hd, auto f16) {
         constexpr int D = decltype(hd)::value;
         constexpr bool F = decltype(f16)::value;
+        constexpr int WIDE = D <= 128 ? 8 : 4, AHEAD = D <= 128 ? 3 : 2;
         if constexpr (D <= 128)
-            if (p.nt == 2) return paged_launch<PagedForm<D, F, 2, D == 64 ? 2 : 1, true>>(a, p, s);
-        if (T > 1 || window) return paged_launch<PagedForm<D, F, 1, 2, true>>(a, p, s);
-        return paged_launch<PagedForm<D, F, 1, D == 256 ? 2 : 3, false>>(a, p, s);
+            if (p.nt == 2) return paged_launch<PagedForm<D, F, 2, D == 128 && F ? 1 : 2, WIDE, true, false>>(a, p, s);
+        if (T > 1 || window) {
+            if (p.fused) return paged_launch<PagedForm<D, F, 1, 2, 4, true, true>>(a, p, s);
+            return paged_launch<PagedForm<D, F, 1, 2, WIDE, true, false>>(a, p, s);
+        }
+        if (p.fused) return paged_launch<PagedForm<D, F, 1, AHEAD, 4, false, true>>(a, p, s);
+        return paged_launch<PagedForm<D, F, 1, AHEAD, WIDE, false, false>>(a, p, s);
     });
 }
 

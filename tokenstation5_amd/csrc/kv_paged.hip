@@ -27,84 +27,135 @@ __device__ inline float max8(float v) {
     return dpp_max<0x141, 0xF, true>(v);  // row_half_mirror
 }
 
-// A row (one head of one token) takes HD / 4 lanes, 4 neighbouring values each. grid (rows of a token / those of a
-// workgroup, tokens).
-template <int HD, bool F16>
-__global__ __launch_bounds__(256) void k_append_paged(const float *__restrict__ qkv, const int32_t *__restrict__ seq,
-                                                      const int32_t *__restrict__ pos, int H,
-                                                      const float *__restrict__ bias, const float *__restrict__ q_norm,
-                                                      const float *__restrict__ k_norm, float eps,
-                                                      const float *__restrict__ rope_cs, int n_pos, int n_rot, int neox,
-                                                      float *__restrict__ q_out, PagedPool p) {
+// A row (one head of one token) takes HD / 4 lanes, 4 neighbouring values each; a thread takes the same head's row of TOK
+// tokens, all requested before the places that they go to. Bytes bound it where there are many.
+// grid (rows of a token / those of a workgroup, tokens / TOK).
+constexpr int APPEND_MANY = 4096;  // rows' workgroups from which a thread takes four tokens
+struct AppendArgs {
+    const float *qkv;  // [ntok][(H + 2 HKV) HD]
+    const int32_t *seq, *pos;
+    const float *bias, *q_norm, *k_norm, *rope_cs;  // the first three may be null
+    float eps;
+    int ntok, H, n_pos, n_rot, neox;
+    float *q_out;
+    PagedPool p;
+};
+template <int HD, bool F16, int TOK>
+__global__ __launch_bounds__(256) void k_append_paged(AppendArgs a) {
     constexpr int LPR = HD / 4, RPW = 256 / LPR;
     __shared__ __align__(16) float rows[RPW][HD];
-    const int t = blockIdx.y, at = pos[t];
-    const int64_t slot0 = paged_slot(p, seq[t], at);
-    if (slot0 < 0 || at >= n_pos) return;  // left out
     const int row = threadIdx.x / LPR, d = 4 * (threadIdx.x % LPR);
-    const int heads = H + 2 * p.HKV, hh = blockIdx.x * RPW + row;
+    const int heads = a.H + 2 * a.p.HKV, hh = blockIdx.x * RPW + row, t0 = blockIdx.y * TOK;
     if (hh >= heads) return;  // (no barrier below: a row is inside one wave)
-    const bool is_q = hh < H, is_k = !is_q && hh < H + p.HKV;
-    float4 x = *(const float4 *)(qkv + ((int64_t)t * heads + hh) * HD + d);
-    if (bias) {
-        const float4 y = *(const float4 *)(bias + (int64_t)hh * HD + d);
-        x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
-    }
-    const float *nw = is_q ? q_norm : is_k ? k_norm : nullptr;
-    if (nw) {
-        float ss = row_sum_dpp(x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w);
-        if constexpr (HD >= 128) ss = add_xor16(ss);
-        if constexpr (HD == 256) ss = add_xor32(ss);
-        const float s = 1.0f / sqrtf(ss / (float)HD + eps);
-        const float4 w = *(const float4 *)(nw + d);
-        x.x = x.x * s * w.x, x.y = x.y * s * w.y, x.z = x.z * s * w.z, x.w = x.w * s * w.w;
-    }
-    if ((is_q || is_k) && d < n_rot) {
-        const float *cs = rope_cs + (int64_t)at * n_rot;  // n_rot / 2 pairs (cos, sin)
-        if (!neox) {
-            rope_pair(x.x, x.y, cs[d], cs[d + 1]);
-            if (d + 2 < n_rot) rope_pair(x.z, x.w, cs[d + 2], cs[d + 3]);
-        } else {
-            const int half = n_rot / 2;
-            *(float4 *)&rows[row][d] = x;
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            float v[4] = {x.x, x.y, x.z, x.w};
+    const bool is_q = hh < a.H, is_k = !is_q && hh < a.H + a.p.HKV;
+    float4 in[TOK];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int e = d + i;
-                if (e < half) {
-                    float y = rows[row][e + half];
-                    rope_pair(v[i], y, cs[2 * e], cs[2 * e + 1]);
-                } else if (e < n_rot) {
-                    float y = rows[row][e - half];
-                    rope_pair(y, v[i], cs[2 * (e - half)], cs[2 * (e - half) + 1]);
+    for (int i = 0; i < TOK; i++) in[i] = *(const float4 *)(a.qkv + ((int64_t)min(t0 + i, a.ntok - 1) * heads + hh) * HD + d);
+    int at[TOK];
+    int64_t slot0[TOK];
+#pragma unroll
+    for (int i = 0; i < TOK; i++) {
+        const int t = min(t0 + i, a.ntok - 1);
+        at[i] = a.pos[t];
+        slot0[i] = paged_slot(a.p, a.seq[t], at[i]);
+        if (t0 + i >= a.ntok || at[i] >= a.n_pos) slot0[i] = -1;  // left out
+    }
+    float4 bias = make_float4(0.f, 0.f, 0.f, 0.f), nw = bias;
+    if (a.bias) bias = *(const float4 *)(a.bias + (int64_t)hh * HD + d);
+    const float *norm = is_q ? a.q_norm : is_k ? a.k_norm : nullptr;
+    if (norm) nw = *(const float4 *)(norm + d);
+    const int half = a.n_rot / 2;
+    const bool turned = (is_q || is_k) && d < a.n_rot;
+    // The lane's four angles: of pairs d / 2 and d / 2 + 1, or of its own place in the lower or upper half.
+    const bool low = d < half, quads = a.neox && half % 4 == 0;
+    float4 cs[TOK][2];
+    if (turned) {
+#pragma unroll
+        for (int i = 0; i < TOK; i++) {
+            const float *c = a.rope_cs + (int64_t)(slot0[i] < 0 ? 0 : at[i]) * a.n_rot;  // half pairs (cos, sin)
+            if (!a.neox) {
+                cs[i][0] = make_float4(c[d], c[d + 1], 0.f, 0.f);
+                if (d + 2 < a.n_rot) cs[i][0].z = c[d + 2], cs[i][0].w = c[d + 3];
+            } else if (quads) {
+                const float4 *q = (const float4 *)(c + 2 * (low ? d : d - half));
+                cs[i][0] = q[0], cs[i][1] = q[1];
+            } else {
+                float2 x[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const int e = d + k;
+                    x[k] = e < a.n_rot ? *(const float2 *)(c + 2 * (e < half ? e : e - half)) : make_float2(1.f, 0.f);
                 }
+                cs[i][0] = make_float4(x[0].x, x[0].y, x[1].x, x[1].y), cs[i][1] = make_float4(x[2].x, x[2].y, x[3].x, x[3].y);
             }
-            x = make_float4(v[0], v[1], v[2], v[3]);
         }
     }
-    if (is_q) {
-        *(float4 *)(q_out + ((int64_t)t * H + hh) * HD + d) = x;
-        return;
-    }
-    const int kvh = is_k ? hh - H : hh - H - p.HKV;
-    const int64_t slot = slot0 + ((int64_t)kvh << p.lp);
-    if constexpr (F16) {  // each value to the nearest half
-        uint2 w;
-        w.x = (uint32_t)f2h(x.x) | (uint32_t)f2h(x.y) << 16, w.y = (uint32_t)f2h(x.z) | (uint32_t)f2h(x.w) << 16;
-        *(uint2 *)((uint16_t *)(is_k ? p.kv.k : p.kv.v) + slot * HD + d) = w;
-    } else {  // per 32 values sc = f16(amax / 127), q = clamp(rint(v / sc), +-127)
-        const float amax = max8(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
-        const uint16_t sh = f2h(amax / 127.0f);
-        const float sc = h2f(sh), v[4] = {x.x, x.y, x.z, x.w};
-        uint32_t w = 0;
-        if (sc > 0.f)
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                w |= (uint32_t)((int)fminf(127.f, fmaxf(-127.f, rintf(v[i] / sc))) & 0xff) << (8 * i);
-        *(uint32_t *)((is_k ? p.kv.k : p.kv.v) + slot * HD + d) = w;
-        if (d % 32 == 0) (is_k ? p.kv.ks : p.kv.vs)[slot * (HD / 32) + d / 32] = sh;
+    for (int i = 0; i < TOK; i++) {
+        if (slot0[i] < 0) continue;
+        const int t = t0 + i;
+        float4 x = in[i];
+        if (a.bias) x.x += bias.x, x.y += bias.y, x.z += bias.z, x.w += bias.w;
+        if (norm) {
+            float ss = row_sum_dpp(x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w);
+            if constexpr (HD >= 128) ss = add_xor16(ss);
+            if constexpr (HD == 256) ss = add_xor32(ss);
+            const float s = 1.0f / sqrtf(ss / (float)HD + a.eps);
+            x.x = x.x * s * nw.x, x.y = x.y * s * nw.y, x.z = x.z * s * nw.z, x.w = x.w * s * nw.w;
+        }
+        if (turned) {
+            if (!a.neox) {
+                rope_pair(x.x, x.y, cs[i][0].x, cs[i][0].y);
+                if (d + 2 < a.n_rot) rope_pair(x.z, x.w, cs[i][0].z, cs[i][0].w);
+            } else {  // the other half's values through LDS
+                *(float4 *)&rows[row][d] = x;
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                float v[4] = {x.x, x.y, x.z, x.w}, y[4];
+                if (quads) {
+                    const float4 o = *(const float4 *)&rows[row][low ? d + half : d - half];
+                    y[0] = o.x, y[1] = o.y, y[2] = o.z, y[3] = o.w;
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const int e = d + k;
+                        y[k] = e < a.n_rot ? rows[row][e < half ? e + half : e - half] : 0.f;
+                    }
+                }
+                const float c[4] = {cs[i][0].x, cs[i][0].z, cs[i][1].x, cs[i][1].z};
+                const float s[4] = {cs[i][0].y, cs[i][0].w, cs[i][1].y, cs[i][1].w};
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    float lo = d + k < half ? v[k] : y[k], hi = d + k < half ? y[k] : v[k];
+                    rope_pair(lo, hi, c[k], s[k]);
+                    if (d + k < a.n_rot) v[k] = d + k < half ? lo : hi;
+                }
+                x = make_float4(v[0], v[1], v[2], v[3]);
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+                __builtin_amdgcn_wave_barrier();  // (the next token's row takes this one's place)
+            }
+        }
+        if (is_q) {
+            *(float4 *)(a.q_out + ((int64_t)t * a.H + hh) * HD + d) = x;
+            continue;
+        }
+        const int64_t slot = slot0[i] + ((int64_t)(is_k ? hh - a.H : hh - a.H - a.p.HKV) << a.p.lp);
+        if constexpr (F16) {  // each value to the nearest half
+            uint2 w;
+            w.x = (uint32_t)f2h(x.x) | (uint32_t)f2h(x.y) << 16, w.y = (uint32_t)f2h(x.z) | (uint32_t)f2h(x.w) << 16;
+            *(uint2 *)((uint16_t *)(is_k ? a.p.kv.k : a.p.kv.v) + slot * HD + d) = w;
+        } else {  // per 32 values sc = f16(amax / 127), q = clamp(rint(v / sc), +-127)
+            const float amax = max8(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
+            const uint16_t sh = f2h(amax / 127.0f);
+            const float sc = h2f(sh), v[4] = {x.x, x.y, x.z, x.w};
+            uint32_t w = 0;
+            if (sc > 0.f)
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    w |= (uint32_t)((int)fminf(127.f, fmaxf(-127.f, rintf(v[k] / sc))) & 0xff) << (8 * k);
+            *(uint32_t *)((is_k ? a.p.kv.k : a.p.kv.v) + slot * HD + d) = w;
+            if (d % 32 == 0) (is_k ? a.p.kv.ks : a.p.kv.vs)[slot * (HD / 32) + d / 32] = sh;
+        }
     }
 }
 
@@ -112,17 +163,22 @@ hipError_t launch_append_paged(const float *qkv, int ntok, const int32_t *seq, c
                                const float *bias, const float *q_norm, const float *k_norm, float eps,
                                const float *rope_cs, int n_pos, int n_rot, int neox, float *q_out, KvLayer kv, int kv_f16,
                                int n_pages, int page, const int32_t *table, int n_seq, int n_table, hipStream_t s) {
-    const PagedPool p{kv, table, n_pages, __builtin_ctz(page), n_seq, n_table, HKV};
-    const int per = 1024 / HD;
-    const dim3 grid((H + 2 * HKV + per - 1) / per, ntok);
-    auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, qkv, seq, pos, H, bias, q_norm, k_norm, eps, rope_cs, n_pos,
-                           n_rot, neox, q_out, p);
+    AppendArgs a{};
+    a.qkv = qkv, a.seq = seq, a.pos = pos, a.bias = bias, a.q_norm = q_norm, a.k_norm = k_norm, a.rope_cs = rope_cs;
+    a.eps = eps, a.ntok = ntok, a.H = H, a.n_pos = n_pos, a.n_rot = n_rot, a.neox = neox, a.q_out = q_out;
+    a.p = PagedPool{kv, table, n_pages, __builtin_ctz(page), n_seq, n_table, HKV};
+    const int per = 1024 / HD, x = (H + 2 * HKV + per - 1) / per;
+    auto go = [&](auto hd, auto f16) {
+        constexpr int D = decltype(hd)::value;
+        constexpr bool F = decltype(f16)::value;
+        if ((int64_t)x * ntok >= APPEND_MANY) hipLaunchKernelGGL((k_append_paged<D, F, 4>), dim3(x, (ntok + 3) / 4), dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((k_append_paged<D, F, 1>), dim3(x, ntok), dim3(256), 0, s, a);
         return hipGetLastError();
     };
-    if (HD == 64) return kv_f16 ? go(k_append_paged<64, true>) : go(k_append_paged<64, false>);
-    if (HD == 128) return kv_f16 ? go(k_append_paged<128, true>) : go(k_append_paged<128, false>);
-    return kv_f16 ? go(k_append_paged<256, true>) : go(k_append_paged<256, false>);
+    auto by_type = [&](auto hd) { return kv_f16 ? go(hd, std::true_type{}) : go(hd, std::false_type{}); };
+    if (HD == 64) return by_type(std::integral_constant<int, 64>{});
+    if (HD == 128) return by_type(std::integral_constant<int, 128>{});
+    return by_type(std::integral_constant<int, 256>{});
 }
 
 // V values a thread of K and V each, READ_TOKENS tokens a workgroup. grid (tokens / READ_TOKENS).
