@@ -27,14 +27,14 @@ struct PagedArgs {
     float *out;    // [B][T][H * HD]
 };
 
-// A sequence's keys: [first, end) are some row's, counted from `first` (a multiple of 16).
+// A sequence's keys: [first, end) are some row's, counted from `first` (a multiple of 32: whole units).
 struct PagedSpan {
     int first, end;
 };
 __device__ inline PagedSpan paged_span(const PagedArgs &a, int n) {
     PagedSpan s;
     s.end = max(0, min(n, a.n_table << a.lp));
-    s.first = a.window ? max(0, s.end - a.T + 1 - a.window) & ~15 : 0;
+    s.first = a.window ? max(0, s.end - a.T + 1 - a.window) & ~31 : 0;
     return s;
 }
 __device__ inline int paged_units(const PagedSpan &s, int unit) { return (s.end - s.first + unit - 1) / unit; }
@@ -54,18 +54,20 @@ __device__ inline int wave_total(int x) { return __builtin_amdgcn_readlane(wave_
 // Slices of u units, `per` each; a sequence without a key has one, which writes its zeros.
 __device__ inline int paged_slices(int u, int per) { return max(1, (u + per - 1) / per); }
 
-// Slice j's sequence, its place among that sequence's slices, how many those are, and the units a slice has. b < 0:
-// there is no such slice. Every lane of a wave calls it with the same j. Slices are whole rounds of NW waves.
+// Slice j's sequence, that one's count of keys, the slice's place among its slices, how many those are, and the units a
+// slice has. b < 0: there is no such slice. Every lane of a wave calls it with the same j. Slices are whole rounds of NW waves.
 struct PagedSlice {
-    int b, at, used, per;
+    int b, n, at, used, per;
 };
 template <int UNIT, int NW, int LEAST>
 __device__ inline PagedSlice paged_slice(const PagedArgs &a, int j) {
     const int lane = threadIdx.x & 63;
-    auto units = [&](int b) { return b < a.B ? paged_units(paged_span(a, a.n_keys[b]), UNIT) : 0; };
+    auto count = [&](int b) { return b < a.B ? a.n_keys[b] : 0; };
+    auto units = [&](int n) { return paged_units(paged_span(a, n), UNIT); };
     PagedSlice s;
-    int sum = 0, u0 = units(lane);
-    for (int b = 0; b < a.B; b += 64) sum += wave_total(b ? units(b + lane) : u0);
+    const int n0 = count(lane), u0 = units(n0);
+    int sum = 0;
+    for (int b = 0; b < a.B; b += 64) sum += wave_total(b ? units(count(b + lane)) : u0);
     // ceil(u / per) <= u / per + 1 summed over the sequences: this many units a slice always fit.
     auto whole = [](int per) { return max(LEAST, (per + NW - 1) / NW * NW); };
     s.per = whole((sum + a.cap - a.B - 1) / max(1, a.cap - a.B));
@@ -78,14 +80,15 @@ __device__ inline PagedSlice paged_slice(const PagedArgs &a, int j) {
         }
         s.per = hi;
     }
-    s.b = -1, s.at = 0, s.used = 0;
+    s.b = -1, s.n = 0, s.at = 0, s.used = 0;
     int before = 0;
     for (int b = 0; b < a.B; b += 64) {
-        const int mine = b + lane < a.B ? paged_slices(b ? units(b + lane) : u0, s.per) : 0, incl = before + wave_scan(mine);
+        const int n = b ? count(b + lane) : n0;
+        const int mine = b + lane < a.B ? paged_slices(b ? units(n) : u0, s.per) : 0, incl = before + wave_scan(mine);
         const uint64_t past = __builtin_amdgcn_ballot_w64(incl > j);
         if (past) {
             const int l = __ffsll((unsigned long long)past) - 1;
-            s.b = b + l, s.used = __builtin_amdgcn_readlane(mine, l);
+            s.b = b + l, s.n = __builtin_amdgcn_readlane(n, l), s.used = __builtin_amdgcn_readlane(mine, l);
             s.at = j - (__builtin_amdgcn_readlane(incl, l) - s.used);
             break;
         }
@@ -94,33 +97,40 @@ __device__ inline PagedSlice paged_slice(const PagedArgs &a, int j) {
     return s;
 }
 
-// Where the wave finds a tile of 16 keys: those from `key` on and below `end`, as bounded buffers (what is past them reads
-// zeros); no page: all of it.
+// The page that a unit is in, as bounded buffers: what is past the sequence's keys reads zeros, and without a page
+// all of it. `id` is the next page's, on its way.
 template <int HD, bool F16>
-__device__ inline RowsKv paged_tile(const PagedArgs &a, int kvh, int page, int key, int end) {
-    const bool ok = (uint32_t)page < (uint32_t)a.n_pages;
-    // (readfirstlane: the compiler takes min and max as one vector instruction, and then each load as a loop over lanes that
-    // might have buffers of their own)
-    const int n = ok ? __builtin_amdgcn_readfirstlane(max(0, min(end - key, 16))) : 0;
-    const int64_t slot = (((int64_t)(ok ? page : 0) * a.HKV + kvh) << a.lp) + (key & ((1 << a.lp) - 1));
-    return rows_kv<HD, F16>(a.kv, slot, n);
-}
+struct PagedPage {
+    RowsKv kv;
+    int at, id;
+    bool has;
+    // The page of index `to` comes next.
+    __device__ void look(const PagedArgs &a, const int32_t *table, int to) { id = table[min(to, a.n_table - 1)]; }
+    __device__ void turn(const PagedArgs &a, int kvh, int end, int to) {
+        at = to, has = to < a.n_table && (uint32_t)id < (uint32_t)a.n_pages;
+        // (readfirstlane: the compiler takes min and max as one vector instruction, and then each load as a loop over lanes
+        // that might have buffers of their own)
+        const int n = __builtin_amdgcn_readfirstlane(max(0, min(end - (to << a.lp), 1 << a.lp)));
+        kv = rows_kv<HD, F16>(a.kv, ((int64_t)(has ? id : 0) * a.HKV + kvh) << a.lp, has ? n : 0);
+    }
+};
+// Tile t of a unit, `slot` keys into its page (or past all pages: zeros).
 template <int HD, bool F16, int KT>
-__device__ inline void paged_load_k(RowsUnit<HD, F16, KT> &u, int t, const RowsKv &kv, int rl, int kq) {
+__device__ inline void paged_load_k(RowsUnit<HD, F16, KT> &u, int t, const RowsKv &kv, uint32_t slot, int rl, int kq) {
     using S = RowsShape<HD, F16, KT>;
+    const uint32_t k0 = (slot + rl) * (HD * S::VB) + 8 * kq * S::VB;
 #pragma unroll
-    for (int c = 0; c < S::NC; c++) rows_words<S::KW>(kv.k, ((uint32_t)rl * HD + 32 * c + 8 * kq) * S::VB, u.k[t][c]);
-    if constexpr (!F16) rows_words<2 * S::NC>(kv.ks, (uint32_t)(4 * kq) * S::NC * 2, u.ks[t]);
+    for (int c = 0; c < S::NC; c++) rows_words<S::KW>(kv.k, k0 + 32 * c * S::VB, u.k[t][c]);
+    if constexpr (!F16) rows_words<2 * S::NC>(kv.ks, (slot + 4 * kq) * (S::NC * 2), u.ks[t]);
 }
 template <int HD, bool F16, int KT>
-__device__ inline void paged_load_v(RowsUnit<HD, F16, KT> &u, int t, const RowsKv &kv, int rl, int kq) {
+__device__ inline void paged_load_v(RowsUnit<HD, F16, KT> &u, int t, const RowsKv &kv, uint32_t slot, int rl, int kq) {
     using S = RowsShape<HD, F16, KT>;
+    const uint32_t v0 = ((slot + 4 * kq) * HD + S::NDT * rl) * S::VB, s0 = (slot + 4 * kq) * (S::NC * 2) + rl * S::NDT / 32 * 2;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const uint32_t key = (uint32_t)(4 * kq + i);
-        rows_words<S::VW>(kv.v, (key * HD + S::NDT * rl) * S::VB, u.v[t][i]);
-        if constexpr (!F16)
-            u.vs[t][i] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(kv.vs, key * S::NC * 2 + rl * S::NDT / 32 * 2, 0, 0);
+        rows_words<S::VW>(kv.v, v0 + i * HD * S::VB, u.v[t][i]);
+        if constexpr (!F16) u.vs[t][i] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(kv.vs, s0 + i * S::NC * 2, 0, 0);
     }
 }
 
@@ -254,13 +264,13 @@ __device__ inline float *paged_out(const PagedArgs &a, int b, int kvh, int r) {
     return a.out + (((int64_t)b * a.T + t) * a.H + kvh * a.G + r - t * a.G) * HD;
 }
 
-// What a kernel is made for: NT row tiles a wave, NS units in its registers (one used, the others on their way; with one,
+// What a kernel is made for: KT tiles of keys a unit (which does not end past a page), NT row tiles a wave, NS units in its registers (one used, the others on their way; with one,
 // the next one's keys are requested once its keys are used and its values once all is), EDGE: rows that do not take the
 // same keys (several tokens, a window).
 // FUSED: the last of a sequence's slices joins them.
-template <int HD_, bool F16_, int NT_, int NS_, int NW_, bool EDGE_, bool FUSED_>
+template <int HD_, bool F16_, int KT_, int NT_, int NS_, int NW_, bool EDGE_, bool FUSED_>
 struct PagedForm {
-    static constexpr int HD = HD_, NT = NT_, NS = NS_, KT = HD == 64 ? 2 : 1, NW = NW_, UNIT = 16 * KT, LEAST = 8 / KT;
+    static constexpr int HD = HD_, KT = KT_, NT = NT_, NS = NS_, NW = NW_, UNIT = 16 * KT, LEAST = 8 / KT < NW ? NW : 8 / KT;
     static constexpr bool F16 = F16_, EDGE = EDGE_, FUSED = FUSED_;
 };
 
@@ -269,9 +279,12 @@ struct PagedForm {
 template <class P>
 __global__ __launch_bounds__(64 * P::NW, P::HD <= 128 ? 2 : 1) void k_attn_paged(PagedArgs a) {
     constexpr int HD = P::HD, NT = P::NT, NS = P::NS, KT = P::KT, NW = P::NW, UNIT = P::UNIT;
-    constexpr bool F16 = P::F16, EDGE = P::EDGE, FUSED = P::FUSED, LOW = NT > 1;  // LOW: the rows' low planes are in LDS
+    constexpr bool F16 = P::F16, EDGE = P::EDGE, FUSED = P::FUSED, LOW = NT > 1;  // LOW: the rows' planes go through LDS, and the low ones stay there
     __shared__ union {
-        uint4 low[LOW ? NT : 1][HD / 32][64];
+        struct {
+            uint4 high[LOW ? NT : 1][HD / 32][64], low[LOW ? NT : 1][HD / 32][64];
+            float p2e[LOW ? NT : 1][16];
+        } q;
         RowsLds<HD, NW> parts;
         RowsJoin join;
     } L;
@@ -283,77 +296,88 @@ __global__ __launch_bounds__(64 * P::NW, P::HD <= 128 ? 2 : 1) void k_attn_paged
     const PagedSlice sl = paged_slice<UNIT, NW, P::LEAST>(a, j);
     if (sl.b < 0) return;
     const int b = sl.b, r0 = blockIdx.y * a.RT, rows = min(a.R - r0, a.RT);
-    RowsIn<HD, NT> in;
-    rows_request<HD, NT>(in, kq, [&](int qt, bool &ok) {
-        const int r = r0 + min(16 * qt + rl, rows - 1), t = rows_div(r, a.g_m);
-        ok = 16 * qt + rl < rows;
-        return a.q + (((int64_t)b * a.T + t) * a.H + kvh * a.G + r - t * a.G) * HD;
-    });
-    const PagedSpan sp = paged_span(a, a.n_keys[b]);
+    constexpr int NQ = LOW ? 1 : NT;  // row tiles that a wave converts (LOW: wave w the w-th)
+    RowsIn<HD, NQ> in;
+    const int tile0 = LOW ? wave : 0;
+    auto request_q = [&] {
+        rows_request<HD, NQ>(in, kq, [&](int qt, bool &ok) {
+            const int at = 16 * (tile0 + qt) + rl, r = r0 + min(at, rows - 1), t = rows_div(r, a.g_m);
+            ok = at < rows;
+            return a.q + (((int64_t)b * a.T + t) * a.H + kvh * a.G + r - t * a.G) * HD;
+        });
+    };
+    if (tile0 < NT) request_q();
+    const PagedSpan sp = paged_span(a, sl.n);
     const int units = paged_units(sp, UNIT), u0 = sl.at * sl.per, u1 = min(units, u0 + sl.per);
     if (!FUSED && kvh == 0 && blockIdx.y == 0 && sl.at == 0 && threadIdx.x == 0) a.plan[b] = make_int2(j, sl.used);
 
-    // The wave's i-th unit: u0 + wave + i NW. Its pages are looked up one request before they are needed.
+    // The wave's i-th unit, of a stretch of its own; its page is looked up one unit before.
     const int32_t *table = a.table + (int64_t)b * a.n_table;
-    const int mine = max(0, (u1 - u0 - wave + NW - 1) / NW);
-    auto key_of = [&](int i, int t) { return sp.first + (u0 + wave + i * NW) * UNIT + 16 * t; };
-    int pages[KT];
-    auto look = [&](int i) {
-#pragma unroll
-        for (int t = 0; t < KT; t++) {
-            const int at = key_of(i, t) >> a.lp;
-            pages[t] = table[min(at, a.n_table - 1)];
-            if (i >= mine || at >= a.n_table) pages[t] = -1;
-        }
-    };
+    const int share = sl.per / NW, w0 = u0 + wave * share, mine = max(0, min(share, u1 - w0));
+    auto key_of = [&](int i) { return sp.first + (w0 + i) * UNIT; };
+    PagedPage<HD, F16> page;
+    page.at = -1, page.look(a, table, key_of(0) >> a.lp);
     RowsUnit<HD, F16, KT> set[NS];
-    uint32_t has[NS];  // bit t: tile t has a page
-    auto tile = [&](int i, int t) { return paged_tile<HD, F16>(a, kvh, pages[t], key_of(i, t), sp.end); };
-    auto request_k = [&](RowsUnit<HD, F16, KT> &u, int i) {
+    bool has[NS];  // the unit has a page
+    auto slot_of = [&](int i) { return i < mine ? (uint32_t)(key_of(i) & ((1 << a.lp) - 1)) : 1u << 20; };
+    auto request_k = [&](RowsUnit<HD, F16, KT> &u, bool &h, int i) {
+        const int to = key_of(i) >> a.lp;
+        if (to != page.at) page.turn(a, kvh, sp.end, to);
+        h = page.has;
+        const int next = key_of(i + 1) >> a.lp;
+        if (next != to) page.look(a, table, next);
 #pragma unroll
-        for (int t = 0; t < KT; t++) paged_load_k<HD, F16, KT>(u, t, tile(i, t), rl, kq);
+        for (int t = 0; t < KT; t++) paged_load_k<HD, F16, KT>(u, t, page.kv, slot_of(i) + 16 * t, rl, kq);
     };
-    auto request_v = [&](RowsUnit<HD, F16, KT> &u, uint32_t &h, int i) {
-        h = 0;
+    auto request_v = [&](RowsUnit<HD, F16, KT> &u, int i) {
 #pragma unroll
-        for (int t = 0; t < KT; t++) {
-            paged_load_v<HD, F16, KT>(u, t, tile(i, t), rl, kq);
-            h |= (uint32_t)pages[t] < (uint32_t)a.n_pages ? 1u << t : 0u;
-        }
-        look(i + 1);
+        for (int t = 0; t < KT; t++) paged_load_v<HD, F16, KT>(u, t, page.kv, slot_of(i) + 16 * t, rl, kq);
     };
-    look(0);
 #pragma unroll
-    for (int s = 0; s < NS; s++) request_k(set[s], s), request_v(set[s], has[s], s);
+    for (int s = 0; s < NS; s++) request_k(set[s], has[s], s), request_v(set[s], s);
 
     RowsQ<HD, NT> q;
-    rows_query<HD, NT, true>(q, in, a.scale);
+    if constexpr (LOW) {
+        if (wave < NT) {
+            RowsQ<HD, 1> mine;
+            rows_query<HD, 1, true>(mine, in, a.scale);
+#pragma unroll
+            for (int c = 0; c < HD / 32; c++) {
+                L.q.high[wave][c][lane] = __builtin_bit_cast(uint4, mine.h[0][c]);
+                L.q.low[wave][c][lane] = __builtin_bit_cast(uint4, mine.l[0][c]);
+            }
+            if (kq == 0) L.q.p2e[wave][rl] = mine.p2e[0];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int qt = 0; qt < NT; qt++) {
+            q.p2e[qt] = L.q.p2e[qt][rl];
+#pragma unroll
+            for (int c = 0; c < HD / 32; c++) q.h[qt][c] = __builtin_bit_cast(ar_h8, L.q.high[qt][c][lane]);
+        }
+    } else {
+        rows_query<HD, NT, true>(q, in, a.scale);
+    }
     // Token t's rows take keys [first(t), last(t)); every row of the workgroup those of [all0, all1).
     auto last = [&](int t) { return sp.end - a.T + t + 1; };
     auto first = [&](int t) { return a.window ? max(0, last(t) - a.window) : 0; };
     const int all1 = last(rows_div(r0, a.g_m)), all0 = first(rows_div(r0 + rows - 1, a.g_m));
-    int from[NT], to[NT];
+    int to[NT];
 #pragma unroll
     for (int qt = 0; qt < NT; qt++) {
         const int t = rows_div(r0 + min(16 * qt + rl, rows - 1), a.g_m);
-        to[qt] = 16 * qt + rl < rows ? last(t) : 0, from[qt] = first(t);
+        to[qt] = 16 * qt + rl < rows ? last(t) : 0;
     }
     auto inside = [&](int key) { return key >= all0 && key + UNIT <= all1; };
     RowsSum<HD, NT> sum;
     rows_clear<HD, NT>(sum);
-    if (LOW && wave == 0) {
-#pragma unroll
-        for (int qt = 0; qt < NT; qt++)
-#pragma unroll
-            for (int c = 0; c < HD / 32; c++) L.low[LOW ? qt : 0][c][lane] = __builtin_bit_cast(uint4, q.l[qt][c]);
-    }
-    if (EDGE) __syncthreads();  // the flag is set, the low planes are there
-    auto low = [&](int qt, int c) { return LOW ? __builtin_bit_cast(ar_h8, L.low[LOW ? qt : 0][c][lane]) : q.l[qt][c]; };
-    auto step = [&](RowsUnit<HD, F16, KT> &u, uint32_t h, int i, auto keys_done) {
-        const bool whole = inside(key_of(i, 0)) && h == (1u << KT) - 1;
+    if (EDGE && !LOW) __syncthreads();  // the flag is set
+    auto low = [&](int qt, int c) { return LOW ? __builtin_bit_cast(ar_h8, L.q.low[LOW ? qt : 0][c][lane]) : q.l[qt][c]; };
+    auto step = [&](RowsUnit<HD, F16, KT> &u, bool h, int i, auto keys_done) {
+        const bool whole = h && inside(key_of(i));
         int kb[KT];
 #pragma unroll
-        for (int t = 0; t < KT; t++) kb[t] = h >> t & 1 ? key_of(i, t) : 0x7fffff00;  // (no page: no row takes its keys)
+        for (int t = 0; t < KT; t++) kb[t] = h ? key_of(i) + 16 * t : 0x7fffff00;  // (no page: no row takes its keys)
         if constexpr (LOW) asm volatile("" ::: "memory");  // (the low planes are read again: registers are what LDS saves)
         if constexpr (EDGE)
             if (!whole && paged_clean<HD, F16, KT>(u)) nonfinite = 1;
@@ -361,7 +385,7 @@ __global__ __launch_bounds__(64 * P::NW, P::HD <= 128 ? 2 : 1) void k_attn_paged
             u, q, low, sum, kb, kq, whole,
             [&](int qt, int key) {
                 const uint32_t x = rows_below(key, to[qt]);
-                return EDGE ? x & ~rows_below(key, from[qt]) : x;
+                return EDGE && a.window ? x & ~rows_below(key, to[qt] - a.window) : x;
             },
             keys_done);
     };
@@ -371,10 +395,10 @@ __global__ __launch_bounds__(64 * P::NW, P::HD <= 128 ? 2 : 1) void k_attn_paged
 #pragma unroll
         for (int s = 0; s < NS; s++) {
             step(set[s], has[s], i + s, [&] {
-                if (NS == 1) request_k(set[s], i + s + NS);
+                if (NS == 1) request_k(set[s], has[s], i + s + NS);
             });
-            if (NS > 1) request_k(set[s], i + s + NS);
-            request_v(set[s], has[s], i + s + NS);
+            if (NS > 1) request_k(set[s], has[s], i + s + NS);
+            request_v(set[s], i + s + NS);
         }
 #pragma unroll
     for (int s = 0; s < NS - 1; s++)
@@ -385,15 +409,9 @@ __global__ __launch_bounds__(64 * P::NW, P::HD <= 128 ? 2 : 1) void k_attn_paged
         const int t = rows_div(r0 + r, a.g_m);
         for (int u = u0; u < u1; u++) {
             const int k0 = sp.first + u * UNIT;
-            bool whole = inside(k0);
-            for (int key = k0; key < k0 + UNIT; key += 16) {
-                const int at = key >> a.lp;
-                if (at >= a.n_table || (uint32_t)table[at] >= (uint32_t)a.n_pages) whole = false;
-            }
-            if (whole) continue;
+            const int page = k0 >> a.lp < a.n_table ? table[k0 >> a.lp] : -1;
+            if ((uint32_t)page >= (uint32_t)a.n_pages || inside(k0)) continue;
             for (int key = max(first(t), k0); key < min(last(t), k0 + UNIT); key++) {
-                const int page = table[key >> a.lp];
-                if ((uint32_t)page >= (uint32_t)a.n_pages) continue;
                 const int64_t slot = (((int64_t)page * a.HKV + kvh) << a.lp) + (key & ((1 << a.lp) - 1));
                 o.x += rows_nonfinite<HD, F16>(a.kv, slot, d), o.y += rows_nonfinite<HD, F16>(a.kv, slot, d + 1);
                 o.z += rows_nonfinite<HD, F16>(a.kv, slot, d + 2), o.w += rows_nonfinite<HD, F16>(a.kv, slot, d + 3);
@@ -490,7 +508,7 @@ static PagedPlan paged_plan(int B, int T, int H, int HKV, int HD, int n_cu) {
     p.blocks = (R + p.rt - 1) / p.rt;
     const int items = B * HKV * p.blocks, slots = (HD <= 128 ? 2 : 1) * n_cu;
     p.fused = items <= 4096 && R <= 16 && 16 * items >= slots;
-    p.nw = !p.fused && HD <= 128 ? 8 : 4;
+    p.nw = p.fused || HD == 256 || (p.nt == 2 && 2 * items >= n_cu) ? 4 : 8;
     p.cap = std::max(2 * B, slots * 4 / p.nw / std::max(1, HKV * p.blocks));
     p.part = align_up((size_t)p.cap * HKV * p.blocks * p.rt * (HD + 4) * sizeof(float), 256);
     p.plan = (size_t)B * sizeof(int2);
@@ -509,6 +527,31 @@ static hipError_t paged_launch(const PagedArgs &a, const PagedPlan &p, hipStream
     hipLaunchKernelGGL(k_paged_merge<P::HD>, dim3((unsigned)((rows + RPW - 1) / RPW)), dim3(256), 0, s, a, rows);
     return hipGetLastError();
 }
+// Forms by the rows and pages: KT the tiles of a unit for one row tile, units ahead as registers allow.
+template <int D, bool F, int KT>
+static hipError_t paged_by_rows(const PagedArgs &a, const PagedPlan &p, hipStream_t s) {
+    constexpr int WIDE = D <= 128 ? 8 : 4, AHEAD = D <= 128 ? 3 : 2;
+    if constexpr (D <= 128) {
+        auto two = [&](auto kt, auto ns) {
+            constexpr int K = decltype(kt)::value, N = decltype(ns)::value;
+            return p.nw == 8 ? paged_launch<PagedForm<D, F, K, 2, N, 8, true, false>>(a, p, s)
+                             : paged_launch<PagedForm<D, F, K, 2, N, 4, true, false>>(a, p, s);
+        };
+        using One = std::integral_constant<int, 1>;
+        using Two = std::integral_constant<int, 2>;
+        if (p.nt == 2) {
+            if constexpr (D == 64) return two(std::integral_constant<int, KT>{}, Two{});
+            else if constexpr (F) return two(One{}, One{});
+            else return a.lp >= 5 ? two(Two{}, One{}) : two(One{}, Two{});
+        }
+    }
+    if (a.T > 1 || a.window) {
+        if (p.fused) return paged_launch<PagedForm<D, F, KT, 1, 2, 4, true, true>>(a, p, s);
+        return paged_launch<PagedForm<D, F, KT, 1, 2, WIDE, true, false>>(a, p, s);
+    }
+    if (p.fused) return paged_launch<PagedForm<D, F, KT, 1, AHEAD, 4, false, true>>(a, p, s);
+    return paged_launch<PagedForm<D, F, KT, 1, AHEAD, WIDE, false, false>>(a, p, s);
+}
 hipError_t launch_attn_paged(const float *q, int B, int T, int H, int HKV, int HD, KvLayer kv, int kv_f16, int n_pages,
                              int page, const int32_t *table, int n_table, const int32_t *n_keys, int window, float scale,
                              void *scratch, int *counters, float *out, int n_cu, hipStream_t s) {
@@ -521,15 +564,9 @@ hipError_t launch_attn_paged(const float *q, int B, int T, int H, int HKV, int H
     return rows_by_shape(HD, kv_f16, [&](auto hd, auto f16) {
         constexpr int D = decltype(hd)::value;
         constexpr bool F = decltype(f16)::value;
-        constexpr int WIDE = D <= 128 ? 8 : 4, AHEAD = D <= 128 ? 3 : 2;
-        if constexpr (D <= 128)
-            if (p.nt == 2) return paged_launch<PagedForm<D, F, 2, D == 128 && F ? 1 : 2, WIDE, true, false>>(a, p, s);
-        if (T > 1 || window) {
-            if (p.fused) return paged_launch<PagedForm<D, F, 1, 2, 4, true, true>>(a, p, s);
-            return paged_launch<PagedForm<D, F, 1, 2, WIDE, true, false>>(a, p, s);
-        }
-        if (p.fused) return paged_launch<PagedForm<D, F, 1, AHEAD, 4, false, true>>(a, p, s);
-        return paged_launch<PagedForm<D, F, 1, AHEAD, WIDE, false, false>>(a, p, s);
+        if constexpr (D == 64)
+            if (page >= 32) return paged_by_rows<D, F, 2>(a, p, s);
+        return paged_by_rows<D, F, 1>(a, p, s);
     });
 }
 
