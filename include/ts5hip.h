@@ -265,8 +265,8 @@ int ts5hip_attn_sparse(ts5hip_ctx *ctx, const float *q, int B, int n_head, int n
 
 /* ts5hip_rope_kv_append into pages: token t (of 1..65535) belongs to position pos_dev[t] (which is its RoPE position too, a
  * row of rope_cs: 0..n_pos - 1) of sequence seq_dev[t] (0..n_seq - 1). A token without a place (padding: -1) is left out,
- * its row of q_out too. No two tokens of a call have one place: what it held then would be parts of both. q_out does not
- * overlap qkv. */
+ * its row of q_out too. No two tokens of a call have one place: what it held then would be parts of both. q_out lies
+ * over none of the inputs and not over the pool. */
 int ts5hip_rope_kv_append_paged(ts5hip_ctx *ctx, const float *qkv, int ntok, const int32_t *seq_dev, const int32_t *pos_dev,
                                 int n_head, int n_head_kv, int head_dim, int n_rot, int neox, const float *rope_cs,
                                 int n_pos, const float *bias, const float *q_norm, const float *k_norm, float eps,
@@ -274,7 +274,7 @@ int ts5hip_rope_kv_append_paged(ts5hip_ctx *ctx, const float *qkv, int ntok, con
                                 const int32_t *table_dev, int n_seq, int n_table);
 /* The cached K and V of ntok (1..2^24) tokens, token t position pos_dev[t] of sequence seq_dev[t], as the values they stand
  * for: k_out, v_out [ntok][n_head_kv * head_dim], out_type TS5HIP_F32 (exact) or TS5HIP_F16 (rounded once). Rows of tokens
- * without a place stay as they are. The outputs overlap neither the pool nor each other. */
+ * without a place stay as they are. The outputs lie over no input, not over the pool and not over each other. */
 int ts5hip_kv_read_paged(ts5hip_ctx *ctx, int ntok, const int32_t *seq_dev, const int32_t *pos_dev, int n_head_kv,
                          int head_dim, int kv_type, const void *k, const void *ks, const void *v, const void *vs,
                          int n_pages, int page, const int32_t *table_dev, int n_seq, int n_table, int out_type,
@@ -282,7 +282,7 @@ int ts5hip_kv_read_paged(ts5hip_ctx *ctx, int ntok, const int32_t *seq_dev, cons
 /* Attention of the n_new (1..16) newest tokens of each of B (1..4096) sequences over its pages: n_keys_dev[b] counts the
  * sequence's keys, those tokens' included (it is taken into 0..n_table x page), and token t reads keys below L = n_keys_dev[b]
  * - n_new + t + 1; with window > 0 only the last `window` of them. table_dev [B][n_table]; q, out [B][n_new][n_head *
- * head_dim], not overlapping; up to 16 query heads a KV head; B x n_table x page up to 2^34. A query without a key (or whose
+ * head_dim], out over no input and not over the pool; up to 16 query heads a KV head; B x n_table x page up to 2^34. A query without a key (or whose
  * scores are all minus infinity, in fp32) gets zeros; infinities and NaN of keys and values that it does not read do not
  * reach it, of those that it reads they do. */
 int ts5hip_attn_paged(ts5hip_ctx *ctx, const float *q, int B, int n_new, int n_head, int n_head_kv, int head_dim,

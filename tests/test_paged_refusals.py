@@ -32,11 +32,13 @@ OWN = {
     "append": [dict(ntok=0), dict(ntok=65536), dict(n_rot=130), dict(n_rot=63), dict(n_rot=-2), dict(n_pos=0), dict(H=7),
                dict(n_seq=0), dict(q_out=6 * P + 8), dict(qkv=7 * P + 4), dict(bias=P + 4), dict(q_norm=P + 8),
                dict(k_norm=P + 4), dict(cs=P + 8), dict(q_out=7 * P), dict(q_out=7 * P + 3 * 12 * 512 - 16),
-               dict(q_out=7 * P - 3 * 8 * 512 + 16)],
+               dict(q_out=7 * P - 3 * 8 * 512 + 16), dict(q_out=P), dict(q_out=5 * P), dict(q_out=4 * P + 1024)],
     "read": [dict(ntok=0), dict(ntok=(1 << 24) + 1), dict(n_seq=0), dict(out_type=2), dict(out_type=-1), dict(k_out=6 * P + 8),
-             dict(v_out=6 * P), dict(v_out=6 * P + 3 * 2 * 512 - 16), dict(k_out=P), dict(v_out=2 * P), dict(k_out=4 * P + 1024)],
+             dict(v_out=6 * P), dict(v_out=6 * P + 3 * 2 * 512 - 16), dict(k_out=P), dict(v_out=2 * P), dict(k_out=4 * P + 1024),
+             dict(v_out=5 * P)],
     "attn": [dict(B=0), dict(B=4097), dict(n_new=0), dict(n_new=17), dict(H=7), dict(H=34), dict(window=-1), dict(q=6 * P + 4),
-             dict(out=7 * P + 8), dict(out=6 * P), dict(out=6 * P + 2 * 8 * 512 - 16), dict(B=4096, n_table=1 << 17)],
+             dict(out=7 * P + 8), dict(out=6 * P), dict(out=6 * P + 2 * 8 * 512 - 16), dict(B=4096, n_table=1 << 17),
+             dict(out=P), dict(out=3 * P + 1024), dict(out=4 * P), dict(out=5 * P)],
     "verify": [dict(V=0), dict(V=(1 << 20) + 1, ld=1 << 21, ld_draft=1 << 21), dict(ld=999), dict(ld_draft=999), dict(B=0),
                dict(B=4097), dict(T=-1), dict(T=64), dict(ld=1 << 41), dict(tokens=3 * P), dict(tokens=P), dict(n_tokens=4 * P),
                dict(n_tokens=7 * P + 4), dict(logp=7 * P), dict(logp=6 * P + 8), dict(tokens=P + 4 * (2 * 6 * 1000 - 1)),

@@ -4,7 +4,16 @@
 // Row (t, head) of sequence b takes keys max(0, L - window) .. L - 1, L = n_keys[b] - T + t + 1. The lengths are in
 // device memory and may differ a hundredfold, so every workgroup computes the same plan from them: the shortest
 // slice length L (in units of the core's keys) for which all sequences' slices together fit the launch's workgroups. A
-// workgroup has one slice of one sequence and KV head and up to 16 rows; slices join through partials.
+// workgroup has one slice of one sequence and KV head and up to 32 rows; slices join through partials.
+//
+// What bounds it: f16 caches memory (16 sequences of 16384 keys, 32/8 heads of 128: 188 us, 5.7 TB/s). q8 caches the vector
+// unit, which turns int8 into fp16 planes: 52 % of the busy cycles, the matrix cores another 28 % (the same sequences 121 us,
+// 4.7 TB/s; a contiguous cache 127). Several tokens the same (8 sequences of 8192, 6 tokens, 40/8 heads 47 us, once all is
+// read 29). Few or short sequences a chain of latencies, 7 us for one key: the lengths, the plan, the table, the keys, the
+// partials, the join.
+//
+// A wave has one unit in registers and requests the next one's keys once it has used this one's, and its values once it is
+// done: with two or three units ahead nothing was faster (T = 1) and some 10 % slower.
 #include <algorithm>
 
 #include "attn_rows.h"
@@ -97,6 +106,9 @@ __device__ inline PagedSlice paged_slice(const PagedArgs &a, int j) {
     return s;
 }
 
+// A sequence's row of the table, which nothing writes while the kernel runs.
+typedef const __attribute__((address_space(4))) int32_t *PagedTable;
+
 // The page that a unit is in, as bounded buffers: what is past the sequence's keys reads zeros, and without a page
 // all of it. `id` is the next page's, on its way.
 template <int HD, bool F16>
@@ -104,8 +116,9 @@ struct PagedPage {
     RowsKv kv;
     int at, id;
     bool has;
-    // The page of index `to` comes next.
-    __device__ void look(const PagedArgs &a, const int32_t *table, int to) { id = table[min(to, a.n_table - 1)]; }
+    // The page of index `to` comes next. (A scalar load: as a vector load its value, wanted as a scalar, was waited for at
+    // once, and with it every key and value on their way.)
+    __device__ void look(const PagedArgs &a, PagedTable table, int to) { id = table[min(to, a.n_table - 1)]; }
     __device__ void turn(const PagedArgs &a, int kvh, int end, int to) {
         at = to, has = to < a.n_table && (uint32_t)id < (uint32_t)a.n_pages;
         // (readfirstlane: the compiler takes min and max as one vector instruction, and then each load as a loop over lanes
@@ -114,24 +127,55 @@ struct PagedPage {
         kv = rows_kv<HD, F16>(a.kv, ((int64_t)(has ? id : 0) * a.HKV + kvh) << a.lp, has ? n : 0);
     }
 };
-// Tile t of a unit, `slot` keys into its page (or past all pages: zeros).
+// The lane's byte offsets in a unit's keys, values and their scales.
 template <int HD, bool F16, int KT>
-__device__ inline void paged_load_k(RowsUnit<HD, F16, KT> &u, int t, const RowsKv &kv, uint32_t slot, int rl, int kq) {
+struct PagedLane {
     using S = RowsShape<HD, F16, KT>;
-    const uint32_t k0 = (slot + rl) * (HD * S::VB) + 8 * kq * S::VB;
+    uint32_t k, v, ks, vs;
+    __device__ PagedLane(int rl, int kq) {
+        k = (rl * HD + 8 * kq) * S::VB, v = (4 * kq * HD + S::NDT * rl) * S::VB;
+        ks = 4 * kq * (S::NC * 2), vs = ks + rl * S::NDT / 32 * 2;
+    }
+    // `x` as a sum of its own: the loads' distances from it are the instructions' then, where the compiler, which sees
+    // disjoint bits, takes an instruction and a register for each.
+    __device__ static uint32_t at(uint32_t lane, uint32_t x) {
+        x += lane;
+        asm("" : "+v"(x));
+        return x;
+    }
+};
+// A unit's keys and values, `slot` keys into its page (or past all pages: zeros).
+template <int HD, bool F16, int KT>
+__device__ inline void paged_load_k(RowsUnit<HD, F16, KT> &u, const RowsKv &kv, uint32_t slot, const PagedLane<HD, F16, KT> &l) {
+    using S = RowsShape<HD, F16, KT>;
+    const uint32_t k0 = l.at(l.k, slot * (HD * S::VB)), s0 = l.at(l.ks, slot * (S::NC * 2));
 #pragma unroll
-    for (int c = 0; c < S::NC; c++) rows_words<S::KW>(kv.k, k0 + 32 * c * S::VB, u.k[t][c]);
-    if constexpr (!F16) rows_words<2 * S::NC>(kv.ks, (slot + 4 * kq) * (S::NC * 2), u.ks[t]);
+    for (int t = 0; t < KT; t++) {
+#pragma unroll
+        for (int c = 0; c < S::NC; c++) rows_words<S::KW>(kv.k, k0 + (16 * t * HD + 32 * c) * S::VB, u.k[t][c]);
+        if constexpr (!F16) rows_words<2 * S::NC>(kv.ks, s0 + 16 * t * (S::NC * 2), u.ks[t]);
+    }
 }
 template <int HD, bool F16, int KT>
-__device__ inline void paged_load_v(RowsUnit<HD, F16, KT> &u, int t, const RowsKv &kv, uint32_t slot, int rl, int kq) {
+__device__ inline void paged_load_v(RowsUnit<HD, F16, KT> &u, const RowsKv &kv, uint32_t slot, const PagedLane<HD, F16, KT> &l) {
     using S = RowsShape<HD, F16, KT>;
-    const uint32_t v0 = ((slot + 4 * kq) * HD + S::NDT * rl) * S::VB, s0 = (slot + 4 * kq) * (S::NC * 2) + rl * S::NDT / 32 * 2;
+    const uint32_t v0 = l.at(l.v, slot * (HD * S::VB)), s0 = l.at(l.vs, slot * (S::NC * 2));
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        rows_words<S::VW>(kv.v, v0 + i * HD * S::VB, u.v[t][i]);
-        if constexpr (!F16) u.vs[t][i] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(kv.vs, s0 + i * S::NC * 2, 0, 0);
-    }
+    for (int t = 0; t < KT; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            rows_words<S::VW>(kv.v, v0 + (16 * t + i) * HD * S::VB, u.v[t][i]);
+            if constexpr (!F16)
+                u.vs[t][i] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(kv.vs, s0 + (16 * t + i) * (S::NC * 2), 0, 0);
+        }
+}
+
+// A value's scale where it is used. (Opaque to the compiler, which otherwise packs two scales into a register where they are
+// loaded, and so waits at the loop's end for the unit that it has just requested.)
+__device__ inline uint32_t paged_scale(uint16_t s) {
+    uint32_t x = s;
+    asm("" : "+v"(x));
+    return x;
 }
 
 // Infinite and NaN values of a unit (as the products see them: fp16's range) replaced by zeros: the product with a row
@@ -144,7 +188,8 @@ __device__ inline bool paged_clean(RowsUnit<HD, F16, KT> &u) {
     for (int t = 0; t < KT; t++)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const _Float16 sc = __builtin_bit_cast(_Float16, F16 ? (uint16_t)0 : u.vs[t][i]);
+            const uint16_t scale = F16 ? 0 : (uint16_t)paged_scale(u.vs[t][i]);
+            const _Float16 sc = __builtin_bit_cast(_Float16, scale);
 #pragma unroll
             for (int w = 0; w < S::VW; w++) {
                 uint32_t x = u.v[t][i][w], out = 0;
@@ -159,17 +204,39 @@ __device__ inline bool paged_clean(RowsUnit<HD, F16, KT> &u) {
                 }
                 any |= out, u.v[t][i][w] = x & ~out;
             }
-            if constexpr (!F16) u.vs[t][i] = (u.vs[t][i] & 0x7c00) == 0x7c00 ? 0 : u.vs[t][i];
+            if constexpr (!F16) u.vs[t][i] = (scale & 0x7c00) == 0x7c00 ? 0 : scale;
         }
     return __builtin_amdgcn_ballot_w64(any != 0) != 0;
 }
 
+// rows_value_tile with q8's pairs of keys from two dims a permutation: 6 instructions for 4 dims of both, not 8.
+template <int HD, bool F16, int KT>
+__device__ inline void paged_value_tile(const RowsUnit<HD, F16, KT> &u, const RowsScale<HD, F16, KT> &sc, int dt,
+                                        uint32_t (&hi)[2 * KT], uint32_t (&lo)[2 * KT]) {
+    if constexpr (F16) {
+        rows_value_tile<HD, F16, KT>(u, sc, dt, hi, lo);
+    } else {
+        const ar_h2 k1152 = {(_Float16)1152.0f, (_Float16)1152.0f};
+#pragma unroll
+        for (int t = 0; t < KT; t++)
+#pragma unroll
+            for (int p = 0; p < 2; p++) {
+                const uint32_t both = __builtin_amdgcn_perm(u.v[t][2 * p + 1][dt / 4], u.v[t][2 * p][dt / 4],
+                                                            dt & 2 ? 0x07030602u : 0x05010400u) ^ 0x80808080u;
+                const uint32_t b = __builtin_amdgcn_perm(0x64646464u, both, dt & 1 ? 0x04030402u : 0x04010400u);
+                const ar_h2 v = __builtin_bit_cast(ar_h2, b) - k1152, h = v * sc.s[t][p];
+                hi[2 * t + p] = __builtin_bit_cast(uint32_t, h);
+                lo[2 * t + p] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(v, sc.s[t][p], -h));
+            }
+    }
+}
+
 // One unit into the sums of NT row tiles, its keys and values converted once. Without `whole`, seen(qt, key) has a bit for each of
 // keys key .. + 3 that the lane's row of tile qt takes. keys_done() comes where the unit's keys are used up.
-// low(qt, c) is the low plane of chunk c of row tile qt.
-template <int HD, bool F16, int KT, int NT, class Low, class Seen, class Done>
-__device__ inline void paged_unit(const RowsUnit<HD, F16, KT> &u, const RowsQ<HD, NT> &q, Low low, RowsSum<HD, NT> &a,
-                                  const int (&kb)[KT], int kq, bool whole, Seen seen, Done keys_done) {
+// high(qt, c) and low(qt, c) are the planes of chunk c of row tile qt.
+template <int HD, bool F16, int KT, int NT, class High, class Low, class Seen, class Done>
+__device__ inline void paged_unit(const RowsUnit<HD, F16, KT> &u, const float (&p2e)[NT], High high, Low low,
+                                  RowsSum<HD, NT> &a, const int (&kb)[KT], int kq, bool whole, Seen seen, Done keys_done) {
     using S = RowsShape<HD, F16, KT>;
     using Op = RowsOp<KT>;
     float s[NT][KT][4];
@@ -186,7 +253,7 @@ __device__ inline void paged_unit(const RowsUnit<HD, F16, KT> &u, const RowsQ<HD
 #pragma unroll
             for (int qt = 0; qt < NT; qt++) {
                 if (!F16 || c == 0) R[qt] = ar_f4{0.f, 0.f, 0.f, 0.f};
-                R[qt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q.h[qt][c], R[qt], 0, 0, 0);
+                R[qt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, high(qt, c), R[qt], 0, 0, 0);
             }
 #pragma unroll
             for (int qt = 0; qt < NT; qt++) R[qt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, low(qt, c), R[qt], 0, 0, 0);
@@ -219,15 +286,15 @@ __device__ inline void paged_unit(const RowsUnit<HD, F16, KT> &u, const RowsQ<HD
         for (int t = 0; t < KT; t++)
 #pragma unroll
             for (int i = 0; i < 4; i++) mx = fmaxf(mx, s[qt][t][i]);
-        const float m0 = rows_reference(a, qt, max_xor32(max_xor16(mx)) * q.p2e[qt]);
+        const float m0 = rows_reference(a, qt, max_xor32(max_xor16(mx)) * p2e[qt]);
         float sum = 0.f;
         uint32_t hi[2 * KT], lo[2 * KT];
 #pragma unroll
         for (int t = 0; t < KT; t++)
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const float p0 = __builtin_amdgcn_exp2f(fmaf(s[qt][t][2 * i], q.p2e[qt], -m0));
-                const float p1 = __builtin_amdgcn_exp2f(fmaf(s[qt][t][2 * i + 1], q.p2e[qt], -m0));
+                const float p0 = __builtin_amdgcn_exp2f(fmaf(s[qt][t][2 * i], p2e[qt], -m0));
+                const float p1 = __builtin_amdgcn_exp2f(fmaf(s[qt][t][2 * i + 1], p2e[qt], -m0));
                 sum += p0 + p1;
                 rows_split(p0, p1, hi[2 * t + i], lo[2 * t + i]);
             }
@@ -240,12 +307,12 @@ __device__ inline void paged_unit(const RowsUnit<HD, F16, KT> &u, const RowsQ<HD
         for (int t = 0; t < KT; t++)
 #pragma unroll
             for (int p = 0; p < 2; p++)
-                sc.s[t][p] = __builtin_bit_cast(ar_h2, (uint32_t)u.vs[t][2 * p] | (uint32_t)u.vs[t][2 * p + 1] << 16);
+                sc.s[t][p] = __builtin_bit_cast(ar_h2, paged_scale(u.vs[t][2 * p]) | paged_scale(u.vs[t][2 * p + 1]) << 16);
     }
 #pragma unroll
     for (int dt = 0; dt < S::NDT; dt++) {
         uint32_t hi[2 * KT], lo[2 * KT];
-        rows_value_tile<HD, F16, KT>(u, sc, dt, hi, lo);
+        paged_value_tile<HD, F16, KT>(u, sc, dt, hi, lo);
         const typename Op::T vh = Op::of(hi), vl = Op::of(lo);
 #pragma unroll
         for (int qt = 0; qt < NT; qt++) a.o[qt][dt] = Op::mfma(vh, ph[qt], a.o[qt][dt]);
@@ -264,13 +331,11 @@ __device__ inline float *paged_out(const PagedArgs &a, int b, int kvh, int r) {
     return a.out + (((int64_t)b * a.T + t) * a.H + kvh * a.G + r - t * a.G) * HD;
 }
 
-// What a kernel is made for: KT tiles of keys a unit (which does not end past a page), NT row tiles a wave, NS units in its registers (one used, the others on their way; with one,
-// the next one's keys are requested once its keys are used and its values once all is), EDGE: rows that do not take the
-// same keys (several tokens, a window).
-// FUSED: the last of a sequence's slices joins them.
-template <int HD_, bool F16_, int KT_, int NT_, int NS_, int NW_, bool EDGE_, bool FUSED_>
+// What a kernel is made for: KT tiles of keys a unit (which does not end past a page), NT row tiles a wave, NW waves, EDGE:
+// rows that do not take the same keys (several tokens, a window), FUSED: the last of a sequence's slices joins them.
+template <int HD_, bool F16_, int KT_, int NT_, int NW_, bool EDGE_, bool FUSED_>
 struct PagedForm {
-    static constexpr int HD = HD_, KT = KT_, NT = NT_, NS = NS_, NW = NW_, UNIT = 16 * KT, LEAST = 8 / KT < NW ? NW : 8 / KT;
+    static constexpr int HD = HD_, KT = KT_, NT = NT_, NW = NW_, UNIT = 16 * KT, LEAST = 8 / KT < NW ? NW : 8 / KT;
     static constexpr bool F16 = F16_, EDGE = EDGE_, FUSED = FUSED_;
 };
 
@@ -278,8 +343,12 @@ struct PagedForm {
 // in turn.
 template <class P>
 __global__ __launch_bounds__(64 * P::NW, P::HD <= 128 ? 2 : 1) void k_attn_paged(PagedArgs a) {
-    constexpr int HD = P::HD, NT = P::NT, NS = P::NS, KT = P::KT, NW = P::NW, UNIT = P::UNIT;
-    constexpr bool F16 = P::F16, EDGE = P::EDGE, FUSED = P::FUSED, LOW = NT > 1;  // LOW: the rows' planes go through LDS, and the low ones stay there
+    constexpr int HD = P::HD, NT = P::NT, KT = P::KT, NW = P::NW, UNIT = P::UNIT;
+    constexpr bool F16 = P::F16, EDGE = P::EDGE, FUSED = P::FUSED;
+    // LOW: the rows' planes go through LDS, where the low ones stay. HIGH: the high ones' chunks in registers: as many as do
+    // not spill.
+    constexpr bool LOW = NT > 1;
+    constexpr int HIGH = LOW && !F16 && HD == 128 && KT == 2 ? 3 : HD / 32;
     __shared__ union {
         struct {
             uint4 high[LOW ? NT : 1][HD / 32][64], low[LOW ? NT : 1][HD / 32][64];
@@ -312,29 +381,25 @@ __global__ __launch_bounds__(64 * P::NW, P::HD <= 128 ? 2 : 1) void k_attn_paged
     if (!FUSED && kvh == 0 && blockIdx.y == 0 && sl.at == 0 && threadIdx.x == 0) a.plan[b] = make_int2(j, sl.used);
 
     // The wave's i-th unit, of a stretch of its own; its page is looked up one unit before.
-    const int32_t *table = a.table + (int64_t)b * a.n_table;
+    const PagedTable table = (PagedTable)(uintptr_t)(a.table + (int64_t)b * a.n_table);
     const int share = sl.per / NW, w0 = u0 + wave * share, mine = max(0, min(share, u1 - w0));
     auto key_of = [&](int i) { return sp.first + (w0 + i) * UNIT; };
     PagedPage<HD, F16> page;
     page.at = -1, page.look(a, table, key_of(0) >> a.lp);
-    RowsUnit<HD, F16, KT> set[NS];
-    bool has[NS];  // the unit has a page
+    RowsUnit<HD, F16, KT> u;
+    const PagedLane<HD, F16, KT> lanes(rl, kq);
+    bool has;  // the unit has a page
     auto slot_of = [&](int i) { return i < mine ? (uint32_t)(key_of(i) & ((1 << a.lp) - 1)) : 1u << 20; };
-    auto request_k = [&](RowsUnit<HD, F16, KT> &u, bool &h, int i) {
+    auto request_k = [&](int i) {
         const int to = key_of(i) >> a.lp;
         if (to != page.at) page.turn(a, kvh, sp.end, to);
-        h = page.has;
+        has = page.has;
         const int next = key_of(i + 1) >> a.lp;
         if (next != to) page.look(a, table, next);
-#pragma unroll
-        for (int t = 0; t < KT; t++) paged_load_k<HD, F16, KT>(u, t, page.kv, slot_of(i) + 16 * t, rl, kq);
+        paged_load_k<HD, F16, KT>(u, page.kv, slot_of(i), lanes);
     };
-    auto request_v = [&](RowsUnit<HD, F16, KT> &u, int i) {
-#pragma unroll
-        for (int t = 0; t < KT; t++) paged_load_v<HD, F16, KT>(u, t, page.kv, slot_of(i) + 16 * t, rl, kq);
-    };
-#pragma unroll
-    for (int s = 0; s < NS; s++) request_k(set[s], has[s], s), request_v(set[s], s);
+    auto request_v = [&](int i) { paged_load_v<HD, F16, KT>(u, page.kv, slot_of(i), lanes); };
+    request_k(0), request_v(0);
 
     RowsQ<HD, NT> q;
     if constexpr (LOW) {
@@ -353,7 +418,7 @@ __global__ __launch_bounds__(64 * P::NW, P::HD <= 128 ? 2 : 1) void k_attn_paged
         for (int qt = 0; qt < NT; qt++) {
             q.p2e[qt] = L.q.p2e[qt][rl];
 #pragma unroll
-            for (int c = 0; c < HD / 32; c++) q.h[qt][c] = __builtin_bit_cast(ar_h8, L.q.high[qt][c][lane]);
+            for (int c = 0; c < HIGH; c++) q.h[qt][c] = __builtin_bit_cast(ar_h8, L.q.high[qt][c][lane]);
         }
     } else {
         rows_query<HD, NT, true>(q, in, a.scale);
@@ -372,9 +437,11 @@ __global__ __launch_bounds__(64 * P::NW, P::HD <= 128 ? 2 : 1) void k_attn_paged
     RowsSum<HD, NT> sum;
     rows_clear<HD, NT>(sum);
     if (EDGE && !LOW) __syncthreads();  // the flag is set
+    auto high = [&](int qt, int c) { return c < HIGH ? q.h[qt][c] : __builtin_bit_cast(ar_h8, L.q.high[LOW ? qt : 0][c][lane]); };
     auto low = [&](int qt, int c) { return LOW ? __builtin_bit_cast(ar_h8, L.q.low[LOW ? qt : 0][c][lane]) : q.l[qt][c]; };
-    auto step = [&](RowsUnit<HD, F16, KT> &u, bool h, int i, auto keys_done) {
-        const bool whole = h && inside(key_of(i));
+    // The next unit's keys are requested once this one's are used, its values once all is.
+    for (int i = 0; i < mine; i++) {
+        const bool h = has, whole = h && inside(key_of(i));
         int kb[KT];
 #pragma unroll
         for (int t = 0; t < KT; t++) kb[t] = h ? key_of(i) + 16 * t : 0x7fffff00;  // (no page: no row takes its keys)
@@ -382,27 +449,14 @@ __global__ __launch_bounds__(64 * P::NW, P::HD <= 128 ? 2 : 1) void k_attn_paged
         if constexpr (EDGE)
             if (!whole && paged_clean<HD, F16, KT>(u)) nonfinite = 1;
         paged_unit<HD, F16, KT, NT>(
-            u, q, low, sum, kb, kq, whole,
+            u, q.p2e, high, low, sum, kb, kq, whole,
             [&](int qt, int key) {
                 const uint32_t x = rows_below(key, to[qt]);
                 return EDGE && a.window ? x & ~rows_below(key, to[qt] - a.window) : x;
             },
-            keys_done);
-    };
-    // (no exit between the steps: the waits for one unit's loads leave the later ones in flight)
-    int i = 0;
-    for (; i + NS <= mine; i += NS)
-#pragma unroll
-        for (int s = 0; s < NS; s++) {
-            step(set[s], has[s], i + s, [&] {
-                if (NS == 1) request_k(set[s], has[s], i + s + NS);
-            });
-            if (NS > 1) request_k(set[s], has[s], i + s + NS);
-            request_v(set[s], i + s + NS);
-        }
-#pragma unroll
-    for (int s = 0; s < NS - 1; s++)
-        if (i + s < mine) step(set[s], has[s], i + s, [] {});
+            [&] { request_k(i + 1); });
+        request_v(i + 1);
+    }
 
     // The infinite and NaN values that were left out, of the keys that row r takes.
     auto add_nonfinite = [&](int r, int d, float4 &o) {
@@ -444,34 +498,34 @@ __global__ __launch_bounds__(64 * P::NW, P::HD <= 128 ? 2 : 1) void k_attn_paged
         });
     }
     if constexpr (FUSED) {
-    if (sl.used == 1) return;
-    __shared__ int is_last;
-    wait_stores();
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        int *c = a.counters + ((b * a.HKV + kvh) * gridDim.y + blockIdx.y) * CTR_STRIDE;
-        is_last = atomicAdd(c, 1) == sl.used - 1;
-        if (is_last) st_dev(c, 0);
-    }
-    __syncthreads();
-    if (!is_last) return;
-    static_assert(64 * NW == 256, "rows_join's threads");
-    auto join = [&](auto sg) {  // rows at a time: few slices leave each to a quarter of the threads
-        constexpr int SG = decltype(sg)::value, TPR = HD / 4 * SG;
-        for (int g0 = 0; g0 < rows; g0 += 256 / TPR) {
-            const int g = g0 + (int)threadIdx.x / TPR;
-            float M, l;
-            const float4 o = rows_join<HD, SG>(L.join, sl.used, M, l, [&](int s, int d, float2 &ml, float4 &x) {
-                const uint32_t at = (uint32_t)s * stride + (uint32_t)min(g, rows - 1) * (HD + 4) * 4;
-                ml = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(part, at, 0, BUF_SC1));
-                x = __builtin_bit_cast(float4, __builtin_amdgcn_raw_buffer_load_b128(part, at + 16 + 4 * d, 0, BUF_SC1));
-            });
-            if (g < rows && threadIdx.x % TPR < HD / 4)
-                *(float4 *)(paged_out<HD>(a, b, kvh, r0 + g) + 4 * (threadIdx.x % TPR)) = rows_over(o, l);
+        if (sl.used == 1) return;
+        __shared__ int is_last;
+        wait_stores();
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            int *c = a.counters + ((b * a.HKV + kvh) * gridDim.y + blockIdx.y) * CTR_STRIDE;
+            is_last = atomicAdd(c, 1) == sl.used - 1;
+            if (is_last) st_dev(c, 0);
         }
-    };
-    if (sl.used <= 8) join(std::integral_constant<int, 1>{});
-    else join(std::integral_constant<int, JOIN_SG>{});
+        __syncthreads();
+        if (!is_last) return;
+        static_assert(64 * NW == 256, "rows_join's threads");
+        auto join = [&](auto sg) {  // rows at a time: few slices leave each to a quarter of the threads
+            constexpr int SG = decltype(sg)::value, TPR = HD / 4 * SG;
+            for (int g0 = 0; g0 < rows; g0 += 256 / TPR) {
+                const int g = g0 + (int)threadIdx.x / TPR;
+                float M, l;
+                const float4 o = rows_join<HD, SG>(L.join, sl.used, M, l, [&](int s, int d, float2 &ml, float4 &x) {
+                    const uint32_t at = (uint32_t)s * stride + (uint32_t)min(g, rows - 1) * (HD + 4) * 4;
+                    ml = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(part, at, 0, BUF_SC1));
+                    x = __builtin_bit_cast(float4, __builtin_amdgcn_raw_buffer_load_b128(part, at + 16 + 4 * d, 0, BUF_SC1));
+                });
+                if (g < rows && threadIdx.x % TPR < HD / 4)
+                    *(float4 *)(paged_out<HD>(a, b, kvh, r0 + g) + 4 * (threadIdx.x % TPR)) = rows_over(o, l);
+            }
+        };
+        if (sl.used <= 8) join(std::integral_constant<int, 1>{});
+        else join(std::integral_constant<int, JOIN_SG>{});
     }
 }
 
@@ -503,11 +557,15 @@ struct PagedPlan {
 static PagedPlan paged_plan(int B, int T, int H, int HKV, int HD, int n_cu) {
     PagedPlan p;
     const int R = T * (H / HKV);
-    p.nt = R > 16 && HD <= 128 ? 2 : 1;
+    p.nt = R > 16 && HD <= 128 ? 2 : 1;  // (two share the keys' and values' conversions; heads of 256 have no registers for it)
     p.rt = std::min(R, 16 * p.nt);
     p.blocks = (R + p.rt - 1) / p.rt;
     const int items = B * HKV * p.blocks, slots = (HD <= 128 ? 2 : 1) * n_cu;
-    p.fused = items <= 4096 && R <= 16 && 16 * items >= slots;
+    // With few slices an item the last one joins them: a launch less (64 x 128 keys 8 us against 13, 24 ragged sequences 63
+    // against 83). With many one workgroup's join is the longer way (1 x 32768 keys 28.6 us against 23, 4 x 4096 17.3 against 16).
+    p.fused = items <= 4096 && R <= 16 && 8 * items >= slots;
+    // Few items want eight waves, which halve the slices to join (1 x 8192 keys, 6 tokens: 19 us, with four 23; 1 x 700 of them
+    // 16 against 13); with many items their long slices no longer even out (24 ragged sequences, 6 tokens: 107 against 81).
     p.nw = p.fused || HD == 256 || (p.nt == 2 && 2 * items >= n_cu) ? 4 : 8;
     p.cap = std::max(2 * B, slots * 4 / p.nw / std::max(1, HKV * p.blocks));
     p.part = align_up((size_t)p.cap * HKV * p.blocks * p.rt * (HD + 4) * sizeof(float), 256);
@@ -527,30 +585,28 @@ static hipError_t paged_launch(const PagedArgs &a, const PagedPlan &p, hipStream
     hipLaunchKernelGGL(k_paged_merge<P::HD>, dim3((unsigned)((rows + RPW - 1) / RPW)), dim3(256), 0, s, a, rows);
     return hipGetLastError();
 }
-// Forms by the rows and pages: KT the tiles of a unit for one row tile, units ahead as registers allow.
+// Two row tiles of q8 heads of 128 take 32 keys a unit if pages allow: half the value products' instructions (24 ragged
+// sequences, 6 tokens: 81 us against 90; 1 x 8192 19 against 18). One row tile takes 16: 1 x 32768 keys 23.6 against 24.6 us,
+// 8 x 8192 of 4 x 4 rows 36 against 42. Heads of 64 always 32 (24 ragged 17.7 against 18.8).
 template <int D, bool F, int KT>
 static hipError_t paged_by_rows(const PagedArgs &a, const PagedPlan &p, hipStream_t s) {
-    constexpr int WIDE = D <= 128 ? 8 : 4, AHEAD = D <= 128 ? 3 : 2;
-    if constexpr (D <= 128) {
-        auto two = [&](auto kt, auto ns) {
-            constexpr int K = decltype(kt)::value, N = decltype(ns)::value;
-            return p.nw == 8 ? paged_launch<PagedForm<D, F, K, 2, N, 8, true, false>>(a, p, s)
-                             : paged_launch<PagedForm<D, F, K, 2, N, 4, true, false>>(a, p, s);
-        };
-        using One = std::integral_constant<int, 1>;
-        using Two = std::integral_constant<int, 2>;
+    constexpr int WIDE = D <= 128 ? 8 : 4;
+    if constexpr (D <= 128)
         if (p.nt == 2) {
-            if constexpr (D == 64) return two(std::integral_constant<int, KT>{}, Two{});
-            else if constexpr (F) return two(One{}, One{});
-            else return a.lp >= 5 ? two(Two{}, One{}) : two(One{}, Two{});
+            if constexpr (D == 128 && !F)
+                if (a.lp >= 5) {
+                    if (p.nw == 8) return paged_launch<PagedForm<D, F, 2, 2, 8, true, false>>(a, p, s);
+                    return paged_launch<PagedForm<D, F, 2, 2, 4, true, false>>(a, p, s);
+                }
+            if (p.nw == 8) return paged_launch<PagedForm<D, F, KT, 2, 8, true, false>>(a, p, s);
+            return paged_launch<PagedForm<D, F, KT, 2, 4, true, false>>(a, p, s);
         }
-    }
     if (a.T > 1 || a.window) {
-        if (p.fused) return paged_launch<PagedForm<D, F, KT, 1, 2, 4, true, true>>(a, p, s);
-        return paged_launch<PagedForm<D, F, KT, 1, 2, WIDE, true, false>>(a, p, s);
+        if (p.fused) return paged_launch<PagedForm<D, F, KT, 1, 4, true, true>>(a, p, s);
+        return paged_launch<PagedForm<D, F, KT, 1, WIDE, true, false>>(a, p, s);
     }
-    if (p.fused) return paged_launch<PagedForm<D, F, KT, 1, AHEAD, 4, false, true>>(a, p, s);
-    return paged_launch<PagedForm<D, F, KT, 1, AHEAD, WIDE, false, false>>(a, p, s);
+    if (p.fused) return paged_launch<PagedForm<D, F, KT, 1, 4, false, true>>(a, p, s);
+    return paged_launch<PagedForm<D, F, KT, 1, WIDE, false, false>>(a, p, s);
 }
 hipError_t launch_attn_paged(const float *q, int B, int T, int H, int HKV, int HD, KvLayer kv, int kv_f16, int n_pages,
                              int page, const int32_t *table, int n_table, const int32_t *n_keys, int window, float scale,

@@ -291,7 +291,12 @@ int ts5hip_rope_kv_append_paged(ts5hip_ctx *ctx, const float *qkv, int ntok, con
         !aligned(rope_cs, 16))
         return fail(ctx, TS5HIP_ERR_ARG, "q, k, v, biases, norms and angles need 16-byte alignment");
     const size_t heads = (size_t)ntok * head_dim * 4;
-    if (int rc = check_apart(ctx, {{q_out, heads * n_head}}, {{qkv, heads * (n_head + 2 * n_head_kv)}})) return rc;
+    const size_t pool = pool_values(n_pages, page, n_head_kv, head_dim, kv_type);
+    const size_t scales = kv_type == KV_Q8 ? pool_scales(n_pages, page, n_head_kv, head_dim) : 0;
+    if (int rc = check_apart(ctx, {{q_out, heads * n_head}},
+                             {{qkv, heads * (n_head + 2 * n_head_kv)}, {k, pool}, {v, pool}, {ks, scales}, {vs, scales},
+                              {table_dev, (size_t)n_seq * n_table * 4}, {seq_dev, (size_t)ntok * 4}, {pos_dev, (size_t)ntok * 4}}))
+        return rc;
     if (!ctx) return fail(nullptr, TS5HIP_ERR_ARG, "ctx is null");
     const OnDevice on(ctx->device);
     TS5_HIP(ctx, launch_append_paged(qkv, ntok, seq_dev, pos_dev, n_head, n_head_kv, head_dim, bias, q_norm, k_norm, eps,
@@ -314,7 +319,10 @@ int ts5hip_kv_read_paged(ts5hip_ctx *ctx, int ntok, const int32_t *seq_dev, cons
     const size_t rows = (size_t)ntok * n_head_kv * head_dim * (out_type == TS5HIP_F32 ? 4 : 2);
     const size_t pool = pool_values(n_pages, page, n_head_kv, head_dim, kv_type);
     const size_t scales = kv_type == KV_Q8 ? pool_scales(n_pages, page, n_head_kv, head_dim) : 0;
-    if (int rc = check_apart(ctx, {{k_out, rows}, {v_out, rows}}, {{k, pool}, {v, pool}, {ks, scales}, {vs, scales}})) return rc;
+    if (int rc = check_apart(ctx, {{k_out, rows}, {v_out, rows}}, {{k, pool}, {v, pool}, {ks, scales}, {vs, scales},
+                                                                  {table_dev, (size_t)n_seq * n_table * 4},
+                                                                  {seq_dev, (size_t)ntok * 4}, {pos_dev, (size_t)ntok * 4}}))
+        return rc;
     if (!ctx) return fail(nullptr, TS5HIP_ERR_ARG, "ctx is null");
     const OnDevice on(ctx->device);
     TS5_HIP(ctx, launch_read_paged(ntok, seq_dev, pos_dev, n_head_kv, head_dim, layer(k, ks, v, vs), kv_type == KV_F16,
@@ -336,7 +344,11 @@ int ts5hip_attn_paged(ts5hip_ctx *ctx, const float *q, int B, int n_new, int n_h
         return fail(ctx, TS5HIP_ERR_ARG, "%d new tokens (1..%d), window %d", n_new, ATTN_MAX_NEW, window);
     if (!aligned(q, 16) || !aligned(out, 16)) return fail(ctx, TS5HIP_ERR_ARG, "q and out need 16-byte alignment");
     const size_t rows = (size_t)B * n_new * n_head * head_dim * 4;
-    if (int rc = check_apart(ctx, {{out, rows}}, {{q, rows}})) return rc;
+    const size_t pool = pool_values(n_pages, page, n_head_kv, head_dim, kv_type);
+    const size_t scales = kv_type == KV_Q8 ? pool_scales(n_pages, page, n_head_kv, head_dim) : 0;
+    if (int rc = check_apart(ctx, {{out, rows}}, {{q, rows}, {k, pool}, {v, pool}, {ks, scales}, {vs, scales},
+                                                  {table_dev, (size_t)B * n_table * 4}, {n_keys_dev, (size_t)B * 4}}))
+        return rc;
     if (!ctx) return fail(nullptr, TS5HIP_ERR_ARG, "ctx is null");
     const OnDevice on(ctx->device);
     if (int rc = ensure_scratch(ctx, attn_paged_scratch_bytes(B, n_new, n_head, n_head_kv, head_dim, ctx->n_cu))) return rc;
