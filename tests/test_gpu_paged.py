@@ -438,6 +438,38 @@ def test_append_as_into_a_contiguous_cache(ctx, kv, H, HKV, HD, neox, bias):
             assert np.array_equal(a[c.table[0, p // 32], :, p % 32], want[:, p]), (m, p)
 
 
+@pytest.mark.parametrize("kv", [Q8, F16])
+@pytest.mark.parametrize("H,HKV,HD,n,n_rot,neox,bias,norms", [
+    (32, 8, 128, 2221, 128, 0, False, False), (40, 8, 128, 1903, 128, 1, True, False), (14, 2, 64, 6659, 64, 1, True, False),
+    (14, 2, 64, 6658, 22, 0, False, True), (8, 4, 256, 3331, 256, 1, False, True), (8, 4, 256, 3329, 0, 0, True, False)])
+def test_append_of_many_tokens(ctx, kv, H, HKV, HD, n, n_rot, neox, bias, norms):
+    """From 13312 workgroups of rows on (6, 7, 2 and 4 of them a token here) a thread takes four tokens: the same bits as in
+    calls of 100 tokens, whatever the count, tokens without a place among them."""
+    rng = np.random.default_rng([31, HD, n, kv])
+    lengths = [n // 2, n - n // 2]
+    c = Pages(ctx, rng, kv, HKV, HD, 64, lengths)
+    seq = np.repeat([0, 1], lengths).astype(np.int32)
+    pos = np.concatenate([np.arange(m) for m in lengths]).astype(np.int32)
+    order = rng.permutation(n)
+    seq, pos = seq[order], pos[order]
+    seq[rng.integers(0, n, 40)] = -1
+    pos[rng.integers(0, n, 40)] = -5
+    width = (H + 2 * HKV) * HD
+    qkv = rng.standard_normal((n, width)).astype(np.float32) * 3
+    cs = rope_angles(max(lengths), n_rot) if n_rot else np.zeros((max(lengths), 2), np.float32)
+    more = dict(bias=rng.standard_normal(width).astype(np.float32) if bias else None,
+                q_norm=(1 + 0.3 * rng.standard_normal(HD)).astype(np.float32) if norms else None,
+                k_norm=(1 + 0.3 * rng.standard_normal(HD)).astype(np.float32) if norms else None)
+    parts = [append(ctx, c, qkv[i:i + 100], seq[i:i + 100], pos[i:i + 100], H, n_rot, neox, cs, **more) for i in range(0, n, 100)]
+    want = c.fetch()
+    for name, b in c.dev.items():
+        b.upload(c.raw[name])
+    got_q = append(ctx, c, qkv, seq, pos, H, n_rot, neox, cs, **more)
+    assert np.array_equal(got_q.view(np.uint32), np.concatenate(parts).view(np.uint32))
+    for name, a in c.fetch().items():
+        assert np.array_equal(a.view(np.uint8), want[name].view(np.uint8)), name
+
+
 # ---- rows back ---------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("kv", [Q8, F16])
