@@ -190,6 +190,31 @@ def test_verify_batches(ctx, kv, H, HKV, HD, T):
 
 
 @pytest.mark.parametrize("kv", [Q8, F16])
+@pytest.mark.parametrize("H,HKV,HD", [(16, 8, 64), (16, 8, 128), (8, 4, 256)])
+@pytest.mark.parametrize("T,page,window", [(1, 16, 0), (1, 64, 0), (1, 32, 50), (1, 16, 300), (2, 16, 0), (3, 64, 41), (9, 16, 0),
+                                           (9, 128, 33), (16, 32, 0)])
+def test_many_items(ctx, kv, H, HKV, HD, T, page, window):
+    """From 64 (heads of 256: 32) pairs of a sequence and a KV head on the last slice joins, and from 128 on two row tiles take
+    four waves: ragged lengths, one of many slices, a page that is missing, infinities and NaN behind the last key."""
+    rng = np.random.default_rng([T, HD, page, kv, window])
+    lengths = [int(x) for x in rng.integers(0, 260, 24)]
+    lengths[5], lengths[11], lengths[20], lengths[23] = 2900, 0, 1, 700
+    c = Pages(ctx, rng, kv, HKV, HD, page, lengths)
+    for b, n in enumerate(lengths):
+        if n % page:
+            at, slot = c.table[b, n // page], n % page
+            for m in "kv":
+                c.raw[m + "s" if kv == Q8 else m][at, :, slot:] = np.inf if b % 2 else np.nan
+    c.table[5, 3], c.table[23, 0] = -1, c.n_pages
+    c.send()
+    q = rng.standard_normal((24, T, H, HD)).astype(np.float32)
+    for again in range(2):  # (the counters are zero again)
+        got = run_attn(ctx, c, q, lengths, window, 0.09, H)
+    check_attn(c, q, lengths, window, 0.09, H, got, (kv, T, page))
+    assert np.all(got[11] == 0)
+
+
+@pytest.mark.parametrize("kv", [Q8, F16])
 def test_counts_outside_the_pages(ctx, kv):
     """Counts in device memory are taken into the table: negative ones as 0, larger ones as all that it holds."""
     rng = np.random.default_rng(7)
