@@ -8,8 +8,8 @@
 //
 // What bounds it: f16 caches memory (16 sequences of 16384 keys, 32/8 heads of 128: 188 us, 5.7 TB/s). q8 caches the vector
 // unit, which turns int8 into fp16 planes: 52 % of the busy cycles, the matrix cores another 28 % (the same sequences 121 us,
-// 4.7 TB/s; a contiguous cache 127). Several tokens the same (8 sequences of 8192, 6 tokens, 40/8 heads 47 us, once all is
-// read 29). Few or short sequences a chain of latencies, 7 us for one key: the lengths, the plan, the table, the keys, the
+// 4.7 TB/s; a contiguous cache 127). Several tokens the same (8 sequences of 8192, 6 tokens, 40/8 heads 47 us; the bytes alone
+// 29). Few or short sequences a chain of latencies, 7 us for one key: the lengths, the plan, the table, the keys, the
 // partials, the join.
 //
 // A wave has one unit in registers and requests the next one's keys once it has used this one's, and its values once it is
