@@ -133,7 +133,7 @@ def test_attention(ctx, kv, H, HKV, HD, T, page, lengths, window):
 
 @pytest.mark.parametrize("kv", [Q8, F16])
 @pytest.mark.parametrize("H,HKV,HD,page,n", [(8, 2, 128, 64, 9001), (14, 2, 64, 256, 5000), (2, 1, 256, 16, 3333),
-                                             (16, 1, 128, 128, 4096)])
+                                             (16, 1, 128, 128, 4096), (4, 1, 64, 16, 1500)])
 def test_one_long_sequence(ctx, kv, H, HKV, HD, page, n):
     """Keys over many workgroups, slices that end inside pages, more pages than a wave looks up at once."""
     rng = np.random.default_rng([n, kv])

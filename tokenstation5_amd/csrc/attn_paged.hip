@@ -339,6 +339,13 @@ struct PagedForm {
     static constexpr bool F16 = F16_, EDGE = EDGE_, FUSED = FUSED_;
 };
 
+// RowsJoin of other workgroups.
+template <int THREADS>
+struct PagedJoin {
+    __align__(16) float4 o[THREADS];
+    float2 ml[THREADS];
+};
+
 // grid (cap * HKV, row blocks): one slice of one sequence's keys for up to 16 NT rows of a KV head; the waves take its units
 // in turn.
 template <class P>
@@ -355,7 +362,7 @@ __global__ __launch_bounds__(64 * P::NW, P::HD <= 128 ? 2 : 1) void k_attn_paged
             float p2e[LOW ? NT : 1][16];
         } q;
         RowsLds<HD, NW> parts;
-        RowsJoin join;
+        PagedJoin<64 * NW> join;
     } L;
     __shared__ int nonfinite;  // a unit that not every row takes whole had infinite or NaN values: they are added at the end
     if (EDGE && threadIdx.x == 0) nonfinite = 0;
@@ -509,10 +516,9 @@ __global__ __launch_bounds__(64 * P::NW, P::HD <= 128 ? 2 : 1) void k_attn_paged
         }
         __syncthreads();
         if (!is_last) return;
-        static_assert(64 * NW == 256, "rows_join's threads");
         auto join = [&](auto sg) {  // rows at a time: few slices leave each to a quarter of the threads
             constexpr int SG = decltype(sg)::value, TPR = HD / 4 * SG;
-            for (int g0 = 0; g0 < rows; g0 += 256 / TPR) {
+            for (int g0 = 0; g0 < rows; g0 += 64 * NW / TPR) {
                 const int g = g0 + (int)threadIdx.x / TPR;
                 float M, l;
                 const float4 o = rows_join<HD, SG>(L.join, sl.used, M, l, [&](int s, int d, float2 &ml, float4 &x) {
@@ -561,13 +567,15 @@ static PagedPlan paged_plan(int B, int T, int H, int HKV, int HD, int n_cu) {
     p.rt = std::min(R, 16 * p.nt);
     p.blocks = (R + p.rt - 1) / p.rt;
     const int items = B * HKV * p.blocks, slots = (HD <= 128 ? 2 : 1) * n_cu;
-    // With few slices an item the last one joins them: a launch less (64 x 128 keys 8 us against 13, 24 ragged sequences 63
-    // against 83). With many one workgroup's join is the longer way (1 x 32768 keys 28.6 us against 23, 4 x 4096 17.3 against 16).
-    p.fused = items <= 4096 && R <= 16 && 8 * items >= slots;
-    // Few items want eight waves, which halve the slices to join (1 x 8192 keys, 6 tokens: 19 us, with four 23; 1 x 700 of them
-    // 16 against 13); with many items their long slices no longer even out (24 ragged sequences, 6 tokens: 107 against 81).
-    p.nw = p.fused || HD == 256 || (p.nt == 2 && 2 * items >= n_cu) ? 4 : 8;
+    // Few items want eight waves, which halve the slices to join (4 x 4096 keys 15.5 us against 17; two row tiles of 1 x 8192
+    // 19 against 23, though of 1 x 700 16 against 13); with many items their long slices no longer even out (24 ragged sequences, 6
+    // tokens: 107 against 81).
+    p.nw = HD == 256 || (p.nt == 2 ? 2 * items >= n_cu : 8 * items >= slots) ? 4 : 8;
     p.cap = std::max(2 * B, slots * 4 / p.nw / std::max(1, HKV * p.blocks));
+    // The last slice joins, a launch less, where sequences of one length leave its threads up to 8 loads each (64 x 128 keys 8 us
+    // against 13, 1 x 32768 22.1 against 23.3, 1 x 700 9.9 against 11). With more its workgroup is the longer way (1 x 8192, 2
+    // tokens 17.8 against 14.9, 16 query heads of one KV head 88 against 28).
+    p.fused = items <= 4096 && R <= 16 && (int64_t)p.cap / B * R * (HD / 4) <= 8 * 64 * p.nw;
     p.part = align_up((size_t)p.cap * HKV * p.blocks * p.rt * (HD + 4) * sizeof(float), 256);
     p.plan = (size_t)B * sizeof(int2);
     return p;
@@ -602,10 +610,12 @@ static hipError_t paged_by_rows(const PagedArgs &a, const PagedPlan &p, hipStrea
             return paged_launch<PagedForm<D, F, KT, 2, 4, true, false>>(a, p, s);
         }
     if (a.T > 1 || a.window) {
-        if (p.fused) return paged_launch<PagedForm<D, F, KT, 1, 4, true, true>>(a, p, s);
+        if (p.fused && p.nw == 4) return paged_launch<PagedForm<D, F, KT, 1, 4, true, true>>(a, p, s);
+        if (p.fused) return paged_launch<PagedForm<D, F, KT, 1, WIDE, true, true>>(a, p, s);
         return paged_launch<PagedForm<D, F, KT, 1, WIDE, true, false>>(a, p, s);
     }
-    if (p.fused) return paged_launch<PagedForm<D, F, KT, 1, 4, false, true>>(a, p, s);
+    if (p.fused && p.nw == 4) return paged_launch<PagedForm<D, F, KT, 1, 4, false, true>>(a, p, s);
+    if (p.fused) return paged_launch<PagedForm<D, F, KT, 1, WIDE, false, true>>(a, p, s);
     return paged_launch<PagedForm<D, F, KT, 1, WIDE, false, false>>(a, p, s);
 }
 hipError_t launch_attn_paged(const float *q, int B, int T, int H, int HKV, int HD, KvLayer kv, int kv_f16, int n_pages,

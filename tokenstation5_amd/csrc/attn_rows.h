@@ -496,8 +496,8 @@ struct RowsJoin {
     float2 ml[256];
 };
 // load(s, d, ml, x) loads slice s's m and l and its dims d .. + 3.
-template <int HD, int SG, class Load>
-__device__ inline float4 rows_join(RowsJoin &J, int used, float &M, float &l, Load load) {
+template <int HD, int SG, class Join, class Load>
+__device__ inline float4 rows_join(Join &J, int used, float &M, float &l, Load load) {
     constexpr int L4 = HD / 4, AHEAD = 8;
     const int tid = threadIdx.x, sg = tid / L4 % SG, d = 4 * (tid % L4);
     M = -INFINITY, l = 0.f;
