@@ -571,11 +571,21 @@ static PagedPlan paged_plan(int B, int T, int H, int HKV, int HD, int n_cu) {
     // 19 against 23, though of 1 x 700 16 against 13); with many items their long slices no longer even out (24 ragged sequences, 6
     // tokens: 107 against 81).
     p.nw = HD == 256 || (p.nt == 2 ? 2 * items >= n_cu : 8 * items >= slots) ? 4 : 8;
-    p.cap = std::max(2 * B, slots * 4 / p.nw / std::max(1, HKV * p.blocks));
+    // Two slices a sequence, which always fit, and whole rounds of the workgroups that run at once (40 ragged sequences 112 us
+    // against 136 in one round and a quarter; three slices 4 % less here, but 64 x 2000 keys 69 against 61).
+    auto cap = [&] {
+        const int round = std::max(1, slots * 4 / p.nw / (HKV * p.blocks));
+        return (2 * B + round - 1) / round * round;
+    };
+    p.cap = cap();
     // The last slice joins, a launch less, where sequences of one length leave its threads up to 8 loads each (64 x 128 keys 8 us
     // against 13, 1 x 32768 22.1 against 23.3, 1 x 700 9.9 against 11). With more its workgroup is the longer way (1 x 8192, 2
-    // tokens 17.8 against 14.9, 16 query heads of one KV head 88 against 28).
+    // tokens 17.8 against 14.9; 8 ragged sequences of 4 tokens 38 against 23; two row tiles of them 22.7 against 13.9).
     p.fused = items <= 4096 && R <= 16 && (int64_t)p.cap / B * R * (HD / 4) <= 8 * 64 * p.nw;
+    if (!p.fused && p.nt == 1 && HD <= 128) {
+        p.nw = 8;
+        p.cap = cap();
+    }
     p.part = align_up((size_t)p.cap * HKV * p.blocks * p.rt * (HD + 4) * sizeof(float), 256);
     p.plan = (size_t)B * sizeof(int2);
     return p;
