@@ -325,6 +325,33 @@ def test_calls_in_turn(ctx):
         assert all(np.array_equal(got[0].view(np.uint32), g.view(np.uint32)) for g in got[1:])
 
 
+def test_two_contexts_at_once(ctx):
+    """Calls of two contexts (streams, scratch and counters of their own) in flight together: the bits of calls alone."""
+    other = ts5hip.Context(0)
+    try:
+        jobs = []
+        for x, seed in ((ctx, 1), (other, 2)):
+            rng = np.random.default_rng(seed)
+            for kv, T, lengths in ((Q8, 1, [3000, 900, 5, 260] * 3), (F16, 1, [8000]), (Q8, 6, [1500, 40])):
+                c = Pages(x, rng, kv, 8, 128, 32, lengths)
+                q = rng.standard_normal((len(lengths), T, 32, 128)).astype(np.float32)
+                args = x.to_device(q), x.to_device(np.array(lengths, np.int32)), [x.alloc(q.nbytes) for _ in range(9)]
+                alone = run_attn(x, c, q, lengths, 0, 0.09, 32)
+                jobs.append((x, c, q, alone, *args))
+        ctx.sync(), other.sync()
+        for turn in range(9):
+            for x, c, q, alone, qd, nd, outs in jobs[turn % 3::3]:
+                x.attn_paged(qd, *q.shape[:2], 32, 8, 128, *c.args, c.n_table, nd, 0, 0.09, outs[turn])
+            for x, c, q, alone, qd, nd, outs in jobs:
+                x.attn_paged(qd, *q.shape[:2], 32, 8, 128, *c.args, c.n_table, nd, 0, 0.09, outs[turn])
+        for x, c, q, alone, qd, nd, outs in jobs:
+            for out in outs:
+                assert np.array_equal(out.download(np.float32, q.shape).view(np.uint32), alone.view(np.uint32))
+        del jobs, x, c, q, alone, qd, nd, outs, out, args  # (the other context's buffers, before it)
+    finally:
+        other.close()
+
+
 def test_same_as_a_contiguous_cache(ctx):
     """Sequences of one length in pages and in caches of their own: the same attention."""
     rng = np.random.default_rng(16)
