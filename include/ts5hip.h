@@ -282,9 +282,9 @@ int ts5hip_kv_read_paged(ts5hip_ctx *ctx, int ntok, const int32_t *seq_dev, cons
 /* Attention of the n_new (1..16) newest tokens of each of B (1..4096) sequences over its pages: n_keys_dev[b] counts the
  * sequence's keys, those tokens' included (it is taken into 0..n_table x page), and token t reads keys below L = n_keys_dev[b]
  * - n_new + t + 1; with window > 0 only the last `window` of them. table_dev [B][n_table]; q, out [B][n_new][n_head *
- * head_dim], out over no input and not over the pool; up to 16 query heads a KV head; B x n_table x page up to 2^34. A query without a key (or whose
- * scores are all minus infinity, in fp32) gets zeros; infinities and NaN of keys and values that it does not read do not
- * reach it, of those that it reads they do. */
+ * head_dim], out over no input and not over the pool; up to 16 query heads a KV head; B x n_table x page up to 2^34. A query
+ * without a key (or whose scores are all minus infinity, in fp32) gets zeros; infinities and NaN of keys and values that it does
+ * not read do not reach it, of those that it reads they do. */
 int ts5hip_attn_paged(ts5hip_ctx *ctx, const float *q, int B, int n_new, int n_head, int n_head_kv, int head_dim,
                       int kv_type, const void *k, const void *ks, const void *v, const void *vs, int n_pages, int page,
                       const int32_t *table_dev, int n_table, const int32_t *n_keys_dev, int window, float scale, float *out);
