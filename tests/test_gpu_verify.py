@@ -338,3 +338,23 @@ def test_conversations_with_drafts(ctx, kv):
             lengths[b] += len(new)
             pending[b] = int(new[-1])
     assert all(len(e) >= 6 for e in emitted) and sum(map(len, emitted)) > 18
+
+
+@pytest.mark.parametrize("V", [37, 4096, 20000, 151936])
+def test_rows_equal_to_the_drafts(ctx, V):
+    """Target and draft rows alike bit for bit, and a draft that is not kept (outside the vocabulary, or of probability 0 in both
+    rows): p - q is 0 everywhere, and the token is drawn from p. The largest entry is shared by two places, and an entry in
+    five has no probability."""
+    rng = np.random.default_rng([10, V])
+    B, T = 24, 2
+    logits, draft, drafts, temp, uni = inputs(rng, B, T, V, True, noise=0.0)
+    logits[:, :, [3, V - 2]] = 11.0
+    logits[:, :, 1:V - 3:5] = -np.inf
+    draft = logits[:, :T].copy()
+    assert np.all(logits[:, :T, 1] == -np.inf)
+    drafts[0::3, 0], drafts[1::3, 0], drafts[2::3, 0] = -1, V, 1
+    temp[::4] = 1.0
+    uni[:4, T], uni[4:8, T] = 0, 1 - 2.0 ** -24
+    got = run(ctx, logits, draft, drafts, None, temp, uni)
+    check(logits, draft, drafts, None, temp, uni, got)
+    assert np.all(got[1] == 1)

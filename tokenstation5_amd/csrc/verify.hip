@@ -311,8 +311,13 @@ __global__ __launch_bounds__(VP_NT) void k_verify_pick(VerifyArgs a) {
             vf_load<VP_NT>(qrow, s0, a.V, y);
             const double inv_q = 1.0 / q.sum;
 #pragma unroll
-            for (int k = 0; k < PER; k++)
-                w[k] = fmax(vf_weight(x[k], p.top, by) * inv_p - vf_weight(y[k], q.top, by) * inv_q, 0.0);
+            for (int k = 0; k < PER; k++) {
+                // (both products rounded: fused, equal rows would leave the rounding error of one, above 0 for half of the
+                // entries, and the token would be drawn by those)
+#pragma clang fp contract(off)
+                const double pk = vf_weight(x[k], p.top, by) * inv_p, qk = vf_weight(y[k], q.top, by) * inv_q;
+                w[k] = fmax(pk - qk, 0.0);
+            }
         } else {
 #pragma unroll
             for (int k = 0; k < PER; k++) {
@@ -341,7 +346,7 @@ __global__ __launch_bounds__(VP_NT) void k_verify_pick(VerifyArgs a) {
         if (!last) return;
         if (tid < a.ns) mine = __hip_atomic_load(sums + tid, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
-    const bool less = by_q && vf_block_sum<VP_NT>(mine, lds) > 0.0;  // (else p and q are equal up to rounding)
+    const bool less = by_q && vf_block_sum<VP_NT>(mine, lds) > 0.0;  // (else they are equal: from p)
     if (!less) {
         mine = 0.0;
         if (tid < a.ns) {
