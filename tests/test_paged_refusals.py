@@ -76,3 +76,24 @@ def test_null_arguments(name, arg):
 def test_refused(name, change):
     rc, text = call(name, **change)
     assert rc in (ARG, UNS) and text not in ("ctx is null", ""), (rc, text)
+
+
+@pytest.mark.parametrize("change", [
+    # q_out over the biases (12 heads of 128), the norms (128) and the angles (64 positions of 128): their first and last bytes
+    dict(bias=6 * P), dict(bias=6 * P - 12 * 512 + 16), dict(q_norm=6 * P + 3 * 8 * 512 - 16), dict(q_norm=6 * P - 512 + 16),
+    dict(k_norm=6 * P), dict(k_norm=6 * P - 512 + 16), dict(cs=6 * P + 16), dict(cs=6 * P - 64 * 512 + 16),
+    # the pool (9 pages of 2 x 64 rows of 128 bytes, 8 of scales) over its own parts, the new rows and the table
+    dict(v=P), dict(v=P + 9 * 128 * 128 - 16), dict(ks=P + 1024), dict(vs=2 * P + 9 * 128 * 8 - 4), dict(vs=3 * P),
+    dict(k=7 * P), dict(v=7 * P + 3 * 12 * 512 - 16), dict(ks=7 * P), dict(vs=7 * P + 16), dict(k=5 * P), dict(vs=5 * P + 4),
+    dict(table=3 * P + 16), dict(kv=F16, ks=None, vs=None, v=P + 9 * 128 * 256 - 16)])
+def test_appends_over_what_they_read_or_write(change):
+    rc, text = call("append", **change)
+    assert (rc, text) == (ARG, "outputs lie over inputs or each other")
+
+
+@pytest.mark.parametrize("change", [
+    dict(bias=6 * P - 12 * 512), dict(bias=6 * P + 3 * 8 * 512), dict(q_norm=6 * P - 512), dict(k_norm=6 * P + 3 * 8 * 512),
+    dict(cs=6 * P - 64 * 512), dict(cs=6 * P, n_rot=0), dict(v=P + 9 * 128 * 128), dict(ks=P + 9 * 128 * 128),
+    dict(kv=F16, ks=P, vs=P), dict(k=7 * P + 3 * 12 * 512)])
+def test_appends_beside_what_they_read_or_write(change):
+    assert call("append", **change) == (ARG, "ctx is null")

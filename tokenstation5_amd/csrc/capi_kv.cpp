@@ -293,9 +293,13 @@ int ts5hip_rope_kv_append_paged(ts5hip_ctx *ctx, const float *qkv, int ntok, con
     const size_t heads = (size_t)ntok * head_dim * 4;
     const size_t pool = pool_values(n_pages, page, n_head_kv, head_dim, kv_type);
     const size_t scales = kv_type == KV_Q8 ? pool_scales(n_pages, page, n_head_kv, head_dim) : 0;
+    const Range table{table_dev, (size_t)n_seq * n_table * 4}, rows{qkv, heads * (n_head + 2 * n_head_kv)};
+    const size_t row = (size_t)(n_head + 2 * n_head_kv) * head_dim * 4, norm = (size_t)head_dim * 4;
+    if (int rc = check_apart(ctx, {{k, pool}, {v, pool}, {ks, scales}, {vs, scales}}, {rows, table})) return rc;
     if (int rc = check_apart(ctx, {{q_out, heads * n_head}},
-                             {{qkv, heads * (n_head + 2 * n_head_kv)}, {k, pool}, {v, pool}, {ks, scales}, {vs, scales},
-                              {table_dev, (size_t)n_seq * n_table * 4}, {seq_dev, (size_t)ntok * 4}, {pos_dev, (size_t)ntok * 4}}))
+                             {rows, {k, pool}, {v, pool}, {ks, scales}, {vs, scales}, table, {seq_dev, (size_t)ntok * 4},
+                              {pos_dev, (size_t)ntok * 4}, {bias, row}, {q_norm, norm}, {k_norm, norm},
+                              {rope_cs, (size_t)n_pos * n_rot * 4}}))
         return rc;
     if (!ctx) return fail(nullptr, TS5HIP_ERR_ARG, "ctx is null");
     const OnDevice on(ctx->device);
