@@ -266,8 +266,9 @@ int ts5hip_attn_sparse(ts5hip_ctx *ctx, const float *q, int B, int n_head, int n
 /* ts5hip_rope_kv_append into pages: token t (of 1..65535) belongs to position pos_dev[t] (which is its RoPE position too, a
  * row of rope_cs: 0..n_pos - 1) of sequence seq_dev[t] (0..n_seq - 1). A token without a place (padding: -1) is left out,
  * its row of q_out too. No two tokens of a call have one place: what it held then would be parts of both. q_out lies
- * over none of the inputs and not over the pool; the pool's arrays lie over no input and not over each other (checked for qkv,
- * the table and each other). */
+ * over none of the inputs and not over the pool; the pool's arrays lie over no input and not over each other (checked
+ * for qkv, the table and each other). A NaN or an infinity that is to be cached stays one, an infinity with its sign; in a q8
+ * cache the values that share its scale are none any more either (NaN beside a NaN, infinities or NaN beside an infinity). */
 int ts5hip_rope_kv_append_paged(ts5hip_ctx *ctx, const float *qkv, int ntok, const int32_t *seq_dev, const int32_t *pos_dev,
                                 int n_head, int n_head_kv, int head_dim, int n_rot, int neox, const float *rope_cs,
                                 int n_pos, const float *bias, const float *q_norm, const float *k_norm, float eps,

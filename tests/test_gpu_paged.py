@@ -589,3 +589,52 @@ def test_pools_past_4_gib(ctx):
             want, _, tol, _ = attend(q[b, :, h].astype(np.float64), rows[:, h], rows[:, HKV + h],
                                      seen_by(n, 2, 0, np.ones(n, bool)), 0.06)
             check_rows(got[b, :, h], want, tol, (b, h))
+
+
+@pytest.mark.parametrize("kv", [Q8, F16])
+@pytest.mark.parametrize("HKV,HD,n", [(8, 128, 7), (2, 64, 7), (4, 256, 7), (8, 128, 3400)])
+def test_append_of_values_that_are_not_finite(ctx, kv, HKV, HD, n):
+    """NaN and infinities in a token's K and V come back as such, an infinity with its sign: f16 caches round each value by
+    itself; of a q8 cache's 32 values that share a scale none is finite then. All others have the bits that they have
+    without them. (3400 tokens of 6 workgroups of rows: four tokens a thread.)"""
+    rng = np.random.default_rng([61, HD, n, kv])
+    H = 2 * HKV if n < 100 else 32
+    c = Pages(ctx, rng, kv, HKV, HD, 16, [n])
+    seq, pos = np.zeros(n, np.int32), np.arange(n, dtype=np.int32)
+    cs = np.zeros((n, 2), np.float32)
+    good = rng.standard_normal((n, H + 2 * HKV, HD)).astype(np.float32)
+    bad = good.copy()
+    hurt = np.zeros((n, 2 * HKV, HD // 32), bool)  # groups of 32 with such a value
+    for t in range(n):
+        for _ in range(4):
+            head, d = rng.integers(0, 2 * HKV), rng.integers(0, HD)
+            bad[t, H + head, d] = rng.choice(np.array([np.nan, -np.nan, np.inf, -np.inf], np.float32))
+            hurt[t, head, d // 32] = True
+    bad[0, H, :32], hurt[0, 0, 0] = np.nan, True  # all of a group
+    caches = []
+    for x in (good, bad):
+        for name, b in c.dev.items():
+            b.upload(c.raw[name])
+        append(ctx, c, x.reshape(n, -1), seq, pos, H, 0, 0, cs)
+        caches.append(c.fetch())
+    page, slot = c.table[0, pos // 16], pos % 16
+    for i, name in enumerate("kv"):
+        want = bad[:, H + i * HKV:H + (i + 1) * HKV]
+        groups = hurt[:, i * HKV:(i + 1) * HKV]
+        was, got = (c.values(name, raw)[page, :, slot] for raw in caches)
+        in_group = np.repeat(groups, 32, axis=-1)
+        assert np.array_equal(got[~in_group], was[~in_group])
+        if kv == F16:
+            assert np.array_equal(got[in_group], want[in_group].astype(np.float16).astype(np.float64), equal_nan=True)
+            continue
+        assert not np.any(np.isfinite(got[in_group]))
+        has_nan = np.repeat(np.isnan(want).reshape(n, HKV, -1, 32).any(-1), 32, axis=-1)
+        assert np.all(np.isnan(got[has_nan]))
+        signed = np.isinf(want) & ~has_nan
+        assert signed.any() and np.array_equal(got[signed], want[signed].astype(np.float64))
+    # Read back they are the same.
+    outs = [ctx.alloc(n * HKV * HD * 4) for _ in range(2)]
+    ctx.kv_read_paged(n, ctx.to_device(seq), ctx.to_device(pos), HKV, HD, *c.args, *c.table.shape, ts5hip.F32, *outs)
+    for name, o in zip("kv", outs):
+        assert np.array_equal(o.download(np.float32, (n, HKV, HD)), c.values(name, caches[1])[page, :, slot].astype(np.float32),
+                              equal_nan=True)

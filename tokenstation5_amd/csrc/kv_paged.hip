@@ -20,11 +20,18 @@ __device__ inline int64_t paged_slot(const PagedPool &p, int seq, int pos) {
     return (((int64_t)page * p.HKV) << p.lp) + (pos & ((1 << p.lp) - 1));
 }
 
-// Max over groups of 8 lanes, in every lane.
-__device__ inline float max8(float v) {
-    v = dpp_max<0xB1, 0xF, true>(v);     // quad_perm [1,0,3,2]
-    v = dpp_max<0x4E, 0xF, true>(v);     // quad_perm [2,3,0,1]
-    return dpp_max<0x141, 0xF, true>(v);  // row_half_mirror
+// The largest |x| over groups of 8 lanes, in every lane: as bits, whose order is the numbers' with infinity and then NaN above.
+template <int CTRL>
+__device__ inline uint32_t max_dpp(uint32_t x) {
+    return max(x, (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, CTRL, 0xF, 0xF, false));
+}
+__device__ inline float amax8(const float (&x)[4]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int k = 0; k < 4; k++) m = max(m, __float_as_uint(x[k]) & 0x7fffffffu);
+    m = max_dpp<0xB1>(m);                    // quad_perm [1,0,3,2]
+    m = max_dpp<0x4E>(m);                    // quad_perm [2,3,0,1]
+    return __uint_as_float(max_dpp<0x141>(m));  // row_half_mirror
 }
 
 // A row (one head of one token) takes HD / 4 lanes, 4 neighbouring values each; a thread takes the same head's row of TOK
@@ -147,15 +154,15 @@ __global__ __launch_bounds__(256) void k_append_paged(AppendArgs a) {
             uint2 w;
             w.x = (uint32_t)f2h(x.x) | (uint32_t)f2h(x.y) << 16, w.y = (uint32_t)f2h(x.z) | (uint32_t)f2h(x.w) << 16;
             *(uint2 *)((uint16_t *)(is_k ? a.p.kv.k : a.p.kv.v) + slot * HD + d) = w;
-        } else {  // per 32 values sc = f16(amax / 127), q = clamp(rint(v / sc), +-127)
-            const float amax = max8(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
+        } else {  // per 32 values sc = f16(amax / 127), q = clamp(rint(v / sc), +-127); a NaN makes sc NaN, an infinity infinite
+            const float v[4] = {x.x, x.y, x.z, x.w}, amax = amax8(v);
             const uint16_t sh = f2h(amax / 127.0f);
-            const float sc = h2f(sh), v[4] = {x.x, x.y, x.z, x.w};
+            const float sc = h2f(sh);
             uint32_t w = 0;
             if (sc > 0.f)
 #pragma unroll
-                for (int k = 0; k < 4; k++)
-                    w |= (uint32_t)((int)fminf(127.f, fmaxf(-127.f, rintf(v[k] / sc))) & 0xff) << (8 * k);
+                for (int k = 0; k < 4; k++)  // (infinity / infinity is NaN: 127 with the value's sign)
+                    w |= (uint32_t)((int)copysignf(fminf(127.f, rintf(fabsf(v[k]) / sc)), v[k]) & 0xff) << (8 * k);
             *(uint32_t *)((is_k ? a.p.kv.k : a.p.kv.v) + slot * HD + d) = w;
             if (d % 32 == 0) (is_k ? a.p.kv.ks : a.p.kv.vs)[slot * (HD / 32) + d / 32] = sh;
         }
