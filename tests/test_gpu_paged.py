@@ -638,3 +638,36 @@ def test_append_of_values_that_are_not_finite(ctx, kv, HKV, HD, n):
     for name, o in zip("kv", outs):
         assert np.array_equal(o.download(np.float32, (n, HKV, HD)), c.values(name, caches[1])[page, :, slot].astype(np.float32),
                               equal_nan=True)
+
+
+def test_joins_of_2_32_values():
+    """4096 sequences of 16 tokens of 256 heads of 256, 16 GiB of rows: more threads than one dimension of a grid takes join
+    the slices. Most sequences have no key; the first, one in the middle and the last have keys in several slices."""
+    ctx = ts5hip.Context(0)
+    try:
+        rng = np.random.default_rng(71)
+        B, T, H, HKV, HD, n_table = 4096, 16, 256, 16, 256, 64
+        k, v = (rng.standard_normal((n_table, HKV, 16, HD)).astype(np.float16) for _ in range(2))
+        kd, vd = ctx.to_device(k), ctx.to_device(v)
+        table = ctx.to_device(np.tile(np.arange(n_table, dtype=np.int32), (B, 1)))
+        lengths = np.zeros(B, np.int32)
+        lengths[[0, 2047, B - 1]] = 900, 1024, 700
+        row = T * H * HD * 4  # bytes of a sequence
+        q, out = ctx.alloc(B * row), ctx.alloc(B * row)
+        rows = {b: rng.standard_normal((T, H, HD)).astype(np.float32) for b in (0, 2047, B - 1)}
+        for b, x in rows.items():
+            ctx.check(ts5hip.lib().ts5hip_upload(ctx.h, q.ptr + b * row, x.ctypes.data, x.nbytes))
+        ctx.attn_paged(q, B, T, H, HKV, HD, F16, kd, None, vd, None, n_table, 16, table, n_table, ctx.to_device(lengths), 0, 0.06,
+                       out)
+        kk, vv = (x.astype(np.float64).transpose(1, 0, 2, 3).reshape(HKV, -1, HD) for x in (k, v))
+        for b, x in rows.items():
+            got, n = out.download(np.float32, (T, H, HD), b * row), int(lengths[b])
+            seen = seen_by(n, T, 0, np.ones(n, bool))
+            for h in (0, 15, 100, 255):
+                want, _, tol, _ = attend(x[:, h].astype(np.float64), kk[h // 16, :n], vv[h // 16, :n], seen, 0.06)
+                check_rows(got[:, h], want, tol, (b, h))
+        for b in (1, 2046, 2048, B - 2):
+            assert np.all(out.download(np.float32, (T * H * HD,), b * row) == 0)
+        del q, out, kd, vd, table
+    finally:
+        ctx.close()

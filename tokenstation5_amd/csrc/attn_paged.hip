@@ -540,7 +540,7 @@ template <int HD>
 __global__ __launch_bounds__(256) void k_paged_merge(PagedArgs a, int64_t rows) {
     constexpr int TPR = HD / 4 * JOIN_SG;
     __shared__ RowsJoin J;
-    const int64_t row = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR, at = min(row, rows - 1);
+    const int64_t row = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * (256 / TPR) + threadIdx.x / TPR, at = min(row, rows - 1);
     const int b = (int)(at / ((int64_t)a.HKV * a.R)), kvh = (int)(at / a.R % a.HKV), r = (int)(at % a.R);
     const int2 plan = a.plan[b];
     const int blocks = (a.R + a.RT - 1) / a.RT;
@@ -600,7 +600,9 @@ static hipError_t paged_launch(const PagedArgs &a, const PagedPlan &p, hipStream
     if (P::FUSED) return hipGetLastError();
     const int64_t rows = (int64_t)a.B * a.HKV * a.R;
     constexpr int RPW = 256 / (P::HD / 4 * JOIN_SG);
-    hipLaunchKernelGGL(k_paged_merge<P::HD>, dim3((unsigned)((rows + RPW - 1) / RPW)), dim3(256), 0, s, a, rows);
+    // (two dimensions: one has up to 2^32 threads, which 4096 sequences of 16 tokens of 256 heads of 256 pass)
+    const int64_t groups = (rows + RPW - 1) / RPW, x = std::min<int64_t>(groups, 1 << 20);
+    hipLaunchKernelGGL(k_paged_merge<P::HD>, dim3((unsigned)x, (unsigned)((groups + x - 1) / x)), dim3(256), 0, s, a, rows);
     return hipGetLastError();
 }
 // Two row tiles of q8 heads of 128 take 32 keys a unit if pages allow: half the value products' instructions (24 ragged
