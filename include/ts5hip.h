@@ -260,8 +260,9 @@ int ts5hip_attn_sparse(ts5hip_ctx *ctx, const float *q, int B, int n_head, int n
  * TS5HIP_KV_Q8: k, v int8 [n_pages][n_head_kv][page][head_dim], ks, vs f16 [..][head_dim / 32]; TS5HIP_KV_F16: k, v f16, ks
  * and vs null. Position p of sequence s is slot p % page of page table_dev[s * n_table + p / page]; sequences may share
  * pages. An entry outside 0..n_pages-1 is no page: tokens there are not written or read back, and their keys are no query's.
- * Head dimension 64, 128 or 256, n_head_kv up to 512, n_table x page up to 2^30; float arrays, cache values and read-back rows are
- * 16-byte aligned. Scratch is the context's, as above. ---- */
+ * Head dimension 64, 128 or 256, n_head_kv up to 512, n_table x page up to 2^30; float arrays, cache values and read-back
+ * rows are 16-byte aligned. Scratch is the context's, as above. A q8 value past f16's range (65504) reads back as it is in
+ * fp32 and is an infinity to the attention. ---- */
 
 /* ts5hip_rope_kv_append into pages: token t (of 1..65535) belongs to position pos_dev[t] (which is its RoPE position too, a
  * row of rope_cs: 0..n_pos - 1) of sequence seq_dev[t] (0..n_seq - 1). A token without a place (padding: -1) is left out,
@@ -285,8 +286,12 @@ int ts5hip_kv_read_paged(ts5hip_ctx *ctx, int ntok, const int32_t *seq_dev, cons
  * sequence's keys, those tokens' included (it is taken into 0..n_table x page), and token t reads keys below L = n_keys_dev[b]
  * - n_new + t + 1; with window > 0 only the last `window` of them. table_dev [B][n_table]; q, out [B][n_new][n_head *
  * head_dim], out over no input and not over the pool; up to 16 query heads a KV head; B x n_table x page up to 2^34. A query
- * without a key (or whose scores are all minus infinity, in fp32) gets zeros; infinities and NaN of keys and values that it does
- * not read do not reach it, of those that it reads they do. */
+ * without a key (or whose scores are all minus infinity, in fp32) gets zeros. Infinities and NaN of keys and values that it
+ * does not read do not reach it; NaN that it reads does, and an infinite value as an infinity or NaN.
+ * The rows are the newest tokens: where sequences have different numbers of them (fewer drafts in some), a row is right
+ * only if n_keys_dev[b] counts n_new tokens for every sequence, padding behind the real ones included, and n_table x page
+ * holds that count (past it the count is cut, and with it each row's L moves). Padding's keys need not be written: only
+ * padding's rows read them. A prompt of more tokens goes in calls of 16. */
 int ts5hip_attn_paged(ts5hip_ctx *ctx, const float *q, int B, int n_new, int n_head, int n_head_kv, int head_dim,
                       int kv_type, const void *k, const void *ks, const void *v, const void *vs, int n_pages, int page,
                       const int32_t *table_dev, int n_table, const int32_t *n_keys_dev, int window, float scale, float *out);
@@ -300,9 +305,9 @@ int ts5hip_attn_paged(ts5hip_ctx *ctx, const float *q, int B, int n_new, int n_h
  * uniform x their sum. uniform_dev [B][n_draft + 1] in [0, 1). At temperature 0 (or below, or NaN) drafts are kept while they
  * are the row's first maximum, and the next token is that. tokens_dev [B][n_draft + 1]: the kept drafts, the next token, -1
  * behind; n_tokens_dev [B]: how many; logp_dev [B][n_draft + 1] (may be null): log p of each (0 at temperature 0 and behind).
- * A draft outside 0..n_vocab-1 is not kept. A row with a NaN or plus infinity, or all minus infinity, is no distribution: a draft's
- * row counts as q = 0 and its draft is not kept; a sequence whose next token would come from one has none (-1, not counted).
- * Computed in fp64. B up to 4096; the outputs overlap no input and not each other. */
+ * A draft outside 0..n_vocab-1 is not kept. A row with a NaN or plus infinity, or all minus infinity, is no distribution: a
+ * draft's row counts as q = 0 and its draft is not kept; a sequence whose next token would come from one has none (-1, not
+ * counted). Computed in fp64. B up to 4096; the outputs overlap no input and not each other. */
 int ts5hip_verify_drafts(ts5hip_ctx *ctx, const float *logits, int64_t ld, const float *draft_logits, int64_t ld_draft,
                          int n_vocab, int B, int n_draft, const int32_t *drafts_dev, const int32_t *n_draft_dev,
                          const float *temperature_dev, const float *uniform_dev, int32_t *tokens_dev,

@@ -2,14 +2,16 @@
 // keys found tile by tile (16 of them, inside one page) through the sequence's table.
 //
 // Row (t, head) of sequence b takes keys max(0, L - window) .. L - 1, L = n_keys[b] - T + t + 1. The lengths are in
-// device memory and may differ a hundredfold, so every workgroup computes the same plan from them: the shortest
-// slice length L (in units of the core's keys) for which all sequences' slices together fit the launch's workgroups. A
-// workgroup has one slice of one sequence and KV head and up to 32 rows; slices join through partials.
+// device memory and may differ a hundredfold, so every workgroup computes the same plan from them: a slice length (in
+// units of the core's keys) with which all sequences' slices together fit the launch's workgroups, up to 64 sequences (a
+// lane each) the shortest such, past that one that always fits. A workgroup has one slice of one sequence and KV head and up
+// to 32 rows; slices join through partials.
 //
-// What bounds it: f16 caches memory (16 sequences of 16384 keys, 32/8 heads of 128: 188 us, 5.7 TB/s). q8 caches the vector
-// unit, which turns int8 into fp16 planes: 52 % of the busy cycles, the matrix cores another 28 % (the same sequences 121 us,
-// 4.7 TB/s; a contiguous cache 127). Several tokens the same (8 sequences of 8192, 6 tokens, 40/8 heads 47 us; the bytes alone
-// 29). Few or short sequences a chain of latencies, 7 us for one key: the lengths, the plan, the table, the keys, the
+// What bounds it: f16 caches memory (16 sequences of 16384 keys, 32/8 heads of 128: 188 us, 5.7 TB/s). q8 caches no unit alone:
+// the vector ALU, which turns int8 into fp16 planes, is busy for 51 % of the cycles and the matrix cores for 27 %, and the two
+// waves a SIMD wait for data for 28 % of theirs (the same sequences 117 us, 4.9 TB/s; a contiguous cache 127). Several tokens
+// the same: 58 %, 27 %, 31 % (8 sequences of 8192, 6 tokens, 40/8 heads 38.9 us and the join's 5.4; the bytes alone 29). Few or
+// short sequences a chain of latencies, 4.1 us and the join's 2.1 for one key: the lengths, the plan, the table, the keys, the
 // partials, the join.
 //
 // A wave has one unit in registers and requests the next one's keys once it has used this one's, and its values once it is
@@ -121,6 +123,8 @@ struct PagedPage {
     __device__ void look(const PagedArgs &a, PagedTable table, int to) { id = table[min(to, a.n_table - 1)]; }
     __device__ void turn(const PagedArgs &a, int kvh, int end, int to) {
         at = to, has = to < a.n_table && (uint32_t)id < (uint32_t)a.n_pages;
+        // A wave also looks at the page past the sequence's last key, and the table may have one there: without max the count is
+        // negative, and as a buffer's size it lets loads (the slot past all pages among them) run on for 4 GiB.
         // (readfirstlane: the compiler takes min and max as one vector instruction, and then each load as a loop over lanes
         // that might have buffers of their own)
         const int n = __builtin_amdgcn_readfirstlane(max(0, min(end - (to << a.lp), 1 << a.lp)));
